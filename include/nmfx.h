@@ -331,6 +331,77 @@ int nmfx_objective(nmfx_ctx *ctx, int alg, const nmfx_opts *opts, double *out);
 int nmfx_pdsolve(nmfx_ctx *ctx, const void *A_host, double lambda, const void *B_host, void *X_host, int project_nn);
 int nmfx_pdrsolve(nmfx_ctx *ctx, const void *A_host, const void *B_host, double lambda, void *X_host, int project_nn);
 
+/* ---- operators on device matrices ---------------------------------------------------------------------------------
+ * Two things a user who trains a factor model by gradients needs beside nmfx_objective and ALSPGrad's projected gradient norms; neither
+ * has a counterpart in the reference.  They take matrices that are in device memory, run on the caller's stream and keep nothing:
+ *   device    the HIP device of all the pointers; it need not be the current one (which is as before when the call returns)
+ *   stream    a hipStream_t of that device (NULL: its default stream).  Calls return once everything is enqueued; nothing is allocated,
+ *             copied to the host or waited for, so they can be captured into a graph.  The results of a call do not depend on timing: the
+ *             same inputs give the same bits
+ *   workspace device memory the caller keeps until the work is done; its size comes from the _workspace call.  Calls that may run at the
+ *             same time (two streams, two captured graphs) need one each
+ * Errors: the status; nmfx_last_op_error() is the text of the calling thread's last call of this section.  Every check is made on the host
+ * before anything is enqueued. */
+
+enum { NMFX_BF16 = 2, NMFX_F16 = 3 };          /* element types of device matrices, beside NMFX_F32 and NMFX_F64 */
+
+/* element (i, j) is at data[i * rs + j * cs] (strides in elements).  One of rs, cs must be 1 and the other at least the extent that it
+ * steps over: a column-major matrix has rs = 1, cs = ld; a row-major one rs = ld, cs = 1.  data is aligned to its element, no more. */
+typedef struct {
+    void *data;
+    int64_t rows, cols, rs, cs;
+    int32_t dtype;
+    int32_t reserved;         /* must be 0 */
+} nmfx_dmat;
+
+const char *nmfx_last_op_error(void);
+
+/* Softmax cross entropy of the logits Z = W*H (W p x k, H k x n) against one class labels[j] in 0..p-1 per column, without keeping Z: the
+ * objective of a factor model whose data are observed classes (words, tokens, items), as 0.5 sqL2dist and gkldiv are of one whose data are
+ * numbers.  With s = opts->label_smoothing:
+ *     lse[j]  = log sum_v exp Z[v, j]
+ *     loss[j] = lse[j] - (1 - s) Z[labels[j], j] - (s / p) sum_v Z[v, j]
+ * Columns with labels[j] = opts->ignore_index are left out whatever H holds there: loss[j] = lse[j] = 0, a zero column of dH, nothing in dW.
+ * A label that is neither that nor a class makes the column's loss and lse NaN (and with them the reduced loss, dW and that column of dH).
+ *   opts->reduction   NMFX_REDUCE_NONE: loss has n values; _SUM, _MEAN: one, the sum over the columns that are not ignored or their mean
+ *                     (0 where there is none)
+ *   lse               n values, or NULL
+ * Types: W and H are both NMFX_F32, NMFX_BF16 or NMFX_F16 (NMFX_F64: NMFX_ERR_UNSUPPORTED); products are summed in Float32, loss and lse are
+ * Float32.  p and n at most 2^21, k at most 2^20.  n = 0 is allowed. */
+typedef struct {
+    double label_smoothing;   /* in [0, 1] */
+    int64_t ignore_index;
+    int32_t reduction;
+    int32_t reserved0;        /* must be 0 */
+} nmfx_xent_opts;
+enum { NMFX_REDUCE_NONE = 0, NMFX_REDUCE_SUM = 1, NMFX_REDUCE_MEAN = 2 };
+int nmfx_xent_workspace(const nmfx_dmat *W, const nmfx_dmat *H, const nmfx_xent_opts *opts, int grad, int64_t *bytes);
+int nmfx_xent(const nmfx_dmat *W, const nmfx_dmat *H, const int64_t *labels, const nmfx_xent_opts *opts, float *loss, float *lse,
+              void *workspace, int64_t workspace_bytes, int device, void *stream);
+
+/* Its gradients dW (p x k) and dH (k x n), of the types of W and H, any strides of their own; overlapping no input.
+ *   gout       the gradient of what follows in the loss: n values for NMFX_REDUCE_NONE, else one; NULL stands for 1
+ *   lse_given  0: loss (or NULL) and lse (or NULL) are computed and written as nmfx_xent does
+ *              1: lse holds what nmfx_xent gave for the same W, H and labels, and is read; loss is not written
+ * dZ is formed per piece of the classes and rounded to the type of W and H in front of the two products (Float16: scaled by a power of two
+ * into its range first); the sums are Float32 and rounded once. */
+int nmfx_xent_grad(const nmfx_dmat *W, const nmfx_dmat *H, const int64_t *labels, const nmfx_xent_opts *opts, const float *gout,
+                   int lse_given, float *loss, float *lse, const nmfx_dmat *dW, const nmfx_dmat *dH, void *workspace,
+                   int64_t workspace_bytes, int device, void *stream);
+
+/* The norm over all elements of a list of matrices -- NMFX_NORM_2: sqrt(sum g^2), NMFX_NORM_INF: max |g| -- and clipping by it:
+ *     coef = min(1, max_norm / (norm + 1e-6)),   out = g * coef
+ * The list may mix all four types; a vector is a matrix of one row.  Squares are summed in Float64.  *norm (device memory) is Float32.
+ * out = NULL: in place (nothing is written where coef = 1); else out[i] has grads[i]'s shape, type and contiguous index.  No two matrices
+ * written may share elements, and none may be part of another's gradient (NMFX_ERR_BAD_ARG).  A NaN among the gradients makes the norm
+ * and every result NaN; an infinite norm makes coef 0. */
+enum { NMFX_NORM_2 = 2, NMFX_NORM_INF = 0 };
+int nmfx_grad_norm_workspace(int count, int64_t *bytes);
+int nmfx_grad_norm(int count, const nmfx_dmat *grads, int norm_type, float *norm, void *workspace, int64_t workspace_bytes, int device,
+                   void *stream);
+int nmfx_clip_grad_norm(int count, const nmfx_dmat *grads, const nmfx_dmat *out, double max_norm, int norm_type, float *norm,
+                        void *workspace, int64_t workspace_bytes, int device, void *stream);
+
 /* Device/timing introspection used by bench.py (no reference counterpart). */
 typedef struct {
     char name[64];

@@ -1,0 +1,389 @@
+// gradnorm.hip -- the norm over all elements of a list of matrices, sqrt(sum g^2) or max |g|, and clipping by it:
+//     coef = min(1, max_norm / (norm + 1e-6)),   out = g * coef
+// Two passes over the list: partial sums (a fixed number of blocks, each over a fixed set of chunks: the same list gives the same bits),
+// and the scaling, whose every block adds up the partial sums for itself (at most ~2048 doubles from L2: cheaper than a launch in between).
+// Squares are summed in Float64: the sum of 10^9 of them loses nothing, and a gradient of 10^30 does not overflow; the conversion and the
+// product-sum cost less than the memory takes.  The scaling walks the chunks backwards, so that it starts on what the first pass read last
+// and the last-level cache still holds.  Bound by memory: one read for the norm, one more and a write for the scaling.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "device_ops.hpp"
+
+namespace nmfx {
+namespace gradnorm {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));   // 16 bytes at any element's address
+
+constexpr int NT = 256;
+constexpr int CHUNK_BYTES = 16384;      // 4 loads of 16 bytes for each of 256 threads
+constexpr int MAXT = 72;                // table entries of a launch: they travel as kernel arguments (4 KB)
+constexpr int BLOCKS = 2048;
+
+struct Entry {
+    const char *in;
+    char *out;
+    int64_t n;              // elements
+    int64_t ldi, ldo;       // elements between rows; 0: dense
+    int cols;               // elements of a row (where not dense)
+    int chunk0;             // first chunk
+};
+struct Table {
+    Entry e[MAXT];
+    int dtype[MAXT];
+    int count, chunks;
+};
+
+template <int INF> __device__ __forceinline__ void take(double &s, double x) {
+    if (INF) {
+        const double a = fabs(x);
+        s = a > s || a != a ? a : s;      // a NaN stays
+    } else s = __builtin_fma(x, x, s);
+}
+template <int INF> __device__ __forceinline__ double both(double a, double b) {
+    if (INF) return a != a ? a : (b > a || b != b ? b : a);
+    return a + b;
+}
+template <int INF> __device__ __forceinline__ double block_total(double s, double *sh, int nt) {
+    for (int o = 32; o; o >>= 1) s = both<INF>(s, __shfl_xor(s, o));
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = sh[0];
+    for (int w = 1; w < nt / 64; ++w) s = both<INF>(s, sh[w]);
+    __syncthreads();
+    return s;
+}
+
+// the entry a chunk belongs to (the table is short and the index the same for the whole block)
+__device__ __forceinline__ int entry_of(const Table &t, int chunk) {
+    int lo = 0, hi = t.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (t.e[mid].chunk0 <= chunk) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+template <typename T> __device__ __forceinline__ int64_t at(const Entry &e, int64_t i, int64_t ld) {
+    if (!e.ldi) return i;
+    const int64_t r = i / e.cols;
+    return r * ld + (i - r * e.cols);
+}
+
+template <typename T, int INF> __device__ __forceinline__ void sum_chunk(const Entry &e, int chunk, int nt, double &s) {
+    constexpr int V = 16 / sizeof(T), PER = CHUNK_BYTES / sizeof(T);
+    const T *in = reinterpret_cast<const T *>(e.in);
+    const int64_t beg = (int64_t)(chunk - e.chunk0) * PER, end = min(e.n, beg + PER);
+    if (!e.ldi) {
+        const int64_t whole = beg + (end - beg) / V * V;
+        if (end - beg == PER && nt == NT) {
+            u32x4 v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const u32x4_any *>(in + beg + (int64_t)(q * NT + threadIdx.x) * V);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const T *x = reinterpret_cast<const T *>(&v[q]);
+#pragma unroll
+                for (int u = 0; u < V; ++u) take<INF>(s, (double)x[u]);
+            }
+            return;
+        }
+        for (int64_t i = beg + (int64_t)threadIdx.x * V; i < whole; i += nt * V) {
+            const u32x4 v = *reinterpret_cast<const u32x4_any *>(in + i);
+            const T *x = reinterpret_cast<const T *>(&v);
+#pragma unroll
+            for (int u = 0; u < V; ++u) take<INF>(s, (double)x[u]);
+        }
+        for (int64_t i = whole + threadIdx.x; i < end; i += nt) take<INF>(s, (double)in[i]);
+    } else
+        for (int64_t i = beg + threadIdx.x; i < end; i += nt) take<INF>(s, (double)in[at<T>(e, i, e.ldi)]);
+}
+
+template <typename T> __device__ __forceinline__ T scaled(T x, double c) {
+    if constexpr (sizeof(T) == 8) return x * c;
+    else return (T)((float)x * (float)c);
+}
+template <typename T> __device__ __forceinline__ void scale_chunk(const Entry &e, int chunk, int nt, double c) {
+    constexpr int V = 16 / sizeof(T), PER = CHUNK_BYTES / sizeof(T);
+    const T *in = reinterpret_cast<const T *>(e.in);
+    T *out = reinterpret_cast<T *>(e.out);
+    const int64_t beg = (int64_t)(chunk - e.chunk0) * PER, end = min(e.n, beg + PER);
+    if (!e.ldi && !e.ldo) {
+        const int64_t whole = beg + (end - beg) / V * V;
+        if (end - beg == PER && nt == NT) {
+            u32x4 v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const u32x4_any *>(in + beg + (int64_t)(q * NT + threadIdx.x) * V);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                T *x = reinterpret_cast<T *>(&v[q]);
+#pragma unroll
+                for (int u = 0; u < V; ++u) x[u] = scaled(x[u], c);
+                *reinterpret_cast<u32x4_any *>(out + beg + (int64_t)(q * NT + threadIdx.x) * V) = v[q];
+            }
+            return;
+        }
+        for (int64_t i = beg + (int64_t)threadIdx.x * V; i < whole; i += nt * V) {
+            u32x4 v = *reinterpret_cast<const u32x4_any *>(in + i);
+            T *x = reinterpret_cast<T *>(&v);
+#pragma unroll
+            for (int u = 0; u < V; ++u) x[u] = scaled(x[u], c);
+            *reinterpret_cast<u32x4_any *>(out + i) = v;
+        }
+        for (int64_t i = whole + threadIdx.x; i < end; i += nt) out[i] = scaled(in[i], c);
+    } else
+        for (int64_t i = beg + threadIdx.x; i < end; i += nt) out[at<T>(e, i, e.ldo)] = scaled(in[at<T>(e, i, e.ldi)], c);
+}
+
+template <int INF> __device__ __forceinline__ void sum_any(const Table &t, int chunk, int nt, double &s) {
+    const int q = entry_of(t, chunk);
+    const Entry &e = t.e[q];
+    switch (t.dtype[q]) {
+        case NMFX_F32: sum_chunk<float, INF>(e, chunk, nt, s); break;
+        case NMFX_F64: sum_chunk<double, INF>(e, chunk, nt, s); break;
+        case NMFX_BF16: sum_chunk<__bf16, INF>(e, chunk, nt, s); break;
+        default: sum_chunk<_Float16, INF>(e, chunk, nt, s); break;
+    }
+}
+__device__ __forceinline__ void scale_any(const Table &t, int chunk, int nt, double c) {
+    const int q = entry_of(t, chunk);
+    const Entry &e = t.e[q];
+    switch (t.dtype[q]) {
+        case NMFX_F32: scale_chunk<float>(e, chunk, nt, c); break;
+        case NMFX_F64: scale_chunk<double>(e, chunk, nt, c); break;
+        case NMFX_BF16: scale_chunk<__bf16>(e, chunk, nt, c); break;
+        default: scale_chunk<_Float16>(e, chunk, nt, c); break;
+    }
+}
+template <int INF> __device__ __forceinline__ double norm_of(double s) { return INF ? s : sqrt(s); }
+__device__ __forceinline__ double coef_of(double norm, double max_norm) {
+    const double c = max_norm / (norm + 1e-6);
+    return c >= 1. ? 1. : c;                 // a NaN norm gives a NaN coefficient
+}
+
+template <int INF> __global__ __launch_bounds__(NT) void partial_kernel(Table t, double *part) {
+    __shared__ double sh[NT / 64];
+    double s = 0.;
+    for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) sum_any<INF>(t, c, NT, s);
+    s = block_total<INF>(s, sh, NT);
+    if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+template <int INF> __global__ __launch_bounds__(1024) void norm_kernel(const double *part, int parts, float *norm) {
+    __shared__ double sh[16];
+    double s = 0.;
+    for (int i = threadIdx.x; i < parts; i += 1024) s = both<INF>(s, part[i]);
+    s = block_total<INF>(s, sh, 1024);
+    if (threadIdx.x == 0) *norm = (float)norm_of<INF>(s);
+}
+template <int INF> __global__ __launch_bounds__(NT) void scale_kernel(Table t, const double *part, int parts, double max_norm, int in_place, float *norm) {
+    __shared__ double sh[NT / 64];
+    double s = 0.;
+    for (int i = threadIdx.x; i < parts; i += NT) s = both<INF>(s, part[i]);
+    const double nrm = norm_of<INF>(block_total<INF>(s, sh, NT)), c = coef_of(nrm, max_norm);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)nrm;
+    if (c == 1. && in_place) return;
+    for (int k = t.chunks - 1 - blockIdx.x; k >= 0; k -= gridDim.x) scale_any(t, k, NT, c);
+}
+// a short list: one block does all
+template <int INF> __global__ __launch_bounds__(1024) void small_kernel(Table t, double max_norm, int in_place, int clip, float *norm) {
+    __shared__ double sh[16];
+    double s = 0.;
+    for (int c = 0; c < t.chunks; ++c) sum_any<INF>(t, c, 1024, s);
+    const double nrm = norm_of<INF>(block_total<INF>(s, sh, 1024));
+    if (threadIdx.x == 0) *norm = (float)nrm;
+    if (!clip) return;
+    const double c = coef_of(nrm, max_norm);
+    if (c == 1. && in_place) return;
+    for (int k = 0; k < t.chunks; ++k) scale_any(t, k, 1024, c);
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------------------------
+constexpr int64_t SMALL_CHUNKS = 8;
+
+struct View {           // a matrix as rows of contiguous elements
+    char *p;
+    int64_t rows, len, ld;   // len: elements of a row, ld: elements between rows
+    int es, dtype;
+    int64_t bytes() const { return ((rows - 1) * ld + len) * es; }
+};
+View view_of(const nmfx_dmat &m, const char *what) {
+    const std::string s(what);
+    const int es = ops::elem_bytes(m.dtype);
+    if (!es) throw ops::OpError{NMFX_ERR_BAD_ARG, s + ": dtype is none of NMFX_F32, NMFX_F64, NMFX_BF16, NMFX_F16"};
+    if (m.reserved != 0) throw ops::OpError{NMFX_ERR_BAD_ARG, s + ": reserved must be 0"};
+    if (m.rows < 0 || m.cols < 0) throw ops::OpError{NMFX_ERR_DIM_MISMATCH, s + ": negative extent"};
+    if (!m.rows || !m.cols) return View{nullptr, 0, 0, 0, es, m.dtype};
+    if (!m.data) throw ops::OpError{NMFX_ERR_BAD_ARG, s + ": data is NULL"};
+    if (reinterpret_cast<uintptr_t>(m.data) % es) throw ops::OpError{NMFX_ERR_BAD_ARG, s + ": data is not aligned to its element"};
+    View v{static_cast<char *>(m.data), 0, 0, 0, es, m.dtype};
+    if (m.cs == 1 && (m.rs >= m.cols || m.rows == 1)) { v.rows = m.rows; v.len = m.cols; v.ld = m.rs; }
+    else if (m.rs == 1 && (m.cs >= m.rows || m.cols == 1)) { v.rows = m.cols; v.len = m.rows; v.ld = m.cs; }
+    else throw ops::OpError{NMFX_ERR_BAD_ARG, s + ": one of rs, cs must be 1 and the other at least the extent it steps over"};
+    if (v.rows == 1 || v.ld == v.len) { v.len *= v.rows; v.rows = 1; v.ld = v.len; }
+    if (v.rows > 1 && v.len > INT32_MAX) throw ops::OpError{NMFX_ERR_UNSUPPORTED, s + ": rows of a strided matrix may have at most 2^31 - 1 elements"};
+    return v;
+}
+
+// whether two views have an element in common; exact for dense views and for views of one row stride, "yes" where that is not clear
+bool meet(const View &a, const View &b) {
+    if (a.p > b.p) return meet(b, a);
+    if (a.p + a.bytes() <= b.p) return false;
+    const int64_t la = a.rows > 1 ? a.ld * a.es : 0, lb = b.rows > 1 ? b.ld * b.es : 0;
+    const int64_t ld = la ? la : lb;
+    if (!ld || (la && lb && la != lb)) return true;
+    if (!la || !lb) return true;
+    const int64_t d = (b.p - a.p) % ld;
+    return !(d >= a.len * a.es && d + b.len * b.es <= ld);
+}
+bool any_meet(std::vector<View> v) {
+    std::sort(v.begin(), v.end(), [](const View &a, const View &b) { return a.p < b.p; });
+    for (size_t i = 0; i < v.size(); ++i)
+        for (size_t j = i + 1; j < v.size() && v[j].p < v[i].p + v[i].bytes(); ++j)
+            if (meet(v[i], v[j])) return true;
+    return false;
+}
+
+struct Plan {
+    std::vector<Table> tables;
+    std::vector<int> blocks;
+    int parts = 0;
+    int64_t chunks = 0;
+};
+int64_t chunks_of(const View &v) { return (v.rows * v.len * v.es + CHUNK_BYTES - 1) / CHUNK_BYTES; }
+
+Plan plan_of(const std::vector<View> &in, const std::vector<View> &out) {
+    Plan p;
+    for (size_t i = 0; i < in.size(); ++i) {
+        const View &a = in[i], &b = out[i];
+        if (!a.rows) continue;
+        const int64_t c = chunks_of(a);
+        ops::require(c <= INT32_MAX / 2, NMFX_ERR_UNSUPPORTED, "a matrix is larger than 2^44 bytes");
+        if (p.tables.empty() || p.tables.back().count == MAXT || p.tables.back().chunks + c > INT32_MAX / 2) p.tables.push_back(Table{});
+        Table &t = p.tables.back();
+        const bool dense = a.rows == 1 && b.rows == 1;
+        // where only one side is dense, both go by the rows of the other
+        const int64_t cols = a.rows > 1 ? a.len : b.len;
+        t.e[t.count] = Entry{a.p, b.p, a.rows * a.len, dense ? 0 : (a.rows > 1 ? a.ld : cols), dense ? 0 : (b.rows > 1 ? b.ld : cols), (int)(dense ? 0 : cols), t.chunks};
+        t.dtype[t.count++] = a.dtype;
+        t.chunks += (int)c;
+        p.chunks += c;
+    }
+    for (const Table &t : p.tables) {
+        const int64_t share = std::max<int64_t>(1, (int64_t)BLOCKS * t.chunks / p.chunks);
+        p.blocks.push_back((int)std::min<int64_t>(t.chunks, share));
+        p.parts += p.blocks.back();
+    }
+    return p;
+}
+int64_t workspace_of(int64_t count) { return 8 * (BLOCKS + count / MAXT + 64); }
+
+template <int INF> void launch(const Plan &p, bool clip, bool in_place, double max_norm, float *norm, double *part, hipStream_t st) {
+    if (p.tables.size() == 1 && p.chunks <= SMALL_CHUNKS) {
+        small_kernel<INF><<<1, 1024, 0, st>>>(p.tables[0], max_norm, in_place, clip, norm);
+        ops::hip_ok(hipGetLastError(), "gradient norm");
+        return;
+    }
+    int at = 0;
+    for (size_t i = 0; i < p.tables.size(); at += p.blocks[i], ++i) {
+        partial_kernel<INF><<<p.blocks[i], NT, 0, st>>>(p.tables[i], part + at);
+        ops::hip_ok(hipGetLastError(), "gradient norm");
+    }
+    if (!clip || p.tables.empty()) {
+        norm_kernel<INF><<<1, 1024, 0, st>>>(part, p.parts, norm);
+        ops::hip_ok(hipGetLastError(), "gradient norm");
+        return;
+    }
+    for (size_t i = p.tables.size(); i-- > 0;) {
+        const int blocks = (int)std::min<int64_t>(p.tables[i].chunks, BLOCKS);
+        scale_kernel<INF><<<blocks, NT, 0, st>>>(p.tables[i], part, p.parts, max_norm, in_place, i == 0 ? norm : nullptr);
+        ops::hip_ok(hipGetLastError(), "gradient scaling");
+    }
+}
+
+void run(int count, const nmfx_dmat *g, const nmfx_dmat *o, bool clip, double max_norm, int norm_type, float *norm, void *ws, int64_t ws_bytes, int device, void *stream) {
+    ops::require(count >= 0, NMFX_ERR_BAD_ARG, "count must not be negative");
+    ops::require(g || !count, NMFX_ERR_BAD_ARG, "the list of matrices is NULL");
+    ops::require(norm != nullptr, NMFX_ERR_BAD_ARG, "norm is NULL");
+    ops::require(norm_type == NMFX_NORM_2 || norm_type == NMFX_NORM_INF, NMFX_ERR_BAD_ARG, "norm_type is neither NMFX_NORM_2 nor NMFX_NORM_INF");
+    ops::require(!clip || max_norm >= 0., NMFX_ERR_BAD_ARG, "max_norm must not be negative");
+    ops::require(ws && ws_bytes >= workspace_of(count), NMFX_ERR_BAD_ARG, "the workspace is smaller than nmfx_grad_norm_workspace says");
+    ops::require((reinterpret_cast<uintptr_t>(ws) & 7) == 0, NMFX_ERR_BAD_ARG, "the workspace must be aligned to 8 bytes");
+    std::vector<View> in, out;
+    in.reserve(count);
+    out.reserve(count);
+    for (int i = 0; i < count; ++i) {
+        in.push_back(view_of(g[i], "a gradient"));
+        out.push_back(clip && o ? view_of(o[i], "a clipped gradient") : in.back());
+        if (clip && o) {
+            ops::require(g[i].rows == o[i].rows && g[i].cols == o[i].cols, NMFX_ERR_DIM_MISMATCH, "a clipped gradient must have its gradient's shape");
+            ops::require(g[i].dtype == o[i].dtype, NMFX_ERR_BAD_ARG, "a clipped gradient must have its gradient's dtype");
+            const bool vec = g[i].rows <= 1 || g[i].cols <= 1;
+            ops::require(vec || (g[i].cs == 1) == (o[i].cs == 1), NMFX_ERR_BAD_ARG, "a clipped gradient must have its gradient's contiguous index");
+        }
+    }
+    if (clip) {
+        // every element is written by one thread once: no two results may share one, and none may be another's input
+        std::vector<View> w;
+        for (int i = 0; i < count; ++i)
+            if (out[i].rows) w.push_back(out[i]);
+        ops::require(!any_meet(w), NMFX_ERR_BAD_ARG, "two of the matrices to write share elements");
+        if (o) {
+            std::vector<View> r;
+            for (int i = 0; i < count; ++i)
+                if (in[i].rows && !(in[i].p == out[i].p && in[i].rows == out[i].rows && in[i].ld == out[i].ld)) r.push_back(in[i]);
+            std::sort(w.begin(), w.end(), [](const View &a, const View &b) { return a.p < b.p; });
+            std::vector<char *> reach;            // how far the written views up to this one reach
+            for (const View &v : w) reach.push_back(std::max(reach.empty() ? v.p : reach.back(), v.p + v.bytes()));
+            for (const View &a : r)
+                for (size_t j = std::upper_bound(reach.begin(), reach.end(), a.p) - reach.begin(); j < w.size() && w[j].p < a.p + a.bytes(); ++j)
+                    ops::require(!meet(a, w[j]), NMFX_ERR_BAD_ARG, "a matrix to write shares elements with a gradient that is not its own");
+        }
+    }
+    const Plan p = plan_of(in, out);
+    ops::require((int64_t)p.parts * 8 <= workspace_of(count), NMFX_ERR_STATE, "partial sums exceed the workspace");
+    ops::OnDevice on(device);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    bool in_place = true;
+    for (int i = 0; i < count; ++i) in_place = in_place && in[i].p == out[i].p;
+    if (norm_type == NMFX_NORM_2) launch<0>(p, clip, in_place, max_norm, norm, static_cast<double *>(ws), st);
+    else launch<1>(p, clip, in_place, max_norm, norm, static_cast<double *>(ws), st);
+}
+
+}  // namespace gradnorm
+
+namespace ops {
+std::string &last_error() {
+    thread_local std::string msg;
+    return msg;
+}
+}  // namespace ops
+}  // namespace nmfx
+
+using namespace nmfx;
+
+extern "C" {
+
+const char *nmfx_last_op_error(void) { return ops::last_error().c_str(); }
+
+int nmfx_grad_norm_workspace(int count, int64_t *bytes) {
+    return ops::guarded([&] {
+        ops::require(bytes && count >= 0, NMFX_ERR_BAD_ARG, "bytes is NULL or count negative");
+        *bytes = gradnorm::workspace_of(count);
+    });
+}
+
+int nmfx_grad_norm(int count, const nmfx_dmat *grads, int norm_type, float *norm, void *workspace, int64_t workspace_bytes, int device, void *stream) {
+    return ops::guarded([&] { gradnorm::run(count, grads, nullptr, false, 0., norm_type, norm, workspace, workspace_bytes, device, stream); });
+}
+
+int nmfx_clip_grad_norm(int count, const nmfx_dmat *grads, const nmfx_dmat *out, double max_norm, int norm_type, float *norm, void *workspace,
+                        int64_t workspace_bytes, int device, void *stream) {
+    return ops::guarded([&] { gradnorm::run(count, grads, out, true, max_norm, norm_type, norm, workspace, workspace_bytes, device, stream); });
+}
+
+}  // extern "C"

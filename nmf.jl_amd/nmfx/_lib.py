@@ -11,7 +11,9 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("NMFX_LIB", os.path.join(_HERE, "..", "lib", "libnmfx.so"))
 
-F32, F64 = 0, 1
+F32, F64, BF16, F16 = 0, 1, 2, 3
+REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2
+NORM_2, NORM_INF = 2, 0
 ALG_MULTMSE, ALG_MULTDIV, ALG_PROJALS, ALG_ALSPGRAD, ALG_CD, ALG_GREEDYCD = 0, 1, 2, 3, 4, 5
 PREC_FP32, PREC_BF16X3 = 0, 1
 OK, ERR_BAD_ARG, ERR_DIM_MISMATCH, ERR_NOT_POSDEF, ERR_ALPHA_NONFINITE, ERR_HIP, ERR_RCCL, ERR_NO_DEVICE, ERR_STATE, ERR_UNSUPPORTED = range(10)
@@ -25,6 +27,7 @@ SYMBOLS = [
     "nmfx_comm_get_unique_id", "nmfx_comm_init", "nmfx_objective", "nmfx_profile_enable", "nmfx_profile_get", "nmfx_set_final_objective",
     "nmfx_device_info", "nmfx_check_nonneg", "nmfx_randinit", "nmfx_solve_replicates", "nmfx_nndsvd", "nmfx_get_iter_trace", "nmfx_rsvd_begin", "nmfx_rsvd_finish",
     "nmfx_local_group_create", "nmfx_local_group_destroy", "nmfx_comm_init_local", "nmfx_comm_set_mode", "nmfx_comm_init_sim", "nmfx_comm_init_p2p", "nmfx_comm_p2p_export", "nmfx_comm_p2p_attach", "nmfx_comm_p2p_stats", "nmfx_pdsolve", "nmfx_pdrsolve", "nmfx_spa_init",
+    "nmfx_last_op_error", "nmfx_xent_workspace", "nmfx_xent", "nmfx_xent_grad", "nmfx_grad_norm_workspace", "nmfx_grad_norm", "nmfx_clip_grad_norm",
 ]
 COMM_ROW_SHARDED, COMM_REPLICATED_W, COMM_PIPELINED, COMM_REPLICAS = 0, 1, 2, 3
 
@@ -47,6 +50,15 @@ class CResult(C.Structure):
 class KernelStat(C.Structure):
     _fields_ = [("name", C.c_char * 64), ("ms_total", C.c_double), ("launches", C.c_int64),
                 ("flops", C.c_double), ("bytes", C.c_double)]
+
+
+class DMat(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64), ("rs", C.c_int64), ("cs", C.c_int64),
+                ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class XentOpts(C.Structure):
+    _fields_ = [("label_smoothing", C.c_double), ("ignore_index", C.c_int64), ("reduction", C.c_int32), ("reserved0", C.c_int32)]
 
 
 _lib = None
@@ -112,6 +124,14 @@ def load():
     lib.nmfx_set_final_objective.argtypes = [vp, i32]
     lib.nmfx_profile_get.argtypes = [vp, C.POINTER(KernelStat), i32, C.POINTER(i32)]
     lib.nmfx_device_info.argtypes = [i32, C.c_char_p, i32, C.POINTER(i32), C.POINTER(i64)]
+    dm, xo = C.POINTER(DMat), C.POINTER(XentOpts)
+    lib.nmfx_last_op_error.restype = C.c_char_p
+    lib.nmfx_xent_workspace.argtypes = [dm, dm, xo, i32, C.POINTER(i64)]
+    lib.nmfx_xent.argtypes = [dm, dm, vp, xo, vp, vp, vp, i64, i32, vp]
+    lib.nmfx_xent_grad.argtypes = [dm, dm, vp, xo, vp, i32, vp, vp, dm, dm, vp, i64, i32, vp]
+    lib.nmfx_grad_norm_workspace.argtypes = [i32, C.POINTER(i64)]
+    lib.nmfx_grad_norm.argtypes = [i32, vp, i32, vp, vp, i64, i32, vp]
+    lib.nmfx_clip_grad_norm.argtypes = [i32, vp, vp, C.c_double, i32, vp, vp, i64, i32, vp]
     for s in SYMBOLS:
         if getattr(lib, s).restype is C.c_int:
             pass

@@ -1,0 +1,232 @@
+"""Operators on matrices that are in device memory (torch tensors): softmax cross entropy of W*H with its gradients, the norm over many
+gradients, clipping by it.
+
+They run on torch's current stream of the tensors' device, take their workspace from torch's allocator, wait for nothing and can be captured
+into a graph.  The reference has no counterpart; the arithmetic is stated at the entry points in include/nmfx.h.  The rest of the package
+works without torch: it is imported with the first call."""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from . import _lib as L
+from .api import ArgumentError, DimensionMismatch, _raise
+
+_DMAT = np.dtype([("data", "u8"), ("rows", "i8"), ("cols", "i8"), ("rs", "i8"), ("cs", "i8"), ("dtype", "i4"), ("reserved", "i4")])
+_REDUCTIONS = {"none": L.REDUCE_NONE, "sum": L.REDUCE_SUM, "mean": L.REDUCE_MEAN}
+_state = {}
+
+
+def _torch():
+    if not _state:
+        import torch
+        _state.update(torch=torch, dtypes={torch.float32: L.F32, torch.float64: L.F64, torch.bfloat16: L.BF16, torch.float16: L.F16})
+    return _state["torch"]
+
+
+def _ck(status):
+    if status != L.OK:
+        _raise(status, L.load().nmfx_last_op_error().decode())
+
+
+def _matrix(t, name, device=None):
+    torch = _torch()
+    if not isinstance(t, torch.Tensor):
+        raise ArgumentError(f"{name} must be a torch tensor")
+    if t.dim() != 2:
+        raise DimensionMismatch(f"{name} must be a matrix, not {t.dim()}-dimensional")
+    if t.dtype not in _state["dtypes"]:
+        raise ArgumentError(f"{name} has dtype {t.dtype}: float32, float64, bfloat16 and float16 are taken")
+    if not t.is_cuda:
+        raise ArgumentError(f"{name} must be in device memory: there is no CPU path")
+    if device is not None and t.device != device:
+        raise ArgumentError(f"{name} is on {t.device}, not on {device}")
+    return L.DMat(t.data_ptr(), t.shape[0], t.shape[1], t.stride(0), t.stride(1), _state["dtypes"][t.dtype], 0)
+
+
+def _vector(t, name, n, dtype, device):
+    torch = _torch()
+    if not isinstance(t, torch.Tensor):
+        raise ArgumentError(f"{name} must be a torch tensor")
+    if t.dtype != dtype:
+        raise ArgumentError(f"{name} must be {dtype}, not {t.dtype}")
+    if t.numel() != n or t.dim() > 1:
+        raise DimensionMismatch(f"{name} must have {n} value(s), not the shape {tuple(t.shape)}")
+    if t.device != device:
+        raise ArgumentError(f"{name} is on {t.device}, not on {device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _xent_args(W, H, labels, ignore_index, label_smoothing, reduction):
+    torch = _torch()
+    if reduction not in _REDUCTIONS:
+        raise ArgumentError(f"reduction must be 'none', 'sum' or 'mean', not {reduction!r}")
+    w = _matrix(W, "W")
+    h = _matrix(H, "H", W.device)
+    labels = _vector(labels, "labels", H.shape[1], torch.int64, W.device)
+    return w, h, labels, L.XentOpts(float(label_smoothing), int(ignore_index), _REDUCTIONS[reduction], 0)
+
+
+def _workspace(w, h, o, grad, device):
+    size = C.c_int64()
+    _ck(L.load().nmfx_xent_workspace(w, h, o, grad, size))
+    return _torch().empty(size.value, dtype=_torch().uint8, device=device), size.value
+
+
+def _stream(device):
+    return _torch().cuda.current_stream(device).cuda_stream
+
+
+def softmax_xent(W, H, labels, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
+    """Softmax cross entropy of the logits W @ H against one class per column, without keeping the logits: (loss, lse).
+
+    W (p x k) and H (k x n) are float32, bfloat16 or float16 with one contiguous index each; labels has n int64 values, classes 0..p-1 or
+    ignore_index.  loss is float32: n values for reduction 'none' (-loss is the label's log-probability), else one, the sum or the mean over
+    the columns that are not ignored (0 where there is none).  lse, the log-sum-exp of every column's logits, has n values; both are 0 in
+    ignored columns.  A label that is no class makes its column's loss NaN."""
+    torch = _torch()
+    w, h, labels, o = _xent_args(W, H, labels, ignore_index, label_smoothing, reduction)
+    dev, n = W.device, H.shape[1]
+    ws, size = _workspace(w, h, o, 0, dev)
+    loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=dev)
+    lse = torch.empty(n, dtype=torch.float32, device=dev)
+    _ck(L.load().nmfx_xent(w, h, labels.data_ptr(), o, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), size, dev.index, _stream(dev)))
+    return loss, lse
+
+
+def _like(t):
+    """An empty matrix of t's shape, type and contiguous index, dense."""
+    if t.stride(1) == 1 or t.stride(0) != 1:
+        return _torch().empty(t.shape, dtype=t.dtype, device=t.device)
+    return _torch().empty((t.shape[1], t.shape[0]), dtype=t.dtype, device=t.device).t()
+
+
+def _grad(W, H, labels, ignore_index, label_smoothing, reduction, gout, lse, dW, dH):
+    torch = _torch()
+    w, h, labels, o = _xent_args(W, H, labels, ignore_index, label_smoothing, reduction)
+    dev, n = W.device, H.shape[1]
+    if gout is not None:
+        gout = _vector(gout, "gout", n if reduction == "none" else 1, torch.float32, dev)
+    given = lse is not None
+    if given:
+        lse, loss = _vector(lse, "lse", n, torch.float32, dev), None
+    else:
+        lse = torch.empty(n, dtype=torch.float32, device=dev)
+        loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=dev)
+    dW = _like(W) if dW is None else dW
+    dH = _like(H) if dH is None else dH
+    gw, gh = _matrix(dW, "dW", dev), _matrix(dH, "dH", dev)
+    ws, size = _workspace(w, h, o, 1, dev)
+    _ck(L.load().nmfx_xent_grad(w, h, labels.data_ptr(), o, None if gout is None else gout.data_ptr(), int(given), None if given else loss.data_ptr(),
+                                lse.data_ptr(), gw, gh, ws.data_ptr(), size, dev.index, _stream(dev)))
+    return loss, lse, dW, dH
+
+
+def softmax_xent_grad(W, H, labels, ignore_index=-100, label_smoothing=0.0, reduction="mean", gout=None, dW=None, dH=None):
+    """softmax_xent with its gradients: (loss, lse, dW, dH).
+
+    gout is the gradient with respect to the loss (float32; n values for reduction 'none', else one; None: 1; with float16 gradients a loss
+    scale belongs here).  dW and dH have the types of W and H and their contiguous index; matrices to write them to can be given."""
+    return _grad(W, H, labels, ignore_index, label_smoothing, reduction, gout, None, dW, dH)
+
+
+def softmax_xent_backward(W, H, labels, lse, gout=None, ignore_index=-100, label_smoothing=0.0, reduction="mean", dW=None, dH=None):
+    """The gradients alone, (dW, dH), from the lse that softmax_xent returned for the same arguments: for a gout that depends on the loss."""
+    if lse is None:
+        raise ArgumentError("lse must be what softmax_xent returned")
+    return _grad(W, H, labels, ignore_index, label_smoothing, reduction, gout, lse, dW, dH)[2:]
+
+
+def _list(ts, name, device=None):
+    """The descriptors of a list of tensors, as an array of nmfx_dmat."""
+    torch = _torch()
+    dtypes = _state["dtypes"]
+    a = np.zeros(len(ts), _DMAT)
+    if not len(ts):
+        return a
+    for t in ts:
+        if not isinstance(t, torch.Tensor):
+            raise ArgumentError(f"{name} must be torch tensors")
+        if t.device != device or t.dtype not in dtypes or not t.is_cuda:
+            if not t.is_cuda:
+                raise ArgumentError(f"{name} must be in device memory: there is no CPU path")
+            if t.dtype not in dtypes:
+                raise ArgumentError(f"one of {name} has dtype {t.dtype}: float32, float64, bfloat16 and float16 are taken")
+            raise ArgumentError(f"one of {name} is on {t.device}, not on {device}")
+    a["data"] = [t.data_ptr() for t in ts]
+    a["cols"] = sizes = [t.numel() for t in ts]
+    a["rs"] = sizes
+    a["rows"] = a["cs"] = 1
+    a["dtype"] = [dtypes[t.dtype] for t in ts]
+    for i, t in enumerate(ts):
+        if not t.is_contiguous():
+            if t.dim() == 1:
+                a[i] = (t.data_ptr(), t.shape[0], 1, t.stride(0), 1, dtypes[t.dtype], 0)
+            elif t.dim() == 2:
+                a[i] = (t.data_ptr(), t.shape[0], t.shape[1], t.stride(0), t.stride(1), dtypes[t.dtype], 0)
+            else:
+                raise ArgumentError(f"one of {name} has more than two indices and is not contiguous")
+    return a
+
+
+def _norm_type(norm_type):
+    if norm_type == 2:
+        return L.NORM_2
+    if norm_type == float("inf"):
+        return L.NORM_INF
+    raise ArgumentError(f"norm_type must be 2 or inf, not {norm_type!r}")
+
+
+def _norm(grads, max_norm, norm_type, out):
+    torch = _torch()
+    kind = _norm_type(norm_type)
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    if not grads:
+        raise ArgumentError("grads is empty")
+    dev = getattr(grads[0], "device", None)
+    a = _list(grads, "grads", dev)
+    b = None
+    if out is not None:
+        out = [out] if isinstance(out, torch.Tensor) else list(out)
+        if len(out) != len(grads):
+            raise DimensionMismatch(f"out has {len(out)} tensors, grads {len(grads)}")
+        for g, o in zip(grads, out):
+            if getattr(o, "shape", None) != g.shape:
+                raise DimensionMismatch("one of out has another shape than its gradient")
+        b = _list(out, "out", dev)
+        # a dense gradient beside a strided result (or the other way round): both go by the strides of their matrix
+        for i in np.nonzero(a["rows"] != b["rows"])[0]:
+            g, o = grads[i], out[i]
+            if g.dim() == 2:
+                a[i] = (g.data_ptr(), *g.shape, *g.stride(), a[i]["dtype"], 0)
+                b[i] = (o.data_ptr(), *o.shape, *o.stride(), b[i]["dtype"], 0)
+            else:
+                for x, t in ((a, g), (b, o)):
+                    x[i] = (t.data_ptr(), t.shape[0], 1, t.stride(0), 1, x[i]["dtype"], 0)
+    lib = L.load()
+    size = C.c_int64()
+    _ck(lib.nmfx_grad_norm_workspace(len(grads), size))
+    ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    common = (norm.data_ptr(), ws.data_ptr(), size.value, dev.index, _stream(dev))
+    if max_norm is None:
+        _ck(lib.nmfx_grad_norm(len(grads), a.ctypes.data, kind, *common))
+    else:
+        _ck(lib.nmfx_clip_grad_norm(len(grads), a.ctypes.data, None if b is None else b.ctypes.data, float(max_norm), kind, *common))
+    return norm
+
+
+def grad_norm(grads, norm_type=2):
+    """The norm over all elements of a list of tensors (or of one), as a float32 tensor on their device: sqrt(sum g^2), or max |g| for
+    norm_type inf.  float32, float64, bfloat16 and float16 may be mixed; squares are summed in float64."""
+    return _norm(grads, None, norm_type, None)
+
+
+def clip_grad_norm(grads, max_norm, norm_type=2, out=None):
+    """Scales a list of tensors by min(1, max_norm / (norm + 1e-6)), in place or into `out`, and returns the norm that they had.
+
+    Tensors are contiguous, or matrices and vectors with a stride; no two that are written may share elements."""
+    if max_norm is None:
+        raise ArgumentError("max_norm is None")
+    return _norm(grads, max_norm, norm_type, out)
