@@ -367,7 +367,8 @@ const char *nmfx_last_op_error(void);
  *                     (0 where there is none)
  *   lse               n values, or NULL
  * Types: W and H are both NMFX_F32, NMFX_BF16 or NMFX_F16 (NMFX_F64: NMFX_ERR_UNSUPPORTED); products are summed in Float32, loss and lse are
- * Float32.  p and n at most 2^21, k at most 2^20.  n = 0 is allowed. */
+ * Float32.  p, n and the stride of W at most
+ * 2^21 - 1024, k half of that.  n = 0 is allowed. */
 typedef struct {
     double label_smoothing;   /* in [0, 1] */
     int64_t ignore_index;

@@ -3,14 +3,19 @@
 // f32.
 //
 // Bytes, not elements, are the unit: a row of an LDS tile is 128 bytes = 8 chunks of 16 (64 contraction steps of a 16-bit type, 32 of
-// f32), so one address path serves all types.  Chunk c of row r sits in slot c ^ (r & 7) of its row: eight consecutive rows of one
-// chunk -- what the eight lanes of one LDS cycle read -- then fall into eight different 16-byte bank groups.  Tiles go from memory to LDS
-// without registers (buffer_load ... lds): lane l of a wave's load writes slot l & 7 of row l >> 3, so it fetches chunk (l & 7) ^ (l >> 3);
-// eight lanes read one whole 128-byte line.  Both operands see the same order of c inside a tile, so any order is right.
+// f32), so one address path serves all types.  Both operands see the same order of c inside a tile, so any order is right.
 //
-// Schedule: two LDS stages, ONE barrier per tile, placed in front of the tile's last quarter of matrix instructions: by then a wave holds
-// the fragments of that quarter in registers, so behind the barrier the freed stage is refilled and the first fragments of the next tile
-// are read while the matrix unit works through the quarter.  The loads of a tile have a whole tile's matrix time to arrive.
+// Feeding the matrix unit (bf16, 256 x 256 tile, 2048 x 32768 x 8192 product; TFLOP/s after each step):
+//   1120  32x32x16 instructions, fragments read a quarter of a tile ahead, one barrier a tile in front of its last quarter, the loads of
+//         the tile after next all issued behind it (two LDS stages)
+//   1212  the loads written out (to_lds), so that the compiler waits for none of them in front of a read, and a main loop without
+//         conditions
+//   1247  loads between the products instead of in a bunch: a bunch fills the address unit's queue and holds the wave's products back
+//   1290  16x16x32 instructions.  At this rate the card runs at its power limit, and they do the same work for less: registers alone,
+//         1985 TFLOP/s against 1745
+//   1318  the loads spread over 20 products, 8 of them in the next tile (12: 1290, 28: 1276, 44: 1198: the last ones then come too late)
+// A row stride that is a large power of two sends the rows of a tile to few memory channels (2048 x 8192 x 32768: 1137 TFLOP/s at 65536
+// bytes, 1317 at 256 more): images made for these products are padded.  Stages of 64-byte rows, 4 or 5 deep, were slower (1174-1195).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -21,28 +26,27 @@ namespace tn {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 template <typename T> struct Elem;
 template <> struct Elem<__bf16> {
-    static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    static constexpr int PARTS = 1;      // matrix instructions for a chunk
+    static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c, int) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
 };
 template <> struct Elem<_Float16> {
-    static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    static constexpr int PARTS = 1;
+    static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c, int) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
 };
-// f32: a chunk is 4 contraction steps; lanes 0-31 hold chunk 2q, lanes 32-63 chunk 2q + 1, and the e-th of four 32x32x2 instructions
-// takes the pair (4 (2q) + e, 4 (2q + 1) + e)
+// f32: a chunk is 4 contraction steps; the four quarters of the wave hold chunks 4 q .. 4 q + 3, and the e-th of four 16x16x4 instructions
+// takes each one's e-th element
 template <> struct Elem<float> {
-    static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
-        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], c, 0, 0, 0);
-        return c;
+    static constexpr int PARTS = 4;
+    static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c, int e) {
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, a)[e], __builtin_bit_cast(f32x4, b)[e], c, 0, 0, 0);
     }
 };
 
@@ -63,52 +67,62 @@ struct Args {
     int ktiles;         // tiles of the contraction, over all splits
 };
 
-// where a wave's part of a tile lies: element (i, j, r) of acc is row m0 + 32 i + 8 (r >> 2) + (r & 3), column n0 + 32 j
+// where a wave's part of a tile lies: element r of acc[i][j] is row m0 + 16 i + r, column n0 + 16 j
 struct Geom {
-    int m0, n0;         // with the lane's own share: m0 includes 4 (lane >> 5), n0 includes lane & 31
+    int m0, n0;         // with the lane's own share: m0 includes 4 (lane >> 4), n0 includes lane & 15
     int tile_m, tile_n, split, wm, wn, lane, tid;
 };
-__device__ __forceinline__ int acc_row(int i, int r) { return 32 * i + 8 * (r >> 2) + (r & 3); }
 
 typedef __attribute__((address_space(3))) void lds_void;
 
+// what a row's chunk numbers are xored with to give their slots: 16 consecutive rows' slots of one chunk fill all 64 banks once
+__device__ __forceinline__ int swizzle(int row) { return row >> 1 & 7; }
+
+// 16 bytes a lane from rsrc + off into LDS at `lds` (the same for the whole wave) + 16 lane.  Written out, so that the compiler, which cannot
+// tell which stage a load is for, does not wait for all of them in front of a read: the waits are tile()'s own.
+__device__ __forceinline__ void to_lds(u32x4 rsrc, char *lds, uint32_t off) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void *)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(at), "v"(off), "s"(rsrc) : "memory", "m0");
+}
+
+// TILE_ROWS rows, by NT threads
 template <int TILE_ROWS, int NT> struct Loader {
-    static constexpr int PER = TILE_ROWS * 8 / NT;   // 16-byte loads of a thread per tile
-    __amdgpu_buffer_rsrc_t rsrc;
-    uint32_t off[PER];
+    static constexpr int LPR = ROW / 16;                   // lanes of a row
+    static constexpr int PER = TILE_ROWS * LPR / NT;       // 16-byte loads of a thread per tile
+    static_assert(NT / LPR % 16 == 0, "a load of the block starts at a row that is a multiple of 16");
+    u32x4 rsrc;
+    uint32_t off, apart;      // of the thread's first load; between one load's row and the next one's
     int chunk, chunks;
     __device__ __forceinline__ void init(const Operand &o, int row0, int tid) {
         const int here = min(TILE_ROWS, o.rows - row0);                 // >= 1: the grid covers existing rows only
-        const char *base = static_cast<const char *>(o.p) + (int64_t)row0 * o.ld;
-        rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, (int)((int64_t)(here - 1) * o.ld + (int64_t)o.chunks * 16), 0x00020000);
-        const int l = tid & 63;
-        chunk = (l & 7) ^ (l >> 3);
+        const uint64_t at = reinterpret_cast<uint64_t>(o.p) + (int64_t)row0 * o.ld;
+        // the buffer ends with the last row that exists: rows behind it read as zero
+        rsrc = u32x4{(uint32_t)at, (uint32_t)(at >> 32), (uint32_t)((int64_t)(here - 1) * o.ld + (int64_t)o.chunks * 16), 0x00020000u};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
+        const int row = tid / LPR;
+        chunk = (tid & (LPR - 1)) ^ swizzle(row);
         chunks = o.chunks;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int row = (i * NT + (tid & ~63)) / 8 + (l >> 3);
-            off[i] = (uint32_t)min(row, here - 1) * (uint32_t)o.ld + chunk * 16;
-        }
+        off = (uint32_t)row * (uint32_t)o.ld + chunk * 16;
+        apart = (uint32_t)(NT / LPR) * (uint32_t)o.ld;
     }
-    __device__ __forceinline__ void load(char *lds, int tid, int kt) const {
-        // a chunk behind the row's end is asked for beyond the buffer: such loads return zero
-        const bool in = kt * 8 + chunk < chunks;
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *)(lds + (i * NT + (tid & ~63)) * 16), 16, in ? off[i] + kt * ROW : 0x80000000u, 0, 0, 0);
-    }
+    // where tile kt's loads start; a chunk behind the row's end is asked for beyond the buffer and reads as zero
+    __device__ __forceinline__ uint32_t start(int kt) const { return kt * LPR + chunk < chunks ? off + kt * ROW : 0x80000000u; }
+    __device__ __forceinline__ void load(char *lds, int tid, uint32_t start, int i) const { to_lds(rsrc, lds + (i * NT + (tid & ~63)) * 16, start + i * apart); }
 };
 
-template <typename T, int BM, int BN, int WM, int WN, typename Epi>
-__global__ __launch_bounds__(WM *WN * 64) void tn_kernel(Args g, Epi epi) {
-#ifdef __HIP_DEVICE_COMPILE__   // the host pass needs the kernel's stub only (with the body it drops the stubs of all but the first uses)
-    constexpr int NT = WM * WN * 64, MI = BM / WM / 32, NJ = BN / WN / 32, STAGE = (BM + BN) * ROW;
-    __shared__ __attribute__((aligned(1024))) char stage0[STAGE];
-    __shared__ __attribute__((aligned(1024))) char stage1[STAGE];
+// vmcnt(n) lgkmcnt(0)
+template <int N> __device__ __forceinline__ void wait_loads() {
+    static_assert(N < 64, "");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
+}
+
+// One tile's sums, in acc; false where the tile lies behind the operand's end.  ST: LDS stages.
+template <typename T, int BM, int BN, int WM, int WN, int ST>
+__device__ __forceinline__ bool tile(const Args &g, int bid, int nblk, char *const (&st)[ST], f32x4 (&acc)[BM / WM / 16][BN / WN / 16], Geom &geo) {
+    constexpr int NT = WM * WN * 64, MI = BM / WM / 16, NJ = BN / WN / 16;
     // consecutive blocks go to the 8 dies in turn: give every die a contiguous range of tiles, and walk a range in columns of 8 row
     // tiles, so that the tiles in flight on a die share rows of A and B in its L2
-    int bid = blockIdx.x;
-    const int nblk = gridDim.x;
     {
         const int die = bid & 7, q = nblk >> 3, rest = nblk & 7;
         bid = die * q + min(die, rest) + (bid >> 3);
@@ -121,7 +135,7 @@ __global__ __launch_bounds__(WM *WN * 64) void tn_kernel(Args g, Epi epi) {
     const int gm = min(8, g.tiles_m - grp * 8);
     const int tile_m = grp * 8 + in % gm, tile_n = in / gm;
     int ktiles = g.ktiles;
-    if (g.limit == LIMIT_N && tile_n * BN >= *g.count) return;
+    if (g.limit == LIMIT_N && tile_n * BN >= *g.count) return false;
     if (g.limit == LIMIT_C) ktiles = min(ktiles, (int)((*g.count * (int64_t)sizeof(T) + ROW - 1) / ROW));
     const int kbeg = (int)((int64_t)ktiles * split / g.splits), kend = (int)((int64_t)ktiles * (split + 1) / g.splits);
 
@@ -131,79 +145,166 @@ __global__ __launch_bounds__(WM *WN * 64) void tn_kernel(Args g, Epi epi) {
     Loader<BN, NT> lb;
     la.init(g.a, tile_m * BM, tid);
     lb.init(g.b, tile_n * BN, tid);
+    constexpr int LA = Loader<BM, NT>::PER, LOADS = LA + Loader<BN, NT>::PER;
 
-    f32x16 acc[MI][NJ];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+        for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // fragment addresses: row (lane & 31) of a 32-row group, chunk 2 q + (lane >> 5)
-    const int arow = wm * (BM / WM) + (lane & 31), brow = wn * (BN / WN) + (lane & 31);
-    const int sw = lane & 7, hi = lane >> 5;
-    u32x4 fa[2][MI], fb[2][NJ];
-    auto frags = [&](const char *st, int q, int set) {
-        const int slot = ((2 * q + hi) ^ sw) * 16;
-#pragma unroll
-        for (int i = 0; i < MI; ++i) fa[set][i] = *reinterpret_cast<const u32x4 *>(st + (arow + 32 * i) * ROW + slot);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) fb[set][j] = *reinterpret_cast<const u32x4 *>(st + BM * ROW + (brow + 32 * j) * ROW + slot);
+    // A tile is 2 halves of the contraction (64 bytes: one matrix instruction's), a half MI steps: A's fragment i times all NJ of B's.
+    // A's fragments are read D steps ahead into a ring of 4 sets of registers, B's a half ahead into the other of 2.
+    constexpr int STEPS = 2 * MI, D = MI < 3 ? MI : 3, MEET = STEPS - D;
+    static_assert(STEPS % 4 == 0, "the ring's place of a step is the same in every tile");
+    const int arow = (wm * (BM / WM) + (lane & 15)) * ROW, brow = BM * ROW + (wn * (BN / WN) + (lane & 15)) * ROW;
+    const int sw = swizzle(lane & 15), hi = lane >> 4;
+    const int slot0 = (hi ^ sw) * 16, slot1 = ((4 + hi) ^ sw) * 16;      // of the two halves
+    u32x4 fa[4], fb[2][NJ];
+    auto read_a = [&](const char *from, int s) { fa[s & 3] = *reinterpret_cast<const u32x4 *>(from + arow + (s % MI) * (16 * ROW) + (s < MI ? slot0 : slot1)); };
+    auto read_b = [&](const char *from, int half, int j) { fb[half][j] = *reinterpret_cast<const u32x4 *>(from + brow + j * (16 * ROW) + (half ? slot1 : slot0)); };
+    uint32_t sa = 0, sb = 0;
+    auto starts = [&](int kt) { sa = la.start(kt); sb = lb.start(kt); };
+    auto load = [&](char *to, int i) {
+        if (i < LA) la.load(to, tid, sa, i);
+        else lb.load(to + BM * ROW, tid, sb, i - LA);
     };
-    auto mult = [&](int set) {
-#pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) acc[i][j] = Elem<T>::mma(fa[set][i], fb[set][j], acc[i][j]);
-    };
-    auto fill = [&](char *st, int kt) {
-        la.load(st, tid, kt);
-        lb.load(st + BM * ROW, tid, kt);
-    };
-    // vmcnt(0) lgkmcnt(0): this wave's loads into LDS are there and its fragments read; then all waves'
-    auto meet = [&]() {
-        __builtin_amdgcn_s_waitcnt(0x0070);
+    // this wave's loads of the next tile are in LDS and its fragments of this one read (`later` tiles may still be on their way);
+    // then all waves'
+    auto meet = [&](int later) {
+        if (ST >= 5 && later >= 3) wait_loads<3 * LOADS>();
+        else if (ST >= 4 && later >= 2) wait_loads<2 * LOADS>();
+        else if (ST >= 3 && later >= 1) wait_loads<LOADS>();
+        else wait_loads<0>();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    auto step = [&](char *cur, char *nxt, int kt) {
-        frags(cur, 1, 1);
-        __builtin_amdgcn_sched_barrier(0);
-        mult(0);
-        __builtin_amdgcn_sched_barrier(0);
-        frags(cur, 2, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        mult(1);
-        __builtin_amdgcn_sched_barrier(0);
-        frags(cur, 3, 1);
-        __builtin_amdgcn_sched_barrier(0);
-        mult(0);
-        __builtin_amdgcn_sched_barrier(0);
-        if (kt + 1 < kend) {
-            meet();
-            if (kt + 2 < kend) fill(cur, kt + 2);
-            frags(nxt, 0, 0);
+    // Tile kt.  In front of step MEET all its fragments are in registers or on the way there: behind the barrier there its stage is free
+    // and tile kt + ST goes into it, the loads and the reads of the next tile's first fragments between the products of the last D steps.
+    // `all`: tiles up to kt + ST exist.
+    // the product behind the barrier after which load l goes out: from BEHIND on in the next tile
+    constexpr int BEHIND = D * NJ, WINDOW = BEHIND + 2 * NJ;
+    constexpr auto place = [](int l) { return (l + 1) * WINDOW / LOADS - 1; };
+    constexpr int LATE = [](auto f) { int n = 0; for (int l = 0; l < LOADS; ++l) n += f(l) >= BEHIND; return n; }(place);
+    auto run = [&](char *prev, char *cur, char *nxt, int kt, bool all) {
+        const bool more = all || kt + 1 < kend, fill = all || kt + ST < kend, late = all || kt - 1 + ST < kend;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const int half = s / MI, i = s % MI;
+            if (s == MEET && more) {
+                meet(all ? ST - 2 : kend - kt - 2);
+                starts(kt + ST);
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                acc[i][j] = Elem<T>::mma(fa[s & 3], fb[half][j], acc[i][j], 0);
+                __builtin_amdgcn_sched_barrier(0);
+                if (s < MEET) {
+                    if (late)
+#pragma unroll
+                        for (int l = 0; l < LOADS; ++l)
+                            if (place(l) == BEHIND + s * NJ + j) load(prev, l);
+                    if (j == 0) read_a(cur, s + D);
+                    // the other half of B: in the first half, spread over its steps
+                    if (half == 0)
+#pragma unroll
+                        for (int b = NJ * (i * NJ + j) / (MI * NJ); b < NJ * (i * NJ + j + 1) / (MI * NJ); ++b) read_b(cur, 1, b);
+                } else {
+                    const int e = (s - MEET) * NJ + j;
+                    if (more) {
+                        if (MEET >= MI) {                // (else B's first set is still in use)
+#pragma unroll
+                            for (int b = NJ * e / BEHIND; b < NJ * (e + 1) / BEHIND; ++b) read_b(nxt, 0, b);
+                        }
+                        if (j == NJ - 1) read_a(nxt, s + D - STEPS);
+                    }
+                    if (fill)
+#pragma unroll
+                        for (int l = 0; l < LOADS; ++l)
+                            if (place(l) == e) load(cur, l);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int e = 1; e < Elem<T>::PARTS; ++e)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[i][j] = Elem<T>::mma(fa[s & 3], fb[half][j], acc[i][j], e);
             __builtin_amdgcn_sched_barrier(0);
         }
-        mult(1);
     };
+    static_assert(MEET >= MI, "the barrier lies in the second half");
     if (kbeg < kend) {
-        fill(stage0, kbeg);
-        meet();
-        if (kbeg + 1 < kend) fill(stage1, kbeg + 1);
-        frags(stage0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < ST; ++i)
+            if (kbeg + i < kend) {
+                starts(kbeg + i);
+#pragma unroll
+                for (int l = 0; l < LOADS; ++l)
+                    if (i + 1 < ST || place(l) < BEHIND) load(st[i], l);
+            }
+        if (kbeg + ST - 1 < kend) wait_loads<(ST - 1) * LOADS - LATE>();
+        else wait_loads<0>();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) read_b(st[0], 0, j);
+#pragma unroll
+        for (int s = 0; s < D; ++s) read_a(st[0], s);
+        __builtin_amdgcn_sched_barrier(0);
         int kt = kbeg;
-        for (; kt + 1 < kend; kt += 2) {
-            step(stage0, stage1, kt);
-            step(stage1, stage0, kt + 1);
+        for (; kt + 2 * ST <= kend; kt += ST) {
+#pragma unroll
+            for (int i = 0; i < ST; ++i) run(st[(i + ST - 1) % ST], st[i], st[(i + 1) % ST], kt + i, true);
         }
-        if (kt < kend) step(stage0, stage1, kt);
+        for (; kt < kend; kt += ST) {
+#pragma unroll
+            for (int i = 0; i < ST; ++i)
+                if (kt + i < kend) run(st[(i + ST - 1) % ST], st[i], st[(i + 1) % ST], kt + i, false);
+        }
     }
-    Geom geo{tile_m * BM + wm * (BM / WM) + 4 * hi, tile_n * BN + wn * (BN / WN) + (lane & 31), tile_m, tile_n, split, wm, wn, lane, tid};
+    geo = Geom{tile_m * BM + wm * (BM / WM) + 4 * hi, tile_n * BN + wn * (BN / WN) + (lane & 15), tile_m, tile_n, split, wm, wn, lane, tid};
     __syncthreads();
-    epi.template finish<BM, BN, WM, WN, MI, NJ>(acc, geo, stage0);
+    return true;
+}
+
+// (separate arrays, not one: the compiler then knows that a load into one stage does not touch what is read from another, and waits for
+// neither)
+#define NMFX_TN_STAGES(BM, BN, ST)                                                        \
+    constexpr int STAGE = (BM + BN) * tn::ROW;                                              \
+    __shared__ __attribute__((aligned(1024))) char st0[STAGE];                            \
+    __shared__ __attribute__((aligned(1024))) char st1[STAGE];                            \
+    __shared__ __attribute__((aligned(1024))) char st2[ST >= 3 ? STAGE : 16];             \
+    __shared__ __attribute__((aligned(1024))) char st3[ST >= 4 ? STAGE : 16];             \
+    __shared__ __attribute__((aligned(1024))) char st4[ST >= 5 ? STAGE : 16];             \
+    char *const all[5] = {st0, st1, st2, st3, st4};                                       \
+    char *st[ST];                                                                         \
+    _Pragma("unroll") for (int i = 0; i < ST; ++i) st[i] = all[i];
+
+// (the host pass needs the kernels' stubs only: with the bodies it drops the stubs of all but the first uses)
+template <typename T, int BM, int BN, int WM, int WN, int ST, typename Epi>
+__global__ __launch_bounds__(WM *WN * 64) void tn_kernel(Args g, Epi epi) {
+#ifdef __HIP_DEVICE_COMPILE__
+    NMFX_TN_STAGES(BM, BN, ST)
+    f32x4 acc[BM / WM / 16][BN / WN / 16];
+    Geom geo;
+    if (!tile<T, BM, BN, WM, WN, ST>(g, blockIdx.x, gridDim.x, st, acc, geo)) return;
+    epi.template finish<BM, BN, WM, WN>(acc, geo, st0, st1);
+#endif
+}
+
+// two products in one launch: the first `first` blocks are one's, the others the other's
+template <typename T, int BM, int BN, int WM, int WN, int ST, typename EpiA, typename EpiB>
+__global__ __launch_bounds__(WM *WN * 64) void tn_pair_kernel(Args ga, EpiA ea, Args gb, EpiB eb, int first) {
+#ifdef __HIP_DEVICE_COMPILE__
+    NMFX_TN_STAGES(BM, BN, ST)
+    f32x4 acc[BM / WM / 16][BN / WN / 16];
+    Geom geo;
+    const bool is_a = (int)blockIdx.x < first;
+    const Args g = is_a ? ga : gb;
+    if (!tile<T, BM, BN, WM, WN, ST>(g, blockIdx.x - (is_a ? 0 : first), is_a ? first : gridDim.x - first, st, acc, geo)) return;
+    if (is_a) ea.template finish<BM, BN, WM, WN>(acc, geo, st0, st1);
+    else eb.template finish<BM, BN, WM, WN>(acc, geo, st0, st1);
 #endif
 }
 

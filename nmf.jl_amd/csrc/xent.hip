@@ -18,7 +18,7 @@
 namespace nmfx {
 namespace xent {
 
-using tn::f32x16;
+using tn::f32x4;
 using tn::Geom;
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -27,7 +27,8 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 struct Info {            // written by select_kernel, read by everything behind it
     int count;           // columns that are not ignored
     float unscale;       // what products with the stored dz are multiplied by
-    int pad[2];
+    unsigned ticket;     // combine_kernel's blocks that are done
+    int pad;
 };
 // What is stored of dz, in the type of W and H, is
 //     f_j ((exp(z_vj - lse_j) - eps / p) / a - [v = y_j]),   a = 1 - eps (1 where eps > 1/2)
@@ -49,47 +50,71 @@ struct Select {
     float *f, *lse_c;         // packed: f_j, log-sum-exp
     float *loss, *lse;        // the caller's: zero in ignored columns (loss only without reduction); NULL: not written
 };
-// One block: the order of the packed columns is that of the columns, so it takes a running count.  It is n / 1024 rounds of a ballot
-// and a 16-entry sum.
-__global__ __launch_bounds__(1024) void select_kernel(Select s) {
-    __shared__ int wsum[16];
-    __shared__ float wmax[16];
+
+// 8 columns a thread: which are not ignored, and how many of them are in front of the thread's first.  Returns their number in the block.
+template <int NT> __device__ __forceinline__ int ranks(const Select &s, int t0, unsigned &on, int &before) {
+    __shared__ int wsum[NT / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    on = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) on |= (t0 + e < s.n && s.labels[min(t0 + e, s.n - 1)] != s.ignore ? 1u : 0u) << e;
+    const int mine = __popc(on);
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(upto, o);
+        if (lane >= o) upto += v;
+    }
+    __syncthreads();                      // (wsum may still be read by the round before)
+    if (lane == 63) wsum[wave] = upto;
+    __syncthreads();
+    int all = 0;
+    before = upto - mine;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+        before += w < wave ? wsum[w] : 0;
+        all += wsum[w];
+    }
+    return all;
+}
+
+// One block: the order of the packed columns is that of the columns, so it takes a running count, 8 NT columns a round.
+template <int NT> __device__ __forceinline__ void select_columns(const Select &s) {
+    __shared__ float wmax[NT / 64];
     __shared__ float sh_scale;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int base = 0;
     float gmax = 0.f;
     const bool per = s.reduction == NMFX_REDUCE_NONE && s.gout != nullptr;
-    for (int t0 = 0; t0 < s.n; t0 += 1024) {
-        const int t = t0 + tid;
-        const int64_t lab = t < s.n ? s.labels[t] : s.ignore;
-        const bool on = t < s.n && lab != s.ignore;
-        const unsigned long long m = __ballot(on);
-        if (lane == 0) wsum[wave] = __popcll(m);
-        __syncthreads();
-        int before = 0, all = 0;
+    for (int t00 = 0; t00 < s.n; t00 += 8 * NT) {
+        unsigned on;
+        int before;
+        const int t0 = t00 + tid * 8, all = ranks<NT>(s, t0, on, before);
+        int i = base + before;
 #pragma unroll
-        for (int w = 0; w < 16; ++w) {
-            before += w < wave ? wsum[w] : 0;
-            all += wsum[w];
-        }
-        const int i = base + before + __popcll(m & ((1ull << lane) - 1));
-        if (t < s.n) s.pos[t] = on ? i : -1;
-        if (on) {
-            const bool bad = lab < 0 || lab >= s.p;
-            s.idx[i] = t;
-            s.y[i] = bad ? -1 : (int)lab;
-            if (s.lse_given) s.lse_c[i] = bad ? __builtin_nanf("") : s.lse_given[t];
-            if (per) {
-                const float g = s.gout[t];
-                s.f[i] = g;
-                gmax = fmaxf(gmax, fabsf(g));
+        for (int e = 0; e < 8; ++e) {
+            const int t = t0 + e;
+            if (t >= s.n) break;
+            if (on >> e & 1) {
+                const int64_t lab = s.labels[t];
+                const bool bad = lab < 0 || lab >= s.p;
+                s.pos[t] = i;
+                s.idx[i] = t;
+                s.y[i] = bad ? -1 : (int)lab;
+                if (s.lse_given) s.lse_c[i] = bad ? __builtin_nanf("") : s.lse_given[t];
+                if (per) {
+                    const float g = s.gout[t];
+                    s.f[i] = g;
+                    gmax = fmaxf(gmax, fabsf(g));
+                }
+                ++i;
+            } else {
+                s.pos[t] = -1;
+                if (s.lse) s.lse[t] = 0.f;
+                if (s.loss && s.reduction == NMFX_REDUCE_NONE) s.loss[t] = 0.f;
             }
-        } else if (t < s.n) {
-            if (s.lse) s.lse[t] = 0.f;
-            if (s.loss && s.reduction == NMFX_REDUCE_NONE) s.loss[t] = 0.f;
         }
         base += all;
-        __syncthreads();
     }
     float g = 1.f;
     if (!per) {
@@ -101,7 +126,7 @@ __global__ __launch_bounds__(1024) void select_kernel(Select s) {
     if (lane == 0) wmax[wave] = gmax;
     __syncthreads();
     if (tid == 0) {
-        for (int w = 1; w < 16; ++w) gmax = fmaxf(gmax, wmax[w]);
+        for (int w = 1; w < NT / 64; ++w) gmax = fmaxf(gmax, wmax[w]);
         float scale = 1.f;
         // the largest factor becomes at most 2^14: with a >= 1/2 what is stored is below 2^15 and finite in f16, and 2^-28 of it normal
         if (s.scaled && gmax > 0.f && gmax < __builtin_inff()) {
@@ -110,37 +135,36 @@ __global__ __launch_bounds__(1024) void select_kernel(Select s) {
             scale = ldexpf(1.f, min(max(14 - e, -100), 100));
         }
         sh_scale = scale;
-        *s.info = Info{base, (per ? 1.f : g) * s.a / scale, {0, 0}};
+        *s.info = Info{base, (per ? 1.f : g) * s.a / scale, 0, 0};
     }
     __syncthreads();
     const float scale = sh_scale;
-    for (int i = tid; i < base; i += 1024) s.f[i] = (per ? s.f[i] : 1.f) * scale;
+    for (int i = tid; i < base; i += NT) s.f[i] = (per ? s.f[i] : 1.f) * scale;
 }
+__global__ __launch_bounds__(1024) void select_kernel(Select s) { select_columns<1024>(s); }
 
 // ---- packed images ----------------------------------------------------------------------------------------------------------------
-// in: element (r, c) at in[r * rs + c * cs], r through idx where given; out1[r * ld1 + c], out2[c * ld2 + r], zero where r or c is
-// behind the end.  64 x 64 tiles through LDS, so that reads follow the contiguous index of `in` and both writes are contiguous.
+// in: element (r, c) at in[r * rs + c * cs]; out1[r * ld1 + c], out2[c * ld2 + r], zero where r or c is behind the end.  64 x 64 tiles
+// through LDS, so that reads follow the contiguous index of `in` and both writes are contiguous.
 template <typename T> struct Pack {
     const T *in;
     int64_t rs, cs;
-    const int *idx, *count;   // NULL: rows as they are
-    int rows, cols;           // that exist (rows: an upper bound where count is given)
+    int rows, cols;           // that exist
     T *out1, *out2;           // NULL: not wanted
     int64_t ld1, ld2;
-    int rpad, cpad;           // written extent
+    int rpad1, rpad2, cpad;   // written extent: rows of out1, of out2 (its columns), columns of out1
+    int tiles_r, tiles;
 };
-template <typename T> __global__ __launch_bounds__(256) void pack_kernel(Pack<T> a) {
-    __shared__ T tile[64][65];
-    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, lo = threadIdx.x & 63, up = threadIdx.x >> 6;
-    const int rows = a.count ? min(a.rows, *a.count) : a.rows;
+template <typename T> __device__ __forceinline__ void pack_tile(const Pack<T> &a, T (*tile)[65], const int *from, int rows, int r0, int c0) {
+    const int lo = threadIdx.x & 63, up = threadIdx.x >> 6;
     if (a.cs == 1) {
         for (int i = up; i < 64; i += 4) {
             const int r = r0 + i, c = c0 + lo;
-            tile[i][lo] = r < rows && c < a.cols ? a.in[(int64_t)(a.idx ? a.idx[r] : r) * a.rs + c] : (T)0.f;
+            tile[i][lo] = r < rows && c < a.cols ? a.in[(int64_t)(from ? from[i] : r) * a.rs + c] : (T)0.f;
         }
     } else {
         const int r = r0 + lo;
-        const T *row = a.in + (r < rows ? (int64_t)(a.idx ? a.idx[r] : r) * a.rs : 0);
+        const T *row = a.in + (r < rows ? (int64_t)(from ? from[lo] : r) * a.rs : 0);
         for (int i = up; i < 64; i += 4) {
             const int c = c0 + i;
             tile[lo][i] = r < rows && c < a.cols ? row[(int64_t)c * a.cs] : (T)0.f;
@@ -149,10 +173,43 @@ template <typename T> __global__ __launch_bounds__(256) void pack_kernel(Pack<T>
     __syncthreads();
     if (a.out1)
         for (int i = up; i < 64; i += 4)
-            if (r0 + i < a.rpad && c0 + lo < a.cpad) a.out1[(int64_t)(r0 + i) * a.ld1 + c0 + lo] = tile[i][lo];
+            if (r0 + i < a.rpad1 && c0 + lo < a.cpad) a.out1[(int64_t)(r0 + i) * a.ld1 + c0 + lo] = tile[i][lo];
     if (a.out2)
         for (int i = up; i < 64; i += 4)
-            if (c0 + i < a.cols && r0 + lo < a.rpad) a.out2[(int64_t)(c0 + i) * a.ld2 + r0 + lo] = tile[lo][i];
+            if (c0 + i < a.cols && r0 + lo < a.rpad2) a.out2[(int64_t)(c0 + i) * a.ld2 + r0 + lo] = tile[lo][i];
+}
+// Everything the products read, in one launch: H packed (first blocks), the images of W that its own order does not serve.  Up to
+// ONE_ROUND columns every block of H finds its 64 packed columns for itself (a round of 256 threads with 8 labels each: less than a launch),
+// and the first one leaves the lists; above, select_kernel has made them.
+constexpr int ONE_ROUND = 2048;
+template <typename T> __global__ __launch_bounds__(256) void prepare_kernel(Select s, Pack<T> h, Pack<T> w) {
+    __shared__ T tile[64][65];
+    __shared__ int from[64];
+    int b = blockIdx.x;
+    if (b >= h.tiles) {
+        b -= h.tiles;
+        pack_tile<T>(w, tile, nullptr, w.rows, (b % w.tiles_r) * 64, (b / w.tiles_r) * 64);
+        return;
+    }
+    const int r0 = (b % h.tiles_r) * 64, c0 = (b / h.tiles_r) * 64;
+    int rows;
+    if (s.n <= ONE_ROUND) {
+        unsigned on;
+        int before;
+        rows = ranks<256>(s, threadIdx.x * 8, on, before);
+        for (int e = 0; e < 8; ++e)
+            if (on >> e & 1) {
+                if (before >= r0 && before < r0 + 64) from[before - r0] = threadIdx.x * 8 + e;
+                ++before;
+            }
+        __syncthreads();
+    } else {
+        rows = s.info->count;
+        if (threadIdx.x < 64 && r0 + (int)threadIdx.x < rows) from[threadIdx.x] = s.idx[r0 + threadIdx.x];
+        __syncthreads();
+    }
+    pack_tile<T>(h, tile, from, rows, r0, c0);
+    if (b == 0 && s.n <= ONE_ROUND) select_columns<256>(s);
 }
 
 // (maximum, sum of exp(z - maximum)) of two sets.  An empty set, or one of minus infinities, is (-inf, 0) and changes nothing; a NaN sum
@@ -171,54 +228,57 @@ struct EpiStats {
     const int *count;
     int p, npad;
     template <int BM, int BN, int WM, int WN, int MI, int NJ>
-    __device__ __forceinline__ void finish(f32x16 (&acc)[MI][NJ], const Geom &g, char *smem) const {
+    __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, char *smem, char *) const {
         float2 *ps = reinterpret_cast<float2 *>(smem);                        // [WM][BN]
         float *zs = reinterpret_cast<float *>(smem + sizeof(float2) * WM * BN);
+        const int cnt = *count;
         if (g.tile_m * BM + BM > p) {
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (g.m0 + tn::acc_row(i, r) >= p)
+                for (int r = 0; r < 4; ++r)
+                    if (g.m0 + 16 * i + r >= p)
 #pragma unroll
                         for (int j = 0; j < NJ; ++j) acc[i][j][r] = -__builtin_inff();
         }
-        const int cnt = *count;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const int n = g.n0 + 32 * j;
+            const int n = g.n0 + 16 * j;
             float mx = -__builtin_inff();
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc[i][j][r]);
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
             const float ref = mx == -__builtin_inff() ? 0.f : mx;
             float s = 0.f;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s += exp2_((acc[i][j][r] - ref) * LOG2E);
+                for (int r = 0; r < 4; ++r) s += exp2_((acc[i][j][r] - ref) * LOG2E);
+            s += __shfl_xor(s, 16);
             s += __shfl_xor(s, 32);
-            const int col = g.wn * (BN / WN) + 32 * j + (g.lane & 31);
-            if (g.lane < 32) ps[g.wm * BN + col] = make_float2(mx, s);
+            const int col = g.wn * (BN / WN) + 16 * j + (g.lane & 15);
+            if (g.lane < 16) ps[g.wm * BN + col] = make_float2(mx, s);
             if (zsum) {
                 float t = 0.f;
 #pragma unroll
                 for (int i = 0; i < MI; ++i)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) t += g.m0 + tn::acc_row(i, r) < p ? acc[i][j][r] : 0.f;
+                    for (int r = 0; r < 4; ++r) t += g.m0 + 16 * i + r < p ? acc[i][j][r] : 0.f;
+                t += __shfl_xor(t, 16);
                 t += __shfl_xor(t, 32);
-                if (g.lane < 32) zs[g.wm * BN + col] = t;
+                if (g.lane < 16) zs[g.wm * BN + col] = t;
             }
             if (n < cnt) {
                 const int d = y[n] - g.m0;
-                if (d >= 0 && d < 32 * MI) {
+                if (d >= 0 && d < 16 * MI && (d & 15) < 4) {
 #pragma unroll
                     for (int i = 0; i < MI; ++i)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            if (d == tn::acc_row(i, r)) zy[n] = acc[i][j][r];
+                        for (int r = 0; r < 4; ++r)
+                            if (d == 16 * i + r) zy[n] = acc[i][j][r];
                 }
             }
         }
@@ -239,97 +299,196 @@ struct EpiStats {
     }
 };
 
-// joins the tiles' statistics: 64 packed columns a block, 4 waves share the tiles
+// joins the tiles' statistics of a column and finishes it
 struct Combine {
     const float2 *part;
     const float *zsum, *zy;
     const int *idx, *y;
-    const Info *info;
+    Info *info;
     int tiles, npad, p, reduction;
     float eps;
     float *lse_c, *loss_c, *lse, *loss;
+    // tiles slice, slice + step, ...
+    __device__ __forceinline__ void some(int i, int slice, int step, float2 &a, float &t) const {
+        a = make_float2(-__builtin_inff(), 0.f);
+        t = 0.f;
+#pragma unroll 4
+        for (int k = slice; k < tiles; k += step) {
+            a = join(a, part[(int64_t)k * npad + i]);
+            if (zsum) t += zsum[(int64_t)k * npad + i];
+        }
+    }
+    __device__ __forceinline__ float finish(int i, float2 a, float t, bool write) const {
+        const int lab = y[i];
+        const float v = lab < 0 ? __builtin_nanf("") : a.x + logf(a.y);     // a label that is no class: the column's loss is NaN
+        if (write) {
+            float l = v - (1.f - eps) * (lab < 0 ? 0.f : zy[i]);
+            if (zsum) l -= eps * (t / (float)p);
+            lse_c[i] = v;
+            loss_c[i] = l;
+            const int col = idx[i];
+            if (lse) lse[col] = v;
+            if (loss && reduction == NMFX_REDUCE_NONE) loss[col] = l;
+        }
+        return v;
+    }
 };
-__global__ __launch_bounds__(256) void combine_kernel(Combine c) {
-    __shared__ float2 ps[4][64];
-    __shared__ float zs[4][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = blockIdx.x * 64 + lane, cnt = c.info->count;
-    if (blockIdx.x * 64 >= cnt) return;
-    float2 a = make_float2(-__builtin_inff(), 0.f);
-    float t = 0.f;
-    for (int k = w; k < c.tiles; k += 4) {
-        const float2 b = c.part[(int64_t)k * c.npad + i];
-        a = join(a, b);
-        if (c.zsum) t += c.zsum[(int64_t)k * c.npad + i];
-    }
-    ps[w][lane] = a;
-    zs[w][lane] = t;
-    __syncthreads();
-    if (w || i >= cnt) return;
-    for (int q = 1; q < 4; ++q) {
-        a = join(a, ps[q][lane]);
-        t += zs[q][lane];
-    }
-    const int y = c.y[i];
-    float lse = a.x + logf(a.y);
-    if (y < 0) lse = __builtin_nanf("");                        // a label that is no class: the column's loss is NaN
-    float l = lse - (1.f - c.eps) * (y < 0 ? 0.f : c.zy[i]);
-    if (c.zsum) l -= c.eps * (t / (float)c.p);
-    c.lse_c[i] = lse;
-    c.loss_c[i] = l;
-    const int col = c.idx[i];
-    if (c.lse) c.lse[col] = lse;
-    if (c.loss && c.reduction == NMFX_REDUCE_NONE) c.loss[col] = l;
-}
 
-// one block, Float64, a fixed order
-__global__ __launch_bounds__(1024) void reduce_kernel(const float *loss_c, const Info *info, int reduction, float *loss) {
-    __shared__ double sh[16];
+// the losses' sum or mean, by one block: Float64, a fixed order
+template <int NT> __device__ __forceinline__ void reduce_losses(const float *loss_c, int cnt, int reduction, float *loss) {
+    __shared__ double sh[NT / 64];
     double s = 0.;
-    const int cnt = info->count;
-    for (int i = threadIdx.x; i < cnt; i += 1024) s += (double)loss_c[i];
+    for (int i = threadIdx.x; i < cnt; i += NT) s += (double)loss_c[i];
     for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) s += sh[w];
+        for (int w = 1; w < NT / 64; ++w) s += sh[w];
         *loss = (float)(reduction == NMFX_REDUCE_MEAN ? s / (double)max(cnt, 1) : s);
     }
+}
+
+// 256 threads share 2^lc packed columns; the block that is done last adds up the losses
+__global__ __launch_bounds__(256) void combine_kernel(Combine c, int lc, int add) {
+    __shared__ float2 ps[256];
+    __shared__ float ts[256];
+    __shared__ unsigned done;
+    const int cols = 1 << lc, step = 256 >> lc, at = threadIdx.x & (cols - 1), slice = threadIdx.x >> lc;
+    const int cnt = c.info->count, i = blockIdx.x * cols + at;
+    if (blockIdx.x * cols < cnt) {
+        float2 a;
+        float t;
+        c.some(i, slice, step, a, t);
+        ps[threadIdx.x] = a;
+        ts[threadIdx.x] = t;
+        for (int o = step / 2; o; o >>= 1) {
+            __syncthreads();
+            if (slice < o) {
+                ps[threadIdx.x] = join(ps[threadIdx.x], ps[threadIdx.x + (o << lc)]);
+                ts[threadIdx.x] += ts[threadIdx.x + (o << lc)];
+            }
+        }
+        if (slice == 0 && i < cnt) c.finish(i, ps[at], ts[at], true);
+    }
+    if (!add) return;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) done = atomicAdd(&c.info->ticket, 1u);
+    __syncthreads();
+    if (done != gridDim.x - 1) return;
+    __threadfence();
+    reduce_losses<256>(c.loss_c, cnt, c.reduction, c.loss);
 }
 
 // ---- dz of a piece of the classes, in both orders -----------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ T to(float x) { return (T)x; }
 
+// A wave's part of a tile in 16-bit elements, in LDS of its own: rows are columns of D (n), M consecutive m each.  The 16-byte slots of a
+// row are xored with its number, so that 16 lanes that write one m of 16 rows fill all banks once.
+template <int M, int WAVES> struct Patch {
+    static constexpr int RB = 2 * M, SLOTS = RB / 16, PER = 256 / RB;       // bytes, slots of a row; rows of 256 bytes
+    static __device__ __forceinline__ char *of(char *st0, char *st1, int wave, int rows) {
+        return (wave < WAVES / 2 ? st0 : st1) + (wave % (WAVES / 2)) * rows * RB;
+    }
+    static __device__ __forceinline__ int at(int row, int slot) { return row * RB + ((slot ^ (row / PER & (SLOTS - 1))) << 4); }
+};
+
 template <typename T> struct EpiDz {
-    T *dz, *dzt;              // [npad][ldc] by packed column, [classes of the piece][npad] by class
-    int64_t ldc;
+    T *dz, *dzt;              // [npad][ldc] by packed column, [classes of the piece][ldn] by class
+    int64_t ldc, ldn;
     const float *lse_c, *f;
     const int *y, *count;
-    int p, v0, npad;          // classes that exist in the piece; its first class
+    int p, v0;                // classes that exist in the piece; its first class
     float inv, label, off;    // 1 / a, (1 - eps) / a, eps / (a p)
+    int few;                  // the tiles' statistics are not joined yet: every block does it for its own columns
+    Combine c;
     template <int BM, int BN, int WM, int WN, int MI, int NJ>
-    __device__ __forceinline__ void finish(f32x16 (&acc)[MI][NJ], const Geom &g, char *) const {
+    __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, char *st0, char *st1) const {
         typedef T T4 __attribute__((ext_vector_type(4)));
         const int cnt = *count;
+        float lse[NJ];
+        if (few) {
+            constexpr int STEP = WM * WN * 64 / BN;
+            float *sl = reinterpret_cast<float *>(st0);                           // [BN]
+            float2 *ps = reinterpret_cast<float2 *>(st0 + BN * sizeof(float));    // [STEP][BN]
+            float *ts = reinterpret_cast<float *>(ps + STEP * BN);
+            const int at = g.tid % BN, slice = g.tid / BN, i = g.tile_n * BN + at;
+            float2 a;
+            float t;
+            c.some(i, slice, STEP, a, t);
+            ps[g.tid] = a;
+            ts[g.tid] = t;
+            __syncthreads();
+            if (slice == 0) {
+#pragma unroll
+                for (int w = 1; w < STEP; ++w) {
+                    a = join(a, ps[w * BN + at]);
+                    t += ts[w * BN + at];
+                }
+                sl[at] = i < cnt ? c.finish(i, a, t, g.tile_m == 0) : 0.f;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) lse[j] = sl[g.n0 + 16 * j - g.tile_n * BN];
+            __syncthreads();
+        } else
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) lse[j] = g.n0 + 16 * j < cnt ? lse_c[g.n0 + 16 * j] : 0.f;
+        using P = Patch<16 * MI, WM * WN>;
+        const int wave = g.tid >> 6;
+        char *patch = P::of(st0, st1, wave, 16 * NJ);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const int n = g.n0 + 32 * j;
+            const int n = g.n0 + 16 * j;
             const bool on = n < cnt;
-            const float lse = on ? lse_c[n] : 0.f, fac = on ? f[n] : 0.f;
+            const float fac = on ? f[n] : 0.f;
             const int d = on ? y[n] - v0 - g.m0 : -1;
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                T4 o;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int m = 16 * i + r;
+                    const float pr = exp2_((acc[i][j][r] - lse[j]) * LOG2E);
+                    const float v = fac * (pr * inv - off - (d == m ? label : 0.f));
+                    o[r] = to<T>(on && g.m0 + m < p ? v : 0.f);
+                }
+                if constexpr (sizeof(T) == 2) {
+                    const int row = 16 * j + (g.lane & 15);
+                    *reinterpret_cast<T4 *>(patch + P::at(row, 2 * i + (g.lane >> 5)) + (g.lane >> 4 & 1) * 8) = o;
+                } else {
+                    *reinterpret_cast<T4 *>(dz + (int64_t)n * ldc + g.m0 + 16 * i) = o;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) dzt[(int64_t)(g.m0 + 16 * i + r) * ldn + n] = o[r];
+                }
+            }
+        }
+        if constexpr (sizeof(T) == 2) {
+            // from the patch both orders go out in 16-byte stores: rows as they are, and transposed by the LDS' own read (of 16 lanes, lane
+            // l gives the address of 4 elements of row l / 4 and gets element l of the 4 rows)
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            const int m0 = g.m0 - 4 * (g.lane >> 4), n0 = g.n0 - (g.lane & 15);
+#pragma unroll
+            for (int e = 0; e < 16 * NJ * P::SLOTS / 64; ++e) {
+                const int at = e * 64 + g.lane, row = at / P::SLOTS, slot = at % P::SLOTS;
+                *reinterpret_cast<tn::u32x4 *>(dz + (int64_t)(n0 + row) * ldc + m0 + slot * 8) = *reinterpret_cast<const tn::u32x4 *>(patch + P::at(row, slot));
+            }
+            const int l = g.lane & 15, rows8 = (g.lane >> 4) * 8;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    T4 o;
+                for (int h = 0; h < NJ / 2; ++h) {
+                    tn::u32x4 o;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int m = tn::acc_row(i, 4 * q + e);
-                        const float pr = exp2_((acc[i][j][4 * q + e] - lse) * LOG2E);
-                        const float v = fac * (pr * inv - off - (d == m ? label : 0.f));
-                        o[e] = to<T>(on && g.m0 + m < p ? v : 0.f);
-                        dzt[(int64_t)(g.m0 + m) * npad + n] = o[e];
+                    for (int q = 0; q < 2; ++q) {
+                        const int row = 32 * h + rows8 + 4 * q + (l >> 2);
+                        const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(patch + P::at(row, 2 * i + (l >> 1 & 1)) + (l & 1) * 8)));
+                        o[2 * q] = v[0];
+                        o[2 * q + 1] = v[1];
                     }
-                    *reinterpret_cast<T4 *>(dz + (int64_t)n * ldc + g.m0 + tn::acc_row(i, 4 * q)) = o;
+                    *reinterpret_cast<tn::u32x4 *>(dzt + (int64_t)(m0 + 16 * i + l) * ldn + n0 + 32 * h + rows8) = o;
                 }
         }
     }
@@ -341,25 +500,20 @@ struct EpiSlot {
     int64_t ld, slot;
     int nmax, add;
     template <int BM, int BN, int WM, int WN, int MI, int NJ>
-    __device__ __forceinline__ void finish(f32x16 (&acc)[MI][NJ], const Geom &g, char *) const {
-        typedef float f4 __attribute__((ext_vector_type(4)));
+    __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, char *, char *) const {
         float *base = out + g.split * slot;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const int n = g.n0 + 32 * j;
+            const int n = g.n0 + 16 * j;
             if (n >= nmax) continue;
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int m = g.m0 + tn::acc_row(i, 4 * q);
-                    if (m < ld) {
-                        f4 *to4 = reinterpret_cast<f4 *>(base + (int64_t)n * ld + m);
-                        f4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                        if (add) v += *to4;
-                        *to4 = v;
-                    }
+            for (int i = 0; i < MI; ++i) {
+                const int m = g.m0 + 16 * i;
+                if (m < ld) {
+                    f32x4 *to4 = reinterpret_cast<f32x4 *>(base + (int64_t)n * ld + m);
+                    *to4 = add ? acc[i][j] + *to4 : acc[i][j];
                 }
+            }
         }
     }
 };
@@ -371,62 +525,84 @@ template <typename T> struct EpiOut {
     const Info *info;
     int mmax, nmax, wide;     // wide: four consecutive m go in one store
     template <int BM, int BN, int WM, int WN, int MI, int NJ>
-    __device__ __forceinline__ void finish(f32x16 (&acc)[MI][NJ], const Geom &g, char *) const {
+    __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, char *, char *) const {
         typedef T T4 __attribute__((ext_vector_type(4)));
         const float u = info->unscale;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const int n = g.n0 + 32 * j;
+            const int n = g.n0 + 16 * j;
             if (n >= nmax) continue;
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
+            for (int i = 0; i < MI; ++i) {
+                const int m = g.m0 + 16 * i;
+                T4 v;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int m = g.m0 + tn::acc_row(i, 4 * q);
-                    T4 v;
+                for (int r = 0; r < 4; ++r) v[r] = to<T>(acc[i][j][r] * u);
+                T *o = out + (int64_t)n * ld + m;
+                if (wide && m + 3 < mmax) *reinterpret_cast<T4 *>(o) = v;
+                else
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = to<T>(acc[i][j][4 * q + e] * u);
-                    T *o = out + (int64_t)n * ld + m;
-                    if (wide && m + 3 < mmax) *reinterpret_cast<T4 *>(o) = v;
-                    else
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (m + e < mmax) o[e] = v[e];
-                }
+                    for (int r = 0; r < 4; ++r)
+                        if (m + r < mmax) o[r] = v[r];
+            }
         }
     }
 };
 
 // out(m, n) = unscale * sum over slots, m < mmax; n through pos where given (-1: zero)
-template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(const float *slots, int64_t ld, int64_t slot, int nslots, const Info *info, const int *pos, int mmax, int nmax, T *out,
-                                                   int64_t ms, int64_t ns) {
-    const int64_t total = (int64_t)mmax * nmax;
-    const float u = info->unscale;
-    for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < total; e += gridDim.x * 256ll) {
-        int m, n;
-        if (ms == 1) { n = (int)(e / mmax); m = (int)(e - (int64_t)n * mmax); }
-        else { m = (int)(e / nmax); n = (int)(e - (int64_t)m * nmax); }
-        const int from = pos ? pos[n] : n;
-        float s = 0.f;
-        if (from >= 0)
-            for (int q = 0; q < nslots; ++q) s += slots[q * slot + (int64_t)from * ld + m];
-        out[m * ms + n * ns] = to<T>(s * u);
+template <typename T> struct Join {
+    const float *slots;
+    int64_t ld, slot;
+    int nslots;
+    const int *pos;
+    int mmax, nmax;
+    T *out;
+    int64_t ms, ns;
+    int blocks;
+    __device__ __forceinline__ void run(int b, float u) const {
+        typedef float f4 __attribute__((ext_vector_type(4)));
+        const int mq = (mmax + 3) / 4;
+        const int64_t total = (int64_t)mq * nmax;
+        for (int64_t e = b * 256ll + threadIdx.x; e < total; e += blocks * 256ll) {
+            int m, n;
+            if (ms == 1) { n = (int)(e / mq); m = (int)(e - (int64_t)n * mq) * 4; }
+            else { m = (int)(e / nmax); n = (int)(e - (int64_t)m * nmax); m *= 4; }
+            const int from = pos ? pos[n] : n;
+            f4 s = {0.f, 0.f, 0.f, 0.f};
+            if (from >= 0) {
+                const float *p = slots + (int64_t)from * ld + m;
+#pragma unroll 4
+                for (int q = 0; q < nslots; ++q) s += *reinterpret_cast<const f4 *>(p + q * slot);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (m + q < mmax) out[(m + q) * ms + n * ns] = to<T>(s[q] * u);
+        }
     }
+};
+// the last launch of a call: dH, dW where it was summed in parts, and the losses' sum
+template <typename T> __global__ __launch_bounds__(256) void join_kernel(Join<T> h, Join<T> w, const Info *info, const float *loss_c, int reduction, float *loss) {
+    const int b = blockIdx.x;
+    if (b < h.blocks) h.run(b, info->unscale);
+    else if (b < h.blocks + w.blocks) w.run(b - h.blocks, info->unscale);
+    else reduce_losses<256>(loss_c, info->count, reduction, loss);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
 inline int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+struct Choice { int kind, splits; };   // of a product: its tiles (KINDS) and into how many parts its contraction is split
 
 struct Shape {
     int64_t p, n, k;
     int es;                       // bytes of an element
     int64_t wrs, wcs;             // strides of W
     bool w_rows_direct, w_cols_direct;   // W can be read in place as [class][component], as [component][class]
-    int64_t npad, kpad, ppad;
+    int64_t npad, kpad, ppad;     // extents as the images have them
+    int64_t ldn, ldp, ldc;        // between rows of the images by columns (ht, dzt), by classes (wt), of dz: padded (tn_gemm.hpp)
     int64_t piece, pieces;        // classes of a piece (a multiple of 256)
     int64_t ldslot;
-    int hsplits, wsplits;
+    Choice z, h, w;               // the products Z, W' dz, dz H'
     bool w_slots;
     // workspace offsets
     int64_t o_info, o_idx, o_pos, o_y, o_f, o_lse, o_loss, o_zy, o_h, o_ht, o_w, o_wt, o_part, o_zsum, o_dz, o_dzt, o_hslot, o_wslot, bytes;
@@ -434,16 +610,30 @@ struct Shape {
 
 constexpr int CUS = 256;
 
-// the 256 x 256 tile reads half as many bytes from LDS and memory per matrix instruction as the 128 x 128 one, but needs as many tiles
-// as the card has compute units to occupy them
-inline bool big_tiles(int64_t m, int64_t n, int splits) { return m > 128 && n > 128 && ((m + 255) / 256) * ((n + 255) / 256) * splits >= CUS - 56; }
+// Tiles of a product.  What a tile of the contraction (128 bytes of it) takes a block, in us: alone on its compute unit (lat: the loads'
+// way), and of the matrix unit (mat); how many blocks a compute unit holds.  Measured on bf16 and f32 products that fill the card (mat) or
+// a few units (lat).  The large tile reads the least from LDS and memory per matrix instruction; the small ones occupy the card where the
+// product is small, and waste less behind its edges.
+struct TileKind { int m, n, cap; double lat16, mat16, lat32, mat32; };
+constexpr TileKind KINDS[3] = {{256, 256, 1, 1.2, 1.65, 7.6, 7.8}, {128, 128, 2, 0.75, 0.52, 2.0, 2.15}, {64, 64, 2, 0.35, 0.23, 0.67, 0.6}};
 
-inline int splits_for(int64_t m, int64_t n, int64_t ktiles) {
-    const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128);
-    // a split shorter than 8 tiles spends more on its sums than on its products
-    const int64_t most = std::max<int64_t>(1, ktiles / 8);
-    if (m > 128 && n > 128 && big >= 32) return (int)std::min<int64_t>(most, std::max<int64_t>(1, CUS / big));
-    return (int)std::min<int64_t>(most, std::max<int64_t>(1, 2 * CUS / small));
+// the kind and number of splits with the least estimated time; a split adds a slot of m x n floats, written and read
+Choice choose(int64_t m, int64_t n, int64_t ktiles, int es, bool split) {
+    Choice best{2, 1};
+    double least = 1e30;
+    for (int k = 0; k < 3; ++k) {
+        const TileKind &t = KINDS[k];
+        const double lat = es == 2 ? t.lat16 : t.lat32, mat = es == 2 ? t.mat16 : t.mat32;
+        const int64_t tiles = ((m + t.m - 1) / t.m) * ((n + t.n - 1) / t.n);
+        const int64_t most = split ? std::min<int64_t>(std::max<int64_t>(1, ktiles / 4), std::max<int64_t>(1, t.cap * CUS / tiles)) : 1;
+        for (int64_t s = 1; s <= most; s = s < most && s * 2 > most ? most : s * 2) {
+            const double kt = (double)((ktiles + s - 1) / s);
+            const int64_t per = (tiles * s + CUS - 1) / CUS;              // blocks of a compute unit
+            const double us = std::max(per * kt * mat, (double)((per + t.cap - 1) / t.cap) * kt * lat) + 2. * (per + t.cap - 1) / t.cap + (s > 1 ? 2. + 8e-6 * s * m * n / 4. : 0.);
+            if (us < least) { least = us; best = Choice{k, (int)s}; }
+        }
+    }
+    return best;
 }
 
 Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
@@ -464,46 +654,68 @@ Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     s.piece = up((s.ppad + s.pieces - 1) / s.pieces, 256);
     s.pieces = (s.ppad + s.piece - 1) / s.piece;
     s.ldslot = up(s.k, 4);
-    s.hsplits = splits_for(s.k, s.npad, s.piece / step);
-    s.wsplits = splits_for(std::min(s.piece, s.p), s.k, s.npad / step);
-    s.w_slots = s.wsplits > 1;
+    s.ldn = s.npad + 256 / s.es; s.ldp = s.ppad + 256 / s.es; s.ldc = s.piece + 256 / s.es;
+    const int64_t n1 = std::max<int64_t>(s.n, 1);
+    s.z = choose(std::min(s.piece, s.p), n1, s.kpad / step, s.es, false);
+    s.h = choose(s.k, n1, (std::min(s.piece, s.p) + step - 1) / step, s.es, true);
+    s.w = choose(std::min(s.piece, s.p), s.k, (n1 + step - 1) / step, s.es, true);
+    s.w_slots = s.w.splits > 1;
     int64_t at = 0;
     auto take = [&](int64_t b) { const int64_t o = at; at = up(at + b, 256); return o; };
     s.o_info = take(sizeof(Info));
     s.o_idx = take(s.npad * 4); s.o_pos = take(s.npad * 4); s.o_y = take(s.npad * 4);
     s.o_f = take(s.npad * 4); s.o_lse = take(s.npad * 4); s.o_loss = take(s.npad * 4); s.o_zy = take(s.npad * 4);
     s.o_h = take(s.npad * s.kpad * s.es);
-    const int64_t tiles = (s.p + 127) / 128;
+    const int64_t tiles = (s.p + KINDS[s.z.kind].m - 1) / KINDS[s.z.kind].m;
     s.o_part = take(tiles * s.npad * sizeof(float2));
     s.o_zsum = smooth ? take(tiles * s.npad * 4) : -1;
     s.o_w = s.w_rows_direct ? -1 : take(s.p * s.kpad * s.es);
     s.o_ht = s.o_wt = s.o_dz = s.o_dzt = s.o_hslot = s.o_wslot = -1;
     if (grad) {
-        s.o_ht = take(s.k * s.npad * s.es);
-        s.o_wt = s.w_cols_direct ? -1 : take(s.k * s.ppad * s.es);
-        s.o_dz = take(s.npad * s.piece * s.es);
-        s.o_dzt = take(s.npad * s.piece * s.es);
-        s.o_hslot = take((int64_t)s.hsplits * s.npad * s.ldslot * 4);
-        if (s.w_slots) s.o_wslot = take((int64_t)s.wsplits * std::max(up(s.piece, 4) * s.k, s.ldslot * s.piece) * 4);
+        s.o_ht = take(s.k * s.ldn * s.es);
+        s.o_wt = s.w_cols_direct ? -1 : take(s.k * s.ldp * s.es);
+        s.o_dz = take(s.npad * s.ldc * s.es);
+        s.o_dzt = take(s.piece * s.ldn * s.es);
+        s.o_hslot = take((int64_t)s.h.splits * s.npad * s.ldslot * 4);
+        if (s.w_slots) s.o_wslot = take((int64_t)s.w.splits * std::max(up(s.piece, 4) * s.k, s.ldslot * s.piece) * 4);
     }
     s.bytes = at;
     return s;
 }
 
-template <typename T, typename Epi> void product(tn::Args a, int64_t m, int64_t n, const Epi &epi, hipStream_t st) {
-    if (big_tiles(m, n, a.splits)) {
-        a.tiles_m = (int)((m + 255) / 256); a.tiles_n = (int)((n + 255) / 256);
-        tn::tn_kernel<T, 256, 256, 2, 4, Epi><<<a.tiles_m * a.tiles_n * a.splits, 512, 0, st>>>(a, epi);
-    } else {
-        a.tiles_m = (int)((m + 127) / 128); a.tiles_n = (int)((n + 127) / 128);
-        tn::tn_kernel<T, 128, 128, 2, 2, Epi><<<a.tiles_m * a.tiles_n * a.splits, 256, 0, st>>>(a, epi);
+inline void grid(tn::Args &a, int64_t m, int64_t n, const Choice &c) {
+    a.tiles_m = (int)((m + KINDS[c.kind].m - 1) / KINDS[c.kind].m);
+    a.tiles_n = (int)((n + KINDS[c.kind].n - 1) / KINDS[c.kind].n);
+    a.splits = c.splits;
+}
+inline int blocks_of(const tn::Args &a) { return a.tiles_m * a.tiles_n * a.splits; }
+
+template <typename T, typename Epi> void product(tn::Args a, int64_t m, int64_t n, const Choice &c, const Epi &epi, hipStream_t st) {
+    grid(a, m, n, c);
+    switch (c.kind) {
+        case 0: tn::tn_kernel<T, 256, 256, 2, 4, 2, Epi><<<blocks_of(a), 512, 0, st>>>(a, epi); break;
+        case 1: tn::tn_kernel<T, 128, 128, 2, 2, 2, Epi><<<blocks_of(a), 256, 0, st>>>(a, epi); break;
+        default: tn::tn_kernel<T, 64, 64, 2, 2, 4, Epi><<<blocks_of(a), 256, 0, st>>>(a, epi); break;
     }
     ops::hip_ok(hipGetLastError(), "product");
 }
-
-template <typename T> void pack(const Pack<T> &a, hipStream_t st) {
-    pack_kernel<T><<<dim3((a.rpad + 63) / 64, (a.cpad + 63) / 64), 256, 0, st>>>(a);
-    ops::hip_ok(hipGetLastError(), "pack");
+// two products at once where they go by the same kind of tile
+template <typename T, typename EA, typename EB>
+void products(tn::Args a, int64_t ma, int64_t na, const Choice &ca, const EA &ea, tn::Args b, int64_t mb, int64_t nb, const Choice &cb, const EB &eb, hipStream_t st) {
+    if (ca.kind != cb.kind) {
+        product<T>(a, ma, na, ca, ea, st);
+        product<T>(b, mb, nb, cb, eb, st);
+        return;
+    }
+    grid(a, ma, na, ca);
+    grid(b, mb, nb, cb);
+    const int first = blocks_of(a), all = first + blocks_of(b);
+    switch (ca.kind) {
+        case 0: tn::tn_pair_kernel<T, 256, 256, 2, 4, 2, EA, EB><<<all, 512, 0, st>>>(a, ea, b, eb, first); break;
+        case 1: tn::tn_pair_kernel<T, 128, 128, 2, 2, 2, EA, EB><<<all, 256, 0, st>>>(a, ea, b, eb, first); break;
+        default: tn::tn_pair_kernel<T, 64, 64, 2, 2, 4, EA, EB><<<all, 256, 0, st>>>(a, ea, b, eb, first); break;
+    }
+    ops::hip_ok(hipGetLastError(), "products");
 }
 
 struct Call {
@@ -530,72 +742,79 @@ template <typename T> void run(const Call &c, const Shape &s) {
 
     Select sel{c.labels, c.grad ? c.gout : nullptr, c.lse_given ? c.lse : nullptr, c.o.ignore_index, n, p, c.o.reduction, c.grad && sizeof(T) == 2 && !std::is_same<T, __bf16>::value,
                (float)a_, info, i32(s.o_idx), i32(s.o_pos), i32(s.o_y), f32(s.o_f), f32(s.o_lse), c.lse_given ? nullptr : c.loss, c.lse_given ? nullptr : c.lse};
-    select_kernel<<<1, 1024, 0, c.st>>>(sel);
-    ops::hip_ok(hipGetLastError(), "select");
+    if (n > ONE_ROUND) {
+        select_kernel<<<1, 1024, 0, c.st>>>(sel);
+        ops::hip_ok(hipGetLastError(), "select");
+    }
 
     T *h = reinterpret_cast<T *>(ws + s.o_h), *ht = c.grad ? reinterpret_cast<T *>(ws + s.o_ht) : nullptr;
-    pack(Pack<T>{static_cast<const T *>(c.H.data), c.H.cs, c.H.rs, i32(s.o_idx), count, n, k, h, ht, s.kpad, s.npad, (int)s.npad, (int)s.kpad}, c.st);
-
+    T *pw = s.o_w >= 0 ? reinterpret_cast<T *>(ws + s.o_w) : nullptr, *pwt = s.o_wt >= 0 ? reinterpret_cast<T *>(ws + s.o_wt) : nullptr;
     const T *w = static_cast<const T *>(c.W.data), *wt = w;
+    const int ct = (int)(s.kpad / 64 + (s.kpad % 64 != 0)), wr = pw || pwt ? (int)(s.ppad / 64) : 0;
+    Pack<T> ph{static_cast<const T *>(c.H.data), c.H.cs, c.H.rs, n, k, h, ht, s.kpad, s.ldn, (int)s.npad, (int)s.npad, (int)s.kpad, (int)(s.npad / 64), (int)(s.npad / 64) * ct};
+    Pack<T> pk{w, s.wrs, s.wcs, p, k, pw, pwt, s.kpad, s.ldp, p, (int)s.ppad, (int)s.kpad, wr, wr * ct};
+    prepare_kernel<T><<<ph.tiles + pk.tiles, 256, 0, c.st>>>(sel, ph, pk);
+    ops::hip_ok(hipGetLastError(), "prepare");
     int64_t ldw = s.wrs, ldwt = s.wcs;
     int wchunks = (int)(s.k / per), wtpad = p;
-    if (s.o_w >= 0 || s.o_wt >= 0) {
-        T *pw = s.o_w >= 0 ? reinterpret_cast<T *>(ws + s.o_w) : nullptr, *pwt = s.o_wt >= 0 ? reinterpret_cast<T *>(ws + s.o_wt) : nullptr;
-        // (rows behind p are written to the transposed image only: the first has none)
-        if (pw) { pack(Pack<T>{w, s.wrs, s.wcs, nullptr, nullptr, p, k, pw, nullptr, s.kpad, 0, p, (int)s.kpad}, c.st); }
-        if (pwt) { pack(Pack<T>{w, s.wrs, s.wcs, nullptr, nullptr, p, k, nullptr, pwt, 0, s.ppad, (int)s.ppad, (int)s.kpad}, c.st); }
-        if (pw) { w = pw; ldw = s.kpad; wchunks = (int)(s.kpad / per); }
-        if (pwt) { wt = pwt; ldwt = s.ppad; wtpad = (int)s.ppad; }
-    }
-    const int kt = (int)(s.kpad / step);
+    if (pw) { w = pw; ldw = s.kpad; wchunks = (int)(s.kpad / per); }
+    if (pwt) { wt = pwt; ldwt = s.ldp; wtpad = (int)s.ppad; }
+
+    const int kt = (int)(s.kpad / step), n1 = std::max(n, 1), tiles = (p + KINDS[s.z.kind].m - 1) / KINDS[s.z.kind].m;
     const tn::Operand hop{h, s.kpad * es, (int)s.npad, (int)(s.kpad / per)};
+    const Combine cb{reinterpret_cast<float2 *>(ws + s.o_part), s.o_zsum >= 0 ? f32(s.o_zsum) : nullptr, f32(s.o_zy), i32(s.o_idx), i32(s.o_y), info, tiles, (int)s.npad, p,
+                     c.o.reduction, eps, f32(s.o_lse), f32(s.o_loss), c.lse, c.loss};
+    // dz's blocks join the tiles' statistics of their columns themselves where that is a few of them: less than a launch
+    const bool few = c.grad && !c.lse_given && s.pieces == 1 && tiles <= 64 && (int64_t)tiles * ((n1 + KINDS[s.z.kind].n - 1) / KINDS[s.z.kind].n) <= 2 * CUS;
     if (!c.lse_given) {
         tn::Args a{{w, ldw * es, p, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt};
-        EpiStats e{reinterpret_cast<float2 *>(ws + s.o_part), s.o_zsum >= 0 ? f32(s.o_zsum) : nullptr, f32(s.o_zy), i32(s.o_y), count, p, (int)s.npad};
-        product<T>(a, p, std::max(n, 1), e, c.st);
-        const bool big = big_tiles(p, std::max(n, 1), 1);
-        Combine cb{e.part, e.zsum, e.zy, i32(s.o_idx), i32(s.o_y), info, big ? (p + 255) / 256 : (p + 127) / 128, (int)s.npad, p, c.o.reduction, eps, f32(s.o_lse), f32(s.o_loss), c.lse, c.loss};
-        combine_kernel<<<(int)(s.npad / 64), 256, 0, c.st>>>(cb);
-        ops::hip_ok(hipGetLastError(), "combine");
-        if (c.loss && c.o.reduction != NMFX_REDUCE_NONE) {
-            reduce_kernel<<<1, 1024, 0, c.st>>>(f32(s.o_loss), info, c.o.reduction, c.loss);
-            ops::hip_ok(hipGetLastError(), "reduce");
+        product<T>(a, p, n1, s.z, EpiStats{reinterpret_cast<float2 *>(ws + s.o_part), s.o_zsum >= 0 ? f32(s.o_zsum) : nullptr, f32(s.o_zy), i32(s.o_y), count, p, (int)s.npad}, c.st);
+        if (!few) {
+            // as many threads for a column as leave every compute unit a block
+            int lc = 6;
+            while (lc > 0 && (n1 >> lc) < CUS) --lc;
+            combine_kernel<<<(n1 + (1 << lc) - 1) >> lc, 256, 0, c.st>>>(cb, lc, !c.grad && c.o.reduction != NMFX_REDUCE_NONE);
+            ops::hip_ok(hipGetLastError(), "combine");
         }
     }
     if (!c.grad) return;
 
     T *dz = reinterpret_cast<T *>(ws + s.o_dz), *dzt = reinterpret_cast<T *>(ws + s.o_dzt);
     T *dw = static_cast<T *>(c.dW.data), *dh = static_cast<T *>(c.dH.data);
+    auto join_blocks = [](int64_t m, int64_t nn) { return (int)std::min<int64_t>((((m + 3) / 4) * nn + 255) / 256, 8 * CUS); };
+    const bool add = !c.lse_given && c.loss && c.o.reduction != NMFX_REDUCE_NONE;
     for (int64_t q = 0; q < s.pieces; ++q) {
         const int64_t v0 = q * s.piece;
         const int pv = (int)std::min(s.piece, s.p - v0), pt = (int)up(pv, step);
+        const bool last = q + 1 == s.pieces;
         tn::Args a{{w + v0 * ldw, ldw * es, pv, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt};
-        product<T>(a, pv, std::max(n, 1), EpiDz<T>{dz, dzt, s.piece, f32(s.o_lse), f32(s.o_f), i32(s.o_y), count, pv, (int)v0, (int)s.npad, (float)(1. / a_), (float)((1. - c.o.label_smoothing) / a_), (float)(c.o.label_smoothing / (a_ * p))}, c.st);
+        product<T>(a, pv, n1, s.z, EpiDz<T>{dz, dzt, s.ldc, s.ldn, f32(s.o_lse), f32(s.o_f), i32(s.o_y), count, pv, (int)v0, (float)(1. / a_),
+                   (float)((1. - c.o.label_smoothing) / a_), (float)(c.o.label_smoothing / (a_ * p)), few, cb}, c.st);
         // dH: rows are components, columns are packed columns
-        tn::Args b{{wt + v0, ldwt * es, k, (int)std::min<int64_t>((wtpad - v0) / per, s.piece / per)}, {dz, s.piece * es, (int)s.npad, (int)(s.piece / per)}, count, tn::LIMIT_N, 0, 0, s.hsplits, pt / step};
-        product<T>(b, k, std::max(n, 1), EpiSlot{f32(s.o_hslot), s.ldslot, s.npad * s.ldslot, (int)s.npad, q > 0}, c.st);
+        tn::Args b{{wt + v0, ldwt * es, k, (int)std::min<int64_t>((wtpad - v0) / per, s.piece / per)}, {dz, s.ldc * es, (int)s.npad, (int)(s.piece / per)}, count, tn::LIMIT_N, 0, 0, 0, pt / step};
+        const EpiSlot eh{f32(s.o_hslot), s.ldslot, s.npad * s.ldslot, (int)s.npad, q > 0};
         // dW: the contiguous index of dW is the row
-        const tn::Operand zop{dzt, s.npad * es, pv, (int)(s.npad / per)}, top{ht, s.npad * es, k, (int)(s.npad / per)};
+        const tn::Operand zop{dzt, s.ldn * es, pv, (int)(s.npad / per)}, top{ht, s.ldn * es, k, (int)(s.npad / per)};
         const bool kfast = c.dW.cs == 1;
         T *out = dw + v0 * c.dW.rs;
         const int64_t ldo = kfast ? c.dW.rs : c.dW.cs;
         const int mm = kfast ? k : pv, nn = kfast ? pv : k;
-        tn::Args d{kfast ? top : zop, kfast ? zop : top, count, tn::LIMIT_C, 0, 0, s.wsplits, (int)(s.npad / step)};
+        tn::Args d{kfast ? top : zop, kfast ? zop : top, count, tn::LIMIT_C, 0, 0, 0, (int)(s.npad / step)};
+        Join<T> jh{}, jw{};
         if (s.w_slots) {
             const int64_t ld = up(mm, 4);
-            product<T>(d, mm, nn, EpiSlot{f32(s.o_wslot), ld, ld * nn, nn, 0}, c.st);
-            const int64_t blocks = std::min<int64_t>(((int64_t)mm * nn + 255) / 256, 8 * CUS);
-            join_kernel<T><<<(int)blocks, 256, 0, c.st>>>(f32(s.o_wslot), ld, ld * nn, s.wsplits, info, nullptr, mm, nn, out, 1, ldo);
-            ops::hip_ok(hipGetLastError(), "join");
+            products<T>(b, k, n1, s.h, eh, d, mm, nn, s.w, EpiSlot{f32(s.o_wslot), ld, ld * nn, nn, 0}, c.st);
+            jw = Join<T>{f32(s.o_wslot), ld, ld * nn, s.w.splits, nullptr, mm, nn, out, 1, ldo, join_blocks(mm, nn)};
         } else {
             const bool wide = ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * es - 1)) == 0;
-            product<T>(d, mm, nn, EpiOut<T>{out, ldo, info, mm, nn, wide}, c.st);
+            products<T>(b, k, n1, s.h, eh, d, mm, nn, s.w, EpiOut<T>{out, ldo, info, mm, nn, wide}, c.st);
         }
-    }
-    if (n > 0) {
-        const int64_t blocks = std::min<int64_t>(((int64_t)k * n + 255) / 256, 8 * CUS);
-        join_kernel<T><<<(int)blocks, 256, 0, c.st>>>(f32(s.o_hslot), s.ldslot, s.npad * s.ldslot, s.hsplits, info, i32(s.o_pos), k, n, dh, c.dH.rs, c.dH.cs);
-        ops::hip_ok(hipGetLastError(), "join");
+        if (last && n) jh = Join<T>{f32(s.o_hslot), s.ldslot, s.npad * s.ldslot, s.h.splits, i32(s.o_pos), k, n, dh, c.dH.rs, c.dH.cs, join_blocks(k, n)};
+        const int jb = jh.blocks + jw.blocks + (last && add);
+        if (jb) {
+            join_kernel<T><<<jb, 256, 0, c.st>>>(jh, jw, info, f32(s.o_loss), c.o.reduction, c.loss);
+            ops::hip_ok(hipGetLastError(), "join");
+        }
     }
 }
 
@@ -621,7 +840,7 @@ nmfx_dmat tidy(nmfx_dmat m) {
     return m;
 }
 
-constexpr int64_t MOST = 1 << 21;   // rows of a tile must stay within the 2 GiB that a buffer descriptor spans
+constexpr int64_t MOST = (1 << 21) - 1024;   // 256 rows of Float32, padded, stay below the 2^31 bytes from which on loads ask for zeros
 
 void check(const nmfx_dmat *W, const nmfx_dmat *H) {
     check_mat(W, "W");
@@ -630,8 +849,8 @@ void check(const nmfx_dmat *W, const nmfx_dmat *H) {
     ops::require(W->dtype != NMFX_F64, NMFX_ERR_UNSUPPORTED, "softmax cross entropy takes NMFX_F32, NMFX_BF16 and NMFX_F16");
     ops::require(W->cols == H->rows, NMFX_ERR_DIM_MISMATCH, "W is p x k and H is k x n: their k differ");
     ops::require(W->rows >= 1 && W->cols >= 1, NMFX_ERR_DIM_MISMATCH, "p and k must be positive");
-    ops::require(W->rows <= MOST && H->cols <= MOST && W->cols <= MOST / 2, NMFX_ERR_UNSUPPORTED, "p and n may be at most 2^21 and k at most 2^20");
-    ops::require((W->cs == 1 ? W->rs : W->cs) <= MOST, NMFX_ERR_UNSUPPORTED, "the stride of W may be at most 2^21 elements");
+    ops::require(W->rows <= MOST && H->cols <= MOST && W->cols <= MOST / 2, NMFX_ERR_UNSUPPORTED, "p and n may be at most 2^21 - 1024 and k half of that");
+    ops::require((W->cs == 1 ? W->rs : W->cs) <= MOST, NMFX_ERR_UNSUPPORTED, "the stride of W may be at most 2^21 - 1024 elements");
 }
 
 void check_opts(const nmfx_xent_opts *o) {
