@@ -22,6 +22,7 @@ using tn::f32x4;
 using tn::Geom;
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 struct Info {            // written by select_kernel, read by everything behind it
@@ -49,103 +50,174 @@ struct Select {
     int *idx, *pos, *y;       // packed -> column, column -> packed or -1, packed label (-1: not a class)
     float *f, *lse_c;         // packed: f_j, log-sum-exp
     float *loss, *lse;        // the caller's: zero in ignored columns (loss only without reduction); NULL: not written
+    int *counts;              // of 2048 columns each
+    float *maxima;
 };
 
-// 8 columns a thread: which are not ignored, and how many of them are in front of the thread's first.  Returns their number in the block.
-template <int NT> __device__ __forceinline__ int ranks(const Select &s, int t0, unsigned &on, int &before) {
-    __shared__ int wsum[NT / 64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    on = 0;
+// 8 NT columns from t00 on, 8 a thread: column(e) is thread's e-th, so that a wave's loads and ranks are of 64 columns in a row.
+template <int NT> struct Columns {
+    int64_t lab[8];
+    int rank[8];              // among the block's columns that are not ignored; -1: ignored, or none
+    int all;                  // of them in the block
+    static __device__ __forceinline__ int column(int t00, int e) { return t00 + (threadIdx.x >> 6) * 512 + e * 64 + (threadIdx.x & 63); }
+    __device__ __forceinline__ void find(const Select &s, int t00) {
+        __shared__ int wsum[NT / 64];
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const unsigned long long below = (1ull << lane) - 1;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) on |= (t0 + e < s.n && s.labels[min(t0 + e, s.n - 1)] != s.ignore ? 1u : 0u) << e;
-    const int mine = __popc(on);
-    int upto = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int v = __shfl_up(upto, o);
-        if (lane >= o) upto += v;
-    }
-    __syncthreads();                      // (wsum may still be read by the round before)
-    if (lane == 63) wsum[wave] = upto;
-    __syncthreads();
-    int all = 0;
-    before = upto - mine;
-#pragma unroll
-    for (int w = 0; w < NT / 64; ++w) {
-        before += w < wave ? wsum[w] : 0;
-        all += wsum[w];
-    }
-    return all;
-}
-
-// One block: the order of the packed columns is that of the columns, so it takes a running count, 8 NT columns a round.
-template <int NT> __device__ __forceinline__ void select_columns(const Select &s) {
-    __shared__ float wmax[NT / 64];
-    __shared__ float sh_scale;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int base = 0;
-    float gmax = 0.f;
-    const bool per = s.reduction == NMFX_REDUCE_NONE && s.gout != nullptr;
-    for (int t00 = 0; t00 < s.n; t00 += 8 * NT) {
-        unsigned on;
-        int before;
-        const int t0 = t00 + tid * 8, all = ranks<NT>(s, t0, on, before);
-        int i = base + before;
+        for (int e = 0; e < 8; ++e) lab[e] = column(t00, e) < s.n ? s.labels[column(t00, e)] : s.ignore;
+        int mine = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int t = t0 + e;
-            if (t >= s.n) break;
-            if (on >> e & 1) {
-                const int64_t lab = s.labels[t];
-                const bool bad = lab < 0 || lab >= s.p;
-                s.pos[t] = i;
-                s.idx[i] = t;
-                s.y[i] = bad ? -1 : (int)lab;
-                if (s.lse_given) s.lse_c[i] = bad ? __builtin_nanf("") : s.lse_given[t];
-                if (per) {
-                    const float g = s.gout[t];
-                    s.f[i] = g;
-                    gmax = fmaxf(gmax, fabsf(g));
-                }
-                ++i;
-            } else {
-                s.pos[t] = -1;
-                if (s.lse) s.lse[t] = 0.f;
-                if (s.loss && s.reduction == NMFX_REDUCE_NONE) s.loss[t] = 0.f;
-            }
+            const unsigned long long m = __ballot(lab[e] != s.ignore);
+            rank[e] = lab[e] != s.ignore ? mine + __popcll(m & below) : -1;
+            mine += __popcll(m);
         }
-        base += all;
+        if (lane == 0) wsum[wave] = mine;
+        __syncthreads();
+        all = 0;
+        int before = 0;
+#pragma unroll
+        for (int w = 0; w < NT / 64; ++w) {
+            before += w < wave ? wsum[w] : 0;
+            all += wsum[w];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rank[e] += rank[e] >= 0 ? before : 0;
     }
-    float g = 1.f;
-    if (!per) {
-        if (s.gout) g = s.gout[0];
-        if (s.reduction == NMFX_REDUCE_MEAN) g /= (float)max(base, 1);
-        gmax = 1.f;
+};
+
+// how many of the first `upto` columns are not ignored, and the largest |gout| among them, by a block
+template <int NT> __device__ __forceinline__ int count_columns(const Select &s, int from, int upto, bool per, float &gmax) {
+    __shared__ int sh[NT / 64];
+    __shared__ float shm[NT / 64];
+    int c = 0;
+    for (int t0 = from + threadIdx.x; t0 < upto; t0 += 16 * NT) {       // 16 loads on their way at a time
+        int64_t lab[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) lab[e] = t0 + e * NT < upto ? s.labels[t0 + e * NT] : s.ignore;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            c += lab[e] != s.ignore;
+            if (per && lab[e] != s.ignore) gmax = fmaxf(gmax, fabsf(s.gout[t0 + e * NT]));
+        }
     }
-    for (int o = 32; o; o >>= 1) gmax = fmaxf(gmax, __shfl_xor(gmax, o));
-    if (lane == 0) wmax[wave] = gmax;
+    for (int o = 32; o; o >>= 1) {
+        c += __shfl_xor(c, o);
+        gmax = fmaxf(gmax, __shfl_xor(gmax, o));
+    }
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < NT / 64; ++w) gmax = fmaxf(gmax, wmax[w]);
-        float scale = 1.f;
+    if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6] = c; shm[threadIdx.x >> 6] = gmax; }
+    __syncthreads();
+    c = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) { c += sh[w]; gmax = fmaxf(gmax, shm[w]); }
+    return c;
+}
+
+// The order of the packed columns is that of the columns: block `blk` places 8 NT of them behind those of the blocks in front, which it
+// counts itself (up to 4096 columns: a few loads a thread) or finds counted (count_kernel).
+constexpr int SELF = 4096;
+template <int NT> __device__ __forceinline__ void select_columns(const Select &s, int blk) {
+    if (!s.n) {
+        if (threadIdx.x == 0) *s.info = Info{0, 0.f, 0, 0};
+        return;
+    }
+    const int t00 = blk * 8 * NT, tid = threadIdx.x;
+    const bool per = s.reduction == NMFX_REDUCE_NONE && s.gout != nullptr, range = per && s.scaled;
+    const int blocks = (s.n + 8 * NT - 1) / (8 * NT);
+    int base = 0;
+    float gmax = 0.f;
+    if (s.n > SELF) {
+        for (int b = 0; b < blocks; ++b) {
+            base += b < blk ? s.counts[b] : 0;
+            if (range) gmax = fmaxf(gmax, s.maxima[b]);
+        }
+    } else {
+        if (blk) base = count_columns<NT>(s, 0, t00, range, gmax);
+        if (range) count_columns<NT>(s, t00, s.n, true, gmax);
+    }
+    float scale = 1.f;
+    if (s.scaled) {
         // the largest factor becomes at most 2^14: with a >= 1/2 what is stored is below 2^15 and finite in f16, and 2^-28 of it normal
-        if (s.scaled && gmax > 0.f && gmax < __builtin_inff()) {
+        if (!per) gmax = 1.f;
+        if (gmax > 0.f && gmax < __builtin_inff()) {
             int e;
             frexpf(gmax, &e);
             scale = ldexpf(1.f, min(max(14 - e, -100), 100));
         }
-        sh_scale = scale;
-        *s.info = Info{base, (per ? 1.f : g) * s.a / scale, 0, 0};
     }
-    __syncthreads();
-    const float scale = sh_scale;
-    for (int i = tid; i < base; i += NT) s.f[i] = (per ? s.f[i] : 1.f) * scale;
+    Columns<NT> c;
+    c.find(s, t00);
+    float g8[8], l8[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int t = min(c.column(t00, e), s.n - 1);
+        g8[e] = per ? s.gout[t] : 1.f;
+        l8[e] = s.lse_given ? s.lse_given[t] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int t = c.column(t00, e);
+        if (t >= s.n) continue;
+        s.pos[t] = c.rank[e] >= 0 ? base + c.rank[e] : -1;
+        if (c.rank[e] >= 0) {
+            const int i = base + c.rank[e];
+            const bool bad = c.lab[e] < 0 || c.lab[e] >= s.p;
+            s.idx[i] = t;
+            s.y[i] = bad ? -1 : (int)c.lab[e];
+            if (s.lse_given) s.lse_c[i] = bad ? __builtin_nanf("") : l8[e];
+            s.f[i] = g8[e] * scale;
+        } else {
+            if (s.lse) s.lse[t] = 0.f;
+            if (s.loss && s.reduction == NMFX_REDUCE_NONE) s.loss[t] = 0.f;
+        }
+    }
+    const int all = c.all;
+    if (tid == 0 && blk == max(blocks, 1) - 1) {
+        float g = 1.f;
+        if (!per && s.gout) g = s.gout[0];
+        if (s.reduction == NMFX_REDUCE_MEAN) g /= (float)max(base + all, 1);
+        *s.info = Info{base + all, g * s.a / scale, 0, 0};
+    }
 }
-__global__ __launch_bounds__(1024) void select_kernel(Select s) { select_columns<1024>(s); }
+__global__ __launch_bounds__(256) void count_kernel(Select s) {
+    float gmax = 0.f;
+    const int c = count_columns<256>(s, blockIdx.x * 2048, min(s.n, (int)(blockIdx.x + 1) * 2048), s.reduction == NMFX_REDUCE_NONE && s.gout != nullptr, gmax);
+    if (threadIdx.x == 0) { s.counts[blockIdx.x] = c; s.maxima[blockIdx.x] = gmax; }
+}
+__global__ __launch_bounds__(256) void select_kernel(Select s) { select_columns<256>(s, blockIdx.x); }
+
+// A patch of a matrix in 16-bit elements in LDS: rows of M elements.  The 16-byte slots of a row are xored with its number, so that 16 lanes
+// at one place of 16 rows touch all banks once.  transposed() reads 8 rows of one element, by the LDS' own transposing read: of 16 lanes,
+// lane l gives the address of 4 elements of row l / 4 and gets element l of the 4 rows.
+template <int M, int WAVES> struct Patch {
+    static constexpr int RB = 2 * M, SLOTS = RB / 16, PER = 256 / RB;       // bytes, slots of a row; rows of 256 bytes
+    static __device__ __forceinline__ char *of(char *st0, char *st1, int wave, int rows) {
+        return (wave < WAVES / 2 ? st0 : st1) + (wave % (WAVES / 2)) * rows * RB;
+    }
+    static __device__ __forceinline__ int at(int row, int slot) { return row * RB + ((slot ^ (row / PER & (SLOTS - 1))) << 4); }
+    // rows row .. row + 7 of element m + (lane & 15), m a multiple of 16
+    static __device__ __forceinline__ tn::u32x4 transposed(const char *patch, int row, int m, int lane) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        const int l = lane & 15;
+        tn::u32x4 o;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const char *from = patch + at(row + 4 * q + (l >> 2), m / 8 + (l >> 1 & 1)) + (l & 1) * 8;
+            const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)from));
+            o[2 * q] = v[0];
+            o[2 * q + 1] = v[1];
+        }
+        return o;
+    }
+};
 
 // ---- packed images ----------------------------------------------------------------------------------------------------------------
-// in: element (r, c) at in[r * rs + c * cs]; out1[r * ld1 + c], out2[c * ld2 + r], zero where r or c is behind the end.  64 x 64 tiles
-// through LDS, so that reads follow the contiguous index of `in` and both writes are contiguous.
+// in: element (r, c) at in[r * rs + c * cs]; out1[r * ld1 + c], out2[c * ld2 + r], zero where r or c is behind the end.  64 x 64 tiles:
+// 16-byte loads along the contiguous index (at any address), 16-byte stores of that order from registers and of the other one through LDS.
 template <typename T> struct Pack {
     const T *in;
     int64_t rs, cs;
@@ -155,73 +227,104 @@ template <typename T> struct Pack {
     int rpad1, rpad2, cpad;   // written extent: rows of out1, of out2 (its columns), columns of out1
     int tiles_r, tiles;
 };
-template <typename T> __device__ __forceinline__ void pack_tile(const Pack<T> &a, T (*tile)[65], const int *from, int rows, int r0, int c0) {
-    const int lo = threadIdx.x & 63, up = threadIdx.x >> 6;
-    if (a.cs == 1) {
-        for (int i = up; i < 64; i += 4) {
-            const int r = r0 + i, c = c0 + lo;
-            tile[i][lo] = r < rows && c < a.cols ? a.in[(int64_t)(from ? from[i] : r) * a.rs + c] : (T)0.f;
+typedef tn::u32x4 u32x4_any __attribute__((aligned(2)));
+template <typename T> __device__ __forceinline__ void pack_tile(const Pack<T> &a, char *tile, const int *from, int rows, int r0, int c0) {
+    constexpr int V = 16 / sizeof(T), CH = 64 / V;
+    using P = Patch<64, 2>;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const bool by_row = a.cs == 1;
+    // y: the index between the contiguous runs of `in`, x: along them
+    const int x0 = by_row ? c0 : r0, y0 = by_row ? r0 : c0, xs = by_row ? a.cols : rows, ys = by_row ? rows : a.cols;
+    const int64_t ld = by_row ? a.rs : a.cs;
+    T *same = by_row ? a.out1 : a.out2, *turn = by_row ? a.out2 : a.out1;
+    const int64_t lds = by_row ? a.ld1 : a.ld2, ldt = by_row ? a.ld2 : a.ld1;
+    const int same_x = by_row ? a.cpad : a.rpad2, same_y = by_row ? a.rpad1 : a.cols, turn_x = by_row ? a.cols : a.rpad1, turn_y = by_row ? a.rpad2 : a.cpad;
+    float (*tf)[65] = reinterpret_cast<float (*)[65]>(tile);
+#pragma unroll
+    for (int i = 0; i < 64 * CH / 256; ++i) {
+        const int q = i * 256 + tid, y = q / CH, xc = q % CH, x = x0 + xc * V;
+        tn::u32x4 v = {0, 0, 0, 0};
+        T *e = reinterpret_cast<T *>(&v);
+        if (y0 + y < ys) {
+            if (by_row || !from) {
+                const T *src = a.in + (int64_t)(from ? from[y] : y0 + y) * ld + x;
+                if (x + V <= xs) v = *reinterpret_cast<const u32x4_any *>(src);
+                else
+#pragma unroll
+                    for (int u = 0; u < V; ++u)
+                        if (x + u < xs) e[u] = src[u];
+            } else
+#pragma unroll
+                for (int u = 0; u < V; ++u)
+                    if (x + u < xs) e[u] = a.in[from[xc * V + u] + (int64_t)(y0 + y) * ld];
         }
-    } else {
-        const int r = r0 + lo;
-        const T *row = a.in + (r < rows ? (int64_t)(from ? from[lo] : r) * a.rs : 0);
-        for (int i = up; i < 64; i += 4) {
-            const int c = c0 + i;
-            tile[lo][i] = r < rows && c < a.cols ? row[(int64_t)c * a.cs] : (T)0.f;
+        if (same && y0 + y < same_y && x < same_x) *reinterpret_cast<tn::u32x4 *>(same + (int64_t)(y0 + y) * lds + x) = v;
+        if (turn) {
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<tn::u32x4 *>(tile + P::at(y, xc)) = v;
+            else
+#pragma unroll
+                for (int u = 0; u < V; ++u) tf[y][xc * V + u] = (float)e[u];
         }
     }
+    if (!turn) return;
     __syncthreads();
-    if (a.out1)
-        for (int i = up; i < 64; i += 4)
-            if (r0 + i < a.rpad1 && c0 + lo < a.cpad) a.out1[(int64_t)(r0 + i) * a.ld1 + c0 + lo] = tile[i][lo];
-    if (a.out2)
-        for (int i = up; i < 64; i += 4)
-            if (c0 + i < a.cols && r0 + lo < a.rpad2) a.out2[(int64_t)(c0 + i) * a.ld2 + r0 + lo] = tile[lo][i];
+    if constexpr (sizeof(T) == 2) {
+        const int x = 16 * (tid >> 6) + (lane & 15), rows8 = (lane >> 4) * 8;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const tn::u32x4 v = P::transposed(tile, 32 * h + rows8, 16 * (tid >> 6), lane);
+            if (x0 + x < turn_x && y0 + 32 * h + rows8 < turn_y) *reinterpret_cast<tn::u32x4 *>(turn + (int64_t)(x0 + x) * ldt + y0 + 32 * h + rows8) = v;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int q = i * 256 + tid, x = q / 16, y = q % 16 * 4;
+            if (x0 + x < turn_x && y0 + y < turn_y) *reinterpret_cast<f32x4 *>(turn + (int64_t)(x0 + x) * ldt + y0 + y) = f32x4{tf[y][x], tf[y + 1][x], tf[y + 2][x], tf[y + 3][x]};
+        }
+    }
 }
 // Everything the products read, in one launch: H packed (first blocks), the images of W that its own order does not serve.  Up to
 // ONE_ROUND columns every block of H finds its 64 packed columns for itself (a round of 256 threads with 8 labels each: less than a launch),
-// and the first one leaves the lists; above, select_kernel has made them.
+// and the last block leaves the lists; above, select_kernel has made them.
 constexpr int ONE_ROUND = 2048;
 template <typename T> __global__ __launch_bounds__(256) void prepare_kernel(Select s, Pack<T> h, Pack<T> w) {
-    __shared__ T tile[64][65];
+    __shared__ __attribute__((aligned(16))) char tile[sizeof(T) == 2 ? 64 * 128 : 64 * 65 * 4];
     __shared__ int from[64];
     int b = blockIdx.x;
     if (b >= h.tiles) {
         b -= h.tiles;
-        pack_tile<T>(w, tile, nullptr, w.rows, (b % w.tiles_r) * 64, (b / w.tiles_r) * 64);
+        if (b < w.tiles) pack_tile<T>(w, tile, nullptr, w.rows, (b % w.tiles_r) * 64, (b / w.tiles_r) * 64);
+        else select_columns<256>(s, 0);
         return;
     }
     const int r0 = (b % h.tiles_r) * 64, c0 = (b / h.tiles_r) * 64;
     int rows;
     if (s.n <= ONE_ROUND) {
-        unsigned on;
-        int before;
-        rows = ranks<256>(s, threadIdx.x * 8, on, before);
+        Columns<256> c;
+        c.find(s, 0);
+        rows = c.all;
+#pragma unroll
         for (int e = 0; e < 8; ++e)
-            if (on >> e & 1) {
-                if (before >= r0 && before < r0 + 64) from[before - r0] = threadIdx.x * 8 + e;
-                ++before;
-            }
-        __syncthreads();
+            if (c.rank[e] >= r0 && c.rank[e] < r0 + 64) from[c.rank[e] - r0] = c.column(0, e);
     } else {
         rows = s.info->count;
         if (threadIdx.x < 64 && r0 + (int)threadIdx.x < rows) from[threadIdx.x] = s.idx[r0 + threadIdx.x];
-        __syncthreads();
     }
+    __syncthreads();
     pack_tile<T>(h, tile, from, rows, r0, c0);
-    if (b == 0 && s.n <= ONE_ROUND) select_columns<256>(s);
 }
 
-// (maximum, sum of exp(z - maximum)) of two sets.  An empty set, or one of minus infinities, is (-inf, 0) and changes nothing; a NaN sum
+// Statistics are kept in units of log 2: (reference r, sum of 2^(z log2(e) - r)), one multiply-add and one exp2 a logit, where r is some
+// set's maximum as it was rounded: its rounding cancels.  Of two sets: an empty one, or one of minus infinities, is (-inf, 0) and changes nothing; a NaN sum
 // is not 0 and goes through.
 __device__ __forceinline__ float2 join(float2 a, float2 b) {
     const float m = fmaxf(a.x, b.x);
-    return make_float2(m, (a.y != 0.f ? a.y * exp2_((a.x - m) * LOG2E) : 0.f) + (b.y != 0.f ? b.y * exp2_((b.x - m) * LOG2E) : 0.f));
+    return make_float2(m, (a.y != 0.f ? a.y * exp2_(a.x - m) : 0.f) + (b.y != 0.f ? b.y * exp2_(b.x - m) : 0.f));
 }
 
 // ---- statistics of the logits: rows of D are classes, columns are packed columns ----------------------------------------------------
 struct EpiStats {
-    float2 *part;         // [tile_m][npad]: maximum and sum of exp(z - maximum) over the tile's classes
+    float2 *part;         // [tile_m][npad]: reference and sum over the tile's classes
     float *zsum;          // [tile_m][npad] or NULL
     float *zy;            // packed: the label's logit
     const int *y;
@@ -251,12 +354,13 @@ struct EpiStats {
                 for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
+            mx *= LOG2E;
             const float ref = mx == -__builtin_inff() ? 0.f : mx;
             float s = 0.f;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s += exp2_((acc[i][j][r] - ref) * LOG2E);
+                for (int r = 0; r < 4; ++r) s += exp2_(__builtin_fmaf(acc[i][j][r], LOG2E, -ref));
             s += __shfl_xor(s, 16);
             s += __shfl_xor(s, 32);
             const int col = g.wn * (BN / WN) + 16 * j + (g.lane & 15);
@@ -320,7 +424,7 @@ struct Combine {
     }
     __device__ __forceinline__ float finish(int i, float2 a, float t, bool write) const {
         const int lab = y[i];
-        const float v = lab < 0 ? __builtin_nanf("") : a.x + logf(a.y);     // a label that is no class: the column's loss is NaN
+        const float v = lab < 0 ? __builtin_nanf("") : (a.x + log2f(a.y)) * LN2;     // a label that is no class: the column's loss is NaN
         if (write) {
             float l = v - (1.f - eps) * (lab < 0 ? 0.f : zy[i]);
             if (zsum) l -= eps * (t / (float)p);
@@ -383,16 +487,6 @@ __global__ __launch_bounds__(256) void combine_kernel(Combine c, int lc, int add
 // ---- dz of a piece of the classes, in both orders -----------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ T to(float x) { return (T)x; }
 
-// A wave's part of a tile in 16-bit elements, in LDS of its own: rows are columns of D (n), M consecutive m each.  The 16-byte slots of a
-// row are xored with its number, so that 16 lanes that write one m of 16 rows fill all banks once.
-template <int M, int WAVES> struct Patch {
-    static constexpr int RB = 2 * M, SLOTS = RB / 16, PER = 256 / RB;       // bytes, slots of a row; rows of 256 bytes
-    static __device__ __forceinline__ char *of(char *st0, char *st1, int wave, int rows) {
-        return (wave < WAVES / 2 ? st0 : st1) + (wave % (WAVES / 2)) * rows * RB;
-    }
-    static __device__ __forceinline__ int at(int row, int slot) { return row * RB + ((slot ^ (row / PER & (SLOTS - 1))) << 4); }
-};
-
 template <typename T> struct EpiDz {
     T *dz, *dzt;              // [npad][ldc] by packed column, [classes of the piece][ldn] by class
     int64_t ldc, ldn;
@@ -437,38 +531,52 @@ template <typename T> struct EpiDz {
         using P = Patch<16 * MI, WM * WN>;
         const int wave = g.tid >> 6;
         char *patch = P::of(st0, st1, wave, 16 * NJ);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
+        // (edge: some of the tile's rows or columns do not exist, and have a zero dz)
+        const bool edge = g.tile_m * BM + BM > p || g.tile_n * BN + BN > cnt;
+        auto column = [&](int j, auto at_edge) {
             const int n = g.n0 + 16 * j;
             const bool on = n < cnt;
-            const float fac = on ? f[n] : 0.f;
-            const int d = on ? y[n] - v0 - g.m0 : -1;
+            const float fac = on ? f[n] : 0.f, mul = fac * inv, sub = -fac * off, ref = lse[j] * -LOG2E;
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 T4 o;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int m = 16 * i + r;
-                    const float pr = exp2_((acc[i][j][r] - lse[j]) * LOG2E);
-                    const float v = fac * (pr * inv - off - (d == m ? label : 0.f));
-                    o[r] = to<T>(on && g.m0 + m < p ? v : 0.f);
+                    const float v = __builtin_fmaf(exp2_(__builtin_fmaf(acc[i][j][r], LOG2E, ref)), mul, sub);
+                    o[r] = to<T>(!at_edge || (on && g.m0 + 16 * i + r < p) ? v : 0.f);
                 }
-                if constexpr (sizeof(T) == 2) {
-                    const int row = 16 * j + (g.lane & 15);
-                    *reinterpret_cast<T4 *>(patch + P::at(row, 2 * i + (g.lane >> 5)) + (g.lane >> 4 & 1) * 8) = o;
-                } else {
+                if constexpr (sizeof(T) == 2) *reinterpret_cast<T4 *>(patch + P::at(16 * j + (g.lane & 15), 2 * i + (g.lane >> 5)) + (g.lane >> 4 & 1) * 8) = o;
+                else {
                     *reinterpret_cast<T4 *>(dz + (int64_t)n * ldc + g.m0 + 16 * i) = o;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) dzt[(int64_t)(g.m0 + 16 * i + r) * ldn + n] = o[r];
                 }
             }
+            // the label's entry, where it is this lane's: written once more
+            const int d = on ? y[n] - v0 - g.m0 : -1;
+            if (d >= 0 && d < 16 * MI && (d & 15) < 4) {
+                float z = 0.f;
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) z = d == 16 * i + r ? acc[i][j][r] : z;
+                const T v = to<T>(__builtin_fmaf(exp2_(__builtin_fmaf(z, LOG2E, ref)), mul, sub - fac * label));
+                if constexpr (sizeof(T) == 2) *reinterpret_cast<T *>(patch + P::at(16 * j + (g.lane & 15), 2 * (d >> 4) + (g.lane >> 5)) + (g.lane >> 4 & 1) * 8 + (d & 3) * 2) = v;
+                else {
+                    dz[(int64_t)n * ldc + g.m0 + d] = v;
+                    dzt[(int64_t)(g.m0 + d) * ldn + n] = v;
+                }
+            }
+        };
+        if (edge) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) column(j, std::true_type{});
+        } else {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) column(j, std::false_type{});
         }
         if constexpr (sizeof(T) == 2) {
-            // from the patch both orders go out in 16-byte stores: rows as they are, and transposed by the LDS' own read (of 16 lanes, lane
-            // l gives the address of 4 elements of row l / 4 and gets element l of the 4 rows)
-            typedef short s16x4 __attribute__((ext_vector_type(4)));
-            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            // from the patch both orders go out in 16-byte stores: its rows as they are, and transposed
             const int m0 = g.m0 - 4 * (g.lane >> 4), n0 = g.n0 - (g.lane & 15);
 #pragma unroll
             for (int e = 0; e < 16 * NJ * P::SLOTS / 64; ++e) {
@@ -479,17 +587,8 @@ template <typename T> struct EpiDz {
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int h = 0; h < NJ / 2; ++h) {
-                    tn::u32x4 o;
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const int row = 32 * h + rows8 + 4 * q + (l >> 2);
-                        const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(patch + P::at(row, 2 * i + (l >> 1 & 1)) + (l & 1) * 8)));
-                        o[2 * q] = v[0];
-                        o[2 * q + 1] = v[1];
-                    }
-                    *reinterpret_cast<tn::u32x4 *>(dzt + (int64_t)(m0 + 16 * i + l) * ldn + n0 + 32 * h + rows8) = o;
-                }
+                for (int h = 0; h < NJ / 2; ++h)
+                    *reinterpret_cast<tn::u32x4 *>(dzt + (int64_t)(m0 + 16 * i + l) * ldn + n0 + 32 * h + rows8) = P::transposed(patch, 32 * h + rows8, 16 * i, g.lane);
         }
     }
 };
@@ -605,7 +704,7 @@ struct Shape {
     Choice z, h, w;               // the products Z, W' dz, dz H'
     bool w_slots;
     // workspace offsets
-    int64_t o_info, o_idx, o_pos, o_y, o_f, o_lse, o_loss, o_zy, o_h, o_ht, o_w, o_wt, o_part, o_zsum, o_dz, o_dzt, o_hslot, o_wslot, bytes;
+    int64_t o_info, o_counts, o_idx, o_pos, o_y, o_f, o_lse, o_loss, o_zy, o_h, o_ht, o_w, o_wt, o_part, o_zsum, o_dz, o_dzt, o_hslot, o_wslot, bytes;
 };
 
 constexpr int CUS = 256;
@@ -663,6 +762,7 @@ Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     int64_t at = 0;
     auto take = [&](int64_t b) { const int64_t o = at; at = up(at + b, 256); return o; };
     s.o_info = take(sizeof(Info));
+    s.o_counts = take(2 * 4096);       // of 2048 columns each: at most 1024 numbers and 1024 maxima
     s.o_idx = take(s.npad * 4); s.o_pos = take(s.npad * 4); s.o_y = take(s.npad * 4);
     s.o_f = take(s.npad * 4); s.o_lse = take(s.npad * 4); s.o_loss = take(s.npad * 4); s.o_zy = take(s.npad * 4);
     s.o_h = take(s.npad * s.kpad * s.es);
@@ -741,9 +841,13 @@ template <typename T> void run(const Call &c, const Shape &s) {
     const int n = (int)s.n, p = (int)s.p, k = (int)s.k;
 
     Select sel{c.labels, c.grad ? c.gout : nullptr, c.lse_given ? c.lse : nullptr, c.o.ignore_index, n, p, c.o.reduction, c.grad && sizeof(T) == 2 && !std::is_same<T, __bf16>::value,
-               (float)a_, info, i32(s.o_idx), i32(s.o_pos), i32(s.o_y), f32(s.o_f), f32(s.o_lse), c.lse_given ? nullptr : c.loss, c.lse_given ? nullptr : c.lse};
+               (float)a_, info, i32(s.o_idx), i32(s.o_pos), i32(s.o_y), f32(s.o_f), f32(s.o_lse), c.lse_given ? nullptr : c.loss, c.lse_given ? nullptr : c.lse, i32(s.o_counts), f32(s.o_counts + 4096)};
     if (n > ONE_ROUND) {
-        select_kernel<<<1, 1024, 0, c.st>>>(sel);
+        if (n > SELF) {
+            count_kernel<<<(n + 2047) / 2048, 256, 0, c.st>>>(sel);
+            ops::hip_ok(hipGetLastError(), "count");
+        }
+        select_kernel<<<(n + 2047) / 2048, 256, 0, c.st>>>(sel);
         ops::hip_ok(hipGetLastError(), "select");
     }
 
@@ -753,7 +857,7 @@ template <typename T> void run(const Call &c, const Shape &s) {
     const int ct = (int)(s.kpad / 64 + (s.kpad % 64 != 0)), wr = pw || pwt ? (int)(s.ppad / 64) : 0;
     Pack<T> ph{static_cast<const T *>(c.H.data), c.H.cs, c.H.rs, n, k, h, ht, s.kpad, s.ldn, (int)s.npad, (int)s.npad, (int)s.kpad, (int)(s.npad / 64), (int)(s.npad / 64) * ct};
     Pack<T> pk{w, s.wrs, s.wcs, p, k, pw, pwt, s.kpad, s.ldp, p, (int)s.ppad, (int)s.kpad, wr, wr * ct};
-    prepare_kernel<T><<<ph.tiles + pk.tiles, 256, 0, c.st>>>(sel, ph, pk);
+    prepare_kernel<T><<<ph.tiles + pk.tiles + (n <= ONE_ROUND), 256, 0, c.st>>>(sel, ph, pk);
     ops::hip_ok(hipGetLastError(), "prepare");
     int64_t ldw = s.wrs, ldwt = s.wcs;
     int wchunks = (int)(s.k / per), wtpad = p;

@@ -21,7 +21,7 @@ _state = {}
 def _torch():
     if not _state:
         import torch
-        _state.update(torch=torch, dtypes={torch.float32: L.F32, torch.float64: L.F64, torch.bfloat16: L.BF16, torch.float16: L.F16})
+        _state.update(raw=getattr(torch._C, "_cuda_getCurrentRawStream", None), torch=torch, dtypes={torch.float32: L.F32, torch.float64: L.F64, torch.bfloat16: L.BF16, torch.float16: L.F16})
     return _state["torch"]
 
 
@@ -75,7 +75,8 @@ def _workspace(w, h, o, grad, device):
 
 
 def _stream(device):
-    return _torch().cuda.current_stream(device).cuda_stream
+    raw = _state["raw"]
+    return raw(device.index) if raw else _torch().cuda.current_stream(device).cuda_stream
 
 
 def softmax_xent(W, H, labels, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
