@@ -9,6 +9,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 #include "device_ops.hpp"
@@ -21,21 +22,40 @@ typedef u32x4 u32x4_any __attribute__((aligned(2)));   // 16 bytes at any elemen
 
 constexpr int NT = 256;
 constexpr int CHUNK_BYTES = 16384;      // 4 loads of 16 bytes for each of 256 threads
-constexpr int MAXT = 72;                // table entries of a launch: they travel as kernel arguments (4 KB)
 constexpr int BLOCKS = 2048;
 
+// The list travels as kernel arguments (an argument's bytes cost the host about a nanosecond each, a launch with 3.6 KB of them 7 us, one
+// with little 2.5: hence 16 bytes an entry, 24 with a result of its own, and a short form of the table).
 struct Entry {
     const char *in;
-    char *out;
-    int64_t n;              // elements
-    int64_t ldi, ldo;       // elements between rows; 0: dense
-    int cols;               // elements of a row (where not dense)
-    int chunk0;             // first chunk
+    uint32_t chunk0;        // first chunk
+    uint32_t bits;          // elements of the last chunk: 14 bits; dtype: 2; place in Table::s + 1, or 0 where dense: 16
 };
-struct Table {
-    Entry e[MAXT];
-    int dtype[MAXT];
-    int count, chunks;
+struct Strided {
+    int64_t ldi, ldo;       // elements between rows
+    int64_t cols;           // elements of a row
+};
+// N entries, S of them strided, OUT with results of their own
+template <int N_, int S_, bool OUT> struct Table {
+    static constexpr int N = N_, S = S_;
+    static constexpr bool HAS_OUT = OUT;
+    Entry e[N];
+    char *out[OUT ? N : 1];
+    Strided s[S];
+    int count, strided, chunks;
+};
+typedef Table<8, 2, true> Short;
+typedef Table<192, 16, false> Long;
+typedef Table<128, 16, true> LongOut;
+static_assert(sizeof(Long) <= 3600 && sizeof(LongOut) <= 3600, "a kernel's arguments");
+
+// an entry as the kernels work with it
+struct Item {
+    const char *in;
+    char *out;
+    int64_t n;
+    int chunk0, dtype;
+    const Strided *strided;
 };
 
 template <int INF> __device__ __forceinline__ void take(double &s, double x) {
@@ -59,27 +79,31 @@ template <int INF> __device__ __forceinline__ double block_total(double s, doubl
 }
 
 // the entry a chunk belongs to (the table is short and the index the same for the whole block)
-__device__ __forceinline__ int entry_of(const Table &t, int chunk) {
+template <typename Tab> __device__ __forceinline__ Item item_of(const Tab &t, int chunk) {
     int lo = 0, hi = t.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (t.e[mid].chunk0 <= chunk) lo = mid;
+        if ((int)t.e[mid].chunk0 <= chunk) lo = mid;
         else hi = mid - 1;
     }
-    return lo;
+    const Entry &e = t.e[lo];
+    const int next = lo + 1 < t.count ? (int)t.e[lo + 1].chunk0 : t.chunks, dtype = e.bits >> 14 & 3, place = e.bits >> 16;
+    const int per = CHUNK_BYTES / (dtype == NMFX_F64 ? 8 : dtype == NMFX_F32 ? 4 : 2);
+    char *out = const_cast<char *>(e.in);
+    if constexpr (Tab::HAS_OUT) out = t.out[lo];
+    return Item{e.in, out, (int64_t)(next - 1 - (int)e.chunk0) * per + (e.bits & 0x3fff), (int)e.chunk0, dtype, place ? &t.s[place - 1] : nullptr};
 }
 
-template <typename T> __device__ __forceinline__ int64_t at(const Entry &e, int64_t i, int64_t ld) {
-    if (!e.ldi) return i;
-    const int64_t r = i / e.cols;
-    return r * ld + (i - r * e.cols);
+__device__ __forceinline__ int64_t at(int64_t cols, int64_t i, int64_t ld) {
+    const int64_t r = i / cols;
+    return r * ld + (i - r * cols);
 }
 
-template <typename T, int INF> __device__ __forceinline__ void sum_chunk(const Entry &e, int chunk, int nt, double &s) {
+template <typename T, int INF> __device__ __forceinline__ void sum_chunk(const Item &e, int chunk, int nt, double &s) {
     constexpr int V = 16 / sizeof(T), PER = CHUNK_BYTES / sizeof(T);
     const T *in = reinterpret_cast<const T *>(e.in);
     const int64_t beg = (int64_t)(chunk - e.chunk0) * PER, end = min(e.n, beg + PER);
-    if (!e.ldi) {
+    if (!e.strided) {
         const int64_t whole = beg + (end - beg) / V * V;
         if (end - beg == PER && nt == NT) {
             u32x4 v[4];
@@ -100,20 +124,22 @@ template <typename T, int INF> __device__ __forceinline__ void sum_chunk(const E
             for (int u = 0; u < V; ++u) take<INF>(s, (double)x[u]);
         }
         for (int64_t i = whole + threadIdx.x; i < end; i += nt) take<INF>(s, (double)in[i]);
-    } else
-        for (int64_t i = beg + threadIdx.x; i < end; i += nt) take<INF>(s, (double)in[at<T>(e, i, e.ldi)]);
+    } else {
+        const Strided &d = *e.strided;
+        for (int64_t i = beg + threadIdx.x; i < end; i += nt) take<INF>(s, (double)in[at(d.cols, i, d.ldi)]);
+    }
 }
 
 template <typename T> __device__ __forceinline__ T scaled(T x, double c) {
     if constexpr (sizeof(T) == 8) return x * c;
     else return (T)((float)x * (float)c);
 }
-template <typename T> __device__ __forceinline__ void scale_chunk(const Entry &e, int chunk, int nt, double c) {
+template <typename T> __device__ __forceinline__ void scale_chunk(const Item &e, int chunk, int nt, double c) {
     constexpr int V = 16 / sizeof(T), PER = CHUNK_BYTES / sizeof(T);
     const T *in = reinterpret_cast<const T *>(e.in);
     T *out = reinterpret_cast<T *>(e.out);
     const int64_t beg = (int64_t)(chunk - e.chunk0) * PER, end = min(e.n, beg + PER);
-    if (!e.ldi && !e.ldo) {
+    if (!e.strided) {
         const int64_t whole = beg + (end - beg) / V * V;
         if (end - beg == PER && nt == NT) {
             u32x4 v[4];
@@ -136,24 +162,24 @@ template <typename T> __device__ __forceinline__ void scale_chunk(const Entry &e
             *reinterpret_cast<u32x4_any *>(out + i) = v;
         }
         for (int64_t i = whole + threadIdx.x; i < end; i += nt) out[i] = scaled(in[i], c);
-    } else
-        for (int64_t i = beg + threadIdx.x; i < end; i += nt) out[at<T>(e, i, e.ldo)] = scaled(in[at<T>(e, i, e.ldi)], c);
+    } else {
+        const Strided &d = *e.strided;
+        for (int64_t i = beg + threadIdx.x; i < end; i += nt) out[at(d.cols, i, d.ldo)] = scaled(in[at(d.cols, i, d.ldi)], c);
+    }
 }
 
-template <int INF> __device__ __forceinline__ void sum_any(const Table &t, int chunk, int nt, double &s) {
-    const int q = entry_of(t, chunk);
-    const Entry &e = t.e[q];
-    switch (t.dtype[q]) {
+template <int INF, typename Tab> __device__ __forceinline__ void sum_any(const Tab &t, int chunk, int nt, double &s) {
+    const Item e = item_of(t, chunk);
+    switch (e.dtype) {
         case NMFX_F32: sum_chunk<float, INF>(e, chunk, nt, s); break;
         case NMFX_F64: sum_chunk<double, INF>(e, chunk, nt, s); break;
         case NMFX_BF16: sum_chunk<__bf16, INF>(e, chunk, nt, s); break;
         default: sum_chunk<_Float16, INF>(e, chunk, nt, s); break;
     }
 }
-__device__ __forceinline__ void scale_any(const Table &t, int chunk, int nt, double c) {
-    const int q = entry_of(t, chunk);
-    const Entry &e = t.e[q];
-    switch (t.dtype[q]) {
+template <typename Tab> __device__ __forceinline__ void scale_any(const Tab &t, int chunk, int nt, double c) {
+    const Item e = item_of(t, chunk);
+    switch (e.dtype) {
         case NMFX_F32: scale_chunk<float>(e, chunk, nt, c); break;
         case NMFX_F64: scale_chunk<double>(e, chunk, nt, c); break;
         case NMFX_BF16: scale_chunk<__bf16>(e, chunk, nt, c); break;
@@ -166,10 +192,10 @@ __device__ __forceinline__ double coef_of(double norm, double max_norm) {
     return c >= 1. ? 1. : c;                 // a NaN norm gives a NaN coefficient
 }
 
-template <int INF> __global__ __launch_bounds__(NT) void partial_kernel(Table t, double *part) {
+template <int INF, typename Tab> __global__ __launch_bounds__(NT) void partial_kernel(Tab t, double *part) {
     __shared__ double sh[NT / 64];
     double s = 0.;
-    for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) sum_any<INF>(t, c, NT, s);
+    for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) sum_any<INF, Tab>(t, c, NT, s);
     s = block_total<INF>(s, sh, NT);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
@@ -180,7 +206,7 @@ template <int INF> __global__ __launch_bounds__(1024) void norm_kernel(const dou
     s = block_total<INF>(s, sh, 1024);
     if (threadIdx.x == 0) *norm = (float)norm_of<INF>(s);
 }
-template <int INF> __global__ __launch_bounds__(NT) void scale_kernel(Table t, const double *part, int parts, double max_norm, int in_place, float *norm) {
+template <int INF, typename Tab> __global__ __launch_bounds__(NT) void scale_kernel(Tab t, const double *part, int parts, double max_norm, int in_place, float *norm) {
     __shared__ double sh[NT / 64];
     double s = 0.;
     for (int i = threadIdx.x; i < parts; i += NT) s = both<INF>(s, part[i]);
@@ -190,10 +216,10 @@ template <int INF> __global__ __launch_bounds__(NT) void scale_kernel(Table t, c
     for (int k = t.chunks - 1 - blockIdx.x; k >= 0; k -= gridDim.x) scale_any(t, k, NT, c);
 }
 // a short list: one block does all
-template <int INF> __global__ __launch_bounds__(1024) void small_kernel(Table t, double max_norm, int in_place, int clip, float *norm) {
+template <int INF> __global__ __launch_bounds__(1024) void small_kernel(Short t, double max_norm, int in_place, int clip, float *norm) {
     __shared__ double sh[16];
     double s = 0.;
-    for (int c = 0; c < t.chunks; ++c) sum_any<INF>(t, c, 1024, s);
+    for (int c = 0; c < t.chunks; ++c) sum_any<INF, Short>(t, c, 1024, s);
     const double nrm = norm_of<INF>(block_total<INF>(s, sh, 1024));
     if (threadIdx.x == 0) *norm = (float)nrm;
     if (!clip) return;
@@ -203,7 +229,7 @@ template <int INF> __global__ __launch_bounds__(1024) void small_kernel(Table t,
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
-constexpr int64_t SMALL_CHUNKS = 8;
+constexpr int64_t SMALL_CHUNKS = 2;
 
 struct View {           // a matrix as rows of contiguous elements
     char *p;
@@ -212,20 +238,20 @@ struct View {           // a matrix as rows of contiguous elements
     int64_t bytes() const { return ((rows - 1) * ld + len) * es; }
 };
 View view_of(const nmfx_dmat &m, const char *what) {
-    const std::string s(what);
+    auto refuse = [&](int status, const char *why) { throw ops::OpError{status, std::string(what) + why}; };
     const int es = ops::elem_bytes(m.dtype);
-    if (!es) throw ops::OpError{NMFX_ERR_BAD_ARG, s + ": dtype is none of NMFX_F32, NMFX_F64, NMFX_BF16, NMFX_F16"};
-    if (m.reserved != 0) throw ops::OpError{NMFX_ERR_BAD_ARG, s + ": reserved must be 0"};
-    if (m.rows < 0 || m.cols < 0) throw ops::OpError{NMFX_ERR_DIM_MISMATCH, s + ": negative extent"};
+    if (!es) refuse(NMFX_ERR_BAD_ARG, ": dtype is none of NMFX_F32, NMFX_F64, NMFX_BF16, NMFX_F16");
+    if (m.reserved != 0) refuse(NMFX_ERR_BAD_ARG, ": reserved must be 0");
+    if (m.rows < 0 || m.cols < 0) refuse(NMFX_ERR_DIM_MISMATCH, ": negative extent");
     if (!m.rows || !m.cols) return View{nullptr, 0, 0, 0, es, m.dtype};
-    if (!m.data) throw ops::OpError{NMFX_ERR_BAD_ARG, s + ": data is NULL"};
-    if (reinterpret_cast<uintptr_t>(m.data) % es) throw ops::OpError{NMFX_ERR_BAD_ARG, s + ": data is not aligned to its element"};
+    if (!m.data) refuse(NMFX_ERR_BAD_ARG, ": data is NULL");
+    if (reinterpret_cast<uintptr_t>(m.data) & (es - 1)) refuse(NMFX_ERR_BAD_ARG, ": data is not aligned to its element");
     View v{static_cast<char *>(m.data), 0, 0, 0, es, m.dtype};
     if (m.cs == 1 && (m.rs >= m.cols || m.rows == 1)) { v.rows = m.rows; v.len = m.cols; v.ld = m.rs; }
     else if (m.rs == 1 && (m.cs >= m.rows || m.cols == 1)) { v.rows = m.cols; v.len = m.rows; v.ld = m.cs; }
-    else throw ops::OpError{NMFX_ERR_BAD_ARG, s + ": one of rs, cs must be 1 and the other at least the extent it steps over"};
+    else refuse(NMFX_ERR_BAD_ARG, ": one of rs, cs must be 1 and the other at least the extent it steps over");
     if (v.rows == 1 || v.ld == v.len) { v.len *= v.rows; v.rows = 1; v.ld = v.len; }
-    if (v.rows > 1 && v.len > INT32_MAX) throw ops::OpError{NMFX_ERR_UNSUPPORTED, s + ": rows of a strided matrix may have at most 2^31 - 1 elements"};
+    if (v.rows > 1 && v.len > INT32_MAX) refuse(NMFX_ERR_UNSUPPORTED, ": rows of a strided matrix may have at most 2^31 - 1 elements");
     return v;
 }
 
@@ -240,69 +266,84 @@ bool meet(const View &a, const View &b) {
     const int64_t d = (b.p - a.p) % ld;
     return !(d >= a.len * a.es && d + b.len * b.es <= ld);
 }
-bool any_meet(std::vector<View> v) {
-    std::sort(v.begin(), v.end(), [](const View &a, const View &b) { return a.p < b.p; });
+bool before(const View &a, const View &b) { return a.p < b.p; }
+// of views in order of address
+bool any_meet(const std::vector<View> &v) {
     for (size_t i = 0; i < v.size(); ++i)
         for (size_t j = i + 1; j < v.size() && v[j].p < v[i].p + v[i].bytes(); ++j)
             if (meet(v[i], v[j])) return true;
     return false;
 }
 
-struct Plan {
-    std::vector<Table> tables;
-    std::vector<int> blocks;
-    int parts = 0;
-    int64_t chunks = 0;
-};
 int64_t chunks_of(const View &v) { return (v.rows * v.len * v.es + CHUNK_BYTES - 1) / CHUNK_BYTES; }
+int64_t workspace_of(int64_t count) { return 8 * (BLOCKS + count / 2 + 64); }    // (a table of the short form takes 2 strided entries)
 
-Plan plan_of(const std::vector<View> &in, const std::vector<View> &out) {
-    Plan p;
-    for (size_t i = 0; i < in.size(); ++i) {
-        const View &a = in[i], &b = out[i];
+struct Work {
+    const std::vector<View> &in, &out;
+    bool clip, in_place;
+    double max_norm;
+    float *norm;
+    double *part;
+    hipStream_t st;
+};
+template <typename Tab> std::vector<Tab> tables_of(const Work &w) {
+    std::vector<Tab> ts;
+    for (size_t i = 0; i < w.in.size(); ++i) {
+        const View &a = w.in[i], &b = w.out[i];
         if (!a.rows) continue;
         const int64_t c = chunks_of(a);
         ops::require(c <= INT32_MAX / 2, NMFX_ERR_UNSUPPORTED, "a matrix is larger than 2^44 bytes");
-        if (p.tables.empty() || p.tables.back().count == MAXT || p.tables.back().chunks + c > INT32_MAX / 2) p.tables.push_back(Table{});
-        Table &t = p.tables.back();
         const bool dense = a.rows == 1 && b.rows == 1;
-        // where only one side is dense, both go by the rows of the other
-        const int64_t cols = a.rows > 1 ? a.len : b.len;
-        t.e[t.count] = Entry{a.p, b.p, a.rows * a.len, dense ? 0 : (a.rows > 1 ? a.ld : cols), dense ? 0 : (b.rows > 1 ? b.ld : cols), (int)(dense ? 0 : cols), t.chunks};
-        t.dtype[t.count++] = a.dtype;
+        if (ts.empty() || ts.back().count == Tab::N || (!dense && ts.back().strided == Tab::S) || ts.back().chunks + c > INT32_MAX / 2) {
+            ts.emplace_back();
+            ts.back().count = ts.back().strided = ts.back().chunks = 0;
+        }
+        Tab &t = ts.back();
+        if (!dense) {
+            // where only one side is dense, both go by the rows of the other
+            const int64_t cols = a.rows > 1 ? a.len : b.len;
+            t.s[t.strided++] = Strided{a.rows > 1 ? a.ld : cols, b.rows > 1 ? b.ld : cols, cols};
+        }
+        const uint32_t last = (uint32_t)(a.rows * a.len - (c - 1) * (CHUNK_BYTES / a.es));
+        if constexpr (Tab::HAS_OUT) t.out[t.count] = b.p;
+        t.e[t.count++] = Entry{a.p, (uint32_t)t.chunks, last | (uint32_t)a.dtype << 14 | (dense ? 0u : (uint32_t)t.strided) << 16};
         t.chunks += (int)c;
-        p.chunks += c;
     }
-    for (const Table &t : p.tables) {
-        const int64_t share = std::max<int64_t>(1, (int64_t)BLOCKS * t.chunks / p.chunks);
-        p.blocks.push_back((int)std::min<int64_t>(t.chunks, share));
-        p.parts += p.blocks.back();
-    }
-    return p;
+    return ts;
 }
-int64_t workspace_of(int64_t count) { return 8 * (BLOCKS + count / MAXT + 64); }
 
-template <int INF> void launch(const Plan &p, bool clip, bool in_place, double max_norm, float *norm, double *part, hipStream_t st) {
-    if (p.tables.size() == 1 && p.chunks <= SMALL_CHUNKS) {
-        small_kernel<INF><<<1, 1024, 0, st>>>(p.tables[0], max_norm, in_place, clip, norm);
+template <int INF, typename Tab> void launch(const Work &w) {
+    const std::vector<Tab> ts = tables_of<Tab>(w);
+    int64_t chunks = 0;
+    for (const Tab &t : ts) chunks += t.chunks;
+    if constexpr (std::is_same<Tab, Short>::value)
+        if (ts.size() == 1 && chunks <= SMALL_CHUNKS) {
+            small_kernel<INF><<<1, 1024, 0, w.st>>>(ts[0], w.max_norm, w.in_place, w.clip, w.norm);
+            ops::hip_ok(hipGetLastError(), "gradient norm");
+            return;
+        }
+    int parts = 0;
+    ops::require((int64_t)(BLOCKS + ts.size()) * 8 <= workspace_of((int64_t)w.in.size()), NMFX_ERR_STATE, "partial sums exceed the workspace");
+    for (const Tab &t : ts) {
+        const int blocks = (int)std::min<int64_t>(t.chunks, std::max<int64_t>(1, (int64_t)BLOCKS * t.chunks / chunks));
+        partial_kernel<INF, Tab><<<blocks, NT, 0, w.st>>>(t, w.part + parts);
+        ops::hip_ok(hipGetLastError(), "gradient norm");
+        parts += blocks;
+    }
+    if (!w.clip || ts.empty()) {
+        norm_kernel<INF><<<1, 1024, 0, w.st>>>(w.part, parts, w.norm);
         ops::hip_ok(hipGetLastError(), "gradient norm");
         return;
     }
-    int at = 0;
-    for (size_t i = 0; i < p.tables.size(); at += p.blocks[i], ++i) {
-        partial_kernel<INF><<<p.blocks[i], NT, 0, st>>>(p.tables[i], part + at);
-        ops::hip_ok(hipGetLastError(), "gradient norm");
-    }
-    if (!clip || p.tables.empty()) {
-        norm_kernel<INF><<<1, 1024, 0, st>>>(part, p.parts, norm);
-        ops::hip_ok(hipGetLastError(), "gradient norm");
-        return;
-    }
-    for (size_t i = p.tables.size(); i-- > 0;) {
-        const int blocks = (int)std::min<int64_t>(p.tables[i].chunks, BLOCKS);
-        scale_kernel<INF><<<blocks, NT, 0, st>>>(p.tables[i], part, p.parts, max_norm, in_place, i == 0 ? norm : nullptr);
+    for (size_t i = ts.size(); i-- > 0;) {
+        scale_kernel<INF, Tab><<<(int)std::min<int64_t>(ts[i].chunks, BLOCKS), NT, 0, w.st>>>(ts[i], w.part, parts, w.max_norm, w.in_place, i == 0 ? w.norm : nullptr);
         ops::hip_ok(hipGetLastError(), "gradient scaling");
     }
+}
+template <int INF> void launch_any(const Work &w) {
+    if (w.in.size() <= 8) launch<INF, Short>(w);
+    else if (w.in_place) launch<INF, Long>(w);
+    else launch<INF, LongOut>(w);
 }
 
 void run(int count, const nmfx_dmat *g, const nmfx_dmat *o, bool clip, double max_norm, int norm_type, float *norm, void *ws, int64_t ws_bytes, int device, void *stream) {
@@ -328,30 +369,30 @@ void run(int count, const nmfx_dmat *g, const nmfx_dmat *o, bool clip, double ma
     }
     if (clip) {
         // every element is written by one thread once: no two results may share one, and none may be another's input
-        std::vector<View> w;
-        for (int i = 0; i < count; ++i)
-            if (out[i].rows) w.push_back(out[i]);
+        std::vector<View> w, r;
+        w.reserve(count);
+        for (int i = 0; i < count; ++i) {
+            if (!out[i].rows) continue;
+            w.push_back(out[i]);
+            if (o && !(in[i].p == out[i].p && in[i].rows == out[i].rows && in[i].ld == out[i].ld)) r.push_back(in[i]);
+        }
+        if (!std::is_sorted(w.begin(), w.end(), before)) std::sort(w.begin(), w.end(), before);
         ops::require(!any_meet(w), NMFX_ERR_BAD_ARG, "two of the matrices to write share elements");
-        if (o) {
-            std::vector<View> r;
-            for (int i = 0; i < count; ++i)
-                if (in[i].rows && !(in[i].p == out[i].p && in[i].rows == out[i].rows && in[i].ld == out[i].ld)) r.push_back(in[i]);
-            std::sort(w.begin(), w.end(), [](const View &a, const View &b) { return a.p < b.p; });
+        if (!r.empty()) {
             std::vector<char *> reach;            // how far the written views up to this one reach
+            reach.reserve(w.size());
             for (const View &v : w) reach.push_back(std::max(reach.empty() ? v.p : reach.back(), v.p + v.bytes()));
             for (const View &a : r)
                 for (size_t j = std::upper_bound(reach.begin(), reach.end(), a.p) - reach.begin(); j < w.size() && w[j].p < a.p + a.bytes(); ++j)
                     ops::require(!meet(a, w[j]), NMFX_ERR_BAD_ARG, "a matrix to write shares elements with a gradient that is not its own");
         }
     }
-    const Plan p = plan_of(in, out);
-    ops::require((int64_t)p.parts * 8 <= workspace_of(count), NMFX_ERR_STATE, "partial sums exceed the workspace");
-    ops::OnDevice on(device);
-    hipStream_t st = static_cast<hipStream_t>(stream);
     bool in_place = true;
-    for (int i = 0; i < count; ++i) in_place = in_place && in[i].p == out[i].p;
-    if (norm_type == NMFX_NORM_2) launch<0>(p, clip, in_place, max_norm, norm, static_cast<double *>(ws), st);
-    else launch<1>(p, clip, in_place, max_norm, norm, static_cast<double *>(ws), st);
+    for (int i = 0; i < count; ++i) in_place = in_place && in[i].p == out[i].p && in[i].rows == out[i].rows && in[i].ld == out[i].ld;
+    ops::OnDevice on(device);
+    const Work w{in, out, clip, in_place, max_norm, norm, static_cast<double *>(ws), static_cast<hipStream_t>(stream)};
+    if (norm_type == NMFX_NORM_2) launch_any<0>(w);
+    else launch_any<1>(w);
 }
 
 }  // namespace gradnorm

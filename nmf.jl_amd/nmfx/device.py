@@ -7,6 +7,7 @@ works without torch: it is imported with the first call."""
 from __future__ import annotations
 
 import ctypes as C
+from operator import attrgetter
 
 import numpy as np
 
@@ -16,6 +17,7 @@ from .api import ArgumentError, DimensionMismatch, _raise
 _DMAT = np.dtype([("data", "u8"), ("rows", "i8"), ("cols", "i8"), ("rs", "i8"), ("cs", "i8"), ("dtype", "i4"), ("reserved", "i4")])
 _REDUCTIONS = {"none": L.REDUCE_NONE, "sum": L.REDUCE_SUM, "mean": L.REDUCE_MEAN}
 _state = {}
+_dtype_of = attrgetter("dtype")
 
 
 def _torch():
@@ -139,36 +141,45 @@ def softmax_xent_backward(W, H, labels, lse, gout=None, ignore_index=-100, label
     return _grad(W, H, labels, ignore_index, label_smoothing, reduction, gout, lse, dW, dH)[2:]
 
 
-def _list(ts, name, device=None):
-    """The descriptors of a list of tensors, as an array of nmfx_dmat."""
+def _list(ts, name, device):
+    """The descriptors of a list of tensors, as an array of nmfx_dmat: contiguous ones as one row.  (A call over hundreds of small tensors
+    takes as long as this does: a few passes over the list, each in C.)"""
     torch = _torch()
-    dtypes = _state["dtypes"]
+    T = torch.Tensor
+    try:
+        devices = set(map(T.get_device, ts))
+        dtypes = list(map(_dtype_of, ts))
+    except (TypeError, AttributeError):
+        raise ArgumentError(f"{name} must be torch tensors") from None
+    if devices != {device.index} or device.type != "cuda":
+        if not all(t.is_cuda for t in ts):
+            raise ArgumentError(f"{name} must be in device memory: there is no CPU path")
+        raise ArgumentError(f"{name} are on several devices")
+    codes = _state["dtypes"]
+    kinds = set(dtypes)
+    if not kinds <= codes.keys():
+        raise ArgumentError(f"one of {name} has dtype {next(d for d in dtypes if d not in codes)}: float32, float64, bfloat16 and float16 are taken")
     a = np.zeros(len(ts), _DMAT)
-    if not len(ts):
-        return a
-    for t in ts:
-        if not isinstance(t, torch.Tensor):
-            raise ArgumentError(f"{name} must be torch tensors")
-        if t.device != device or t.dtype not in dtypes or not t.is_cuda:
-            if not t.is_cuda:
-                raise ArgumentError(f"{name} must be in device memory: there is no CPU path")
-            if t.dtype not in dtypes:
-                raise ArgumentError(f"one of {name} has dtype {t.dtype}: float32, float64, bfloat16 and float16 are taken")
-            raise ArgumentError(f"one of {name} is on {t.device}, not on {device}")
-    a["data"] = [t.data_ptr() for t in ts]
-    a["cols"] = sizes = [t.numel() for t in ts]
-    a["rs"] = sizes
+    sizes = list(map(T.numel, ts))
+    a["data"] = list(map(T.data_ptr, ts))
+    a["cols"] = a["rs"] = sizes
     a["rows"] = a["cs"] = 1
-    a["dtype"] = [dtypes[t.dtype] for t in ts]
-    for i, t in enumerate(ts):
-        if not t.is_contiguous():
-            if t.dim() == 1:
-                a[i] = (t.data_ptr(), t.shape[0], 1, t.stride(0), 1, dtypes[t.dtype], 0)
-            elif t.dim() == 2:
-                a[i] = (t.data_ptr(), t.shape[0], t.shape[1], t.stride(0), t.stride(1), dtypes[t.dtype], 0)
-            else:
-                raise ArgumentError(f"one of {name} has more than two indices and is not contiguous")
-    return a
+    a["dtype"] = codes[dtypes[0]] if len(kinds) == 1 else [codes[d] for d in dtypes]
+    dense = list(map(T.is_contiguous, ts))
+    if not all(dense):
+        for i in range(len(ts)):
+            if not dense[i]:
+                _strided(a, i, ts[i], name)
+    return a, sizes
+
+
+def _strided(a, i, t, name):
+    if t.dim() == 1:
+        a[i] = (t.data_ptr(), t.shape[0], 1, t.stride(0), 1, a[i]["dtype"], 0)
+    elif t.dim() == 2:
+        a[i] = (t.data_ptr(), *t.shape, *t.stride(), a[i]["dtype"], 0)
+    else:
+        raise ArgumentError(f"one of {name} has more than two indices and is not contiguous")
 
 
 def _norm_type(norm_type):
@@ -185,26 +196,26 @@ def _norm(grads, max_norm, norm_type, out):
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     if not grads:
         raise ArgumentError("grads is empty")
-    dev = getattr(grads[0], "device", None)
-    a = _list(grads, "grads", dev)
+    if not isinstance(grads[0], torch.Tensor):
+        raise ArgumentError("grads must be torch tensors")
+    dev = grads[0].device
+    a, sizes = _list(grads, "grads", dev)
     b = None
     if out is not None:
         out = [out] if isinstance(out, torch.Tensor) else list(out)
         if len(out) != len(grads):
             raise DimensionMismatch(f"out has {len(out)} tensors, grads {len(grads)}")
-        for g, o in zip(grads, out):
-            if getattr(o, "shape", None) != g.shape:
-                raise DimensionMismatch("one of out has another shape than its gradient")
-        b = _list(out, "out", dev)
-        # a dense gradient beside a strided result (or the other way round): both go by the strides of their matrix
-        for i in np.nonzero(a["rows"] != b["rows"])[0]:
-            g, o = grads[i], out[i]
-            if g.dim() == 2:
-                a[i] = (g.data_ptr(), *g.shape, *g.stride(), a[i]["dtype"], 0)
-                b[i] = (o.data_ptr(), *o.shape, *o.stride(), b[i]["dtype"], 0)
-            else:
-                for x, t in ((a, g), (b, o)):
-                    x[i] = (t.data_ptr(), t.shape[0], 1, t.stride(0), 1, x[i]["dtype"], 0)
+        b, counts = _list(out, "out", dev)
+        if sizes != counts:
+            raise DimensionMismatch("one of out has another number of elements than its gradient")
+        # where one of the two is not contiguous both go by the strides of their matrix
+        odd = (a["rows"] != 1) | (b["rows"] != 1)
+        if odd.any():
+            for i in np.nonzero(odd)[0]:
+                if grads[i].shape != out[i].shape:
+                    raise DimensionMismatch("one of out has another shape than its gradient")
+                _strided(a, i, grads[i], "grads")
+                _strided(b, i, out[i], "out")
     lib = L.load()
     size = C.c_int64()
     _ck(lib.nmfx_grad_norm_workspace(len(grads), size))
@@ -227,7 +238,8 @@ def grad_norm(grads, norm_type=2):
 def clip_grad_norm(grads, max_norm, norm_type=2, out=None):
     """Scales a list of tensors by min(1, max_norm / (norm + 1e-6)), in place or into `out`, and returns the norm that they had.
 
-    Tensors are contiguous, or matrices and vectors with a stride; no two that are written may share elements."""
+    Tensors are contiguous, or matrices and vectors with a stride; out's have as many elements as their gradients (where one of the two is
+    strided, the same shape), and no two that are written may share elements."""
     if max_norm is None:
         raise ArgumentError("max_norm is None")
     return _norm(grads, max_norm, norm_type, out)
