@@ -73,6 +73,10 @@ struct Geom {
     int tile_m, tile_n, split, wm, wn, lane, tid;
 };
 
+// An epilogue functor has finish(acc, where, early, shared, st0, st1), with the LDS stages free for its use; what it reads ahead, in
+// begin(where, early, shared), is kept in an Early (registers) and a Shared (LDS of its own).
+struct None {};
+
 typedef __attribute__((address_space(3))) void lds_void;
 
 // what a row's chunk numbers are xored with to give their slots: 16 consecutive rows' slots of one chunk fill all 64 banks once
@@ -117,10 +121,8 @@ template <int N> __device__ __forceinline__ void wait_loads() {
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
 }
 
-// One tile's sums, in acc; false where the tile lies behind the operand's end.  ST: LDS stages.
-template <typename T, int BM, int BN, int WM, int WN, int ST>
-__device__ __forceinline__ bool tile(const Args &g, int bid, int nblk, char *const (&st)[ST], f32x4 (&acc)[BM / WM / 16][BN / WN / 16], Geom &geo) {
-    constexpr int NT = WM * WN * 64, MI = BM / WM / 16, NJ = BN / WN / 16;
+struct Place { int tile_m, tile_n, split; };
+__device__ __forceinline__ Place place_of(const Args &g, int bid, int nblk) {
     // consecutive blocks go to the 8 dies in turn: give every die a contiguous range of tiles, and walk a range in columns of 8 row
     // tiles, so that the tiles in flight on a die share rows of A and B in its L2
     {
@@ -133,12 +135,25 @@ __device__ __forceinline__ bool tile(const Args &g, int bid, int nblk, char *con
     const int per = 8 * g.tiles_n, grp = in / per;
     in -= grp * per;
     const int gm = min(8, g.tiles_m - grp * 8);
-    const int tile_m = grp * 8 + in % gm, tile_n = in / gm;
-    int ktiles = g.ktiles;
-    if (g.limit == LIMIT_N && tile_n * BN >= *g.count) return false;
-    if (g.limit == LIMIT_C) ktiles = min(ktiles, (int)((*g.count * (int64_t)sizeof(T) + ROW - 1) / ROW));
-    const int kbeg = (int)((int64_t)ktiles * split / g.splits), kend = (int)((int64_t)ktiles * (split + 1) / g.splits);
+    return Place{grp * 8 + in % gm, in / gm, split};
+}
 
+// One tile's sums, in acc; false where the tile lies behind the operand's end.  ST: LDS stages.  `meanwhile` runs while the first loads are
+// on their way: in a small product they and what the consumer reads take longer than the products.
+template <typename T, int BM, int BN, int WM, int WN, int ST, typename F>
+__device__ __forceinline__ bool tile(const Args &g, const Place &at, char *const (&st)[ST], f32x4 (&acc)[BM / WM / 16][BN / WN / 16], Geom &geo, F &&meanwhile) {
+    constexpr int NT = WM * WN * 64, MI = BM / WM / 16, NJ = BN / WN / 16;
+    const int tile_m = at.tile_m, tile_n = at.tile_n, split = at.split;
+    int kbeg, kend;
+    // the number of columns is read while loads are on their way, but where it decides what to load
+    if (g.limit == LIMIT_C && g.splits > 1) {
+        const int ktiles = min(g.ktiles, (int)((*g.count * (int64_t)sizeof(T) + ROW - 1) / ROW));
+        kbeg = (int)((int64_t)ktiles * split / g.splits);
+        kend = (int)((int64_t)ktiles * (split + 1) / g.splits);
+    } else {
+        kbeg = (int)((int64_t)g.ktiles * split / g.splits);
+        kend = (int)((int64_t)g.ktiles * (split + 1) / g.splits);
+    }
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave % WM, wn = wave / WM;
     Loader<BM, NT> la;
@@ -146,11 +161,6 @@ __device__ __forceinline__ bool tile(const Args &g, int bid, int nblk, char *con
     la.init(g.a, tile_m * BM, tid);
     lb.init(g.b, tile_n * BN, tid);
     constexpr int LA = Loader<BM, NT>::PER, LOADS = LA + Loader<BN, NT>::PER;
-
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     // A tile is 2 halves of the contraction (64 bytes: one matrix instruction's), a half MI steps: A's fragment i times all NJ of B's.
     // A's fragments are read D steps ahead into a ring of 4 sets of registers, B's a half ahead into the other of 2.
@@ -233,15 +243,29 @@ __device__ __forceinline__ bool tile(const Args &g, int bid, int nblk, char *con
         }
     };
     static_assert(MEET >= MI, "the barrier lies in the second half");
+    geo = Geom{tile_m * BM + wm * (BM / WM) + 4 * hi, tile_n * BN + wn * (BN / WN) + (lane & 15), tile_m, tile_n, split, wm, wn, lane, tid};
+#pragma unroll
+    for (int i = 0; i < ST; ++i)
+        if (kbeg + i < kend) {
+            starts(kbeg + i);
+#pragma unroll
+            for (int l = 0; l < LOADS; ++l)
+                if (i + 1 < ST || place(l) < BEHIND) load(st[i], l);
+        }
+    const int count = g.limit == LIMIT_NONE ? 0 : *g.count;
+    if (g.limit == LIMIT_N && tile_n * BN >= count) {
+        wait_loads<0>();
+        return false;
+    }
+    meanwhile(geo);
+    // (loads of tiles behind the end that the count gives are waited for, and not looked at)
+    if (g.limit == LIMIT_C && g.splits == 1) kend = min(kend, (int)((count * (int64_t)sizeof(T) + ROW - 1) / ROW));
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
     if (kbeg < kend) {
-#pragma unroll
-        for (int i = 0; i < ST; ++i)
-            if (kbeg + i < kend) {
-                starts(kbeg + i);
-#pragma unroll
-                for (int l = 0; l < LOADS; ++l)
-                    if (i + 1 < ST || place(l) < BEHIND) load(st[i], l);
-            }
         if (kbeg + ST - 1 < kend) wait_loads<(ST - 1) * LOADS - LATE>();
         else wait_loads<0>();
         asm volatile("" ::: "memory");
@@ -263,7 +287,7 @@ __device__ __forceinline__ bool tile(const Args &g, int bid, int nblk, char *con
                 if (kt + i < kend) run(st[(i + ST - 1) % ST], st[i], st[(i + 1) % ST], kt + i, false);
         }
     }
-    geo = Geom{tile_m * BM + wm * (BM / WM) + 4 * hi, tile_n * BN + wn * (BN / WN) + (lane & 15), tile_m, tile_n, split, wm, wn, lane, tid};
+    wait_loads<0>();
     __syncthreads();
     return true;
 }
@@ -286,10 +310,12 @@ template <typename T, int BM, int BN, int WM, int WN, int ST, typename Epi>
 __global__ __launch_bounds__(WM *WN * 64) void tn_kernel(Args g, Epi epi) {
 #ifdef __HIP_DEVICE_COMPILE__
     NMFX_TN_STAGES(BM, BN, ST)
+    __shared__ typename Epi::template Shared<BM, BN, WM, WN> sh;
+    typename Epi::template Early<BM / WM / 16, BN / WN / 16> early;
     f32x4 acc[BM / WM / 16][BN / WN / 16];
     Geom geo;
-    if (!tile<T, BM, BN, WM, WN, ST>(g, blockIdx.x, gridDim.x, st, acc, geo)) return;
-    epi.template finish<BM, BN, WM, WN>(acc, geo, st0, st1);
+    if (!tile<T, BM, BN, WM, WN, ST>(g, place_of(g, blockIdx.x, gridDim.x), st, acc, geo, [&](const Geom &at) { epi.template begin<BM, BN, WM, WN>(at, early, sh); })) return;
+    epi.template finish<BM, BN, WM, WN>(acc, geo, early, sh, st0, st1);
 #endif
 }
 
@@ -298,13 +324,14 @@ template <typename T, int BM, int BN, int WM, int WN, int ST, typename EpiA, typ
 __global__ __launch_bounds__(WM *WN * 64) void tn_pair_kernel(Args ga, EpiA ea, Args gb, EpiB eb, int first) {
 #ifdef __HIP_DEVICE_COMPILE__
     NMFX_TN_STAGES(BM, BN, ST)
+    None none;
     f32x4 acc[BM / WM / 16][BN / WN / 16];
     Geom geo;
     const bool is_a = (int)blockIdx.x < first;
     const Args g = is_a ? ga : gb;
-    if (!tile<T, BM, BN, WM, WN, ST>(g, blockIdx.x - (is_a ? 0 : first), is_a ? first : gridDim.x - first, st, acc, geo)) return;
-    if (is_a) ea.template finish<BM, BN, WM, WN>(acc, geo, st0, st1);
-    else eb.template finish<BM, BN, WM, WN>(acc, geo, st0, st1);
+    if (!tile<T, BM, BN, WM, WN, ST>(g, place_of(g, blockIdx.x - (is_a ? 0 : first), is_a ? first : gridDim.x - first), st, acc, geo, [](const Geom &) {})) return;
+    if (is_a) ea.template finish<BM, BN, WM, WN>(acc, geo, none, none, st0, st1);
+    else eb.template finish<BM, BN, WM, WN>(acc, geo, none, none, st0, st1);
 #endif
 }
 

@@ -330,11 +330,17 @@ struct EpiStats {
     const int *y;
     const int *count;
     int p, npad;
-    template <int BM, int BN, int WM, int WN, int MI, int NJ>
-    __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, char *smem, char *) const {
+    template <int MI, int NJ> struct Early { int cnt, y[NJ]; };
+    template <int BM, int BN, int WM, int WN> using Shared = tn::None;
+    template <int BM, int BN, int WM, int WN, typename E> __device__ __forceinline__ void begin(const Geom &g, E &early, tn::None &) const {
+        early.cnt = *count;
+#pragma unroll
+        for (int j = 0; j < BN / WN / 16; ++j) early.y[j] = g.n0 + 16 * j < early.cnt ? y[g.n0 + 16 * j] : -1;
+    }
+    template <int BM, int BN, int WM, int WN, int MI, int NJ, typename E>
+    __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, const E &early, tn::None &, char *smem, char *) const {
         float2 *ps = reinterpret_cast<float2 *>(smem);                        // [WM][BN]
         float *zs = reinterpret_cast<float *>(smem + sizeof(float2) * WM * BN);
-        const int cnt = *count;
         if (g.tile_m * BM + BM > p) {
 #pragma unroll
             for (int i = 0; i < MI; ++i)
@@ -375,8 +381,8 @@ struct EpiStats {
                 t += __shfl_xor(t, 32);
                 if (g.lane < 16) zs[g.wm * BN + col] = t;
             }
-            if (n < cnt) {
-                const int d = y[n] - g.m0;
+            {
+                const int d = early.y[j] - g.m0;           // (-1 where there is no column or no class: below every m0)
                 if (d >= 0 && d < 16 * MI && (d & 15) < 4) {
 #pragma unroll
                     for (int i = 0; i < MI; ++i)
@@ -496,38 +502,47 @@ template <typename T> struct EpiDz {
     float inv, label, off;    // 1 / a, (1 - eps) / a, eps / (a p)
     int few;                  // the tiles' statistics are not joined yet: every block does it for its own columns
     Combine c;
-    template <int BM, int BN, int WM, int WN, int MI, int NJ>
-    __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, char *st0, char *st1) const {
-        typedef T T4 __attribute__((ext_vector_type(4)));
-        const int cnt = *count;
-        float lse[NJ];
+    // per column: log-sum-exp, factor, label's class in the piece.  The large tile has no registers for them to wait in: it reads them late.
+    template <int MI, int NJ> struct Early { int cnt, y[NJ]; float lse[NJ], f[NJ]; };
+    template <int BM, int BN, int WM, int WN> struct Shared { float lse[BN], t[WM * WN * 64]; float2 s[WM * WN * 64]; };
+    template <int BM, int BN, int WM, int WN, typename E, typename S> __device__ __forceinline__ void begin(const Geom &g, E &early, S &sh) const {
+        early.cnt = *count;
         if (few) {
             constexpr int STEP = WM * WN * 64 / BN;
-            float *sl = reinterpret_cast<float *>(st0);                           // [BN]
-            float2 *ps = reinterpret_cast<float2 *>(st0 + BN * sizeof(float));    // [STEP][BN]
-            float *ts = reinterpret_cast<float *>(ps + STEP * BN);
             const int at = g.tid % BN, slice = g.tid / BN, i = g.tile_n * BN + at;
             float2 a;
             float t;
             c.some(i, slice, STEP, a, t);
-            ps[g.tid] = a;
-            ts[g.tid] = t;
+            sh.s[g.tid] = a;
+            sh.t[g.tid] = t;
             __syncthreads();
             if (slice == 0) {
 #pragma unroll
                 for (int w = 1; w < STEP; ++w) {
-                    a = join(a, ps[w * BN + at]);
-                    t += ts[w * BN + at];
+                    a = join(a, sh.s[w * BN + at]);
+                    t += sh.t[w * BN + at];
                 }
-                sl[at] = i < cnt ? c.finish(i, a, t, g.tile_m == 0) : 0.f;
+                sh.lse[at] = i < early.cnt ? c.finish(i, a, t, g.tile_m == 0) : 0.f;
             }
             __syncthreads();
+        }
+        if (BM < 256) read<BN, BN / WN / 16>(g, early, sh);
+    }
+    template <int BN, int NJ, typename E, typename S> __device__ __forceinline__ void read(const Geom &g, E &early, S &sh) const {
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) lse[j] = sl[g.n0 + 16 * j - g.tile_n * BN];
-            __syncthreads();
-        } else
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) lse[j] = g.n0 + 16 * j < cnt ? lse_c[g.n0 + 16 * j] : 0.f;
+        for (int j = 0; j < NJ; ++j) {
+            const int n = g.n0 + 16 * j;
+            const bool on = n < early.cnt;
+            early.lse[j] = few ? sh.lse[n - g.tile_n * BN] : on ? lse_c[n] : 0.f;
+            early.f[j] = on ? f[n] : 0.f;
+            early.y[j] = on ? y[n] - v0 : -1;
+        }
+    }
+    template <int BM, int BN, int WM, int WN, int MI, int NJ, typename E, typename S>
+    __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, E &early, S &sh, char *st0, char *st1) const {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        if (BM == 256) read<BN, NJ>(g, early, sh);
+        const int cnt = early.cnt;
         using P = Patch<16 * MI, WM * WN>;
         const int wave = g.tid >> 6;
         char *patch = P::of(st0, st1, wave, 16 * NJ);
@@ -536,7 +551,7 @@ template <typename T> struct EpiDz {
         auto column = [&](int j, auto at_edge) {
             const int n = g.n0 + 16 * j;
             const bool on = n < cnt;
-            const float fac = on ? f[n] : 0.f, mul = fac * inv, sub = -fac * off, ref = lse[j] * -LOG2E;
+            const float fac = early.f[j], mul = fac * inv, sub = -fac * off, ref = early.lse[j] * -LOG2E;
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 T4 o;
@@ -553,8 +568,8 @@ template <typename T> struct EpiDz {
                 }
             }
             // the label's entry, where it is this lane's: written once more
-            const int d = on ? y[n] - v0 - g.m0 : -1;
-            if (d >= 0 && d < 16 * MI && (d & 15) < 4) {
+            const int d = early.y[j] - g.m0;
+            if (early.y[j] >= 0 && d >= 0 && d < 16 * MI && (d & 15) < 4) {
                 float z = 0.f;
 #pragma unroll
                 for (int i = 0; i < MI; ++i)
@@ -598,8 +613,11 @@ struct EpiSlot {
     float *out;
     int64_t ld, slot;
     int nmax, add;
+    template <int MI, int NJ> using Early = tn::None;
+    template <int BM, int BN, int WM, int WN> using Shared = tn::None;
+    template <int BM, int BN, int WM, int WN> __device__ __forceinline__ void begin(const Geom &, tn::None &, tn::None &) const {}
     template <int BM, int BN, int WM, int WN, int MI, int NJ>
-    __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, char *, char *) const {
+    __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, tn::None &, tn::None &, char *, char *) const {
         float *base = out + g.split * slot;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
@@ -623,8 +641,11 @@ template <typename T> struct EpiOut {
     int64_t ld;
     const Info *info;
     int mmax, nmax, wide;     // wide: four consecutive m go in one store
+    template <int MI, int NJ> using Early = tn::None;
+    template <int BM, int BN, int WM, int WN> using Shared = tn::None;
+    template <int BM, int BN, int WM, int WN> __device__ __forceinline__ void begin(const Geom &, tn::None &, tn::None &) const {}
     template <int BM, int BN, int WM, int WN, int MI, int NJ>
-    __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, char *, char *) const {
+    __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, tn::None &, tn::None &, char *, char *) const {
         typedef T T4 __attribute__((ext_vector_type(4)));
         const float u = info->unscale;
 #pragma unroll
