@@ -1,9 +1,9 @@
 // gradnorm.hip -- the norm over all elements of a list of matrices, sqrt(sum g^2) or max |g|, and clipping by it:
 //     coef = min(1, max_norm / (norm + 1e-6)),   out = g * coef
 // Two passes over the list: partial sums (a fixed number of blocks, each over a fixed set of chunks: the same list gives the same bits),
-// and the scaling, whose every block adds up the partial sums for itself (at most ~2048 doubles from L2: cheaper than a launch in between).
-// Squares are summed in Float64: the sum of 10^9 of them loses nothing, and a gradient of 10^30 does not overflow; the conversion and the
-// product-sum cost less than the memory takes.  The scaling walks the chunks backwards, so that it starts on what the first pass read last
+// and the scaling, whose every block adds up the partial sums for itself (some thousand doubles from L2: cheaper than a launch in between).
+// Squares are summed in Float64: the sum of 10^9 of them loses nothing, and a gradient of 10^30 does not overflow.  (For 16-bit elements
+// eight squares summed in Float32 first, where that is safe, were no faster: 416 us either way for 680 MB of bf16, clipped.)  The scaling walks the chunks backwards, so that it starts on what the first pass read last
 // and the last-level cache still holds.  Bound by memory: one read for the norm, one more and a write for the scaling.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -22,7 +22,9 @@ typedef u32x4 u32x4_any __attribute__((aligned(2)));   // 16 bytes at any elemen
 
 constexpr int NT = 256;
 constexpr int CHUNK_BYTES = 16384;      // 4 loads of 16 bytes for each of 256 threads
-constexpr int BLOCKS = 2048;
+// as many blocks as the card holds at a time (4 and 8 a compute unit, by their registers): their shares are equal, so more would only make a
+// second, short round
+constexpr int SUM_BLOCKS = 1024, SCALE_BLOCKS = 2048;
 
 // The list travels as kernel arguments (an argument's bytes cost the host about a nanosecond each, a launch with 3.6 KB of them 7 us, one
 // with little 2.5: hence 16 bytes an entry, 24 with a result of its own, and a short form of the table).
@@ -54,7 +56,7 @@ struct Item {
     const char *in;
     char *out;
     int64_t n;
-    int chunk0, dtype;
+    int chunk0, next, dtype;      // its first chunk, the next entry's
     const Strided *strided;
 };
 
@@ -91,7 +93,7 @@ template <typename Tab> __device__ __forceinline__ Item item_of(const Tab &t, in
     const int per = CHUNK_BYTES / (dtype == NMFX_F64 ? 8 : dtype == NMFX_F32 ? 4 : 2);
     char *out = const_cast<char *>(e.in);
     if constexpr (Tab::HAS_OUT) out = t.out[lo];
-    return Item{e.in, out, (int64_t)(next - 1 - (int)e.chunk0) * per + (e.bits & 0x3fff), (int)e.chunk0, dtype, place ? &t.s[place - 1] : nullptr};
+    return Item{e.in, out, (int64_t)(next - 1 - (int)e.chunk0) * per + (e.bits & 0x3fff), (int)e.chunk0, next, dtype, place ? &t.s[place - 1] : nullptr};
 }
 
 __device__ __forceinline__ int64_t at(int64_t cols, int64_t i, int64_t ld) {
@@ -99,92 +101,96 @@ __device__ __forceinline__ int64_t at(int64_t cols, int64_t i, int64_t ld) {
     return r * ld + (i - r * cols);
 }
 
-template <typename T, int INF> __device__ __forceinline__ void sum_chunk(const Item &e, int chunk, int nt, double &s) {
-    constexpr int V = 16 / sizeof(T), PER = CHUNK_BYTES / sizeof(T);
+// Elements beg .. end - 1 of an entry, by a block of nt threads: U loads of 16 bytes a thread on their way at a time.
+template <typename T, int INF> __device__ __forceinline__ void sum_span(const Item &e, int64_t beg, int64_t end, int nt, double &s) {
+    constexpr int V = 16 / sizeof(T), U = 8;
     const T *in = reinterpret_cast<const T *>(e.in);
-    const int64_t beg = (int64_t)(chunk - e.chunk0) * PER, end = min(e.n, beg + PER);
-    if (!e.strided) {
-        const int64_t whole = beg + (end - beg) / V * V;
-        if (end - beg == PER && nt == NT) {
-            u32x4 v[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const u32x4_any *>(in + beg + (int64_t)(q * NT + threadIdx.x) * V);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const T *x = reinterpret_cast<const T *>(&v[q]);
-#pragma unroll
-                for (int u = 0; u < V; ++u) take<INF>(s, (double)x[u]);
-            }
-            return;
-        }
-        for (int64_t i = beg + (int64_t)threadIdx.x * V; i < whole; i += nt * V) {
-            const u32x4 v = *reinterpret_cast<const u32x4_any *>(in + i);
-            const T *x = reinterpret_cast<const T *>(&v);
-#pragma unroll
-            for (int u = 0; u < V; ++u) take<INF>(s, (double)x[u]);
-        }
-        for (int64_t i = whole + threadIdx.x; i < end; i += nt) take<INF>(s, (double)in[i]);
-    } else {
+    if (e.strided) {
         const Strided &d = *e.strided;
         for (int64_t i = beg + threadIdx.x; i < end; i += nt) take<INF>(s, (double)in[at(d.cols, i, d.ldi)]);
+        return;
     }
+    double part[4] = {0., 0., 0., 0.};
+    auto add = [&](const u32x4 &v) {
+        const T *x = reinterpret_cast<const T *>(&v);
+#pragma unroll
+        for (int u = 0; u < V; ++u) take<INF>(part[u & 3], (double)x[u]);
+    };
+    const int64_t step = (int64_t)nt * V;
+    int64_t i = beg;
+    for (; i + U * step <= end; i += U * step) {
+        u32x4 v[U];
+#pragma unroll
+        for (int q = 0; q < U; ++q) v[q] = *reinterpret_cast<const u32x4_any *>(in + i + q * step + threadIdx.x * V);
+#pragma unroll
+        for (int q = 0; q < U; ++q) add(v[q]);
+    }
+    for (; i + step <= end; i += step) add(*reinterpret_cast<const u32x4_any *>(in + i + threadIdx.x * V));
+    for (int64_t j = i + threadIdx.x; j < end; j += nt) take<INF>(s, (double)in[j]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) s = both<INF>(s, part[u]);
 }
 
 template <typename T> __device__ __forceinline__ T scaled(T x, double c) {
     if constexpr (sizeof(T) == 8) return x * c;
     else return (T)((float)x * (float)c);
 }
-template <typename T> __device__ __forceinline__ void scale_chunk(const Item &e, int chunk, int nt, double c) {
-    constexpr int V = 16 / sizeof(T), PER = CHUNK_BYTES / sizeof(T);
+template <typename T> __device__ __forceinline__ void scale_span(const Item &e, int64_t beg, int64_t end, int nt, double c) {
+    constexpr int V = 16 / sizeof(T), U = 4;
     const T *in = reinterpret_cast<const T *>(e.in);
     T *out = reinterpret_cast<T *>(e.out);
-    const int64_t beg = (int64_t)(chunk - e.chunk0) * PER, end = min(e.n, beg + PER);
-    if (!e.strided) {
-        const int64_t whole = beg + (end - beg) / V * V;
-        if (end - beg == PER && nt == NT) {
-            u32x4 v[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const u32x4_any *>(in + beg + (int64_t)(q * NT + threadIdx.x) * V);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                T *x = reinterpret_cast<T *>(&v[q]);
-#pragma unroll
-                for (int u = 0; u < V; ++u) x[u] = scaled(x[u], c);
-                *reinterpret_cast<u32x4_any *>(out + beg + (int64_t)(q * NT + threadIdx.x) * V) = v[q];
-            }
-            return;
-        }
-        for (int64_t i = beg + (int64_t)threadIdx.x * V; i < whole; i += nt * V) {
-            u32x4 v = *reinterpret_cast<const u32x4_any *>(in + i);
-            T *x = reinterpret_cast<T *>(&v);
-#pragma unroll
-            for (int u = 0; u < V; ++u) x[u] = scaled(x[u], c);
-            *reinterpret_cast<u32x4_any *>(out + i) = v;
-        }
-        for (int64_t i = whole + threadIdx.x; i < end; i += nt) out[i] = scaled(in[i], c);
-    } else {
+    if (e.strided) {
         const Strided &d = *e.strided;
         for (int64_t i = beg + threadIdx.x; i < end; i += nt) out[at(d.cols, i, d.ldo)] = scaled(in[at(d.cols, i, d.ldi)], c);
+        return;
     }
+    auto put = [&](u32x4 v, int64_t i) {
+        T *x = reinterpret_cast<T *>(&v);
+#pragma unroll
+        for (int u = 0; u < V; ++u) x[u] = scaled(x[u], c);
+        *reinterpret_cast<u32x4_any *>(out + i) = v;
+    };
+    const int64_t step = (int64_t)nt * V;
+    int64_t i = beg;
+    for (; i + U * step <= end; i += U * step) {
+        u32x4 v[U];
+#pragma unroll
+        for (int q = 0; q < U; ++q) v[q] = *reinterpret_cast<const u32x4_any *>(in + i + q * step + threadIdx.x * V);
+#pragma unroll
+        for (int q = 0; q < U; ++q) put(v[q], i + q * step + threadIdx.x * V);
+    }
+    for (; i + step <= end; i += step) put(*reinterpret_cast<const u32x4_any *>(in + i + threadIdx.x * V), i + threadIdx.x * V);
+    for (int64_t j = i + threadIdx.x; j < end; j += nt) out[j] = scaled(in[j], c);
 }
 
-template <int INF, typename Tab> __device__ __forceinline__ void sum_any(const Tab &t, int chunk, int nt, double &s) {
-    const Item e = item_of(t, chunk);
-    switch (e.dtype) {
-        case NMFX_F32: sum_chunk<float, INF>(e, chunk, nt, s); break;
-        case NMFX_F64: sum_chunk<double, INF>(e, chunk, nt, s); break;
-        case NMFX_BF16: sum_chunk<__bf16, INF>(e, chunk, nt, s); break;
-        default: sum_chunk<_Float16, INF>(e, chunk, nt, s); break;
+// calls f(entry, first, last element) for the pieces of chunks c .. last - 1, entry by entry
+template <typename Tab, typename F> __device__ __forceinline__ void spans(const Tab &t, int c, int last, F &&f) {
+    while (c < last) {
+        const Item e = item_of(t, c);
+        const int upto = min(last, e.next), per = CHUNK_BYTES / (e.dtype == NMFX_F64 ? 8 : e.dtype == NMFX_F32 ? 4 : 2);
+        f(e, (int64_t)(c - e.chunk0) * per, min(e.n, (int64_t)(upto - e.chunk0) * per));
+        c = upto;
     }
 }
-template <typename Tab> __device__ __forceinline__ void scale_any(const Tab &t, int chunk, int nt, double c) {
-    const Item e = item_of(t, chunk);
-    switch (e.dtype) {
-        case NMFX_F32: scale_chunk<float>(e, chunk, nt, c); break;
-        case NMFX_F64: scale_chunk<double>(e, chunk, nt, c); break;
-        case NMFX_BF16: scale_chunk<__bf16>(e, chunk, nt, c); break;
-        default: scale_chunk<_Float16>(e, chunk, nt, c); break;
-    }
+template <int INF, typename Tab> __device__ __forceinline__ void sum_chunks(const Tab &t, int c, int last, int nt, double &s) {
+    spans(t, c, last, [&](const Item &e, int64_t beg, int64_t end) {
+        switch (e.dtype) {
+            case NMFX_F32: sum_span<float, INF>(e, beg, end, nt, s); break;
+            case NMFX_F64: sum_span<double, INF>(e, beg, end, nt, s); break;
+            case NMFX_BF16: sum_span<__bf16, INF>(e, beg, end, nt, s); break;
+            default: sum_span<_Float16, INF>(e, beg, end, nt, s); break;
+        }
+    });
+}
+template <typename Tab> __device__ __forceinline__ void scale_chunks(const Tab &t, int c, int last, int nt, double coef) {
+    spans(t, c, last, [&](const Item &e, int64_t beg, int64_t end) {
+        switch (e.dtype) {
+            case NMFX_F32: scale_span<float>(e, beg, end, nt, coef); break;
+            case NMFX_F64: scale_span<double>(e, beg, end, nt, coef); break;
+            case NMFX_BF16: scale_span<__bf16>(e, beg, end, nt, coef); break;
+            default: scale_span<_Float16>(e, beg, end, nt, coef); break;
+        }
+    });
 }
 template <int INF> __device__ __forceinline__ double norm_of(double s) { return INF ? s : sqrt(s); }
 __device__ __forceinline__ double coef_of(double norm, double max_norm) {
@@ -195,7 +201,8 @@ __device__ __forceinline__ double coef_of(double norm, double max_norm) {
 template <int INF, typename Tab> __global__ __launch_bounds__(NT) void partial_kernel(Tab t, double *part) {
     __shared__ double sh[NT / 64];
     double s = 0.;
-    for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) sum_any<INF, Tab>(t, c, NT, s);
+    // neighbouring chunks: an entry is looked up once for all of its chunks that the block has
+    sum_chunks<INF>(t, (int)((int64_t)t.chunks * blockIdx.x / gridDim.x), (int)((int64_t)t.chunks * (blockIdx.x + 1) / gridDim.x), NT, s);
     s = block_total<INF>(s, sh, NT);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
@@ -213,23 +220,24 @@ template <int INF, typename Tab> __global__ __launch_bounds__(NT) void scale_ker
     const double nrm = norm_of<INF>(block_total<INF>(s, sh, NT)), c = coef_of(nrm, max_norm);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)nrm;
     if (c == 1. && in_place) return;
-    for (int k = t.chunks - 1 - blockIdx.x; k >= 0; k -= gridDim.x) scale_any(t, k, NT, c);
+    const int b = gridDim.x - 1 - blockIdx.x;
+    scale_chunks(t, (int)((int64_t)t.chunks * b / gridDim.x), (int)((int64_t)t.chunks * (b + 1) / gridDim.x), NT, c);
 }
 // a short list: one block does all
 template <int INF> __global__ __launch_bounds__(1024) void small_kernel(Short t, double max_norm, int in_place, int clip, float *norm) {
     __shared__ double sh[16];
     double s = 0.;
-    for (int c = 0; c < t.chunks; ++c) sum_any<INF, Short>(t, c, 1024, s);
+    sum_chunks<INF>(t, 0, t.chunks, 1024, s);
     const double nrm = norm_of<INF>(block_total<INF>(s, sh, 1024));
     if (threadIdx.x == 0) *norm = (float)nrm;
     if (!clip) return;
     const double c = coef_of(nrm, max_norm);
     if (c == 1. && in_place) return;
-    for (int k = 0; k < t.chunks; ++k) scale_any(t, k, 1024, c);
+    scale_chunks(t, 0, t.chunks, 1024, c);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
-constexpr int64_t SMALL_CHUNKS = 2;
+constexpr int64_t SMALL_CHUNKS = 4;
 
 struct View {           // a matrix as rows of contiguous elements
     char *p;
@@ -276,7 +284,8 @@ bool any_meet(const std::vector<View> &v) {
 }
 
 int64_t chunks_of(const View &v) { return (v.rows * v.len * v.es + CHUNK_BYTES - 1) / CHUNK_BYTES; }
-int64_t workspace_of(int64_t count) { return 8 * (BLOCKS + count / 2 + 64); }    // (a table of the short form takes 2 strided entries)
+// a table is full with 16 strided entries at the earliest (of the short form: 2)
+int64_t workspace_of(int64_t count) { return 8ll * SUM_BLOCKS * (count / Long::S + 5); }
 
 struct Work {
     const std::vector<View> &in, &out;
@@ -323,9 +332,9 @@ template <int INF, typename Tab> void launch(const Work &w) {
             return;
         }
     int parts = 0;
-    ops::require((int64_t)(BLOCKS + ts.size()) * 8 <= workspace_of((int64_t)w.in.size()), NMFX_ERR_STATE, "partial sums exceed the workspace");
+    ops::require((int64_t)(SUM_BLOCKS * ts.size()) * 8 <= workspace_of((int64_t)w.in.size()), NMFX_ERR_STATE, "partial sums exceed the workspace");
     for (const Tab &t : ts) {
-        const int blocks = (int)std::min<int64_t>(t.chunks, std::max<int64_t>(1, (int64_t)BLOCKS * t.chunks / chunks));
+        const int blocks = std::min(t.chunks, SUM_BLOCKS);
         partial_kernel<INF, Tab><<<blocks, NT, 0, w.st>>>(t, w.part + parts);
         ops::hip_ok(hipGetLastError(), "gradient norm");
         parts += blocks;
@@ -336,7 +345,7 @@ template <int INF, typename Tab> void launch(const Work &w) {
         return;
     }
     for (size_t i = ts.size(); i-- > 0;) {
-        scale_kernel<INF, Tab><<<(int)std::min<int64_t>(ts[i].chunks, BLOCKS), NT, 0, w.st>>>(ts[i], w.part, parts, w.max_norm, w.in_place, i == 0 ? w.norm : nullptr);
+        scale_kernel<INF, Tab><<<std::min(ts[i].chunks, SCALE_BLOCKS), NT, 0, w.st>>>(ts[i], w.part, parts, w.max_norm, w.in_place, i == 0 ? w.norm : nullptr);
         ops::hip_ok(hipGetLastError(), "gradient scaling");
     }
 }

@@ -402,6 +402,16 @@ def test_norm_range():
     for value in (1e30, 1e-30):
         t = torch.full((5000,), value, device=DEV)
         assert abs(float(nmfx.grad_norm([t])) / (value * math.sqrt(5000)) - 1) < 1e-6
+    for value in (1e30, 1e-30, 1e-18, 2e19, 3e38):        # bf16, in whole groups and beside others
+        t = torch.full((50001,), value, device=DEV).bfloat16()
+        norm = float(t[0].double()) * math.sqrt(50001)
+        got = float(nmfx.grad_norm([t]))
+        assert abs(got / norm - 1) < 1e-6 if norm < 3e38 else math.isinf(got)
+        t[::7] = 0
+        assert abs(float(nmfx.grad_norm([t])) / (float(t[1].double()) * math.sqrt(50001 - 7143)) - 1) < 1e-6 or norm > 1e38
+    for value in (65504.0, 2.0 ** -24):
+        t = torch.full((50001,), value, device=DEV).half()
+        assert abs(float(nmfx.grad_norm([t])) / (value * math.sqrt(50001)) - 1) < 1e-6
     t = torch.full((3,), 3e38, device=DEV)
     nmfx.clip_grad_norm([t], 1.0)
     assert abs(float(t[0]) * math.sqrt(3) - 1) < 1e-6          # the norm is beyond Float32, the coefficient is not
