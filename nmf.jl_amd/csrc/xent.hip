@@ -490,6 +490,152 @@ __global__ __launch_bounds__(256) void combine_kernel(Combine c, int lc, int add
     reduce_losses<256>(c.loss_c, cnt, c.reduction, c.loss);
 }
 
+// ---- a few columns (scoring tokens): one pass over W, two launches -----------------------------------------------------------------------
+// Up to 16 columns are the 16 columns of a matrix instruction.  H is in LDS, each wave streams 16 rows of W at a time from memory into the
+// other operand's registers (no LDS: nobody else reads them) and keeps the running statistics of its rows; ignored columns stay, as zeros.
+// Bound by reading W: 200 MB (100003 x 1000, f16) in 38 us, 5.2 TB/s.
+struct Score {
+    const void *w, *h;
+    int64_t ldw, hrs, hcs;    // bytes between rows of W; elements between components and columns of H
+    const int64_t *labels;
+    int64_t ignore;
+    int p, n, k, steps, per;  // steps: of 4 chunks; per: groups of 16 rows of a wave
+    float2 *part;             // [block][16]
+    float *zsum, *zy;         // [block][16] or NULL; [16]
+};
+template <typename T> __global__ __launch_bounds__(512) void score_kernel(Score a) {
+#ifdef __HIP_DEVICE_COMPILE__
+    extern __shared__ __attribute__((aligned(16))) char hs[];        // [steps][4 chunks][16 columns] of 16 bytes
+    __shared__ float2 ps[8][16];
+    __shared__ float zs[8][16];
+    constexpr int PER = 16 / sizeof(T), U = 8;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, hi = lane >> 4;
+    const int chunks = a.k / PER, groups = (a.p + 15) / 16, parts = (a.steps + U - 1) / U;
+    // a wave's work: groups of 16 rows, each in parts of U steps; a part's loads go out before the products of the part in front of it
+    int g = (blockIdx.x * 8 + wave) * a.per, q = 0;
+    const int last = min(groups, g + a.per);
+    tn::u32x4 f[2][U];
+    auto fetch = [&](int set, int gg, int qq) {
+        const char *src = static_cast<const char *>(a.w) + (int64_t)min(gg * 16 + col, a.p - 1) * a.ldw + hi * 16;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            f[set][u] = tn::u32x4{0, 0, 0, 0};
+            if ((qq * U + u) * 4 + hi < chunks) f[set][u] = *reinterpret_cast<const tn::u32x4 *>(src + (qq * U + u) * 64);
+        }
+    };
+    if (g < last) fetch(0, g, 0);
+    const int64_t lab = col < a.n ? a.labels[col] : a.ignore;
+    for (int e = tid; e < a.steps * 64; e += 512) {                  // (e & 15 is col)
+        const int chunk = e >> 4;
+        tn::u32x4 v = {0, 0, 0, 0};
+        T *x = reinterpret_cast<T *>(&v);
+        if (lab != a.ignore) {
+            const T *src = static_cast<const T *>(a.h) + col * a.hcs + (int64_t)chunk * PER * a.hrs;
+            if (a.hrs == 1 && chunk < chunks) v = *reinterpret_cast<const u32x4_any *>(src);
+            else
+#pragma unroll
+                for (int u = 0; u < PER; ++u)
+                    if (chunk * PER + u < a.k) x[u] = src[u * a.hrs];
+        }
+        *reinterpret_cast<tn::u32x4 *>(hs + e * 16) = v;
+    }
+    __syncthreads();
+    float ref = -__builtin_inff(), sum = 0.f, zsum = 0.f;
+    f32x4 z = {0.f, 0.f, 0.f, 0.f};
+    auto work = [&](int set) {
+        const int gn = q + 1 < parts ? g : g + 1, qn = q + 1 < parts ? q + 1 : 0;
+        if (gn < last) fetch(set ^ 1, gn, qn);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (q * U + u < a.steps) {
+                const tn::u32x4 b = *reinterpret_cast<const tn::u32x4 *>(hs + ((q * U + u) * 64 + lane) * 16);
+#pragma unroll
+                for (int e = 0; e < tn::Elem<T>::PARTS; ++e) z = tn::Elem<T>::mma(f[set][u], b, z, e);
+            }
+        if (qn == 0) {                                               // the group is done
+            float mx = -__builtin_inff();
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int v = g * 16 + 4 * hi + r;
+                if (v >= a.p) z[r] = -__builtin_inff();
+                else if (a.zsum) zsum += z[r];
+                if (v == lab) a.zy[col] = z[r];
+                mx = fmaxf(mx, z[r]);
+            }
+            mx *= LOG2E;
+            if (mx > ref) {
+                sum *= sum != 0.f ? exp2_(ref - mx) : 0.f;
+                ref = mx;
+            }
+            const float at = ref == -__builtin_inff() ? 0.f : ref;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum += exp2_(__builtin_fmaf(z[r], LOG2E, -at));
+            z = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        g = gn;
+        q = qn;
+    };
+    while (g < last) {
+        work(0);
+        if (g < last) work(1);
+    }
+    float2 s = make_float2(ref, sum);
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1) {
+        s = join(s, make_float2(__shfl_xor(s.x, o), __shfl_xor(s.y, o)));
+        zsum += __shfl_xor(zsum, o);
+    }
+    if (lane < 16) { ps[wave][lane] = s; zs[wave][lane] = zsum; }
+    __syncthreads();
+    if (tid < 16) {
+#pragma unroll
+        for (int w = 1; w < 8; ++w) { s = join(s, ps[w][tid]); zsum += zs[w][tid]; }
+        a.part[blockIdx.x * 16 + tid] = s;
+        if (a.zsum) a.zsum[blockIdx.x * 16 + tid] = zsum;
+    }
+#endif
+}
+// one block, a wave a column
+__global__ __launch_bounds__(1024) void score_join_kernel(Score a, int blocks, float eps, int reduction, float *lse, float *loss) {
+    __shared__ float ls[16];
+    __shared__ int on[16];
+    const int col = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t lab = col < a.n ? a.labels[col] : a.ignore;
+    float2 s = make_float2(-__builtin_inff(), 0.f);
+    float t = 0.f;
+#pragma unroll 4
+    for (int b = lane; b < blocks; b += 64) {
+        s = join(s, a.part[b * 16 + col]);
+        if (a.zsum) t += a.zsum[b * 16 + col];
+    }
+    for (int o = 32; o; o >>= 1) {
+        s = join(s, make_float2(__shfl_xor(s.x, o), __shfl_xor(s.y, o)));
+        t += __shfl_xor(t, o);
+    }
+    if (lane == 0) {
+        float v = 0.f, l = 0.f;
+        if (lab != a.ignore) {
+            const bool bad = lab < 0 || lab >= a.p;
+            v = bad ? __builtin_nanf("") : (s.x + log2f(s.y)) * LN2;
+            l = v - (1.f - eps) * (bad ? 0.f : a.zy[col]);
+            if (a.zsum) l -= eps * (t / (float)a.p);
+        }
+        if (col < a.n) {
+            if (lse) lse[col] = v;
+            if (reduction == NMFX_REDUCE_NONE) loss[col] = l;
+        }
+        ls[col] = l;
+        on[col] = lab != a.ignore;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && reduction != NMFX_REDUCE_NONE) {
+        double sum = 0.;
+        int cnt = 0;
+        for (int c = 0; c < 16; ++c) { sum += (double)ls[c]; cnt += on[c]; }
+        *loss = (float)(reduction == NMFX_REDUCE_MEAN ? sum / (double)max(cnt, 1) : sum);
+    }
+}
+
 // ---- dz of a piece of the classes, in both orders -----------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ T to(float x) { return (T)x; }
 
@@ -787,9 +933,9 @@ Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     s.o_idx = take(s.npad * 4); s.o_pos = take(s.npad * 4); s.o_y = take(s.npad * 4);
     s.o_f = take(s.npad * 4); s.o_lse = take(s.npad * 4); s.o_loss = take(s.npad * 4); s.o_zy = take(s.npad * 4);
     s.o_h = take(s.npad * s.kpad * s.es);
-    const int64_t tiles = (s.p + KINDS[s.z.kind].m - 1) / KINDS[s.z.kind].m;
-    s.o_part = take(tiles * s.npad * sizeof(float2));
-    s.o_zsum = smooth ? take(tiles * s.npad * 4) : -1;
+    const int64_t tiles = (s.p + KINDS[s.z.kind].m - 1) / KINDS[s.z.kind].m, parts = std::max<int64_t>(tiles * s.npad, 16 * 4 * CUS);
+    s.o_part = take(parts * sizeof(float2));
+    s.o_zsum = smooth ? take(parts * 4) : -1;
     s.o_w = s.w_rows_direct ? -1 : take(s.p * s.kpad * s.es);
     s.o_ht = s.o_wt = s.o_dz = s.o_dzt = s.o_hslot = s.o_wslot = -1;
     if (grad) {
@@ -850,7 +996,22 @@ struct Call {
     hipStream_t st;
 };
 
+// The short way: few columns, W in an order and alignment that a wave can load fragments from, H small enough for LDS.
+constexpr int SCORE_LDS = 65536;
+inline bool scored(const Shape &s) { return s.n > 0 && s.n <= 16 && s.w_rows_direct && up(s.k * s.es, 64) * 16 <= SCORE_LDS; }
+template <typename T> void score(const Call &c, const Shape &s) {
+    // one round of blocks, 2 a compute unit (16 waves of up to 16 loads each), with the same number of groups for every wave
+    const int steps = (int)(up(s.k * s.es, 64) / 64), groups = (int)((s.p + 15) / 16), per = (groups + 16 * CUS - 1) / (16 * CUS), blocks = (groups + 8 * per - 1) / (8 * per);
+    Score a{c.W.data, c.H.data, s.wrs * s.es, c.H.rs, c.H.cs, c.labels, c.o.ignore_index, (int)s.p, (int)s.n, (int)s.k, steps, per, reinterpret_cast<float2 *>(c.ws + s.o_part),
+            s.o_zsum >= 0 ? reinterpret_cast<float *>(c.ws + s.o_zsum) : nullptr, reinterpret_cast<float *>(c.ws + s.o_zy)};
+    score_kernel<T><<<blocks, 512, steps * 1024, c.st>>>(a);
+    ops::hip_ok(hipGetLastError(), "score");
+    score_join_kernel<<<1, 1024, 0, c.st>>>(a, blocks, (float)c.o.label_smoothing, c.o.reduction, c.lse, c.loss);
+    ops::hip_ok(hipGetLastError(), "score");
+}
+
 template <typename T> void run(const Call &c, const Shape &s) {
+    if (!c.grad && scored(s)) return score<T>(c, s);
     const int es = sizeof(T), step = 128 / es, per = 16 / es;
     char *ws = c.ws;
     auto f32 = [&](int64_t o) { return reinterpret_cast<float *>(ws + o); };
