@@ -319,17 +319,21 @@ __global__ __launch_bounds__(WM *WN * 64) void tn_kernel(Args g, Epi epi) {
 #endif
 }
 
-// two products in one launch: the first `first` blocks are one's, the others the other's
-template <typename T, int BM, int BN, int WM, int WN, int ST, typename EpiA, typename EpiB>
-__global__ __launch_bounds__(WM *WN * 64) void tn_pair_kernel(Args ga, EpiA ea, Args gb, EpiB eb, int first) {
+// two products in one launch: the first `first` blocks are one's, those up to `last` the other's; a block behind them runs `more`
+template <typename T, int BM, int BN, int WM, int WN, int ST, typename EpiA, typename EpiB, typename More>
+__global__ __launch_bounds__(WM *WN * 64) void tn_pair_kernel(Args ga, EpiA ea, Args gb, EpiB eb, int first, int last, More more) {
 #ifdef __HIP_DEVICE_COMPILE__
+    if ((int)blockIdx.x >= last) {
+        more.template run<WM * WN * 64>();
+        return;
+    }
     NMFX_TN_STAGES(BM, BN, ST)
     None none;
     f32x4 acc[BM / WM / 16][BN / WN / 16];
     Geom geo;
     const bool is_a = (int)blockIdx.x < first;
     const Args g = is_a ? ga : gb;
-    if (!tile<T, BM, BN, WM, WN, ST>(g, place_of(g, blockIdx.x - (is_a ? 0 : first), is_a ? first : gridDim.x - first), st, acc, geo, [](const Geom &) {})) return;
+    if (!tile<T, BM, BN, WM, WN, ST>(g, place_of(g, blockIdx.x - (is_a ? 0 : first), is_a ? first : last - first), st, acc, geo, [](const Geom &) {})) return;
     if (is_a) ea.template finish<BM, BN, WM, WN>(acc, geo, none, none, st0, st1);
     else eb.template finish<BM, BN, WM, WN>(acc, geo, none, none, st0, st1);
 #endif

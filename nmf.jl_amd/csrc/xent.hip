@@ -287,13 +287,25 @@ template <typename T> __device__ __forceinline__ void pack_tile(const Pack<T> &a
 // ONE_ROUND columns every block of H finds its 64 packed columns for itself (a round of 256 threads with 8 labels each: less than a launch),
 // and the last block leaves the lists; above, select_kernel has made them.
 constexpr int ONE_ROUND = 2048;
-template <typename T> __global__ __launch_bounds__(256) void prepare_kernel(Select s, Pack<T> h, Pack<T> w) {
+template <typename T> struct Blank {           // zero in the ignored columns of a matrix with contiguous columns
+    T *out;
+    int64_t ld;
+    int k, blocks;            // of 64 columns each
+    __device__ __forceinline__ void run(const Select &s, int b) const {
+        const int lane = threadIdx.x & 63;
+        for (int t = b * 64 + (threadIdx.x >> 6); t < min(s.n, b * 64 + 64); t += 4)
+            if (s.labels[t] == s.ignore)
+                for (int c = lane; c < k; c += 64) out[t * ld + c] = (T)0.f;
+    }
+};
+template <typename T> __global__ __launch_bounds__(256) void prepare_kernel(Select s, Pack<T> h, Pack<T> w, Blank<T> z) {
     __shared__ __attribute__((aligned(16))) char tile[sizeof(T) == 2 ? 64 * 128 : 64 * 65 * 4];
     __shared__ int from[64];
     int b = blockIdx.x;
     if (b >= h.tiles) {
         b -= h.tiles;
         if (b < w.tiles) pack_tile<T>(w, tile, nullptr, w.rows, (b % w.tiles_r) * 64, (b / w.tiles_r) * 64);
+        else if (b < w.tiles + z.blocks) z.run(s, b - w.tiles);
         else select_columns<256>(s, 0);
         return;
     }
@@ -457,6 +469,14 @@ template <int NT> __device__ __forceinline__ void reduce_losses(const float *los
         *loss = (float)(reduction == NMFX_REDUCE_MEAN ? s / (double)max(cnt, 1) : s);
     }
 }
+
+struct Losses {          // as a block of another launch
+    const float *loss_c;
+    const Info *info;
+    int reduction;
+    float *loss;              // NULL: not wanted
+    template <int NT> __device__ __forceinline__ void run() const { reduce_losses<NT>(loss_c, info->count, reduction, loss); }
+};
 
 // 256 threads share 2^lc packed columns; the block that is done last adds up the losses
 __global__ __launch_bounds__(256) void combine_kernel(Combine c, int lc, int add) {
@@ -787,6 +807,7 @@ template <typename T> struct EpiOut {
     int64_t ld;
     const Info *info;
     int mmax, nmax, wide;     // wide: four consecutive m go in one store
+    const int *cols, *count;  // column n goes to column cols[n], for n < *count; or NULL
     template <int MI, int NJ> using Early = tn::None;
     template <int BM, int BN, int WM, int WN> using Shared = tn::None;
     template <int BM, int BN, int WM, int WN> __device__ __forceinline__ void begin(const Geom &, tn::None &, tn::None &) const {}
@@ -796,8 +817,9 @@ template <typename T> struct EpiOut {
         const float u = info->unscale;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const int n = g.n0 + 16 * j;
-            if (n >= nmax) continue;
+            int n = g.n0 + 16 * j;
+            if (n >= (cols ? *count : nmax)) continue;
+            if (cols) n = cols[n];
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 const int m = g.m0 + 16 * i;
@@ -869,7 +891,7 @@ struct Shape {
     int64_t piece, pieces;        // classes of a piece (a multiple of 256)
     int64_t ldslot;
     Choice z, h, w;               // the products Z, W' dz, dz H'
-    bool w_slots;
+    bool w_slots, direct;         // direct: dH need not be summed from slots
     // workspace offsets
     int64_t o_info, o_counts, o_idx, o_pos, o_y, o_f, o_lse, o_loss, o_zy, o_h, o_ht, o_w, o_wt, o_part, o_zsum, o_dz, o_dzt, o_hslot, o_wslot, bytes;
 };
@@ -883,23 +905,43 @@ constexpr int CUS = 256;
 struct TileKind { int m, n, cap; double lat16, mat16, lat32, mat32; };
 constexpr TileKind KINDS[3] = {{256, 256, 1, 1.2, 1.65, 7.6, 7.8}, {128, 128, 2, 0.75, 0.52, 2.0, 2.15}, {64, 64, 2, 0.35, 0.23, 0.67, 0.6}};
 
-// the kind and number of splits with the least estimated time; a split adds a slot of m x n floats, written and read
-Choice choose(int64_t m, int64_t n, int64_t ktiles, int es, bool split) {
-    Choice best{2, 1};
-    double least = 1e30;
-    for (int k = 0; k < 3; ++k) {
-        const TileKind &t = KINDS[k];
-        const double lat = es == 2 ? t.lat16 : t.lat32, mat = es == 2 ? t.mat16 : t.mat32;
-        const int64_t tiles = ((m + t.m - 1) / t.m) * ((n + t.n - 1) / t.n);
-        const int64_t most = split ? std::min<int64_t>(std::max<int64_t>(1, ktiles / 4), std::max<int64_t>(1, t.cap * CUS / tiles)) : 1;
-        for (int64_t s = 1; s <= most; s = s < most && s * 2 > most ? most : s * 2) {
-            const double kt = (double)((ktiles + s - 1) / s);
-            const int64_t per = (tiles * s + CUS - 1) / CUS;              // blocks of a compute unit
-            const double us = std::max(per * kt * mat, (double)((per + t.cap - 1) / t.cap) * kt * lat) + 2. * (per + t.cap - 1) / t.cap + (s > 1 ? 2. + 8e-6 * s * m * n / 4. : 0.);
-            if (us < least) { least = us; best = Choice{k, (int)s}; }
-        }
+// The least estimated time of a product by tiles of one kind, over the numbers of splits; a split adds a slot of m x n floats, written and
+// read.
+struct Guess { Choice c; double us; };
+Guess guess(int kind, int64_t m, int64_t n, int64_t ktiles, int es, bool split) {
+    const TileKind &t = KINDS[kind];
+    const double lat = es == 2 ? t.lat16 : t.lat32, mat = es == 2 ? t.mat16 : t.mat32;
+    const int64_t tiles = ((m + t.m - 1) / t.m) * ((n + t.n - 1) / t.n);
+    const int64_t most = split ? std::min<int64_t>(std::max<int64_t>(1, ktiles / 4), std::max<int64_t>(1, t.cap * CUS / tiles)) : 1;
+    Guess best{{kind, 1}, 1e30};
+    for (int64_t s = 1; s <= most; s = s < most && s * 2 > most ? most : s * 2) {
+        const double kt = (double)((ktiles + s - 1) / s);
+        const int64_t per = (tiles * s + CUS - 1) / CUS;              // blocks of a compute unit
+        const double us = std::max(per * kt * mat, (double)((per + t.cap - 1) / t.cap) * kt * lat) + 2. * (per + t.cap - 1) / t.cap + (s > 1 ? 2. + 8e-6 * s * m * n / 4. : 0.);
+        if (us < best.us) best = Guess{{kind, (int)s}, us};
     }
     return best;
+}
+Choice choose(int64_t m, int64_t n, int64_t ktiles, int es) {
+    Guess best{{2, 1}, 1e30};
+    for (int k = 0; k < 3; ++k) {
+        const Guess g = guess(k, m, n, ktiles, es, false);
+        if (g.us < best.us) best = g;
+    }
+    return best.c;
+}
+// The two gradient products: each by the kind that suits it, or both by one kind in one launch; and, where neither is split, without the
+// launch that joins the slots (dH then goes straight to its columns).  A launch costs about LAUNCH us, the host's part or the gap it leaves.
+constexpr double LAUNCH = 4.;
+void choose_two(int64_t hm, int64_t hn, int64_t hk, int64_t wm, int64_t wn, int64_t wk, int es, bool direct, Choice &h, Choice &w) {
+    double least = 1e30;
+    auto take = [&](const Guess &a, const Guess &b, double more) {
+        if (a.us + b.us + more < least) { least = a.us + b.us + more; h = a.c; w = b.c; }
+    };
+    for (int k = 0; k < 3; ++k) {
+        for (int l = 0; l < 3; ++l) take(guess(k, hm, hn, hk, es, true), guess(l, wm, wn, wk, es, true), k == l ? LAUNCH - 2. : 2. * LAUNCH);
+        if (direct) take(guess(k, hm, hn, hk, es, false), guess(k, wm, wn, wk, es, false), -2.);
+    }
 }
 
 Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
@@ -922,9 +964,10 @@ Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     s.ldslot = up(s.k, 4);
     s.ldn = s.npad + 256 / s.es; s.ldp = s.ppad + 256 / s.es; s.ldc = s.piece + 256 / s.es;
     const int64_t n1 = std::max<int64_t>(s.n, 1);
-    s.z = choose(std::min(s.piece, s.p), n1, s.kpad / step, s.es, false);
-    s.h = choose(s.k, n1, (std::min(s.piece, s.p) + step - 1) / step, s.es, true);
-    s.w = choose(std::min(s.piece, s.p), s.k, (n1 + step - 1) / step, s.es, true);
+    const int64_t pp = std::min(s.piece, s.p);
+    s.z = choose(pp, n1, s.kpad / step, s.es);
+    choose_two(s.k, n1, (pp + step - 1) / step, pp, s.k, (n1 + step - 1) / step, s.es, s.pieces == 1, s.h, s.w);
+    s.direct = s.pieces == 1 && s.h.splits == 1 && s.w.splits == 1 && s.h.kind == s.w.kind;
     s.w_slots = s.w.splits > 1;
     int64_t at = 0;
     auto take = [&](int64_t b) { const int64_t o = at; at = up(at + b, 256); return o; };
@@ -968,7 +1011,7 @@ template <typename T, typename Epi> void product(tn::Args a, int64_t m, int64_t 
 }
 // two products at once where they go by the same kind of tile
 template <typename T, typename EA, typename EB>
-void products(tn::Args a, int64_t ma, int64_t na, const Choice &ca, const EA &ea, tn::Args b, int64_t mb, int64_t nb, const Choice &cb, const EB &eb, hipStream_t st) {
+void products(tn::Args a, int64_t ma, int64_t na, const Choice &ca, const EA &ea, tn::Args b, int64_t mb, int64_t nb, const Choice &cb, const EB &eb, const Losses &more, hipStream_t st) {
     if (ca.kind != cb.kind) {
         product<T>(a, ma, na, ca, ea, st);
         product<T>(b, mb, nb, cb, eb, st);
@@ -976,11 +1019,11 @@ void products(tn::Args a, int64_t ma, int64_t na, const Choice &ca, const EA &ea
     }
     grid(a, ma, na, ca);
     grid(b, mb, nb, cb);
-    const int first = blocks_of(a), all = first + blocks_of(b);
+    const int first = blocks_of(a), last = first + blocks_of(b), all = last + (more.loss != nullptr);
     switch (ca.kind) {
-        case 0: tn::tn_pair_kernel<T, 256, 256, 2, 4, 2, EA, EB><<<all, 512, 0, st>>>(a, ea, b, eb, first); break;
-        case 1: tn::tn_pair_kernel<T, 128, 128, 2, 2, 2, EA, EB><<<all, 256, 0, st>>>(a, ea, b, eb, first); break;
-        default: tn::tn_pair_kernel<T, 64, 64, 2, 2, 4, EA, EB><<<all, 256, 0, st>>>(a, ea, b, eb, first); break;
+        case 0: tn::tn_pair_kernel<T, 256, 256, 2, 4, 2, EA, EB, Losses><<<all, 512, 0, st>>>(a, ea, b, eb, first, last, more); break;
+        case 1: tn::tn_pair_kernel<T, 128, 128, 2, 2, 2, EA, EB, Losses><<<all, 256, 0, st>>>(a, ea, b, eb, first, last, more); break;
+        default: tn::tn_pair_kernel<T, 64, 64, 2, 2, 4, EA, EB, Losses><<<all, 256, 0, st>>>(a, ea, b, eb, first, last, more); break;
     }
     ops::hip_ok(hipGetLastError(), "products");
 }
@@ -1039,7 +1082,9 @@ template <typename T> void run(const Call &c, const Shape &s) {
     const int ct = (int)(s.kpad / 64 + (s.kpad % 64 != 0)), wr = pw || pwt ? (int)(s.ppad / 64) : 0;
     Pack<T> ph{static_cast<const T *>(c.H.data), c.H.cs, c.H.rs, n, k, h, ht, s.kpad, s.ldn, (int)s.npad, (int)s.npad, (int)s.kpad, (int)(s.npad / 64), (int)(s.npad / 64) * ct};
     Pack<T> pk{w, s.wrs, s.wcs, p, k, pw, pwt, s.kpad, s.ldp, p, (int)s.ppad, (int)s.kpad, wr, wr * ct};
-    prepare_kernel<T><<<ph.tiles + pk.tiles + (n <= ONE_ROUND), 256, 0, c.st>>>(sel, ph, pk);
+    const bool direct = c.grad && s.direct && c.dH.rs == 1;
+    const Blank<T> blank{static_cast<T *>(c.dH.data), c.dH.cs, k, direct ? (n + 63) / 64 : 0};
+    prepare_kernel<T><<<ph.tiles + pk.tiles + blank.blocks + (n <= ONE_ROUND), 256, 0, c.st>>>(sel, ph, pk, blank);
     ops::hip_ok(hipGetLastError(), "prepare");
     int64_t ldw = s.wrs, ldwt = s.wcs;
     int wchunks = (int)(s.k / per), wtpad = p;
@@ -1087,14 +1132,18 @@ template <typename T> void run(const Call &c, const Shape &s) {
         const int mm = kfast ? k : pv, nn = kfast ? pv : k;
         tn::Args d{kfast ? top : zop, kfast ? zop : top, count, tn::LIMIT_C, 0, 0, 0, (int)(s.npad / step)};
         Join<T> jh{}, jw{};
+        const bool wide = ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * es - 1)) == 0;
+        const EpiOut<T> ew{out, ldo, info, mm, nn, wide, nullptr, nullptr};
+        if (direct) {
+            const bool hwide = c.dH.cs % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & (4 * es - 1)) == 0;
+            products<T>(b, k, n1, s.h, EpiOut<T>{dh, c.dH.cs, info, k, n, hwide, i32(s.o_idx), count}, d, mm, nn, s.w, ew, Losses{f32(s.o_loss), info, c.o.reduction, add ? c.loss : nullptr}, c.st);
+            return;
+        }
         if (s.w_slots) {
             const int64_t ld = up(mm, 4);
-            products<T>(b, k, n1, s.h, eh, d, mm, nn, s.w, EpiSlot{f32(s.o_wslot), ld, ld * nn, nn, 0}, c.st);
+            products<T>(b, k, n1, s.h, eh, d, mm, nn, s.w, EpiSlot{f32(s.o_wslot), ld, ld * nn, nn, 0}, Losses{}, c.st);
             jw = Join<T>{f32(s.o_wslot), ld, ld * nn, s.w.splits, nullptr, mm, nn, out, 1, ldo, join_blocks(mm, nn)};
-        } else {
-            const bool wide = ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * es - 1)) == 0;
-            products<T>(b, k, n1, s.h, eh, d, mm, nn, s.w, EpiOut<T>{out, ldo, info, mm, nn, wide}, c.st);
-        }
+        } else products<T>(b, k, n1, s.h, eh, d, mm, nn, s.w, ew, Losses{}, c.st);
         if (last && n) jh = Join<T>{f32(s.o_hslot), s.ldslot, s.npad * s.ldslot, s.h.splits, i32(s.o_pos), k, n, dh, c.dH.rs, c.dH.cs, join_blocks(k, n)};
         const int jb = jh.blocks + jw.blocks + (last && add);
         if (jb) {
