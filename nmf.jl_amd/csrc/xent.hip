@@ -712,7 +712,10 @@ template <typename T> struct EpiDz {
         using P = Patch<16 * MI, WM * WN>;
         const int wave = g.tid >> 6;
         char *patch = P::of(st0, st1, wave, 16 * NJ);
-        // (edge: some of the tile's rows or columns do not exist, and have a zero dz)
+        // edge: some of the tile's rows or columns do not exist, and have a zero dz.  Of the columns that do not exist dz is never looked at,
+        // dzt up to where the tiles of its contraction end.
+        constexpr int CT = tn::ROW / (int)sizeof(T);
+        const int ends = (cnt + CT - 1) / CT * CT;
         const bool edge = g.tile_m * BM + BM > p || g.tile_n * BN + BN > cnt;
         auto column = [&](int j, auto at_edge) {
             const int n = g.n0 + 16 * j;
@@ -728,9 +731,10 @@ template <typename T> struct EpiDz {
                 }
                 if constexpr (sizeof(T) == 2) *reinterpret_cast<T4 *>(patch + P::at(16 * j + (g.lane & 15), 2 * i + (g.lane >> 5)) + (g.lane >> 4 & 1) * 8) = o;
                 else {
-                    *reinterpret_cast<T4 *>(dz + (int64_t)n * ldc + g.m0 + 16 * i) = o;
+                    if (!at_edge || n < cnt) *reinterpret_cast<T4 *>(dz + (int64_t)n * ldc + g.m0 + 16 * i) = o;
+                    if (!at_edge || n < ends)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) dzt[(int64_t)(g.m0 + 16 * i + r) * ldn + n] = o[r];
+                        for (int r = 0; r < 4; ++r) dzt[(int64_t)(g.m0 + 16 * i + r) * ldn + n] = o[r];
                 }
             }
             // the label's entry, where it is this lane's: written once more
@@ -762,14 +766,14 @@ template <typename T> struct EpiDz {
 #pragma unroll
             for (int e = 0; e < 16 * NJ * P::SLOTS / 64; ++e) {
                 const int at = e * 64 + g.lane, row = at / P::SLOTS, slot = at % P::SLOTS;
-                *reinterpret_cast<tn::u32x4 *>(dz + (int64_t)(n0 + row) * ldc + m0 + slot * 8) = *reinterpret_cast<const tn::u32x4 *>(patch + P::at(row, slot));
+                if (!edge || n0 + row < cnt) *reinterpret_cast<tn::u32x4 *>(dz + (int64_t)(n0 + row) * ldc + m0 + slot * 8) = *reinterpret_cast<const tn::u32x4 *>(patch + P::at(row, slot));
             }
             const int l = g.lane & 15, rows8 = (g.lane >> 4) * 8;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
                 for (int h = 0; h < NJ / 2; ++h)
-                    *reinterpret_cast<tn::u32x4 *>(dzt + (int64_t)(m0 + 16 * i + l) * ldn + n0 + 32 * h + rows8) = P::transposed(patch, 32 * h + rows8, 16 * i, g.lane);
+                    if (!edge || n0 + 32 * h + rows8 < ends) *reinterpret_cast<tn::u32x4 *>(dzt + (int64_t)(m0 + 16 * i + l) * ldn + n0 + 32 * h + rows8) = P::transposed(patch, 32 * h + rows8, 16 * i, g.lane);
         }
     }
 };
