@@ -83,7 +83,7 @@ typedef __attribute__((address_space(3))) void lds_void;
 __device__ __forceinline__ int swizzle(int row) { return row >> 1 & 7; }
 
 // 16 bytes a lane from rsrc + off into LDS at `lds` (the same for the whole wave) + 16 lane.  Written out, so that the compiler, which cannot
-// tell which stage a load is for, does not wait for all of them in front of a read: the waits are tile()'s own.
+// tell which stage a load is for, does not wait for all of them in front of a read: the waits are walk()'s own.
 __device__ __forceinline__ void to_lds(u32x4 rsrc, char *lds, uint32_t off) {
     const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void *)lds);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(at), "v"(off), "s"(rsrc) : "memory", "m0");
@@ -121,45 +121,34 @@ template <int N> __device__ __forceinline__ void wait_loads() {
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
 }
 
+// Tiles in columns of 8 row tiles, so that those in flight on a die share rows of A and B in its L2.
 struct Place { int tile_m, tile_n, split; };
-__device__ __forceinline__ Place place_of(const Args &g, int bid, int nblk) {
-    // consecutive blocks go to the 8 dies in turn: give every die a contiguous range of tiles, and walk a range in columns of 8 row
-    // tiles, so that the tiles in flight on a die share rows of A and B in its L2
-    {
-        const int die = bid & 7, q = nblk >> 3, rest = nblk & 7;
-        bid = die * q + min(die, rest) + (bid >> 3);
-    }
+__device__ __forceinline__ Place place_at(const Args &g, int id) {
     const int tiles = g.tiles_m * g.tiles_n;
-    const int split = bid / tiles;
-    int in = bid - split * tiles;
+    const int split = id / tiles;
+    int in = id - split * tiles;
     const int per = 8 * g.tiles_n, grp = in / per;
     in -= grp * per;
     const int gm = min(8, g.tiles_m - grp * 8);
     return Place{grp * 8 + in % gm, in / gm, split};
 }
+// consecutive blocks go to the 8 dies in turn: every die gets a contiguous range of tiles
+__device__ __forceinline__ Place place_of(const Args &g, int bid, int nblk) {
+    const int die = bid & 7, q = nblk >> 3, rest = nblk & 7;
+    return place_at(g, die * q + min(die, rest) + (bid >> 3));
+}
 
-// One tile's sums, in acc; false where the tile lies behind the operand's end.  ST: LDS stages.  `meanwhile` runs while the first loads are
-// on their way: in a small product they and what the consumer reads take longer than the products.
-template <typename T, int BM, int BN, int WM, int WN, int ST, typename F>
-__device__ __forceinline__ bool tile(const Args &g, const Place &at, char *const (&st)[ST], f32x4 (&acc)[BM / WM / 16][BN / WN / 16], Geom &geo, F &&meanwhile) {
+// A tile's sums, in acc; then use(acc, where), and on to the tile that next(place) gives, if any, whose first loads go out before use() runs
+// (which then has to leave the stages alone).  Nothing where the tile lies behind the operand's end.  ST: LDS stages.  meanwhile(where) runs
+// while the first loads are on their way: in a small product they and what the consumer reads take longer than the products.
+template <typename T, int BM, int BN, int WM, int WN, int ST, typename Next, typename Mid, typename Use>
+__device__ __forceinline__ void walk(const Args &g, Place at, char *const (&st)[ST], f32x4 (&acc)[BM / WM / 16][BN / WN / 16], Next &&next, Mid &&meanwhile, Use &&use) {
     constexpr int NT = WM * WN * 64, MI = BM / WM / 16, NJ = BN / WN / 16;
-    const int tile_m = at.tile_m, tile_n = at.tile_n, split = at.split;
     int kbeg, kend;
-    // the number of columns is read while loads are on their way, but where it decides what to load
-    if (g.limit == LIMIT_C && g.splits > 1) {
-        const int ktiles = min(g.ktiles, (int)((*g.count * (int64_t)sizeof(T) + ROW - 1) / ROW));
-        kbeg = (int)((int64_t)ktiles * split / g.splits);
-        kend = (int)((int64_t)ktiles * (split + 1) / g.splits);
-    } else {
-        kbeg = (int)((int64_t)g.ktiles * split / g.splits);
-        kend = (int)((int64_t)g.ktiles * (split + 1) / g.splits);
-    }
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave % WM, wn = wave / WM;
     Loader<BM, NT> la;
     Loader<BN, NT> lb;
-    la.init(g.a, tile_m * BM, tid);
-    lb.init(g.b, tile_n * BN, tid);
     constexpr int LA = Loader<BM, NT>::PER, LOADS = LA + Loader<BN, NT>::PER;
 
     // A tile is 2 halves of the contraction (64 bytes: one matrix instruction's), a half MI steps: A's fragment i times all NJ of B's.
@@ -243,53 +232,68 @@ __device__ __forceinline__ bool tile(const Args &g, const Place &at, char *const
         }
     };
     static_assert(MEET >= MI, "the barrier lies in the second half");
-    geo = Geom{tile_m * BM + wm * (BM / WM) + 4 * hi, tile_n * BN + wn * (BN / WN) + (lane & 15), tile_m, tile_n, split, wm, wn, lane, tid};
+    auto aim = [&]() {
+        // the number of columns is read while loads are on their way, but where it decides what to load
+        int ktiles = g.ktiles;
+        if (g.limit == LIMIT_C && g.splits > 1) ktiles = min(ktiles, (int)((*g.count * (int64_t)sizeof(T) + ROW - 1) / ROW));
+        kbeg = (int)((int64_t)ktiles * at.split / g.splits);
+        kend = (int)((int64_t)ktiles * (at.split + 1) / g.splits);
+        la.init(g.a, at.tile_m * BM, tid);
+        lb.init(g.b, at.tile_n * BN, tid);
 #pragma unroll
-    for (int i = 0; i < ST; ++i)
-        if (kbeg + i < kend) {
-            starts(kbeg + i);
+        for (int i = 0; i < ST; ++i)
+            if (kbeg + i < kend) {
+                starts(kbeg + i);
 #pragma unroll
-            for (int l = 0; l < LOADS; ++l)
-                if (i + 1 < ST || place(l) < BEHIND) load(st[i], l);
-        }
+                for (int l = 0; l < LOADS; ++l)
+                    if (i + 1 < ST || place(l) < BEHIND) load(st[i], l);
+            }
+    };
+    aim();
     const int count = g.limit == LIMIT_NONE ? 0 : *g.count;
-    if (g.limit == LIMIT_N && tile_n * BN >= count) {
+    if (g.limit == LIMIT_N && at.tile_n * BN >= count) {
         wait_loads<0>();
-        return false;
+        return;
     }
-    meanwhile(geo);
-    // (loads of tiles behind the end that the count gives are waited for, and not looked at)
-    if (g.limit == LIMIT_C && g.splits == 1) kend = min(kend, (int)((count * (int64_t)sizeof(T) + ROW - 1) / ROW));
+    for (;;) {
+        const Geom geo{at.tile_m * BM + wm * (BM / WM) + 4 * hi, at.tile_n * BN + wn * (BN / WN) + (lane & 15), at.tile_m, at.tile_n, at.split, wm, wn, lane, tid};
+        meanwhile(geo);
+        // (loads of tiles behind the end that the count gives are waited for, and not looked at)
+        if (g.limit == LIMIT_C && g.splits == 1) kend = min(kend, (int)((count * (int64_t)sizeof(T) + ROW - 1) / ROW));
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    if (kbeg < kend) {
-        if (kbeg + ST - 1 < kend) wait_loads<(ST - 1) * LOADS - LATE>();
-        else wait_loads<0>();
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
+        if (kbeg < kend) {
+            if (kbeg + ST - 1 < kend) wait_loads<(ST - 1) * LOADS - LATE>();
+            else wait_loads<0>();
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) read_b(st[0], 0, j);
+            for (int j = 0; j < NJ; ++j) read_b(st[0], 0, j);
 #pragma unroll
-        for (int s = 0; s < D; ++s) read_a(st[0], s);
-        __builtin_amdgcn_sched_barrier(0);
-        int kt = kbeg;
-        for (; kt + 2 * ST <= kend; kt += ST) {
+            for (int s = 0; s < D; ++s) read_a(st[0], s);
+            __builtin_amdgcn_sched_barrier(0);
+            int kt = kbeg;
+            for (; kt + 2 * ST <= kend; kt += ST) {
 #pragma unroll
-            for (int i = 0; i < ST; ++i) run(st[(i + ST - 1) % ST], st[i], st[(i + 1) % ST], kt + i, true);
+                for (int i = 0; i < ST; ++i) run(st[(i + ST - 1) % ST], st[i], st[(i + 1) % ST], kt + i, true);
+            }
+            for (; kt < kend; kt += ST) {
+#pragma unroll
+                for (int i = 0; i < ST; ++i)
+                    if (kt + i < kend) run(st[(i + ST - 1) % ST], st[i], st[(i + 1) % ST], kt + i, false);
+            }
         }
-        for (; kt < kend; kt += ST) {
-#pragma unroll
-            for (int i = 0; i < ST; ++i)
-                if (kt + i < kend) run(st[(i + ST - 1) % ST], st[i], st[(i + 1) % ST], kt + i, false);
-        }
+        wait_loads<0>();
+        __syncthreads();
+        const bool more = next(at);
+        if (more) aim();
+        use(acc, geo);
+        if (!more) return;
     }
-    wait_loads<0>();
-    __syncthreads();
-    return true;
 }
 
 // (separate arrays, not one: the compiler then knows that a load into one stage does not touch what is read from another, and waits for
@@ -301,9 +305,9 @@ __device__ __forceinline__ bool tile(const Args &g, const Place &at, char *const
     __shared__ __attribute__((aligned(1024))) char st2[ST >= 3 ? STAGE : 16];             \
     __shared__ __attribute__((aligned(1024))) char st3[ST >= 4 ? STAGE : 16];             \
     __shared__ __attribute__((aligned(1024))) char st4[ST >= 5 ? STAGE : 16];             \
-    char *const all[5] = {st0, st1, st2, st3, st4};                                       \
+    char *const stages[5] = {st0, st1, st2, st3, st4};                                    \
     char *st[ST];                                                                         \
-    _Pragma("unroll") for (int i = 0; i < ST; ++i) st[i] = all[i];
+    _Pragma("unroll") for (int i = 0; i < ST; ++i) st[i] = stages[i];
 
 // (the host pass needs the kernels' stubs only: with the bodies it drops the stubs of all but the first uses)
 template <typename T, int BM, int BN, int WM, int WN, int ST, typename Epi>
@@ -313,9 +317,34 @@ __global__ __launch_bounds__(WM *WN * 64) void tn_kernel(Args g, Epi epi) {
     __shared__ typename Epi::template Shared<BM, BN, WM, WN> sh;
     typename Epi::template Early<BM / WM / 16, BN / WN / 16> early;
     f32x4 acc[BM / WM / 16][BN / WN / 16];
-    Geom geo;
-    if (!tile<T, BM, BN, WM, WN, ST>(g, place_of(g, blockIdx.x, gridDim.x), st, acc, geo, [&](const Geom &at) { epi.template begin<BM, BN, WM, WN>(at, early, sh); })) return;
-    epi.template finish<BM, BN, WM, WN>(acc, geo, early, sh, st0, st1);
+    walk<T, BM, BN, WM, WN, ST>(g, place_of(g, blockIdx.x, gridDim.x), st, acc, [](Place &) { return false; }, [&](const Geom &at) { epi.template begin<BM, BN, WM, WN>(at, early, sh); },
+                                [&](auto &sums, const Geom &at) { epi.template finish<BM, BN, WM, WN>(sums, at, early, sh, st0, st1); });
+#endif
+}
+
+// The same with a block for every compute unit, which takes tile after tile of its die's range: the first loads of a tile pass under the
+// epilogue of the one before.  For LIMIT_N, unsplit, and an epilogue that leaves the stages alone.
+template <typename T, int BM, int BN, int WM, int WN, int ST, typename Epi>
+__global__ __launch_bounds__(WM *WN * 64) void tn_stream_kernel(Args g, Epi epi) {
+#ifdef __HIP_DEVICE_COMPILE__
+    NMFX_TN_STAGES(BM, BN, ST)
+    __shared__ typename Epi::template Shared<BM, BN, WM, WN> sh;
+    typename Epi::template Early<BM / WM / 16, BN / WN / 16> early;
+    f32x4 acc[BM / WM / 16][BN / WN / 16];
+    g.tiles_n = min(g.tiles_n, (*g.count + BN - 1) / BN);
+    const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
+    const int die = blockIdx.x & 7, last = (int)(tiles * (die + 1) / 8), step = gridDim.x / 8;
+    int id = (int)(tiles * die / 8) + (blockIdx.x >> 3);
+    if (id >= last) return;
+    walk<T, BM, BN, WM, WN, ST>(
+        g, place_at(g, id), st, acc,
+        [&](Place &at) {
+            id += step;
+            if (id >= last) return false;
+            at = place_at(g, id);
+            return true;
+        },
+        [&](const Geom &at) { epi.template begin<BM, BN, WM, WN>(at, early, sh); }, [&](auto &sums, const Geom &at) { epi.template finish<BM, BN, WM, WN>(sums, at, early, sh, st0, st1); });
 #endif
 }
 
@@ -330,12 +359,13 @@ __global__ __launch_bounds__(WM *WN * 64) void tn_pair_kernel(Args ga, EpiA ea, 
     NMFX_TN_STAGES(BM, BN, ST)
     None none;
     f32x4 acc[BM / WM / 16][BN / WN / 16];
-    Geom geo;
     const bool is_a = (int)blockIdx.x < first;
     const Args g = is_a ? ga : gb;
-    if (!tile<T, BM, BN, WM, WN, ST>(g, place_of(g, blockIdx.x - (is_a ? 0 : first), is_a ? first : last - first), st, acc, geo, [](const Geom &) {})) return;
-    if (is_a) ea.template finish<BM, BN, WM, WN>(acc, geo, none, none, st0, st1);
-    else eb.template finish<BM, BN, WM, WN>(acc, geo, none, none, st0, st1);
+    walk<T, BM, BN, WM, WN, ST>(g, place_of(g, blockIdx.x - (is_a ? 0 : first), is_a ? first : last - first), st, acc, [](Place &) { return false; }, [](const Geom &) {},
+                                [&](auto &sums, const Geom &at) {
+                                    if (is_a) ea.template finish<BM, BN, WM, WN>(sums, at, none, none, st0, st1);
+                                    else eb.template finish<BM, BN, WM, WN>(sums, at, none, none, st0, st1);
+                                });
 #endif
 }
 

@@ -343,16 +343,16 @@ struct EpiStats {
     const int *count;
     int p, npad;
     template <int MI, int NJ> struct Early { int cnt, y[NJ]; };
-    template <int BM, int BN, int WM, int WN> using Shared = tn::None;
-    template <int BM, int BN, int WM, int WN, typename E> __device__ __forceinline__ void begin(const Geom &g, E &early, tn::None &) const {
+    template <int BM, int BN, int WM, int WN> struct Shared { float2 s[WM * BN]; float t[WM * BN]; };
+    template <int BM, int BN, int WM, int WN, typename E, typename S> __device__ __forceinline__ void begin(const Geom &g, E &early, S &) const {
         early.cnt = *count;
 #pragma unroll
         for (int j = 0; j < BN / WN / 16; ++j) early.y[j] = g.n0 + 16 * j < early.cnt ? y[g.n0 + 16 * j] : -1;
     }
-    template <int BM, int BN, int WM, int WN, int MI, int NJ, typename E>
-    __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, const E &early, tn::None &, char *smem, char *) const {
-        float2 *ps = reinterpret_cast<float2 *>(smem);                        // [WM][BN]
-        float *zs = reinterpret_cast<float *>(smem + sizeof(float2) * WM * BN);
+    template <int BM, int BN, int WM, int WN, int MI, int NJ, typename E, typename S>
+    __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, const E &early, S &sh, char *, char *) const {
+        float2 *ps = sh.s;                        // [WM][BN]
+        float *zs = sh.t;
         if (g.tile_m * BM + BM > p) {
 #pragma unroll
             for (int i = 0; i < MI; ++i)
@@ -851,27 +851,43 @@ template <typename T> struct Join {
     T *out;
     int64_t ms, ns;
     int blocks;
+    // 2^lanes threads share four outputs' slots
+    int lanes;
     __device__ __forceinline__ void run(int b, float u) const {
-        typedef float f4 __attribute__((ext_vector_type(4)));
-        const int mq = (mmax + 3) / 4;
-        const int64_t total = (int64_t)mq * nmax;
-        for (int64_t e = b * 256ll + threadIdx.x; e < total; e += blocks * 256ll) {
-            int m, n;
-            if (ms == 1) { n = (int)(e / mq); m = (int)(e - (int64_t)n * mq) * 4; }
-            else { m = (int)(e / nmax); n = (int)(e - (int64_t)m * nmax); m *= 4; }
-            const int from = pos ? pos[n] : n;
-            f4 s = {0.f, 0.f, 0.f, 0.f};
+        const int mq = (mmax + 3) / 4, part = threadIdx.x & ((1 << lanes) - 1);
+        const int64_t total = (int64_t)mq * nmax, threads = blocks * 256ll >> lanes;
+        for (int64_t e0 = 0; e0 < total; e0 += threads) {                 // (whole waves stay together: they exchange sums)
+            const int64_t e = e0 + ((b * 256ll + threadIdx.x) >> lanes);
+            int m = 0, n = 0, from = -1;
+            if (e < total) {
+                if (ms == 1) { n = (int)(e / mq); m = (int)(e - (int64_t)n * mq) * 4; }
+                else { m = (int)(e / nmax); n = (int)(e - (int64_t)m * nmax); m *= 4; }
+                from = pos ? pos[n] : n;
+            }
+            f32x4 s = {0.f, 0.f, 0.f, 0.f};
             if (from >= 0) {
                 const float *p = slots + (int64_t)from * ld + m;
 #pragma unroll 4
-                for (int q = 0; q < nslots; ++q) s += *reinterpret_cast<const f4 *>(p + q * slot);
+                for (int q = part; q < nslots; q += 1 << lanes) s += *reinterpret_cast<const f32x4 *>(p + q * slot);
             }
+            for (int o = 1; o < 1 << lanes; o <<= 1)
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (m + q < mmax) out[(m + q) * ms + n * ns] = to<T>(s[q] * u);
+                for (int q = 0; q < 4; ++q) s[q] += __shfl_xor(s[q], o);
+            if (e < total && part == 0)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (m + q < mmax) out[(m + q) * ms + n * ns] = to<T>(s[q] * u);
         }
     }
 };
+// (blocks, lanes) of a join: the slots are shared where the outputs alone would not fill the card
+struct JoinGrid { int blocks, lanes; };
+inline JoinGrid join_grid(int64_t m, int64_t n, int slots) {
+    const int64_t quads = (m + 3) / 4 * n;
+    int lanes = 0;
+    while (lanes < 6 && (2 << lanes) <= slots && (quads << lanes) < 65536) ++lanes;
+    return JoinGrid{(int)std::min<int64_t>(((quads << lanes) + 255) / 256, 2048), lanes};
+}
 // the last launch of a call: dH, dW where it was summed in parts, and the losses' sum
 template <typename T> __global__ __launch_bounds__(256) void join_kernel(Join<T> h, Join<T> w, const Info *info, const float *loss_c, int reduction, float *loss) {
     const int b = blockIdx.x;
@@ -1013,6 +1029,13 @@ template <typename T, typename Epi> void product(tn::Args a, int64_t m, int64_t 
     }
     ops::hip_ok(hipGetLastError(), "product");
 }
+// the large tile, several tiles for every compute unit: their loads pass under one another's epilogues
+template <typename T, typename Epi> void stream(tn::Args a, int64_t m, int64_t n, const Choice &c, const Epi &epi, hipStream_t st) {
+    grid(a, m, n, c);
+    if (c.kind != 0 || blocks_of(a) < 2 * CUS) return product<T>(a, m, n, c, epi, st);
+    tn::tn_stream_kernel<T, 256, 256, 2, 4, 2, Epi><<<CUS, 512, 0, st>>>(a, epi);
+    ops::hip_ok(hipGetLastError(), "product");
+}
 // two products at once where they go by the same kind of tile
 template <typename T, typename EA, typename EB>
 void products(tn::Args a, int64_t ma, int64_t na, const Choice &ca, const EA &ea, tn::Args b, int64_t mb, int64_t nb, const Choice &cb, const EB &eb, const Losses &more, hipStream_t st) {
@@ -1103,7 +1126,7 @@ template <typename T> void run(const Call &c, const Shape &s) {
     const bool few = c.grad && !c.lse_given && s.pieces == 1 && tiles <= 64 && (int64_t)tiles * ((n1 + KINDS[s.z.kind].n - 1) / KINDS[s.z.kind].n) <= 2 * CUS;
     if (!c.lse_given) {
         tn::Args a{{w, ldw * es, p, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt};
-        product<T>(a, p, n1, s.z, EpiStats{reinterpret_cast<float2 *>(ws + s.o_part), s.o_zsum >= 0 ? f32(s.o_zsum) : nullptr, f32(s.o_zy), i32(s.o_y), count, p, (int)s.npad}, c.st);
+        stream<T>(a, p, n1, s.z, EpiStats{reinterpret_cast<float2 *>(ws + s.o_part), s.o_zsum >= 0 ? f32(s.o_zsum) : nullptr, f32(s.o_zy), i32(s.o_y), count, p, (int)s.npad}, c.st);
         if (!few) {
             // as many threads for a column as leave every compute unit a block
             int lc = 6;
@@ -1116,7 +1139,6 @@ template <typename T> void run(const Call &c, const Shape &s) {
 
     T *dz = reinterpret_cast<T *>(ws + s.o_dz), *dzt = reinterpret_cast<T *>(ws + s.o_dzt);
     T *dw = static_cast<T *>(c.dW.data), *dh = static_cast<T *>(c.dH.data);
-    auto join_blocks = [](int64_t m, int64_t nn) { return (int)std::min<int64_t>((((m + 3) / 4) * nn + 255) / 256, 8 * CUS); };
     const bool add = !c.lse_given && c.loss && c.o.reduction != NMFX_REDUCE_NONE;
     for (int64_t q = 0; q < s.pieces; ++q) {
         const int64_t v0 = q * s.piece;
@@ -1146,9 +1168,13 @@ template <typename T> void run(const Call &c, const Shape &s) {
         if (s.w_slots) {
             const int64_t ld = up(mm, 4);
             products<T>(b, k, n1, s.h, eh, d, mm, nn, s.w, EpiSlot{f32(s.o_wslot), ld, ld * nn, nn, 0}, Losses{}, c.st);
-            jw = Join<T>{f32(s.o_wslot), ld, ld * nn, s.w.splits, nullptr, mm, nn, out, 1, ldo, join_blocks(mm, nn)};
+            const JoinGrid jg = join_grid(mm, nn, s.w.splits);
+            jw = Join<T>{f32(s.o_wslot), ld, ld * nn, s.w.splits, nullptr, mm, nn, out, 1, ldo, jg.blocks, jg.lanes};
         } else products<T>(b, k, n1, s.h, eh, d, mm, nn, s.w, ew, Losses{}, c.st);
-        if (last && n) jh = Join<T>{f32(s.o_hslot), s.ldslot, s.npad * s.ldslot, s.h.splits, i32(s.o_pos), k, n, dh, c.dH.rs, c.dH.cs, join_blocks(k, n)};
+        if (last && n) {
+            const JoinGrid jg = join_grid(k, n, s.h.splits);
+            jh = Join<T>{f32(s.o_hslot), s.ldslot, s.npad * s.ldslot, s.h.splits, i32(s.o_pos), k, n, dh, c.dH.rs, c.dH.cs, jg.blocks, jg.lanes};
+        }
         const int jb = jh.blocks + jw.blocks + (last && add);
         if (jb) {
             join_kernel<T><<<jb, 256, 0, c.st>>>(jh, jw, info, f32(s.o_loss), c.o.reduction, c.loss);
