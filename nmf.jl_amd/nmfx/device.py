@@ -23,7 +23,7 @@ _dtype_of = attrgetter("dtype")
 def _torch():
     if not _state:
         import torch
-        _state.update(raw=getattr(torch._C, "_cuda_getCurrentRawStream", None), torch=torch, dtypes={torch.float32: L.F32, torch.float64: L.F64, torch.bfloat16: L.BF16, torch.float16: L.F16})
+        _state.update(raw=getattr(torch._C, "_cuda_getCurrentRawStream", None), torch=torch, bytes=torch.uint8, dtypes={torch.float32: L.F32, torch.float64: L.F64, torch.bfloat16: L.BF16, torch.float16: L.F16})
     return _state["torch"]
 
 
@@ -32,7 +32,21 @@ def _ck(status):
         _raise(status, L.load().nmfx_last_op_error().decode())
 
 
-def _matrix(t, name, device=None):
+def _matrix(t, name, index=None):
+    """The descriptor of a matrix; index: the device that it has to be on."""
+    try:
+        rows, cols = t.shape
+        rs, cs = t.stride()
+        d = L.DMat(t.data_ptr(), rows, cols, rs, cs, _state["dtypes"][t.dtype], 0)
+        on = t.get_device()
+    except (TypeError, ValueError, AttributeError, KeyError):
+        on = None
+    if on is None or on < 0 or (index is not None and on != index):
+        _refuse_matrix(t, name, index)
+    return d
+
+
+def _refuse_matrix(t, name, index):
     torch = _torch()
     if not isinstance(t, torch.Tensor):
         raise ArgumentError(f"{name} must be a torch tensor")
@@ -42,12 +56,10 @@ def _matrix(t, name, device=None):
         raise ArgumentError(f"{name} has dtype {t.dtype}: float32, float64, bfloat16 and float16 are taken")
     if not t.is_cuda:
         raise ArgumentError(f"{name} must be in device memory: there is no CPU path")
-    if device is not None and t.device != device:
-        raise ArgumentError(f"{name} is on {t.device}, not on {device}")
-    return L.DMat(t.data_ptr(), t.shape[0], t.shape[1], t.stride(0), t.stride(1), _state["dtypes"][t.dtype], 0)
+    raise ArgumentError(f"{name} is on {t.device}, not on cuda:{index}")
 
 
-def _vector(t, name, n, dtype, device):
+def _vector(t, name, n, dtype, index):
     torch = _torch()
     if not isinstance(t, torch.Tensor):
         raise ArgumentError(f"{name} must be a torch tensor")
@@ -55,8 +67,8 @@ def _vector(t, name, n, dtype, device):
         raise ArgumentError(f"{name} must be {dtype}, not {t.dtype}")
     if t.numel() != n or t.dim() > 1:
         raise DimensionMismatch(f"{name} must have {n} value(s), not the shape {tuple(t.shape)}")
-    if t.device != device:
-        raise ArgumentError(f"{name} is on {t.device}, not on {device}")
+    if t.get_device() != index:
+        raise ArgumentError(f"{name} is on {t.device}, not on cuda:{index}")
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -65,20 +77,22 @@ def _xent_args(W, H, labels, ignore_index, label_smoothing, reduction):
     if reduction not in _REDUCTIONS:
         raise ArgumentError(f"reduction must be 'none', 'sum' or 'mean', not {reduction!r}")
     w = _matrix(W, "W")
-    h = _matrix(H, "H", W.device)
-    labels = _vector(labels, "labels", H.shape[1], torch.int64, W.device)
-    return w, h, labels, L.XentOpts(float(label_smoothing), int(ignore_index), _REDUCTIONS[reduction], 0)
+    index = W.get_device()
+    h = _matrix(H, "H", index)
+    return w, h, _vector(labels, "labels", h.cols, torch.int64, index), L.XentOpts(label_smoothing, ignore_index, _REDUCTIONS[reduction], 0), index
 
 
-def _workspace(w, h, o, grad, device):
+def _workspace(lib, w, h, o, grad, device):
     size = C.c_int64()
-    _ck(L.load().nmfx_xent_workspace(w, h, o, grad, size))
-    return _torch().empty(size.value, dtype=_torch().uint8, device=device), size.value
+    status = lib.nmfx_xent_workspace(w, h, o, grad, size)
+    if status:
+        _ck(status)
+    return _state["torch"].empty(size.value, dtype=_state["bytes"], device=device), size.value
 
 
-def _stream(device):
+def _stream(index):
     raw = _state["raw"]
-    return raw(device.index) if raw else _torch().cuda.current_stream(device).cuda_stream
+    return raw(index) if raw else _torch().cuda.current_stream(index).cuda_stream
 
 
 def softmax_xent(W, H, labels, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
@@ -89,40 +103,44 @@ def softmax_xent(W, H, labels, ignore_index=-100, label_smoothing=0.0, reduction
     the columns that are not ignored (0 where there is none).  lse, the log-sum-exp of every column's logits, has n values; both are 0 in
     ignored columns.  A label that is no class makes its column's loss NaN."""
     torch = _torch()
-    w, h, labels, o = _xent_args(W, H, labels, ignore_index, label_smoothing, reduction)
-    dev, n = W.device, H.shape[1]
-    ws, size = _workspace(w, h, o, 0, dev)
+    w, h, labels, o, index = _xent_args(W, H, labels, ignore_index, label_smoothing, reduction)
+    lib, dev, n = L.load(), W.device, h.cols
+    ws, size = _workspace(lib, w, h, o, 0, dev)
     loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=dev)
     lse = torch.empty(n, dtype=torch.float32, device=dev)
-    _ck(L.load().nmfx_xent(w, h, labels.data_ptr(), o, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), size, dev.index, _stream(dev)))
+    status = lib.nmfx_xent(w, h, labels.data_ptr(), o, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), size, index, _stream(index))
+    if status:
+        _ck(status)
     return loss, lse
 
 
-def _like(t):
-    """An empty matrix of t's shape, type and contiguous index, dense."""
-    if t.stride(1) == 1 or t.stride(0) != 1:
-        return _torch().empty(t.shape, dtype=t.dtype, device=t.device)
-    return _torch().empty((t.shape[1], t.shape[0]), dtype=t.dtype, device=t.device).t()
+def _like(t, d, device):
+    """An empty matrix of t's shape, type and contiguous index, dense (d: t's descriptor)."""
+    if d.cs == 1 or d.rs != 1:
+        return _state["torch"].empty((d.rows, d.cols), dtype=t.dtype, device=device)
+    return _state["torch"].empty((d.cols, d.rows), dtype=t.dtype, device=device).t()
 
 
 def _grad(W, H, labels, ignore_index, label_smoothing, reduction, gout, lse, dW, dH):
     torch = _torch()
-    w, h, labels, o = _xent_args(W, H, labels, ignore_index, label_smoothing, reduction)
-    dev, n = W.device, H.shape[1]
+    w, h, labels, o, index = _xent_args(W, H, labels, ignore_index, label_smoothing, reduction)
+    lib, dev, n = L.load(), W.device, h.cols
     if gout is not None:
-        gout = _vector(gout, "gout", n if reduction == "none" else 1, torch.float32, dev)
+        gout = _vector(gout, "gout", n if reduction == "none" else 1, torch.float32, index)
     given = lse is not None
     if given:
-        lse, loss = _vector(lse, "lse", n, torch.float32, dev), None
+        lse, loss = _vector(lse, "lse", n, torch.float32, index), None
     else:
         lse = torch.empty(n, dtype=torch.float32, device=dev)
         loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=dev)
-    dW = _like(W) if dW is None else dW
-    dH = _like(H) if dH is None else dH
-    gw, gh = _matrix(dW, "dW", dev), _matrix(dH, "dH", dev)
-    ws, size = _workspace(w, h, o, 1, dev)
-    _ck(L.load().nmfx_xent_grad(w, h, labels.data_ptr(), o, None if gout is None else gout.data_ptr(), int(given), None if given else loss.data_ptr(),
-                                lse.data_ptr(), gw, gh, ws.data_ptr(), size, dev.index, _stream(dev)))
+    dW = _like(W, w, dev) if dW is None else dW
+    dH = _like(H, h, dev) if dH is None else dH
+    gw, gh = _matrix(dW, "dW", index), _matrix(dH, "dH", index)
+    ws, size = _workspace(lib, w, h, o, 1, dev)
+    status = lib.nmfx_xent_grad(w, h, labels.data_ptr(), o, None if gout is None else gout.data_ptr(), given, None if given else loss.data_ptr(), lse.data_ptr(), gw, gh,
+                                ws.data_ptr(), size, index, _stream(index))
+    if status:
+        _ck(status)
     return loss, lse, dW, dH
 
 
@@ -221,7 +239,7 @@ def _norm(grads, max_norm, norm_type, out):
     _ck(lib.nmfx_grad_norm_workspace(len(grads), size))
     ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    common = (norm.data_ptr(), ws.data_ptr(), size.value, dev.index, _stream(dev))
+    common = (norm.data_ptr(), ws.data_ptr(), size.value, dev.index, _stream(dev.index))
     if max_norm is None:
         _ck(lib.nmfx_grad_norm(len(grads), a.ctypes.data, kind, *common))
     else:
