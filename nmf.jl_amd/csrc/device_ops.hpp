@@ -36,6 +36,7 @@ struct OnDevice {
             throw OpError{NMFX_ERR_NO_DEVICE, "no HIP device visible: libnmfx has no CPU fallback"};
         }
         require(device >= 0 && device < n, NMFX_ERR_BAD_ARG, "device ordinal out of range");
+        (void)hipGetLastError();      // an error that somebody else's call left behind is not a launch's of this one
         hip_ok(hipGetDevice(&before), "hipGetDevice");
         if (before != device) hip_ok(hipSetDevice(device), "hipSetDevice");
         else before = -1;
@@ -70,6 +71,24 @@ inline int elem_bytes(int dtype) {
         case NMFX_BF16: case NMFX_F16: return 2;
         default: return 0;
     }
+}
+
+struct View {           // a matrix as rows of contiguous elements
+    char *p;
+    int64_t rows, len, ld;   // len: elements of a row, ld: elements between rows
+    int es, dtype;
+    int64_t bytes() const { return ((rows - 1) * ld + len) * es; }
+};
+
+// whether two views have an element in common: exact where one is dense or both have one row stride, else "yes" where their extents overlap
+inline bool meet(const View &a, const View &b) {
+    if (!a.rows || !b.rows) return false;
+    if (a.p > b.p) return meet(b, a);
+    if (a.p + a.bytes() <= b.p) return false;
+    const int64_t la = a.rows > 1 ? a.ld * a.es : 0, lb = b.rows > 1 ? b.ld * b.es : 0;
+    if (!la || (lb && la != lb)) return true;
+    const int64_t d = (b.p - a.p) % la;
+    return !(d >= a.len * a.es && d + b.len * b.es <= la);
 }
 
 }  // namespace ops

@@ -239,12 +239,8 @@ template <int INF> __global__ __launch_bounds__(1024) void small_kernel(Short t,
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
 constexpr int64_t SMALL_CHUNKS = 4;
 
-struct View {           // a matrix as rows of contiguous elements
-    char *p;
-    int64_t rows, len, ld;   // len: elements of a row, ld: elements between rows
-    int es, dtype;
-    int64_t bytes() const { return ((rows - 1) * ld + len) * es; }
-};
+using ops::View;
+using ops::meet;
 View view_of(const nmfx_dmat &m, const char *what) {
     auto refuse = [&](int status, const char *why) { throw ops::OpError{status, std::string(what) + why}; };
     const int es = ops::elem_bytes(m.dtype);
@@ -263,17 +259,6 @@ View view_of(const nmfx_dmat &m, const char *what) {
     return v;
 }
 
-// whether two views have an element in common; exact for dense views and for views of one row stride, "yes" where that is not clear
-bool meet(const View &a, const View &b) {
-    if (a.p > b.p) return meet(b, a);
-    if (a.p + a.bytes() <= b.p) return false;
-    const int64_t la = a.rows > 1 ? a.ld * a.es : 0, lb = b.rows > 1 ? b.ld * b.es : 0;
-    const int64_t ld = la ? la : lb;
-    if (!ld || (la && lb && la != lb)) return true;
-    if (!la || !lb) return true;
-    const int64_t d = (b.p - a.p) % ld;
-    return !(d >= a.len * a.es && d + b.len * b.es <= ld);
-}
 bool before(const View &a, const View &b) { return a.p < b.p; }
 // of views in order of address
 bool any_meet(const std::vector<View> &v) {

@@ -86,7 +86,10 @@ __device__ __forceinline__ int swizzle(int row) { return row >> 1 & 7; }
 // tell which stage a load is for, does not wait for all of them in front of a read: the waits are walk()'s own.
 __device__ __forceinline__ void to_lds(u32x4 rsrc, char *lds, uint32_t off) {
     const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void *)lds);
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"        // m0 is said to be reserved: it is written here and named for that
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(at), "v"(off), "s"(rsrc) : "memory", "m0");
+#pragma clang diagnostic pop
 }
 
 // TILE_ROWS rows, by NT threads
@@ -170,9 +173,8 @@ __device__ __forceinline__ void walk(const Args &g, Place at, char *const (&st)[
     // this wave's loads of the next tile are in LDS and its fragments of this one read (`later` tiles may still be on their way);
     // then all waves'
     auto meet = [&](int later) {
-        if (ST >= 5 && later >= 3) wait_loads<3 * LOADS>();
-        else if (ST >= 4 && later >= 2) wait_loads<2 * LOADS>();
-        else if (ST >= 3 && later >= 1) wait_loads<LOADS>();
+        if (ST == 4 && later >= 2) wait_loads<2 * LOADS>();
+        else if (ST == 4 && later >= 1) wait_loads<LOADS>();
         else wait_loads<0>();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
@@ -296,16 +298,15 @@ __device__ __forceinline__ void walk(const Args &g, Place at, char *const (&st)[
     }
 }
 
-// (separate arrays, not one: the compiler then knows that a load into one stage does not touch what is read from another, and waits for
-// neither)
+// (the epilogues take the first two for their own use)
 #define NMFX_TN_STAGES(BM, BN, ST)                                                        \
-    constexpr int STAGE = (BM + BN) * tn::ROW;                                              \
+    static_assert(ST == 2 || ST == 4, "meet()'s waits");                                  \
+    constexpr int STAGE = (BM + BN) * tn::ROW;                                            \
     __shared__ __attribute__((aligned(1024))) char st0[STAGE];                            \
     __shared__ __attribute__((aligned(1024))) char st1[STAGE];                            \
-    __shared__ __attribute__((aligned(1024))) char st2[ST >= 3 ? STAGE : 16];             \
-    __shared__ __attribute__((aligned(1024))) char st3[ST >= 4 ? STAGE : 16];             \
-    __shared__ __attribute__((aligned(1024))) char st4[ST >= 5 ? STAGE : 16];             \
-    char *const stages[5] = {st0, st1, st2, st3, st4};                                    \
+    __shared__ __attribute__((aligned(1024))) char st2[ST == 4 ? STAGE : 16];             \
+    __shared__ __attribute__((aligned(1024))) char st3[ST == 4 ? STAGE : 16];             \
+    char *const stages[4] = {st0, st1, st2, st3};                                         \
     char *st[ST];                                                                         \
     _Pragma("unroll") for (int i = 0; i < ST; ++i) st[i] = stages[i];
 

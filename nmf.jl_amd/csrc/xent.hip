@@ -1205,6 +1205,14 @@ nmfx_dmat tidy(nmfx_dmat m) {
     return m;
 }
 
+ops::View view_of(const nmfx_dmat &m) {
+    const bool by_row = m.cs == 1;
+    ops::View v{static_cast<char *>(m.data), by_row ? m.rows : m.cols, by_row ? m.cols : m.rows, by_row ? m.rs : m.cs, ops::elem_bytes(m.dtype), m.dtype};
+    if (!m.rows || !m.cols) v.rows = 0;
+    else if (v.rows == 1 || v.ld == v.len) v = ops::View{v.p, 1, v.rows * v.len, v.rows * v.len, v.es, v.dtype};
+    return v;
+}
+
 constexpr int64_t MOST = (1 << 21) - 1024;   // 256 rows of Float32, padded, stay below the 2^31 bytes from which on loads ask for zeros
 
 void check(const nmfx_dmat *W, const nmfx_dmat *H) {
@@ -1279,6 +1287,8 @@ int nmfx_xent_grad(const nmfx_dmat *W, const nmfx_dmat *H, const int64_t *labels
         ops::require(lse || !H->cols || !lse_given, NMFX_ERR_BAD_ARG, "lse is NULL, yet lse_given is set");
         xent::Call c{xent::tidy(*W), xent::tidy(*H), xent::tidy(*dW), xent::tidy(*dH), labels, *opts, gout, loss, lse, true, lse_given != 0, static_cast<char *>(workspace),
                      static_cast<hipStream_t>(stream)};
+        const ops::View w = xent::view_of(c.W), h = xent::view_of(c.H), gw = xent::view_of(c.dW), gh = xent::view_of(c.dH);
+        ops::require(!ops::meet(gw, gh) && !ops::meet(gw, w) && !ops::meet(gw, h) && !ops::meet(gh, w) && !ops::meet(gh, h), NMFX_ERR_BAD_ARG, "dW and dH may share no elements with each other, W or H");
         const xent::Shape s = xent::shape_of(c.W, c.H, true, opts->label_smoothing != 0.);
         ops::require(workspace && workspace_bytes >= s.bytes, NMFX_ERR_BAD_ARG, "the workspace is smaller than nmfx_xent_workspace says");
         ops::require((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, NMFX_ERR_BAD_ARG, "the workspace must be aligned to 256 bytes");

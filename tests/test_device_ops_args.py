@@ -63,12 +63,23 @@ def test_xent_grad_arguments(lib):
     L = lib
 
     def grad(dW=None, dH=None, lse=0x50000, given=0):
-        return L.load().nmfx_xent_grad(mat(L), mat(L, 32, 8, 1, 32), 0x20000, opts(L), None, given, None, lse, dW or mat(L), dH or mat(L, 32, 8, 1, 32), 0x40000, 1 << 40, 0, None)
+        return L.load().nmfx_xent_grad(mat(L), mat(L, 32, 8, 1, 32, data=0x60000), 0x20000, opts(L), None, given, None, lse, dW or mat(L, data=0x70000),
+                                       dH or mat(L, 32, 8, 1, 32, data=0x80000), 0x40000, 1 << 40, 0, None)
 
     assert grad() == L.ERR_NO_DEVICE and grad(lse=None) == L.ERR_NO_DEVICE
     assert grad(lse=None, given=1) == L.ERR_BAD_ARG
     assert grad(dW=mat(L, rows=63)) == L.ERR_DIM_MISMATCH and grad(dH=mat(L, 32, 9, 1, 32)) == L.ERR_DIM_MISMATCH
     assert grad(dW=mat(L, dtype=2)) == L.ERR_BAD_ARG and grad(dH=mat(L, 32, 8, 0, 1)) == L.ERR_BAD_ARG
+    # W: 64 x 32 at 0x10000, H: 32 x 8 at 0x60000, Float32
+    assert grad(dW=mat(L)) == L.ERR_BAD_ARG and grad(dW=mat(L, data=0x60000 - 64 * 32 * 4 + 4)) == L.ERR_BAD_ARG
+    assert grad(dW=mat(L, data=0x60000 - 64 * 32 * 4)) == L.ERR_NO_DEVICE and grad(dW=mat(L, data=0x60000 + 8 * 32 * 4)) == L.ERR_NO_DEVICE
+    assert grad(dH=mat(L, 32, 8, 1, 32, data=0x60000)) == L.ERR_BAD_ARG and grad(dH=mat(L, 32, 8, 1, 32, data=0x70000 + 512)) == L.ERR_BAD_ARG
+    assert grad(dH=mat(L, 32, 8, 1, 32, data=0x10000 + 64 * 32 * 4 - 4)) == L.ERR_BAD_ARG
+    # side by side in one buffer's rows of 64
+    side = mat(L, rs=64, data=0x70000)
+    assert grad(dW=side, dH=mat(L, 32, 8, 8, 1, data=0x70000 + 32 * 4)) == L.ERR_BAD_ARG       # longer than the gap
+    assert grad(dW=side, dH=mat(L, 32, 8, 64, 1, data=0x70000 + 32 * 4)) == L.ERR_NO_DEVICE
+    assert grad(dW=side, dH=mat(L, 32, 8, 64, 1, data=0x70000 + 31 * 4)) == L.ERR_BAD_ARG
 
 
 def test_workspace_is_bounded(lib):
@@ -106,6 +117,9 @@ def test_norm_arguments(lib):
     assert clip([left, right]) == L.ERR_NO_DEVICE                         # two halves of one buffer's rows
     assert clip([left, mat(L, 64, 16, 32, 1, data=0x10000 + 60)]) == bad
     assert clip([mat(L, 64, 17, 32, 1), right]) == bad
+    gap = mat(L, 1, 16, 16, 1, data=0x10000 + 5 * 128 + 64)               # 16 elements behind a row's left half, dense
+    assert clip([left, gap]) == L.ERR_NO_DEVICE and clip([right, gap]) == bad and clip([left, mat(L, 1, 17, 17, 1, data=0x10000 + 5 * 128 + 64)]) == bad
+    assert clip([left, mat(L, 1, 16, 16, 1, data=0x10000 - 64)]) == L.ERR_NO_DEVICE and clip([left, mat(L, 1, 17, 17, 1, data=0x10000 - 64)]) == bad
     other = mat(L, data=0x80000)
     assert clip([one], [other]) == L.ERR_NO_DEVICE and clip([one], [one]) == L.ERR_NO_DEVICE
     assert clip([one, other], [other, one]) == bad                        # exchanged: one's result is another's gradient

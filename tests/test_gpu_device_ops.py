@@ -264,6 +264,17 @@ def test_xent_float16_range(dtype):
     check(W, H, y, dtype, reduction="none", gout=gout)
 
 
+@pytest.mark.parametrize("n", [1, 2048, 2049, 5000, 9000])
+def test_xent_factors_of_many_columns(n):
+    """A factor of its own for every column, the largest (which sets Float16's scale) in the last: found over one round and over several."""
+    for dtype in TYPES:
+        W, H, y = problem(130, n, 16, dtype, seed=n, ignored=0.3)
+        y[-1] = 5
+        gout = torch.rand(n, device=DEV) - 0.5
+        gout[-1] = -512.0
+        check(W, H, y, dtype, reduction="none", gout=gout)
+
+
 def test_xent_same_bits_twice_and_given_outputs():
     W, H, y = problem(3000, 500, 136, "bf16", ignored=0.2)
     a = nmfx.softmax_xent_grad(W, H, y)
@@ -318,6 +329,88 @@ def test_two_streams_at_once():
         for g in got[i]:
             for a, b in zip(g, want[i]):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_xent_many_components(dtype):
+    for n in (1, 5, 40):
+        check(*problem(300, n, 9000, dtype, seed=n), dtype)
+
+
+def _guarded(nbytes, guard=4096):
+    """nbytes of 0xff (NaN in every type) between guards, 256-byte aligned; and the check that the guards are as they were."""
+    room = (nbytes + 255) // 256 * 256
+    buf = torch.full((room + 2 * guard,), 0xff, dtype=torch.uint8, device=DEV)
+    buf[:guard] = buf[guard + room:] = 0x5a
+
+    def untouched():
+        assert (buf[:guard] == 0x5a).all() and (buf[guard + room:] == 0x5a).all() and (buf[guard + nbytes:guard + room] == 0xff).all()
+
+    return buf[guard:guard + nbytes], untouched
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("p,n,k,wl,ignored", [(1, 1, 1, "r", 0.0), (70, 3, 8, "r", 0.0), (70, 3, 9, "c", 0.5), (777, 65, 40, "c", 0.3), (5000, 300, 64, "r", 0.9), (257, 2100, 33, "r", 0.5), (300, 5000, 24, "r", 0.4),
+                                              (20000, 4200, 40, "r", 0.2)])
+def test_xent_stays_in_its_buffers_and_takes_nothing_from_them(dtype, p, n, k, wl, ignored):
+    """Workspace and outputs full of NaN beforehand and between guards: same bits as with torch's memory, guards untouched."""
+    L = nmfx._lib
+    lib = L.load()
+    W, H, y = problem(p, n, k, dtype, seed=p, ignored=ignored, wl=wl)
+    code = {"f32": L.F32, "bf16": L.BF16, "f16": L.F16}[dtype]
+    es = W.element_size()
+
+    def mat(t, rows, cols, rs, cs):
+        return L.DMat(t.data_ptr(), rows, cols, rs, cs, code, 0)
+
+    w, h = mat(W, p, k, *W.stride()), mat(H, k, n, *H.stride())
+    import ctypes as C
+    for eps in (0.0, 0.1):
+        o, size = L.XentOpts(eps, -100, L.REDUCE_MEAN, 0), C.c_int64()
+        for grad in (0, 1):
+            assert lib.nmfx_xent_workspace(w, h, o, grad, size) == L.OK
+            bufs = [_guarded(b) for b in (size.value, 4, 4 * n, p * k * es, k * n * es)]
+            ws, loss, lse, dW, dH = (b[0] for b in bufs)
+            stream = torch.cuda.current_stream().cuda_stream
+            if grad:
+                st = lib.nmfx_xent_grad(w, h, y.data_ptr(), o, None, 0, loss.data_ptr(), lse.data_ptr(), mat(dW, p, k, k, 1), mat(dH, k, n, 1, k), ws.data_ptr(), size.value, 0, stream)
+                got = (loss.view(torch.float32)[0], lse.view(torch.float32), dW.view(W.dtype).view(p, k), dH.view(W.dtype).view(n, k).t())
+                want = nmfx.softmax_xent_grad(W, H, y, label_smoothing=eps, dW=torch.empty(p, k, dtype=W.dtype, device=DEV))
+            else:
+                st = lib.nmfx_xent(w, h, y.data_ptr(), o, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), size.value, 0, stream)
+                got, want = (loss.view(torch.float32)[0], lse.view(torch.float32)), nmfx.softmax_xent(W, H, y, label_smoothing=eps)
+            assert st == L.OK, lib.nmfx_last_op_error()
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+            for _, untouched in bufs:
+                untouched()
+
+
+def test_norm_stays_in_its_buffers():
+    L = nmfx._lib
+    lib = L.load()
+    import ctypes as C
+    sizes = [1, 7, 8191, 40000, 3] * 40
+    flat, flat_ok = _guarded(4 * sum(sizes))
+    flat.view(torch.float32).copy_(torch.randn(sum(sizes), device=DEV))
+    views = flat.view(torch.float32).split(sizes)
+    want = [v.clone() for v in views]
+    norm = nmfx.clip_grad_norm(want, 0.5)
+    for count in (5, 200):
+        data = [v.clone() for v in views[:count]]
+        out, out_ok = _guarded(4 * sum(sizes[:count]))
+        outs = out.view(torch.float32).split(sizes[:count])
+        a = (L.DMat * count)(*[L.DMat(t.data_ptr(), 1, t.numel(), t.numel(), 1, L.F32, 0) for t in data])
+        b = (L.DMat * count)(*[L.DMat(t.data_ptr(), 1, t.numel(), t.numel(), 1, L.F32, 0) for t in outs])
+        size = C.c_int64()
+        assert lib.nmfx_grad_norm_workspace(count, size) == L.OK
+        ws, ws_ok = _guarded(size.value)
+        got, got_ok = _guarded(4)
+        assert lib.nmfx_clip_grad_norm(count, C.addressof(a), C.addressof(b), 0.5, L.NORM_2, got.data_ptr(), ws.data_ptr(), size.value, 0, torch.cuda.current_stream().cuda_stream) == L.OK
+        if count == 200:
+            assert torch.equal(got.view(torch.float32)[0], norm) and all(torch.equal(x, y) for x, y in zip(outs, want))
+        assert not out.view(torch.float32).isnan().any()
+        out_ok(), ws_ok(), got_ok(), flat_ok()
 
 
 # ---- norm and clipping ---------------------------------------------------------------------------------------------------------------
