@@ -656,9 +656,8 @@ template <typename T> class Solver : public SolverBase {
     hipEvent_t ev_fork = nullptr, ev_join = nullptr;
     void ensure_fstream() {
         if (fstream) return;
-        int lo = 0, hi = 0;
-        HIP_TRY(hipDeviceGetStreamPriorityRange(&lo, &hi));
-        HIP_TRY(hipStreamCreateWithPriority(&fstream, hipStreamNonBlocking, hi));
+        // (at the default priority like every other stream: work on streams of different priorities can hang the queues)
+        HIP_TRY(hipStreamCreateWithFlags(&fstream, hipStreamNonBlocking));
         HIP_TRY(hipEventCreateWithFlags(&ev_fork, hipEventDisableTiming));
         HIP_TRY(hipEventCreateWithFlags(&ev_join, hipEventDisableTiming));
     }
