@@ -261,11 +261,43 @@ struct PeerHandle {
 static_assert(sizeof(PeerHandle) <= 128, "NMFX_P2P_HANDLE_BYTES");
 constexpr uint64_t PEER_MAGIC = 0x4e4d465850325031ull;
 
+// Windows are kept for the process's next communicator instead of being freed: memory that was allocated uncached and read by a kernel must
+// not go back to the runtime (allocations that got it afterwards have held wrong values), and a rank whose peer has failed may still store into
+// the peer's window.  What is kept is at most what was in use at once.
+struct WindowPool {
+    struct Kept { int dev; unsigned flags; size_t bytes; unsigned char *p; };
+    std::mutex m;
+    std::vector<Kept> kept;
+    static WindowPool &get() {
+        static WindowPool *pool = new WindowPool;       // never destroyed: contexts may outlive static destructors
+        return *pool;
+    }
+    hipError_t take(int dev, unsigned flags, size_t &bytes, unsigned char *&p) {
+        {
+            std::lock_guard<std::mutex> lock(m);
+            for (size_t i = 0; i < kept.size(); ++i)
+                if (kept[i].dev == dev && kept[i].flags == flags && kept[i].bytes >= bytes) {
+                    p = kept[i].p;
+                    bytes = kept[i].bytes;
+                    kept.erase(kept.begin() + (ptrdiff_t)i);
+                    return hipSuccess;
+                }
+        }
+        return hipExtMallocWithFlags(reinterpret_cast<void **>(&p), bytes, flags);
+    }
+    void give(int dev, unsigned flags, size_t bytes, unsigned char *p) {
+        std::lock_guard<std::mutex> lock(m);
+        kept.push_back(Kept{dev, flags, bytes, p});
+    }
+};
+
 struct PeerComm : Comm {
     Comm *base;                       // bootstrap transport; carries whatever does not fit a slot (owned)
     int dev;
     unsigned char *mine = nullptr;    // this rank's window
     size_t win_bytes = 0, slot_bytes = 0;
+    unsigned mem_flags = 0;           // how the window was allocated, and how much of it
+    size_t mem_bytes = 0;
     PeerWin win;                      // every rank's window as mapped HERE
     bool opened[LOCAL_MAX_RANKS] = {};
     bool attached = false, sim = false;
@@ -290,9 +322,9 @@ struct PeerComm : Comm {
         if (const char *e = dev_env("NMFX_P2P_TINY")) tiny_enabled = std::atoi(e) != 0;
         // uncached: remote stores and local reads both bypass the (non-coherent) L2s; NMFX_P2P_MEM=finegrained|plain for experiments
         const char *kind = dev_env("NMFX_P2P_MEM");
-        hipError_t e;
-        if (kind && std::strcmp(kind, "plain") == 0) e = hipMalloc(reinterpret_cast<void **>(&mine), win_bytes);
-        else e = hipExtMallocWithFlags(reinterpret_cast<void **>(&mine), win_bytes, (kind && std::strcmp(kind, "finegrained") == 0) ? hipDeviceMallocFinegrained : hipDeviceMallocUncached);
+        mem_flags = kind && std::strcmp(kind, "plain") == 0 ? hipDeviceMallocDefault : kind && std::strcmp(kind, "finegrained") == 0 ? hipDeviceMallocFinegrained : hipDeviceMallocUncached;
+        mem_bytes = win_bytes;
+        const hipError_t e = WindowPool::get().take(dev, mem_flags, mem_bytes, mine);
         if (e != hipSuccess) throw CommError{std::string("peer window allocation failed: ") + hipGetErrorString(e)};
         if (hipMemset(mine, 0, win_bytes) != hipSuccess || hipDeviceSynchronize() != hipSuccess) throw CommError{"peer window memset failed"};
         for (int q = 0; q < LOCAL_MAX_RANKS; ++q) win.p[q] = nullptr;
@@ -301,7 +333,9 @@ struct PeerComm : Comm {
     ~PeerComm() override {
         for (int q = 0; q < nranks; ++q)
             if (opened[q] && win.p[q]) (void)hipIpcCloseMemHandle(win.p[q]);
-        if (mine) (void)hipFree(mine);
+        // (a window that saw a time-out stays mapped and is not used again: a rank that has not failed yet may still store into it)
+        unsigned aborted = 1;
+        if (mine && hipMemcpy(&aborted, mine + PEER_ABORT_OFF, 4, hipMemcpyDeviceToHost) == hipSuccess && !aborted) WindowPool::get().give(dev, mem_flags, mem_bytes, mine);
         delete base;
     }
     const char *transport() const override { return "peer"; }
