@@ -7,7 +7,9 @@ import pytest
 # spins on the device until its peers' signal kernels have run, so no two ranks' streams may share a hardware queue (HIP multiplexes a
 # process's streams onto GPU_MAX_HW_QUEUES = 4 queues by default; a signal queued behind a spinning wait would never run).  Read by
 # the HIP runtime at initialisation, hence before torch.  One process per GPU -- the production layout -- needs nothing of the kind.
-os.environ.setdefault("GPU_MAX_HW_QUEUES", "24")
+# (At least 24: an environment that states the runtime's own default of 4 would leave the ranks sharing queues.)
+if not os.environ.get("GPU_MAX_HW_QUEUES", "").isdigit() or int(os.environ["GPU_MAX_HW_QUEUES"]) < 24:
+    os.environ["GPU_MAX_HW_QUEUES"] = "24"
 # the library's development switches (NMFX_POTRS, NMFX_K_GRANULE, NMFX_RS_FUSED, ...: alternative kernels the tests run against each
 # other) are dead unless NMFX_DEV=1 is set as well (csrc/comm.hpp: dev_env)
 os.environ.setdefault("NMFX_DEV", "1")
