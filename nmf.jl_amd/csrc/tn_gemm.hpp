@@ -349,6 +349,38 @@ __global__ __launch_bounds__(WM *WN * 64) void tn_stream_kernel(Args g, Epi epi)
 #endif
 }
 
+// A block for each column of tiles that `on` names: all its tiles with one epilogue, between(tile_n), then all with the other.
+template <typename T, int BM, int BN, int WM, int WN, int ST, typename EpiA, typename Between, typename EpiB>
+__global__ __launch_bounds__(WM *WN * 64) void tn_again_kernel(Args g, EpiA ea, Between between, EpiB eb, const int *on) {
+#ifdef __HIP_DEVICE_COMPILE__
+    if (!on[blockIdx.x]) return;
+    NMFX_TN_STAGES(BM, BN, ST)
+    f32x4 acc[BM / WM / 16][BN / WN / 16];
+    auto all = [&](const auto &epi, auto &sh, auto &early) {
+        for (int m = 0; m < g.tiles_m; ++m) {
+            walk<T, BM, BN, WM, WN, ST>(g, Place{m, (int)blockIdx.x, 0}, st, acc, [](Place &) { return false; }, [&](const Geom &at) { epi.template begin<BM, BN, WM, WN>(at, early, sh); },
+                                        [&](auto &sums, const Geom &at) { epi.template finish<BM, BN, WM, WN>(sums, at, early, sh, st0, st1); });
+            __syncthreads();
+        }
+        __threadfence();
+        __syncthreads();
+    };
+    {
+        __shared__ typename EpiA::template Shared<BM, BN, WM, WN> sh;
+        typename EpiA::template Early<BM / WM / 16, BN / WN / 16> early;
+        all(ea, sh, early);
+    }
+    between.template run<BN>(blockIdx.x * BN);
+    __threadfence();
+    __syncthreads();
+    {
+        __shared__ typename EpiB::template Shared<BM, BN, WM, WN> sh;
+        typename EpiB::template Early<BM / WM / 16, BN / WN / 16> early;
+        all(eb, sh, early);
+    }
+#endif
+}
+
 // two products in one launch: the first `first` blocks are one's, those up to `last` the other's; a block behind them runs `more`
 template <typename T, int BM, int BN, int WM, int WN, int ST, typename EpiA, typename EpiB, typename More>
 __global__ __launch_bounds__(WM *WN * 64) void tn_pair_kernel(Args ga, EpiA ea, Args gb, EpiB eb, int first, int last, More more) {

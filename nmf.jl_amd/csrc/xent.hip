@@ -456,6 +456,19 @@ struct Combine {
     }
 };
 
+// the columns from n0 on of a tile, by a thread each
+struct Columnwise {
+    Combine c;
+    template <int BN> __device__ __forceinline__ void run(int n0) const {
+        const int i = n0 + threadIdx.x;
+        if (threadIdx.x >= BN || i >= c.info->count) return;
+        float2 a;
+        float t;
+        c.some(i, 0, 1, a, t);
+        c.finish(i, a, t, true);
+    }
+};
+
 // the losses' sum or mean, by one block: Float64, a fixed order
 template <int NT> __device__ __forceinline__ void reduce_losses(const float *loss_c, int cnt, int reduction, float *loss) {
     __shared__ double sh[NT / 64];
@@ -478,7 +491,7 @@ struct Losses {          // as a block of another launch
     template <int NT> __device__ __forceinline__ void run() const { reduce_losses<NT>(loss_c, info->count, reduction, loss); }
 };
 
-// 256 threads share 2^lc packed columns; the block that is done last adds up the losses
+// 256 threads share 2^lc packed columns; the block that is done last adds up the losses.
 __global__ __launch_bounds__(256) void combine_kernel(Combine c, int lc, int add) {
     __shared__ float2 ps[256];
     __shared__ float ts[256];
@@ -659,15 +672,17 @@ __global__ __launch_bounds__(1024) void score_join_kernel(Score a, int blocks, f
 // ---- dz of a piece of the classes, in both orders -----------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ T to(float x) { return (T)x; }
 
-template <typename T> struct EpiDz {
+// KEEP: the same images of E = exp(z - r_j) instead, before the log-sum-exp is known, with the tiles' sums of E and the labels' logits.
+template <typename T, bool KEEP = false> struct EpiDz {
     T *dz, *dzt;              // [npad][ldc] by packed column, [classes of the piece][ldn] by class
     int64_t ldc, ldn;
-    const float *lse_c, *f;
+    const float *lse_c, *f;   // KEEP: lse_c is the reference, in units of log 2
     const int *y, *count;
     int p, v0;                // classes that exist in the piece; its first class
     float inv, label, off;    // 1 / a, (1 - eps) / a, eps / (a p)
     int few;                  // the tiles' statistics are not joined yet: every block does it for its own columns
     Combine c;
+    float *part, *zy;         // KEEP: [tile_m][npad]; the labels' logits
     // per column: log-sum-exp, factor, label's class in the piece.  The large tile has no registers for them to wait in: it reads them late.
     template <int MI, int NJ> struct Early { int cnt, y[NJ]; float lse[NJ], f[NJ]; };
     template <int BM, int BN, int WM, int WN> struct Shared { float lse[BN], t[WM * WN * 64]; float2 s[WM * WN * 64]; };
@@ -700,7 +715,7 @@ template <typename T> struct EpiDz {
             const int n = g.n0 + 16 * j;
             const bool on = n < early.cnt;
             early.lse[j] = few ? sh.lse[n - g.tile_n * BN] : on ? lse_c[n] : 0.f;
-            early.f[j] = on ? f[n] : 0.f;
+            early.f[j] = KEEP ? 1.f : on ? f[n] : 0.f;
             early.y[j] = on ? y[n] - v0 : -1;
         }
     }
@@ -720,14 +735,17 @@ template <typename T> struct EpiDz {
         auto column = [&](int j, auto at_edge) {
             const int n = g.n0 + 16 * j;
             const bool on = n < cnt;
-            const float fac = early.f[j], mul = fac * inv, sub = -fac * off, ref = early.lse[j] * -LOG2E;
+            const float fac = early.f[j], mul = fac * inv, sub = -fac * off, ref = early.lse[j] * (KEEP ? -1.f : -LOG2E);
+            float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 T4 o;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float v = __builtin_fmaf(exp2_(__builtin_fmaf(acc[i][j][r], LOG2E, ref)), mul, sub);
-                    o[r] = to<T>(!at_edge || (on && g.m0 + 16 * i + r < p) ? v : 0.f);
+                    const float e = exp2_(__builtin_fmaf(acc[i][j][r], LOG2E, ref));
+                    const float v = !at_edge || (on && g.m0 + 16 * i + r < p) ? (KEEP ? e : __builtin_fmaf(e, mul, sub)) : 0.f;
+                    sum += v;
+                    o[r] = to<T>(v);
                 }
                 if constexpr (sizeof(T) == 2) *reinterpret_cast<T4 *>(patch + P::at(16 * j + (g.lane & 15), 2 * i + (g.lane >> 5)) + (g.lane >> 4 & 1) * 8) = o;
                 else {
@@ -745,12 +763,20 @@ template <typename T> struct EpiDz {
                 for (int i = 0; i < MI; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) z = d == 16 * i + r ? acc[i][j][r] : z;
+                if constexpr (KEEP) zy[n] = z;
+                else {
                 const T v = to<T>(__builtin_fmaf(exp2_(__builtin_fmaf(z, LOG2E, ref)), mul, sub - fac * label));
                 if constexpr (sizeof(T) == 2) *reinterpret_cast<T *>(patch + P::at(16 * j + (g.lane & 15), 2 * (d >> 4) + (g.lane >> 5)) + (g.lane >> 4 & 1) * 8 + (d & 3) * 2) = v;
                 else {
                     dz[(int64_t)n * ldc + g.m0 + d] = v;
                     dzt[(int64_t)(g.m0 + d) * ldn + n] = v;
                 }
+                }
+            }
+            if constexpr (KEEP) {
+                sum += __shfl_xor(sum, 16);
+                sum += __shfl_xor(sum, 32);
+                if (g.lane < 16) sh.t[g.wm * BN + n - g.tile_n * BN] = sum;
             }
         };
         if (edge) {
@@ -759,6 +785,15 @@ template <typename T> struct EpiDz {
         } else {
 #pragma unroll
             for (int j = 0; j < NJ; ++j) column(j, std::false_type{});
+        }
+        if constexpr (KEEP) {
+            __syncthreads();
+            if (g.tid < BN) {
+                float t = sh.t[g.tid];
+#pragma unroll
+                for (int w = 1; w < WM; ++w) t += sh.t[w * BN + g.tid];
+                part[(int64_t)g.tile_m * c.npad + g.tile_n * BN + g.tid] = t;
+            }
         }
         if constexpr (sizeof(T) == 2) {
             // from the patch both orders go out in 16-byte stores: its rows as they are, and transposed
@@ -777,6 +812,93 @@ template <typename T> struct EpiDz {
         }
     }
 };
+
+// ---- E kept from the first pass ---------------------------------------------------------------------------------------------------------
+// Without smoothing dz_j = f_j / S_j (E_vj - S_j [v = y_j]) with E_vj = exp(z_vj - r_j), S_j = sum_v E_vj, whatever r_j is.  With r_j the
+// label's logit S_j = exp(l_j): between 1 and 10^30 for every loss that training sees.  So E is written by the pass that sums it, and the
+// logits are formed once: the column's factor f_j / S_j goes on dH's result and, rounded once more, on H's image for dW.
+struct Keep {
+    const float *part;        // [tile_m][npad]
+    const float *f, *ref, *zy;
+    const int *idx, *y;
+    const Info *info;
+    int tiles, npad, reduction, k, per;   // per: columns of a tile of the product (what is done again)
+    float *lse_c, *loss_c, *lse, *loss;
+    float *scale, *again_f;   // of a column: f_j / S_j, and what its dz is multiplied by if it is formed again
+    int *again;               // per tile: some column's sum is out of range
+    int64_t ldc, ldn;
+};
+constexpr float SUM_MOST = 1e30f;
+// r_j, by a wave a column; and no tile is to be done again
+template <typename T> __global__ __launch_bounds__(256) void label_kernel(Keep s, const T *w, int64_t ldw, int wchunks, const T *h, int64_t ldh, float *ref, int tiles_n) {
+    if (blockIdx.x == 0)
+        for (int t = threadIdx.x; t < tiles_n; t += 256) s.again[t] = 0;
+    const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (i >= s.info->count) return;
+    const int v = s.y[i];
+    float d = 0.f;
+    if (v >= 0)
+        for (int q = lane; q < wchunks; q += 64) {
+            const tn::u32x4 a = *reinterpret_cast<const tn::u32x4 *>(reinterpret_cast<const char *>(w + v * ldw) + q * 16), b = *reinterpret_cast<const tn::u32x4 *>(reinterpret_cast<const char *>(h + i * ldh) + q * 16);
+            const T *x = reinterpret_cast<const T *>(&a), *y = reinterpret_cast<const T *>(&b);
+#pragma unroll
+            for (int u = 0; u < 16 / (int)sizeof(T); ++u) d = __builtin_fmaf((float)x[u], (float)y[u], d);
+        }
+    for (int o = 32; o; o >>= 1) d += __shfl_xor(d, o);
+    if (lane == 0) ref[i] = d * LOG2E;
+}
+// joins the tiles' sums of 2^lc (at least 8) columns, finishes them, puts the label's entry right and scales H's image
+template <typename T> __global__ __launch_bounds__(256) void keep_kernel(Keep s, T *dz, T *dzt, T *ht, int lc) {
+    __shared__ float ps[256], by[256];
+    const int cols = 1 << lc, step = 256 >> lc, at = threadIdx.x & (cols - 1), slice = threadIdx.x >> lc;
+    const int cnt = s.info->count, i0 = blockIdx.x * cols, i = i0 + at;
+    if (i0 >= cnt) return;
+    float a = 0.f;
+#pragma unroll 4
+    for (int q = slice; q < s.tiles; q += step) a += s.part[(int64_t)q * s.npad + i];
+    ps[threadIdx.x] = a;
+    for (int o = step / 2; o; o >>= 1) {
+        __syncthreads();
+        if (slice < o) ps[threadIdx.x] += ps[threadIdx.x + (o << lc)];
+    }
+    if (slice == 0) {
+        by[at] = 0.f;
+        if (i < cnt) {
+            const float sum = ps[at], r = s.ref[i], f = s.f[i];
+            const int lab = s.y[i];
+            const bool good = sum < SUM_MOST;
+            float v = __builtin_nanf(""), l = v, c = v;
+            if (lab >= 0) {
+                v = (r + log2f(sum)) * LN2;
+                l = v - s.zy[i];
+                c = good ? f / sum : 1.f;
+                const T e = to<T>(exp2_(__builtin_fmaf(s.zy[i], LOG2E, -r)) - sum);
+                dz[i * s.ldc + lab] = e;
+                dzt[lab * s.ldn + i] = e;
+            }
+            if (!good) s.again[i / s.per] = 1;
+            s.lse_c[i] = v;
+            s.loss_c[i] = l;
+            const int col = s.idx[i];
+            if (s.lse) s.lse[col] = v;
+            if (s.loss && s.reduction == NMFX_REDUCE_NONE) s.loss[col] = l;
+            s.scale[i] = by[at] = c;
+            s.again_f[i] = good ? sum : f;
+        }
+    }
+    __syncthreads();
+    constexpr int V = 16 / sizeof(T);
+    const int chunks = cols / V;
+    for (int e = threadIdx.x; e < s.k * chunks; e += 256) {
+        const int c = e / chunks, o = e % chunks * V;
+        tn::u32x4 *x = reinterpret_cast<tn::u32x4 *>(ht + c * s.ldn + i0 + o);
+        tn::u32x4 v = *x;
+        T *t = reinterpret_cast<T *>(&v);
+#pragma unroll
+        for (int u = 0; u < V; ++u) t[u] = to<T>((float)t[u] * by[o + u]);
+        *x = v;
+    }
+}
 
 // ---- sums of products kept in f32: slot s of [split][n][ld], m contiguous -------------------------------------------------------------
 struct EpiSlot {
@@ -812,17 +934,18 @@ template <typename T> struct EpiOut {
     const Info *info;
     int mmax, nmax, wide;     // wide: four consecutive m go in one store
     const int *cols, *count;  // column n goes to column cols[n], for n < *count; or NULL
+    const float *scale;       // of column n, or NULL
     template <int MI, int NJ> using Early = tn::None;
     template <int BM, int BN, int WM, int WN> using Shared = tn::None;
     template <int BM, int BN, int WM, int WN> __device__ __forceinline__ void begin(const Geom &, tn::None &, tn::None &) const {}
     template <int BM, int BN, int WM, int WN, int MI, int NJ>
     __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, tn::None &, tn::None &, char *, char *) const {
         typedef T T4 __attribute__((ext_vector_type(4)));
-        const float u = info->unscale;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             int n = g.n0 + 16 * j;
             if (n >= (cols ? *count : nmax)) continue;
+            const float u = info->unscale * (scale ? scale[n] : 1.f);
             if (cols) n = cols[n];
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
@@ -847,6 +970,7 @@ template <typename T> struct Join {
     int64_t ld, slot;
     int nslots;
     const int *pos;
+    const float *scale;       // of a packed column, or NULL
     int mmax, nmax;
     T *out;
     int64_t ms, ns;
@@ -873,10 +997,11 @@ template <typename T> struct Join {
             for (int o = 1; o < 1 << lanes; o <<= 1)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) s[q] += __shfl_xor(s[q], o);
+            const float by = scale && from >= 0 ? u * scale[from] : u;
             if (e < total && part == 0)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    if (m + q < mmax) out[(m + q) * ms + n * ns] = to<T>(s[q] * u);
+                    if (m + q < mmax) out[(m + q) * ms + n * ns] = to<T>(s[q] * by);
         }
     }
 };
@@ -912,8 +1037,9 @@ struct Shape {
     int64_t ldslot;
     Choice z, h, w;               // the products Z, W' dz, dz H'
     bool w_slots, direct;         // direct: dH need not be summed from slots
+    bool keep;                    // E is kept from the first pass
     // workspace offsets
-    int64_t o_info, o_counts, o_idx, o_pos, o_y, o_f, o_lse, o_loss, o_zy, o_h, o_ht, o_w, o_wt, o_part, o_zsum, o_dz, o_dzt, o_hslot, o_wslot, bytes;
+    int64_t o_info, o_counts, o_idx, o_pos, o_y, o_f, o_lse, o_loss, o_zy, o_h, o_ht, o_w, o_wt, o_part, o_zsum, o_ref, o_scale, o_again_f, o_again, o_dz, o_dzt, o_hslot, o_wslot, bytes;
 };
 
 constexpr int CUS = 256;
@@ -942,13 +1068,13 @@ Guess guess(int kind, int64_t m, int64_t n, int64_t ktiles, int es, bool split) 
     }
     return best;
 }
-Choice choose(int64_t m, int64_t n, int64_t ktiles, int es) {
+Guess choose(int64_t m, int64_t n, int64_t ktiles, int es) {
     Guess best{{2, 1}, 1e30};
     for (int k = 0; k < 3; ++k) {
         const Guess g = guess(k, m, n, ktiles, es, false);
         if (g.us < best.us) best = g;
     }
-    return best.c;
+    return best;
 }
 // The two gradient products: each by the kind that suits it, or both by one kind in one launch; and, where neither is split, without the
 // launch that joins the slots (dH then goes straight to its columns).  A launch costs about LAUNCH us, the host's part or the gap it leaves.
@@ -963,6 +1089,14 @@ void choose_two(int64_t hm, int64_t hn, int64_t hk, int64_t wm, int64_t wn, int6
         if (direct) take(guess(k, hm, hn, hk, es, false), guess(k, wm, wn, wk, es, false), -2.);
     }
 }
+
+// E is kept from the first pass where a pass over the logits takes longer than this estimate (us), and so more than the two launches that come
+// with it: f32, 5000 x 1000, k = 100 (estimate 18): 100 -> 83 us; 2000 x 400, k = 42 (3.3): 33 -> 35 us.  In bf16 it costs dW a rounding (of the
+// scaled H; 32768 x 4096, k = 1024: 1067 -> 894 us), from few columns not averaged: more is asked for.  1551 x 2221, k = 1568 (21): 105 -> 109 us;
+// 8192 x 2048, k = 1024 (28): 180 -> 163.  (f16 has not the range for E, smoothing takes a part from every entry that E's rounding would
+// show in, and of several pieces the first ones' E would have to wait for the last one's sums.)
+constexpr double KEEP_US_F32 = 6., KEEP_US_BF16 = 25.;
+constexpr int KEEP_COLUMNS = 256;
 
 Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     Shape s{};
@@ -985,7 +1119,9 @@ Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     s.ldn = s.npad + 256 / s.es; s.ldp = s.ppad + 256 / s.es; s.ldc = s.piece + 256 / s.es;
     const int64_t n1 = std::max<int64_t>(s.n, 1);
     const int64_t pp = std::min(s.piece, s.p);
-    s.z = choose(pp, n1, s.kpad / step, s.es);
+    const Guess z = choose(pp, n1, s.kpad / step, s.es);
+    s.z = z.c;
+    s.keep = grad && !smooth && W.dtype != NMFX_F16 && s.pieces == 1 && s.n >= KEEP_COLUMNS && z.us > (W.dtype == NMFX_F32 ? KEEP_US_F32 : KEEP_US_BF16);
     choose_two(s.k, n1, (pp + step - 1) / step, pp, s.k, (n1 + step - 1) / step, s.es, s.pieces == 1, s.h, s.w);
     s.direct = s.pieces == 1 && s.h.splits == 1 && s.w.splits == 1 && s.h.kind == s.w.kind;
     s.w_slots = s.w.splits > 1;
@@ -999,6 +1135,8 @@ Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     const int64_t tiles = (s.p + KINDS[s.z.kind].m - 1) / KINDS[s.z.kind].m, parts = std::max<int64_t>(tiles * s.npad, 16 * 4 * CUS);
     s.o_part = take(parts * sizeof(float2));
     s.o_zsum = smooth ? take(parts * 4) : -1;
+    s.o_ref = s.o_scale = s.o_again_f = s.o_again = -1;
+    if (s.keep) { s.o_ref = take(s.npad * 4); s.o_scale = take(s.npad * 4); s.o_again_f = take(s.npad * 4); s.o_again = take(s.npad / 64 * 4); }
     s.o_w = s.w_rows_direct ? -1 : take(s.p * s.kpad * s.es);
     s.o_ht = s.o_wt = s.o_dz = s.o_dzt = s.o_hslot = s.o_wslot = -1;
     if (grad) {
@@ -1080,6 +1218,33 @@ template <typename T> void score(const Call &c, const Shape &s) {
     ops::hip_ok(hipGetLastError(), "score");
 }
 
+// the first pass with E kept, up to the images that the gradient products read
+template <typename T, typename F, typename I>
+void keep_first(const Call &c, const Shape &s, const T *w, int64_t ldw, int wchunks, const tn::Operand &hop, const T *h, T *ht, T *dz, T *dzt, const Combine &cb, F f32, I i32) {
+    const int n = (int)s.n, p = (int)s.p, es = sizeof(T), n1 = std::max(n, 1);
+    const int *count = &cb.info->count;
+    tn::Args a{{w, ldw * es, p, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, (int)(s.kpad * es / 128)};
+    grid(a, p, n1, s.z);
+    const Keep kp{f32(s.o_part), f32(s.o_f), f32(s.o_ref), f32(s.o_zy), i32(s.o_idx), i32(s.o_y), cb.info, a.tiles_m, (int)s.npad, c.o.reduction, (int)s.k, KINDS[s.z.kind].n,
+                  f32(s.o_lse), f32(s.o_loss), c.lse, c.loss, f32(s.o_scale), f32(s.o_again_f), i32(s.o_again), s.ldc, s.ldn};
+    label_kernel<T><<<(n1 + 3) / 4, 256, 0, c.st>>>(kp, w, ldw, wchunks, h, s.kpad, f32(s.o_ref), a.tiles_n);
+    ops::hip_ok(hipGetLastError(), "label");
+    product<T>(a, p, n1, s.z, EpiDz<T, true>{dz, dzt, s.ldc, s.ldn, f32(s.o_ref), nullptr, i32(s.o_y), count, p, 0, 1.f, 0.f, 0.f, 0, cb, f32(s.o_part), f32(s.o_zy)}, c.st);
+    int lc = 6;
+    while (lc > 3 && (n1 >> lc) < CUS) --lc;
+    keep_kernel<T><<<(n1 + (1 << lc) - 1) >> lc, 256, 0, c.st>>>(kp, dz, dzt, ht, lc);
+    ops::hip_ok(hipGetLastError(), "keep");
+    // columns whose sums left the range of E, by tiles: the way with a pass for the log-sum-exp in front
+    const EpiStats ea{const_cast<float2 *>(cb.part), nullptr, f32(s.o_zy), i32(s.o_y), count, p, (int)s.npad};
+    const EpiDz<T> eb{dz, dzt, s.ldc, s.ldn, f32(s.o_lse), f32(s.o_again_f), i32(s.o_y), count, p, 0, 1.f, 1.f, 0.f, 0, cb, nullptr, nullptr};
+    switch (s.z.kind) {
+        case 0: tn::tn_again_kernel<T, 256, 256, 2, 4, 2, EpiStats, Columnwise, EpiDz<T>><<<a.tiles_n, 512, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
+        case 1: tn::tn_again_kernel<T, 128, 128, 2, 2, 2, EpiStats, Columnwise, EpiDz<T>><<<a.tiles_n, 256, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
+        default: tn::tn_again_kernel<T, 64, 64, 2, 2, 4, EpiStats, Columnwise, EpiDz<T>><<<a.tiles_n, 256, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
+    }
+    ops::hip_ok(hipGetLastError(), "again");
+}
+
 template <typename T> void run(const Call &c, const Shape &s) {
     if (!c.grad && scored(s)) return score<T>(c, s);
     const int es = sizeof(T), step = 128 / es, per = 16 / es;
@@ -1123,8 +1288,13 @@ template <typename T> void run(const Call &c, const Shape &s) {
     const Combine cb{reinterpret_cast<float2 *>(ws + s.o_part), s.o_zsum >= 0 ? f32(s.o_zsum) : nullptr, f32(s.o_zy), i32(s.o_idx), i32(s.o_y), info, tiles, (int)s.npad, p,
                      c.o.reduction, eps, f32(s.o_lse), f32(s.o_loss), c.lse, c.loss};
     // dz's blocks join the tiles' statistics of their columns themselves where that is a few of them: less than a launch
-    const bool few = c.grad && !c.lse_given && s.pieces == 1 && tiles <= 64 && (int64_t)tiles * ((n1 + KINDS[s.z.kind].n - 1) / KINDS[s.z.kind].n) <= 2 * CUS;
-    if (!c.lse_given) {
+    const bool keep = s.keep && !c.lse_given;
+    const bool few = c.grad && !c.lse_given && !keep && s.pieces == 1 && tiles <= 64 && (int64_t)tiles * ((n1 + KINDS[s.z.kind].n - 1) / KINDS[s.z.kind].n) <= 2 * CUS;
+    T *dz = c.grad ? reinterpret_cast<T *>(ws + s.o_dz) : nullptr, *dzt = c.grad ? reinterpret_cast<T *>(ws + s.o_dzt) : nullptr;
+    const float inv = (float)(1. / a_), label = (float)((1. - c.o.label_smoothing) / a_), off = (float)(c.o.label_smoothing / (a_ * p));
+    if (keep) {
+        if constexpr (!std::is_same<T, _Float16>::value) keep_first<T>(c, s, w, ldw, wchunks, hop, h, ht, dz, dzt, cb, f32, i32);
+    } else if (!c.lse_given) {
         tn::Args a{{w, ldw * es, p, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt};
         stream<T>(a, p, n1, s.z, EpiStats{reinterpret_cast<float2 *>(ws + s.o_part), s.o_zsum >= 0 ? f32(s.o_zsum) : nullptr, f32(s.o_zy), i32(s.o_y), count, p, (int)s.npad}, c.st);
         if (!few) {
@@ -1137,7 +1307,7 @@ template <typename T> void run(const Call &c, const Shape &s) {
     }
     if (!c.grad) return;
 
-    T *dz = reinterpret_cast<T *>(ws + s.o_dz), *dzt = reinterpret_cast<T *>(ws + s.o_dzt);
+    const float *scale = keep ? f32(s.o_scale) : nullptr;
     T *dw = static_cast<T *>(c.dW.data), *dh = static_cast<T *>(c.dH.data);
     const bool add = !c.lse_given && c.loss && c.o.reduction != NMFX_REDUCE_NONE;
     for (int64_t q = 0; q < s.pieces; ++q) {
@@ -1145,8 +1315,8 @@ template <typename T> void run(const Call &c, const Shape &s) {
         const int pv = (int)std::min(s.piece, s.p - v0), pt = (int)up(pv, step);
         const bool last = q + 1 == s.pieces;
         tn::Args a{{w + v0 * ldw, ldw * es, pv, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt};
-        product<T>(a, pv, n1, s.z, EpiDz<T>{dz, dzt, s.ldc, s.ldn, f32(s.o_lse), f32(s.o_f), i32(s.o_y), count, pv, (int)v0, (float)(1. / a_),
-                   (float)((1. - c.o.label_smoothing) / a_), (float)(c.o.label_smoothing / (a_ * p)), few, cb}, c.st);
+        if (!keep)
+            product<T>(a, pv, n1, s.z, EpiDz<T>{dz, dzt, s.ldc, s.ldn, f32(s.o_lse), f32(s.o_f), i32(s.o_y), count, pv, (int)v0, inv, label, off, few, cb, nullptr, nullptr}, c.st);
         // dH: rows are components, columns are packed columns
         tn::Args b{{wt + v0, ldwt * es, k, (int)std::min<int64_t>((wtpad - v0) / per, s.piece / per)}, {dz, s.ldc * es, (int)s.npad, (int)(s.piece / per)}, count, tn::LIMIT_N, 0, 0, 0, pt / step};
         const EpiSlot eh{f32(s.o_hslot), s.ldslot, s.npad * s.ldslot, (int)s.npad, q > 0};
@@ -1159,21 +1329,21 @@ template <typename T> void run(const Call &c, const Shape &s) {
         tn::Args d{kfast ? top : zop, kfast ? zop : top, count, tn::LIMIT_C, 0, 0, 0, (int)(s.npad / step)};
         Join<T> jh{}, jw{};
         const bool wide = ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * es - 1)) == 0;
-        const EpiOut<T> ew{out, ldo, info, mm, nn, wide, nullptr, nullptr};
+        const EpiOut<T> ew{out, ldo, info, mm, nn, wide, nullptr, nullptr, nullptr};
         if (direct) {
             const bool hwide = c.dH.cs % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & (4 * es - 1)) == 0;
-            products<T>(b, k, n1, s.h, EpiOut<T>{dh, c.dH.cs, info, k, n, hwide, i32(s.o_idx), count}, d, mm, nn, s.w, ew, Losses{f32(s.o_loss), info, c.o.reduction, add ? c.loss : nullptr}, c.st);
+            products<T>(b, k, n1, s.h, EpiOut<T>{dh, c.dH.cs, info, k, n, hwide, i32(s.o_idx), count, scale}, d, mm, nn, s.w, ew, Losses{f32(s.o_loss), info, c.o.reduction, add ? c.loss : nullptr}, c.st);
             return;
         }
         if (s.w_slots) {
             const int64_t ld = up(mm, 4);
             products<T>(b, k, n1, s.h, eh, d, mm, nn, s.w, EpiSlot{f32(s.o_wslot), ld, ld * nn, nn, 0}, Losses{}, c.st);
             const JoinGrid jg = join_grid(mm, nn, s.w.splits);
-            jw = Join<T>{f32(s.o_wslot), ld, ld * nn, s.w.splits, nullptr, mm, nn, out, 1, ldo, jg.blocks, jg.lanes};
+            jw = Join<T>{f32(s.o_wslot), ld, ld * nn, s.w.splits, nullptr, nullptr, mm, nn, out, 1, ldo, jg.blocks, jg.lanes};
         } else products<T>(b, k, n1, s.h, eh, d, mm, nn, s.w, ew, Losses{}, c.st);
         if (last && n) {
             const JoinGrid jg = join_grid(k, n, s.h.splits);
-            jh = Join<T>{f32(s.o_hslot), s.ldslot, s.npad * s.ldslot, s.h.splits, i32(s.o_pos), k, n, dh, c.dH.rs, c.dH.cs, jg.blocks, jg.lanes};
+            jh = Join<T>{f32(s.o_hslot), s.ldslot, s.npad * s.ldslot, s.h.splits, i32(s.o_pos), scale, k, n, dh, c.dH.rs, c.dH.cs, jg.blocks, jg.lanes};
         }
         const int jb = jh.blocks + jw.blocks + (last && add);
         if (jb) {

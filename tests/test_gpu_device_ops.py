@@ -87,7 +87,7 @@ def oracle(W, H, y, eps=0.0, reduction="mean", gout=None, ignore=-100, dtype="f3
         total, etotal = loss.sum(), eloss.sum() + V * loss.abs().sum()
         if reduction == "mean":
             total, etotal = total / cnt, etotal / cnt
-    return dict(loss=total, lse=torch.where(on, lse, 0.0), dW=dW, dH=dH, eloss=etotal, else_=torch.where(on, elog, 0.0), edW=edW, edH=edH)
+    return dict(adz=dz.abs(), loss=total, lse=torch.where(on, lse, 0.0), dW=dW, dH=dH, eloss=etotal, else_=torch.where(on, elog, 0.0), edW=edW, edH=edH)
 
 
 def near(name, got, want, bound):
@@ -97,9 +97,13 @@ def near(name, got, want, bound):
     assert (over <= 0).all(), f"{name}: off by {float(off.flatten()[over.argmax()]):.3e} where {float(bound.expand_as(off).flatten()[over.argmax()]):.3e} is allowed"
 
 
-def check(W, H, y, dtype, eps=0.0, reduction="mean", gout=None, ignore=-100):
+def check(W, H, y, dtype, eps=0.0, reduction="mean", gout=None, ignore=-100, scaled_h=False):
+    """scaled_h: dW's product may take H times a factor of its column, rounded: half a step of every |dz| |h| more."""
     kw = dict(ignore_index=ignore, label_smoothing=eps, reduction=reduction)
     want = oracle(W, H, y, eps, reduction, gout, ignore, dtype)
+    if scaled_h:
+        on = y != ignore
+        want["edW"] = want["edW"] + HALF_STEP[dtype] * (want["adz"] @ torch.where(on[None, :], H.double(), 0.0).abs().t())
     loss, lse = nmfx.softmax_xent(W, H, y, **kw)
     near("loss", loss, want["loss"], want["eloss"])
     near("lse", lse, want["lse"], want["else_"])
@@ -273,6 +277,70 @@ def test_xent_factors_of_many_columns(n):
         gout = torch.rand(n, device=DEV) - 0.5
         gout[-1] = -512.0
         check(W, H, y, dtype, reduction="none", gout=gout)
+
+
+# sizes that form the logits once
+ONCE = [("f32", 1024, 300, 300), ("f32", 5000, 1000, 100), ("f32", 1537, 2500, 129), ("bf16", 8192, 2048, 1024), ("bf16", 9001, 2100, 1000)]
+
+
+@pytest.mark.parametrize("dtype,p,n,k", ONCE)
+@pytest.mark.parametrize("wl,ignored,reduction", [("r", 0.0, "mean"), ("c", 0.4, "none"), ("r+o", 0.95, "sum"), ("r", 1.0, "mean")])
+def test_xent_logits_formed_once(dtype, p, n, k, wl, ignored, reduction):
+    W, H, y = problem(p, n, k, dtype, seed=p + n, ignored=ignored, wl=wl)
+    gout = torch.linspace(-2, 2, n, device=DEV) if reduction == "none" else None
+    check(W, H, y, dtype, reduction=reduction, gout=gout, scaled_h=True)
+
+
+@pytest.mark.parametrize("dtype,p,n,k", ONCE[1:4])
+def test_xent_losses_beyond_any_exponential(dtype, p, n, k):
+    """Columns whose losses are near and far beyond where exp() of them leaves Float32 (88.7), among ordinary ones, in some column tiles."""
+    W, H, y = problem(p, n, k, dtype, seed=k)
+    cols = torch.tensor([3, 4, 5, 6, n // 2, n - 1], device=DEV)
+    z = W.double() @ H[:, cols].double()
+    y[cols] = z.argmin(0)
+    spread = z.max(0).values - z.min(0).values
+    H = H.clone()
+    H[:, cols] = (H[:, cols].double() * (torch.tensor([50.0, 68.0, 75.0, 87.0, 200.0, 1000.0], device=DEV, dtype=torch.float64) / spread)).to(H.dtype)
+    check(W, H, y, dtype, reduction="none", gout=torch.linspace(-1, 1, n, device=DEV), scaled_h=True)
+
+
+@pytest.mark.parametrize("dtype,p,n,k", ONCE[1:4])
+def test_xent_formed_once_keeps_nan_and_no_classes_to_their_columns(dtype, p, n, k):
+    W, H, y = problem(p, n, k, dtype, seed=1, ignored=0.3)
+    good = nmfx.softmax_xent_grad(W, H, y, reduction="none")
+    on = torch.nonzero(y != -100).flatten()
+    H2, y2 = H.clone(), y.clone()
+    H2[1, on[0]] = float("nan")
+    H2[0, on[7]] = float("inf")
+    y2[on[9]] = p
+    y2[on[11]] = -1
+    loss, lse, dW, dH = nmfx.softmax_xent_grad(W, H2, y2, reduction="none")
+    bad = torch.zeros(n, dtype=torch.bool, device=DEV)
+    bad[on[[0, 7, 9, 11]]] = True
+    assert loss[bad].isnan().all() and lse[bad][[0, 2, 3]].isnan().all() and dH[:, bad].isnan().all(0).all() and dW.isnan().all()
+    for name, a, b, t in (("loss", loss, good[0], 2.0 ** -20), ("lse", lse, good[1], 2.0 ** -20), ("dH", dH, good[3], 4 * HALF_STEP[dtype])):
+        a, b = a[..., ~bad].double(), b[..., ~bad].double()
+        assert ((a - b).abs() <= t * b.abs().max()).all(), name
+
+
+def test_xent_formed_once_in_a_graph():
+    W, H, y = problem(4000, 900, 120, "f32", ignored=0.2)
+    kw = dict(reduction="sum", dW=torch.empty_like(W), dH=torch.empty_like(H.t()).t())
+    nmfx.softmax_xent_grad(W, H, y, **kw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, lse, dW, dH = nmfx.softmax_xent_grad(W, H, y, **kw)
+    for r in range(4):
+        H.copy_(torch.randn_like(H))
+        if r == 2:
+            H[:, 5] *= 300
+            y[5] = (W @ H[:, 5]).argmin()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (loss, lse, dW, dH)]
+        for a, b in zip(got, nmfx.softmax_xent_grad(W, H, y, reduction="sum")):
+            assert torch.equal(a, b), r
 
 
 def test_xent_same_bits_twice_and_given_outputs():
