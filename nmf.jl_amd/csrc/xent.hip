@@ -341,13 +341,13 @@ struct EpiStats {
     float *zy;            // packed: the label's logit
     const int *y;
     const int *count;
-    int p, npad;
+    int p, v0, npad;      // classes of the piece that exist; its first class
     template <int MI, int NJ> struct Early { int cnt, y[NJ]; };
     template <int BM, int BN, int WM, int WN> struct Shared { float2 s[WM * BN]; float t[WM * BN]; };
     template <int BM, int BN, int WM, int WN, typename E, typename S> __device__ __forceinline__ void begin(const Geom &g, E &early, S &) const {
         early.cnt = *count;
 #pragma unroll
-        for (int j = 0; j < BN / WN / 16; ++j) early.y[j] = g.n0 + 16 * j < early.cnt ? y[g.n0 + 16 * j] : -1;
+        for (int j = 0; j < BN / WN / 16; ++j) early.y[j] = g.n0 + 16 * j < early.cnt ? y[g.n0 + 16 * j] - v0 : -1;
     }
     template <int BM, int BN, int WM, int WN, int MI, int NJ, typename E, typename S>
     __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, const E &early, S &sh, char *, char *) const {
@@ -814,15 +814,18 @@ template <typename T, bool KEEP = false> struct EpiDz {
 };
 
 // ---- E kept from the first pass ---------------------------------------------------------------------------------------------------------
+// (Of the last piece of the classes: the first ones' E would have to wait for its sums.)
 // Without smoothing dz_j = f_j / S_j (E_vj - S_j [v = y_j]) with E_vj = exp(z_vj - r_j), S_j = sum_v E_vj, whatever r_j is.  With r_j the
 // label's logit S_j = exp(l_j): between 1 and 10^30 for every loss that training sees.  So E is written by the pass that sums it, and the
-// logits are formed once: the column's factor f_j / S_j goes on dH's result and, rounded once more, on H's image for dW.
+// logits are formed once: the column's factor f_j / S_j goes on dH's result and, rounded once more, on H's image for dW.  The other pieces'
+// dz are formed to go with that: times S_j / f_j.
 struct Keep {
-    const float *part;        // [tile_m][npad]
+    const float2 *before;     // [tile_m][npad]: statistics of the pieces in front
+    const float *part;        // [tile_m][npad]: sums of E
     const float *f, *ref, *zy;
     const int *idx, *y;
     const Info *info;
-    int tiles, npad, reduction, k, per;   // per: columns of a tile of the product (what is done again)
+    int tiles_before, tiles, v0, npad, reduction, k, per;   // v0: the piece's first class; per: columns of a tile of the product (what is done again)
     float *lse_c, *loss_c, *lse, *loss;
     float *scale, *again_f;   // of a column: f_j / S_j, and what its dz is multiplied by if it is formed again
     int *again;               // per tile: some column's sum is out of range
@@ -856,6 +859,12 @@ template <typename T> __global__ __launch_bounds__(256) void keep_kernel(Keep s,
     float a = 0.f;
 #pragma unroll 4
     for (int q = slice; q < s.tiles; q += step) a += s.part[(int64_t)q * s.npad + i];
+    const float r = i < cnt ? s.ref[i] : 0.f;
+#pragma unroll 4
+    for (int q = slice; q < s.tiles_before; q += step) {
+        const float2 b = s.before[(int64_t)q * s.npad + i];
+        a += b.y != 0.f ? b.y * exp2_(b.x - r) : 0.f;
+    }
     ps[threadIdx.x] = a;
     for (int o = step / 2; o; o >>= 1) {
         __syncthreads();
@@ -864,7 +873,7 @@ template <typename T> __global__ __launch_bounds__(256) void keep_kernel(Keep s,
     if (slice == 0) {
         by[at] = 0.f;
         if (i < cnt) {
-            const float sum = ps[at], r = s.ref[i], f = s.f[i];
+            const float sum = ps[at], f = s.f[i];
             const int lab = s.y[i];
             const bool good = sum < SUM_MOST;
             float v = __builtin_nanf(""), l = v, c = v;
@@ -872,9 +881,11 @@ template <typename T> __global__ __launch_bounds__(256) void keep_kernel(Keep s,
                 v = (r + log2f(sum)) * LN2;
                 l = v - s.zy[i];
                 c = good ? f / sum : 1.f;
-                const T e = to<T>(exp2_(__builtin_fmaf(s.zy[i], LOG2E, -r)) - sum);
-                dz[i * s.ldc + lab] = e;
-                dzt[lab * s.ldn + i] = e;
+                if (lab >= s.v0) {
+                    const T e = to<T>(exp2_(__builtin_fmaf(s.zy[i], LOG2E, -r)) - sum);
+                    dz[i * s.ldc + (lab - s.v0)] = e;
+                    dzt[(lab - s.v0) * s.ldn + i] = e;
+                }
             }
             if (!good) s.again[i / s.per] = 1;
             s.lse_c[i] = v;
@@ -1093,8 +1104,8 @@ void choose_two(int64_t hm, int64_t hn, int64_t hk, int64_t wm, int64_t wn, int6
 // E is kept from the first pass where a pass over the logits takes longer than this estimate (us), and so more than the two launches that come
 // with it: f32, 5000 x 1000, k = 100 (estimate 18): 100 -> 83 us; 2000 x 400, k = 42 (3.3): 33 -> 35 us.  In bf16 it costs dW a rounding (of the
 // scaled H; 32768 x 4096, k = 1024: 1067 -> 894 us), from few columns not averaged: more is asked for.  1551 x 2221, k = 1568 (21): 105 -> 109 us;
-// 8192 x 2048, k = 1024 (28): 180 -> 163.  (f16 has not the range for E, smoothing takes a part from every entry that E's rounding would
-// show in, and of several pieces the first ones' E would have to wait for the last one's sums.)
+// 8192 x 2048, k = 1024 (28): 180 -> 163; of several pieces, where only the last one's E is kept, the rounding is not taken.  (f16 has not the range for E, and smoothing takes a part from every entry that E's rounding would
+// show in.)
 constexpr double KEEP_US_F32 = 6., KEEP_US_BF16 = 25.;
 constexpr int KEEP_COLUMNS = 256;
 
@@ -1121,7 +1132,7 @@ Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     const int64_t pp = std::min(s.piece, s.p);
     const Guess z = choose(pp, n1, s.kpad / step, s.es);
     s.z = z.c;
-    s.keep = grad && !smooth && W.dtype != NMFX_F16 && s.pieces == 1 && s.n >= KEEP_COLUMNS && z.us > (W.dtype == NMFX_F32 ? KEEP_US_F32 : KEEP_US_BF16);
+    s.keep = grad && !smooth && W.dtype != NMFX_F16 && s.n >= KEEP_COLUMNS && (s.pieces == 1 || W.dtype == NMFX_F32) && z.us > (W.dtype == NMFX_F32 ? KEEP_US_F32 : KEEP_US_BF16);
     choose_two(s.k, n1, (pp + step - 1) / step, pp, s.k, (n1 + step - 1) / step, s.es, s.pieces == 1, s.h, s.w);
     s.direct = s.pieces == 1 && s.h.splits == 1 && s.w.splits == 1 && s.h.kind == s.w.kind;
     s.w_slots = s.w.splits > 1;
@@ -1221,22 +1232,25 @@ template <typename T> void score(const Call &c, const Shape &s) {
 // the first pass with E kept, up to the images that the gradient products read
 template <typename T, typename F, typename I>
 void keep_first(const Call &c, const Shape &s, const T *w, int64_t ldw, int wchunks, const tn::Operand &hop, const T *h, T *ht, T *dz, T *dzt, const Combine &cb, F f32, I i32) {
-    const int n = (int)s.n, p = (int)s.p, es = sizeof(T), n1 = std::max(n, 1);
+    const int n = (int)s.n, es = sizeof(T), n1 = std::max(n, 1), v0 = (int)((s.pieces - 1) * s.piece), p = (int)s.p - v0, before = v0 / KINDS[s.z.kind].m, kt = (int)(s.kpad * es / 128);
     const int *count = &cb.info->count;
-    tn::Args a{{w, ldw * es, p, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, (int)(s.kpad * es / 128)};
+    float2 *part = const_cast<float2 *>(cb.part), *here = part + (int64_t)before * s.npad;      // (a piece is whole tiles)
+    if (v0) stream<T>(tn::Args{{w, ldw * es, v0, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt}, v0, n1, s.z, EpiStats{part, nullptr, f32(s.o_zy), i32(s.o_y), count, v0, 0, (int)s.npad}, c.st);
+    tn::Args a{{w + v0 * ldw, ldw * es, p, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt};
     grid(a, p, n1, s.z);
-    const Keep kp{f32(s.o_part), f32(s.o_f), f32(s.o_ref), f32(s.o_zy), i32(s.o_idx), i32(s.o_y), cb.info, a.tiles_m, (int)s.npad, c.o.reduction, (int)s.k, KINDS[s.z.kind].n,
+    float *sums = reinterpret_cast<float *>(here);
+    const Keep kp{part, sums, f32(s.o_f), f32(s.o_ref), f32(s.o_zy), i32(s.o_idx), i32(s.o_y), cb.info, before, a.tiles_m, v0, (int)s.npad, c.o.reduction, (int)s.k, KINDS[s.z.kind].n,
                   f32(s.o_lse), f32(s.o_loss), c.lse, c.loss, f32(s.o_scale), f32(s.o_again_f), i32(s.o_again), s.ldc, s.ldn};
     label_kernel<T><<<(n1 + 3) / 4, 256, 0, c.st>>>(kp, w, ldw, wchunks, h, s.kpad, f32(s.o_ref), a.tiles_n);
     ops::hip_ok(hipGetLastError(), "label");
-    product<T>(a, p, n1, s.z, EpiDz<T, true>{dz, dzt, s.ldc, s.ldn, f32(s.o_ref), nullptr, i32(s.o_y), count, p, 0, 1.f, 0.f, 0.f, 0, cb, f32(s.o_part), f32(s.o_zy)}, c.st);
+    product<T>(a, p, n1, s.z, EpiDz<T, true>{dz, dzt, s.ldc, s.ldn, f32(s.o_ref), nullptr, i32(s.o_y), count, p, v0, 1.f, 0.f, 0.f, 0, cb, sums, f32(s.o_zy)}, c.st);
     int lc = 6;
     while (lc > 3 && (n1 >> lc) < CUS) --lc;
     keep_kernel<T><<<(n1 + (1 << lc) - 1) >> lc, 256, 0, c.st>>>(kp, dz, dzt, ht, lc);
     ops::hip_ok(hipGetLastError(), "keep");
     // columns whose sums left the range of E, by tiles: the way with a pass for the log-sum-exp in front
-    const EpiStats ea{const_cast<float2 *>(cb.part), nullptr, f32(s.o_zy), i32(s.o_y), count, p, (int)s.npad};
-    const EpiDz<T> eb{dz, dzt, s.ldc, s.ldn, f32(s.o_lse), f32(s.o_again_f), i32(s.o_y), count, p, 0, 1.f, 1.f, 0.f, 0, cb, nullptr, nullptr};
+    const EpiStats ea{here, nullptr, f32(s.o_zy), i32(s.o_y), count, p, v0, (int)s.npad};
+    const EpiDz<T> eb{dz, dzt, s.ldc, s.ldn, f32(s.o_lse), f32(s.o_again_f), i32(s.o_y), count, p, v0, 1.f, 1.f, 0.f, 0, cb, nullptr, nullptr};
     switch (s.z.kind) {
         case 0: tn::tn_again_kernel<T, 256, 256, 2, 4, 2, EpiStats, Columnwise, EpiDz<T>><<<a.tiles_n, 512, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
         case 1: tn::tn_again_kernel<T, 128, 128, 2, 2, 2, EpiStats, Columnwise, EpiDz<T>><<<a.tiles_n, 256, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
@@ -1296,7 +1310,7 @@ template <typename T> void run(const Call &c, const Shape &s) {
         if constexpr (!std::is_same<T, _Float16>::value) keep_first<T>(c, s, w, ldw, wchunks, hop, h, ht, dz, dzt, cb, f32, i32);
     } else if (!c.lse_given) {
         tn::Args a{{w, ldw * es, p, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt};
-        stream<T>(a, p, n1, s.z, EpiStats{reinterpret_cast<float2 *>(ws + s.o_part), s.o_zsum >= 0 ? f32(s.o_zsum) : nullptr, f32(s.o_zy), i32(s.o_y), count, p, (int)s.npad}, c.st);
+        stream<T>(a, p, n1, s.z, EpiStats{reinterpret_cast<float2 *>(ws + s.o_part), s.o_zsum >= 0 ? f32(s.o_zsum) : nullptr, f32(s.o_zy), i32(s.o_y), count, p, 0, (int)s.npad}, c.st);
         if (!few) {
             // as many threads for a column as leave every compute unit a block
             int lc = 6;
@@ -1310,16 +1324,16 @@ template <typename T> void run(const Call &c, const Shape &s) {
     const float *scale = keep ? f32(s.o_scale) : nullptr;
     T *dw = static_cast<T *>(c.dW.data), *dh = static_cast<T *>(c.dH.data);
     const bool add = !c.lse_given && c.loss && c.o.reduction != NMFX_REDUCE_NONE;
-    for (int64_t q = 0; q < s.pieces; ++q) {
-        const int64_t v0 = q * s.piece;
+    for (int64_t t = 0; t < s.pieces; ++t) {
+        const int64_t q = keep ? s.pieces - 1 - t : t, v0 = q * s.piece;      // (the piece whose E was kept first)
         const int pv = (int)std::min(s.piece, s.p - v0), pt = (int)up(pv, step);
-        const bool last = q + 1 == s.pieces;
+        const bool last = t + 1 == s.pieces;
         tn::Args a{{w + v0 * ldw, ldw * es, pv, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt};
-        if (!keep)
-            product<T>(a, pv, n1, s.z, EpiDz<T>{dz, dzt, s.ldc, s.ldn, f32(s.o_lse), f32(s.o_f), i32(s.o_y), count, pv, (int)v0, inv, label, off, few, cb, nullptr, nullptr}, c.st);
+        if (!keep || t)
+            product<T>(a, pv, n1, s.z, EpiDz<T>{dz, dzt, s.ldc, s.ldn, f32(s.o_lse), f32(keep ? s.o_again_f : s.o_f), i32(s.o_y), count, pv, (int)v0, inv, label, off, few, cb, nullptr, nullptr}, c.st);
         // dH: rows are components, columns are packed columns
         tn::Args b{{wt + v0, ldwt * es, k, (int)std::min<int64_t>((wtpad - v0) / per, s.piece / per)}, {dz, s.ldc * es, (int)s.npad, (int)(s.piece / per)}, count, tn::LIMIT_N, 0, 0, 0, pt / step};
-        const EpiSlot eh{f32(s.o_hslot), s.ldslot, s.npad * s.ldslot, (int)s.npad, q > 0};
+        const EpiSlot eh{f32(s.o_hslot), s.ldslot, s.npad * s.ldslot, (int)s.npad, t > 0};
         // dW: the contiguous index of dW is the row
         const tn::Operand zop{dzt, s.ldn * es, pv, (int)(s.npad / per)}, top{ht, s.ldn * es, k, (int)(s.npad / per)};
         const bool kfast = c.dW.cs == 1;

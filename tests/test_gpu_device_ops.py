@@ -280,7 +280,7 @@ def test_xent_factors_of_many_columns(n):
 
 
 # sizes that form the logits once
-ONCE = [("f32", 1024, 300, 300), ("f32", 5000, 1000, 100), ("f32", 1537, 2500, 129), ("bf16", 8192, 2048, 1024), ("bf16", 9001, 2100, 1000)]
+ONCE = [("f32", 300001, 600, 9), ("f32", 1024, 300, 300), ("f32", 5000, 1000, 100), ("f32", 1537, 2500, 129), ("bf16", 8192, 2048, 1024), ("bf16", 9001, 2100, 1000)]
 
 
 @pytest.mark.parametrize("dtype,p,n,k", ONCE)
@@ -291,7 +291,7 @@ def test_xent_logits_formed_once(dtype, p, n, k, wl, ignored, reduction):
     check(W, H, y, dtype, reduction=reduction, gout=gout, scaled_h=True)
 
 
-@pytest.mark.parametrize("dtype,p,n,k", ONCE[1:4])
+@pytest.mark.parametrize("dtype,p,n,k", ONCE[:1] + ONCE[2:5])
 def test_xent_losses_beyond_any_exponential(dtype, p, n, k):
     """Columns whose losses are near and far beyond where exp() of them leaves Float32 (88.7), among ordinary ones, in some column tiles."""
     W, H, y = problem(p, n, k, dtype, seed=k)
@@ -304,7 +304,7 @@ def test_xent_losses_beyond_any_exponential(dtype, p, n, k):
     check(W, H, y, dtype, reduction="none", gout=torch.linspace(-1, 1, n, device=DEV), scaled_h=True)
 
 
-@pytest.mark.parametrize("dtype,p,n,k", ONCE[1:4])
+@pytest.mark.parametrize("dtype,p,n,k", ONCE[2:5])
 def test_xent_formed_once_keeps_nan_and_no_classes_to_their_columns(dtype, p, n, k):
     W, H, y = problem(p, n, k, dtype, seed=1, ignored=0.3)
     good = nmfx.softmax_xent_grad(W, H, y, reduction="none")
