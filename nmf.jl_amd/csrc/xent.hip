@@ -672,7 +672,7 @@ __global__ __launch_bounds__(1024) void score_join_kernel(Score a, int blocks, f
 // ---- dz of a piece of the classes, in both orders -----------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ T to(float x) { return (T)x; }
 
-// KEEP: the same images of E = exp(z - r_j) instead, before the log-sum-exp is known, with the tiles' sums of E and the labels' logits.
+// KEEP (f32): the same images of E = exp(z - r_j) instead, before the log-sum-exp is known, with the tiles' sums of E and the labels' logits.
 template <typename T, bool KEEP = false> struct EpiDz {
     T *dz, *dzt;              // [npad][ldc] by packed column, [classes of the piece][ldn] by class
     int64_t ldc, ldn;
@@ -817,7 +817,7 @@ template <typename T, bool KEEP = false> struct EpiDz {
 // (Of the last piece of the classes: the first ones' E would have to wait for its sums.)
 // Without smoothing dz_j = f_j / S_j (E_vj - S_j [v = y_j]) with E_vj = exp(z_vj - r_j), S_j = sum_v E_vj, whatever r_j is.  With r_j the
 // label's logit S_j = exp(l_j): between 1 and 10^30 for every loss that training sees.  So E is written by the pass that sums it, and the
-// logits are formed once: the column's factor f_j / S_j goes on dH's result and, rounded once more, on H's image for dW.  The other pieces'
+// logits are formed once: the column's factor f_j / S_j goes on dH's result and on H's image for dW.  The other pieces'
 // dz are formed to go with that: times S_j / f_j.
 struct Keep {
     const float2 *before;     // [tile_m][npad]: statistics of the pieces in front
@@ -833,7 +833,7 @@ struct Keep {
 };
 constexpr float SUM_MOST = 1e30f;
 // r_j, by a wave a column; and no tile is to be done again
-template <typename T> __global__ __launch_bounds__(256) void label_kernel(Keep s, const T *w, int64_t ldw, int wchunks, const T *h, int64_t ldh, float *ref, int tiles_n) {
+__global__ __launch_bounds__(256) void label_kernel(Keep s, const float *w, int64_t ldw, int chunks, const float *h, int64_t ldh, float *ref, int tiles_n) {
     if (blockIdx.x == 0)
         for (int t = threadIdx.x; t < tiles_n; t += 256) s.again[t] = 0;
     const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -841,17 +841,16 @@ template <typename T> __global__ __launch_bounds__(256) void label_kernel(Keep s
     const int v = s.y[i];
     float d = 0.f;
     if (v >= 0)
-        for (int q = lane; q < wchunks; q += 64) {
-            const tn::u32x4 a = *reinterpret_cast<const tn::u32x4 *>(reinterpret_cast<const char *>(w + v * ldw) + q * 16), b = *reinterpret_cast<const tn::u32x4 *>(reinterpret_cast<const char *>(h + i * ldh) + q * 16);
-            const T *x = reinterpret_cast<const T *>(&a), *y = reinterpret_cast<const T *>(&b);
+        for (int q = lane; q < chunks; q += 64) {
+            const f32x4 a = reinterpret_cast<const f32x4 *>(w + v * ldw)[q], b = reinterpret_cast<const f32x4 *>(h + i * ldh)[q];
 #pragma unroll
-            for (int u = 0; u < 16 / (int)sizeof(T); ++u) d = __builtin_fmaf((float)x[u], (float)y[u], d);
+            for (int u = 0; u < 4; ++u) d = __builtin_fmaf(a[u], b[u], d);
         }
     for (int o = 32; o; o >>= 1) d += __shfl_xor(d, o);
     if (lane == 0) ref[i] = d * LOG2E;
 }
 // joins the tiles' sums of 2^lc (at least 8) columns, finishes them, puts the label's entry right and scales H's image
-template <typename T> __global__ __launch_bounds__(256) void keep_kernel(Keep s, T *dz, T *dzt, T *ht, int lc) {
+__global__ __launch_bounds__(256) void keep_kernel(Keep s, float *dz, float *dzt, float *ht, int lc) {
     __shared__ float ps[256], by[256];
     const int cols = 1 << lc, step = 256 >> lc, at = threadIdx.x & (cols - 1), slice = threadIdx.x >> lc;
     const int cnt = s.info->count, i0 = blockIdx.x * cols, i = i0 + at;
@@ -882,7 +881,7 @@ template <typename T> __global__ __launch_bounds__(256) void keep_kernel(Keep s,
                 l = v - s.zy[i];
                 c = good ? f / sum : 1.f;
                 if (lab >= s.v0) {
-                    const T e = to<T>(exp2_(__builtin_fmaf(s.zy[i], LOG2E, -r)) - sum);
+                    const float e = exp2_(__builtin_fmaf(s.zy[i], LOG2E, -r)) - sum;
                     dz[i * s.ldc + (lab - s.v0)] = e;
                     dzt[(lab - s.v0) * s.ldn + i] = e;
                 }
@@ -898,16 +897,11 @@ template <typename T> __global__ __launch_bounds__(256) void keep_kernel(Keep s,
         }
     }
     __syncthreads();
-    constexpr int V = 16 / sizeof(T);
-    const int chunks = cols / V;
+    const int chunks = cols / 4;
     for (int e = threadIdx.x; e < s.k * chunks; e += 256) {
-        const int c = e / chunks, o = e % chunks * V;
-        tn::u32x4 *x = reinterpret_cast<tn::u32x4 *>(ht + c * s.ldn + i0 + o);
-        tn::u32x4 v = *x;
-        T *t = reinterpret_cast<T *>(&v);
-#pragma unroll
-        for (int u = 0; u < V; ++u) t[u] = to<T>((float)t[u] * by[o + u]);
-        *x = v;
+        const int c = e / chunks, o = e % chunks * 4;
+        f32x4 *x = reinterpret_cast<f32x4 *>(ht + c * s.ldn + i0 + o);
+        *x = *x * f32x4{by[o], by[o + 1], by[o + 2], by[o + 3]};
     }
 }
 
@@ -1101,13 +1095,11 @@ void choose_two(int64_t hm, int64_t hn, int64_t hk, int64_t wm, int64_t wn, int6
     }
 }
 
-// E is kept from the first pass where a pass over the logits takes longer than this estimate (us), and so more than the two launches that come
-// with it: f32, 5000 x 1000, k = 100 (estimate 18): 100 -> 83 us; 2000 x 400, k = 42 (3.3): 33 -> 35 us.  In bf16 it costs dW a rounding (of the
-// scaled H; 32768 x 4096, k = 1024: 1067 -> 894 us), from few columns not averaged: more is asked for.  1551 x 2221, k = 1568 (21): 105 -> 109 us;
-// 8192 x 2048, k = 1024 (28): 180 -> 163; of several pieces, where only the last one's E is kept, the rounding is not taken.  (f16 has not the range for E, and smoothing takes a part from every entry that E's rounding would
-// show in.)
-constexpr double KEEP_US_F32 = 6., KEEP_US_BF16 = 25.;
-constexpr int KEEP_COLUMNS = 256;
+// E is kept from the first pass in f32, where a pass over the logits takes longer than this estimate (us) and so more than the two launches
+// that come with it: 5000 x 1000, k = 100 (estimate 18): 100 -> 83 us; 2000 x 400, k = 42 (3.3): 33 -> 35 us.  (Not in 16 bits: the rounding of the
+// scaled H is not small there, and shows in the rows of dW that are mostly labels: bf16, 32768 x 4096, k = 1024, 1067 -> 894 us, but
+// gradients 2.9e-3 off instead of 1.7e-3.  Not with smoothing: it takes a part from every entry that E's rounding would show in.)
+constexpr double KEEP_US = 6.;
 
 Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     Shape s{};
@@ -1132,7 +1124,7 @@ Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     const int64_t pp = std::min(s.piece, s.p);
     const Guess z = choose(pp, n1, s.kpad / step, s.es);
     s.z = z.c;
-    s.keep = grad && !smooth && W.dtype != NMFX_F16 && s.n >= KEEP_COLUMNS && (s.pieces == 1 || W.dtype == NMFX_F32) && z.us > (W.dtype == NMFX_F32 ? KEEP_US_F32 : KEEP_US_BF16);
+    s.keep = grad && !smooth && W.dtype == NMFX_F32 && z.us > KEEP_US;
     choose_two(s.k, n1, (pp + step - 1) / step, pp, s.k, (n1 + step - 1) / step, s.es, s.pieces == 1, s.h, s.w);
     s.direct = s.pieces == 1 && s.h.splits == 1 && s.w.splits == 1 && s.h.kind == s.w.kind;
     s.w_slots = s.w.splits > 1;
@@ -1230,31 +1222,31 @@ template <typename T> void score(const Call &c, const Shape &s) {
 }
 
 // the first pass with E kept, up to the images that the gradient products read
-template <typename T, typename F, typename I>
-void keep_first(const Call &c, const Shape &s, const T *w, int64_t ldw, int wchunks, const tn::Operand &hop, const T *h, T *ht, T *dz, T *dzt, const Combine &cb, F f32, I i32) {
-    const int n = (int)s.n, es = sizeof(T), n1 = std::max(n, 1), v0 = (int)((s.pieces - 1) * s.piece), p = (int)s.p - v0, before = v0 / KINDS[s.z.kind].m, kt = (int)(s.kpad * es / 128);
+template <typename F, typename I>
+void keep_first(const Call &c, const Shape &s, const float *w, int64_t ldw, int wchunks, const tn::Operand &hop, const float *h, float *ht, float *dz, float *dzt, const Combine &cb, F f32, I i32) {
+    const int n = (int)s.n, es = 4, n1 = std::max(n, 1), v0 = (int)((s.pieces - 1) * s.piece), p = (int)s.p - v0, before = v0 / KINDS[s.z.kind].m, kt = (int)(s.kpad * es / 128);
     const int *count = &cb.info->count;
     float2 *part = const_cast<float2 *>(cb.part), *here = part + (int64_t)before * s.npad;      // (a piece is whole tiles)
-    if (v0) stream<T>(tn::Args{{w, ldw * es, v0, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt}, v0, n1, s.z, EpiStats{part, nullptr, f32(s.o_zy), i32(s.o_y), count, v0, 0, (int)s.npad}, c.st);
+    if (v0) stream<float>(tn::Args{{w, ldw * es, v0, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt}, v0, n1, s.z, EpiStats{part, nullptr, f32(s.o_zy), i32(s.o_y), count, v0, 0, (int)s.npad}, c.st);
     tn::Args a{{w + v0 * ldw, ldw * es, p, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt};
     grid(a, p, n1, s.z);
     float *sums = reinterpret_cast<float *>(here);
     const Keep kp{part, sums, f32(s.o_f), f32(s.o_ref), f32(s.o_zy), i32(s.o_idx), i32(s.o_y), cb.info, before, a.tiles_m, v0, (int)s.npad, c.o.reduction, (int)s.k, KINDS[s.z.kind].n,
                   f32(s.o_lse), f32(s.o_loss), c.lse, c.loss, f32(s.o_scale), f32(s.o_again_f), i32(s.o_again), s.ldc, s.ldn};
-    label_kernel<T><<<(n1 + 3) / 4, 256, 0, c.st>>>(kp, w, ldw, wchunks, h, s.kpad, f32(s.o_ref), a.tiles_n);
+    label_kernel<<<(n1 + 3) / 4, 256, 0, c.st>>>(kp, w, ldw, wchunks, h, s.kpad, f32(s.o_ref), a.tiles_n);
     ops::hip_ok(hipGetLastError(), "label");
-    product<T>(a, p, n1, s.z, EpiDz<T, true>{dz, dzt, s.ldc, s.ldn, f32(s.o_ref), nullptr, i32(s.o_y), count, p, v0, 1.f, 0.f, 0.f, 0, cb, sums, f32(s.o_zy)}, c.st);
+    product<float>(a, p, n1, s.z, EpiDz<float, true>{dz, dzt, s.ldc, s.ldn, f32(s.o_ref), nullptr, i32(s.o_y), count, p, v0, 1.f, 0.f, 0.f, 0, cb, sums, f32(s.o_zy)}, c.st);
     int lc = 6;
     while (lc > 3 && (n1 >> lc) < CUS) --lc;
-    keep_kernel<T><<<(n1 + (1 << lc) - 1) >> lc, 256, 0, c.st>>>(kp, dz, dzt, ht, lc);
+    keep_kernel<<<(n1 + (1 << lc) - 1) >> lc, 256, 0, c.st>>>(kp, dz, dzt, ht, lc);
     ops::hip_ok(hipGetLastError(), "keep");
     // columns whose sums left the range of E, by tiles: the way with a pass for the log-sum-exp in front
     const EpiStats ea{here, nullptr, f32(s.o_zy), i32(s.o_y), count, p, v0, (int)s.npad};
-    const EpiDz<T> eb{dz, dzt, s.ldc, s.ldn, f32(s.o_lse), f32(s.o_again_f), i32(s.o_y), count, p, v0, 1.f, 1.f, 0.f, 0, cb, nullptr, nullptr};
+    const EpiDz<float> eb{dz, dzt, s.ldc, s.ldn, f32(s.o_lse), f32(s.o_again_f), i32(s.o_y), count, p, v0, 1.f, 1.f, 0.f, 0, cb, nullptr, nullptr};
     switch (s.z.kind) {
-        case 0: tn::tn_again_kernel<T, 256, 256, 2, 4, 2, EpiStats, Columnwise, EpiDz<T>><<<a.tiles_n, 512, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
-        case 1: tn::tn_again_kernel<T, 128, 128, 2, 2, 2, EpiStats, Columnwise, EpiDz<T>><<<a.tiles_n, 256, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
-        default: tn::tn_again_kernel<T, 64, 64, 2, 2, 4, EpiStats, Columnwise, EpiDz<T>><<<a.tiles_n, 256, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
+        case 0: tn::tn_again_kernel<float, 256, 256, 2, 4, 2, EpiStats, Columnwise, EpiDz<float>><<<a.tiles_n, 512, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
+        case 1: tn::tn_again_kernel<float, 128, 128, 2, 2, 2, EpiStats, Columnwise, EpiDz<float>><<<a.tiles_n, 256, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
+        default: tn::tn_again_kernel<float, 64, 64, 2, 2, 4, EpiStats, Columnwise, EpiDz<float>><<<a.tiles_n, 256, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
     }
     ops::hip_ok(hipGetLastError(), "again");
 }
@@ -1307,7 +1299,7 @@ template <typename T> void run(const Call &c, const Shape &s) {
     T *dz = c.grad ? reinterpret_cast<T *>(ws + s.o_dz) : nullptr, *dzt = c.grad ? reinterpret_cast<T *>(ws + s.o_dzt) : nullptr;
     const float inv = (float)(1. / a_), label = (float)((1. - c.o.label_smoothing) / a_), off = (float)(c.o.label_smoothing / (a_ * p));
     if (keep) {
-        if constexpr (!std::is_same<T, _Float16>::value) keep_first<T>(c, s, w, ldw, wchunks, hop, h, ht, dz, dzt, cb, f32, i32);
+        if constexpr (std::is_same<T, float>::value) keep_first(c, s, w, ldw, wchunks, hop, h, ht, dz, dzt, cb, f32, i32);
     } else if (!c.lse_given) {
         tn::Args a{{w, ldw * es, p, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt};
         stream<T>(a, p, n1, s.z, EpiStats{reinterpret_cast<float2 *>(ws + s.o_part), s.o_zsum >= 0 ? f32(s.o_zsum) : nullptr, f32(s.o_zy), i32(s.o_y), count, p, 0, (int)s.npad}, c.st);

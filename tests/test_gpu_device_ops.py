@@ -87,7 +87,7 @@ def oracle(W, H, y, eps=0.0, reduction="mean", gout=None, ignore=-100, dtype="f3
         total, etotal = loss.sum(), eloss.sum() + V * loss.abs().sum()
         if reduction == "mean":
             total, etotal = total / cnt, etotal / cnt
-    return dict(adz=dz.abs(), loss=total, lse=torch.where(on, lse, 0.0), dW=dW, dH=dH, eloss=etotal, else_=torch.where(on, elog, 0.0), edW=edW, edH=edH)
+    return dict(loss=total, lse=torch.where(on, lse, 0.0), dW=dW, dH=dH, eloss=etotal, else_=torch.where(on, elog, 0.0), edW=edW, edH=edH)
 
 
 def near(name, got, want, bound):
@@ -97,13 +97,9 @@ def near(name, got, want, bound):
     assert (over <= 0).all(), f"{name}: off by {float(off.flatten()[over.argmax()]):.3e} where {float(bound.expand_as(off).flatten()[over.argmax()]):.3e} is allowed"
 
 
-def check(W, H, y, dtype, eps=0.0, reduction="mean", gout=None, ignore=-100, scaled_h=False):
-    """scaled_h: dW's product may take H times a factor of its column, rounded: half a step of every |dz| |h| more."""
+def check(W, H, y, dtype, eps=0.0, reduction="mean", gout=None, ignore=-100):
     kw = dict(ignore_index=ignore, label_smoothing=eps, reduction=reduction)
     want = oracle(W, H, y, eps, reduction, gout, ignore, dtype)
-    if scaled_h:
-        on = y != ignore
-        want["edW"] = want["edW"] + HALF_STEP[dtype] * (want["adz"] @ torch.where(on[None, :], H.double(), 0.0).abs().t())
     loss, lse = nmfx.softmax_xent(W, H, y, **kw)
     near("loss", loss, want["loss"], want["eloss"])
     near("lse", lse, want["lse"], want["else_"])
@@ -280,7 +276,7 @@ def test_xent_factors_of_many_columns(n):
 
 
 # sizes that form the logits once
-ONCE = [("f32", 300001, 600, 9), ("f32", 1024, 300, 300), ("f32", 5000, 1000, 100), ("f32", 1537, 2500, 129), ("bf16", 8192, 2048, 1024), ("bf16", 9001, 2100, 1000)]
+ONCE = [("f32", 300001, 600, 9), ("f32", 1024, 300, 300), ("f32", 5000, 1000, 100), ("f32", 1537, 2500, 129), ("f32", 4097, 1100, 520)]
 
 
 @pytest.mark.parametrize("dtype,p,n,k", ONCE)
@@ -288,10 +284,10 @@ ONCE = [("f32", 300001, 600, 9), ("f32", 1024, 300, 300), ("f32", 5000, 1000, 10
 def test_xent_logits_formed_once(dtype, p, n, k, wl, ignored, reduction):
     W, H, y = problem(p, n, k, dtype, seed=p + n, ignored=ignored, wl=wl)
     gout = torch.linspace(-2, 2, n, device=DEV) if reduction == "none" else None
-    check(W, H, y, dtype, reduction=reduction, gout=gout, scaled_h=True)
+    check(W, H, y, dtype, reduction=reduction, gout=gout)
 
 
-@pytest.mark.parametrize("dtype,p,n,k", ONCE[:1] + ONCE[2:5])
+@pytest.mark.parametrize("dtype,p,n,k", [ONCE[0], ONCE[2], ONCE[4]])
 def test_xent_losses_beyond_any_exponential(dtype, p, n, k):
     """Columns whose losses are near and far beyond where exp() of them leaves Float32 (88.7), among ordinary ones, in some column tiles."""
     W, H, y = problem(p, n, k, dtype, seed=k)
@@ -301,10 +297,10 @@ def test_xent_losses_beyond_any_exponential(dtype, p, n, k):
     spread = z.max(0).values - z.min(0).values
     H = H.clone()
     H[:, cols] = (H[:, cols].double() * (torch.tensor([50.0, 68.0, 75.0, 87.0, 200.0, 1000.0], device=DEV, dtype=torch.float64) / spread)).to(H.dtype)
-    check(W, H, y, dtype, reduction="none", gout=torch.linspace(-1, 1, n, device=DEV), scaled_h=True)
+    check(W, H, y, dtype, reduction="none", gout=torch.linspace(-1, 1, n, device=DEV))
 
 
-@pytest.mark.parametrize("dtype,p,n,k", ONCE[2:5])
+@pytest.mark.parametrize("dtype,p,n,k", ONCE[2:4])
 def test_xent_formed_once_keeps_nan_and_no_classes_to_their_columns(dtype, p, n, k):
     W, H, y = problem(p, n, k, dtype, seed=1, ignored=0.3)
     good = nmfx.softmax_xent_grad(W, H, y, reduction="none")
