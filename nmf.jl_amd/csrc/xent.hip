@@ -116,7 +116,8 @@ template <int NT> __device__ __forceinline__ int count_columns(const Select &s, 
 }
 
 // The order of the packed columns is that of the columns: block `blk` places 8 NT of them behind those of the blocks in front, which it
-// counts itself (up to 4096 columns: a few loads a thread) or finds counted (count_kernel).
+// counts itself (up to 4096 columns: a few loads a thread, 23.6 -> 21.4 us for a small call) or finds counted by count_kernel (16384 columns:
+// 37.4 -> 33.4 us, 200000: 285 -> 97).
 constexpr int SELF = 4096;
 template <int NT> __device__ __forceinline__ void select_columns(const Select &s, int blk) {
     if (!s.n) {
@@ -284,8 +285,9 @@ template <typename T> __device__ __forceinline__ void pack_tile(const Pack<T> &a
     }
 }
 // Everything the products read, in one launch: H packed (first blocks), the images of W that its own order does not serve.  Up to
-// ONE_ROUND columns every block of H finds its 64 packed columns for itself (a round of 256 threads with 8 labels each: less than a launch),
-// and the last block leaves the lists; above, select_kernel has made them.
+// ONE_ROUND columns every block of H finds its 64 packed columns for itself (a round of 256 threads with 8 labels each: less than a launch; a
+// call of 2048 columns 17.5 -> 15.9 us), and the last block leaves the lists; above, select_kernel has made them.  Bound by memory: W' of
+// 131072 x 2048 bf16 with 8192 columns of H, 1.2 GB read and written in 257 us, 4.7 TB/s.
 constexpr int ONE_ROUND = 2048;
 template <typename T> struct Blank {           // zero in the ignored columns of a matrix with contiguous columns
     T *out;
@@ -335,6 +337,8 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
 }
 
 // ---- statistics of the logits: rows of D are classes, columns are packed columns ----------------------------------------------------
+// Bound by the product where k is long (131072 x 8192, k = 2048: 3.26 ms, 1350 TFLOP/s); where it is short by the exponentials, which go in
+// the products' shadow only between blocks (131072 x 16384, k = 256: 1.30 ms, 845 TFLOP/s: 1.65 10^12 logits a second).
 struct EpiStats {
     float2 *part;         // [tile_m][npad]: reference and sum over the tile's classes
     float *zsum;          // [tile_m][npad] or NULL
@@ -526,7 +530,8 @@ __global__ __launch_bounds__(256) void combine_kernel(Combine c, int lc, int add
 // ---- a few columns (scoring tokens): one pass over W, two launches -----------------------------------------------------------------------
 // Up to 16 columns are the 16 columns of a matrix instruction.  H is in LDS, each wave streams 16 rows of W at a time from memory into the
 // other operand's registers (no LDS: nobody else reads them) and keeps the running statistics of its rows; ignored columns stay, as zeros.
-// Bound by reading W: 200 MB (100003 x 1000, f16) in 38 us, 5.2 TB/s.
+// Bound by reading W: 200 MB (100003 x 1000, f16) in 35.6 us, 5.6 TB/s.  Against the general way: 49.7 -> 40.6 us a call; 32768 x 512 and one
+// column 15.3 -> 12.6 (the call), 16 columns of 50000 x 512 22.5 -> 18.4.
 struct Score {
     const void *w, *h;
     int64_t ldw, hrs, hcs;    // bytes between rows of W; elements between components and columns of H
@@ -670,6 +675,9 @@ __global__ __launch_bounds__(1024) void score_join_kernel(Score a, int blocks, f
 }
 
 // ---- dz of a piece of the classes, in both orders -----------------------------------------------------------------------------------
+// Both gradient products contract an index that has to be contiguous, so dz is written twice: 32768 x 8192, k = 2048: 995 us (1105 TFLOP/s
+// with 1.07 GB of stores); 16384 x 16384, k = 256, 400 us: bound by the stores (2.7 TB/s) and the exponentials.  It is rounded to the type of
+// W and H there, the one rounding in front of the products: in f32 they would run at an eighth of the rate.
 template <typename T> __device__ __forceinline__ T to(float x) { return (T)x; }
 
 // KEEP (f32): the same images of E = exp(z - r_j) instead, before the log-sum-exp is known, with the tiles' sums of E and the labels' logits.
@@ -932,12 +940,26 @@ struct EpiSlot {
     }
 };
 
+// up to four results in the caller's type, in one store at whatever address
+template <typename T> __device__ __forceinline__ void put4(T *o, f32x4 x, int there) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    typedef T4 T4_any __attribute__((aligned(sizeof(T))));
+    T4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = to<T>(x[r]);
+    if (there >= 4) *reinterpret_cast<T4_any *>(o) = v;
+    else
+#pragma unroll
+        for (int r = 0; r < 3; ++r)
+            if (r < there) o[r] = v[r];
+}
+
 // ---- a finished product in the caller's type: element (m, n) at out[m + n * ld] ------------------------------------------------------
 template <typename T> struct EpiOut {
     T *out;
     int64_t ld;
     const Info *info;
-    int mmax, nmax, wide;     // wide: four consecutive m go in one store
+    int mmax, nmax;
     const int *cols, *count;  // column n goes to column cols[n], for n < *count; or NULL
     const float *scale;       // of column n, or NULL
     template <int MI, int NJ> using Early = tn::None;
@@ -945,7 +967,6 @@ template <typename T> struct EpiOut {
     template <int BM, int BN, int WM, int WN> __device__ __forceinline__ void begin(const Geom &, tn::None &, tn::None &) const {}
     template <int BM, int BN, int WM, int WN, int MI, int NJ>
     __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NJ], const Geom &g, tn::None &, tn::None &, char *, char *) const {
-        typedef T T4 __attribute__((ext_vector_type(4)));
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             int n = g.n0 + 16 * j;
@@ -955,15 +976,7 @@ template <typename T> struct EpiOut {
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 const int m = g.m0 + 16 * i;
-                T4 v;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = to<T>(acc[i][j][r] * u);
-                T *o = out + (int64_t)n * ld + m;
-                if (wide && m + 3 < mmax) *reinterpret_cast<T4 *>(o) = v;
-                else
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (m + r < mmax) o[r] = v[r];
+                put4(out + (int64_t)n * ld + m, acc[i][j] * u, mmax - m);
             }
         }
     }
@@ -985,12 +998,14 @@ template <typename T> struct Join {
     __device__ __forceinline__ void run(int b, float u) const {
         const int mq = (mmax + 3) / 4, part = threadIdx.x & ((1 << lanes) - 1);
         const int64_t total = (int64_t)mq * nmax, threads = blocks * 256ll >> lanes;
+        const int inner = ms == 1 ? mq : nmax;                            // of the two indexes the one that neighbouring threads step
         for (int64_t e0 = 0; e0 < total; e0 += threads) {                 // (whole waves stay together: they exchange sums)
             const int64_t e = e0 + ((b * 256ll + threadIdx.x) >> lanes);
             int m = 0, n = 0, from = -1;
             if (e < total) {
-                if (ms == 1) { n = (int)(e / mq); m = (int)(e - (int64_t)n * mq) * 4; }
-                else { m = (int)(e / nmax); n = (int)(e - (int64_t)m * nmax); m *= 4; }
+                const int o = total >> 32 ? (int)(e / inner) : (int)((uint32_t)e / (uint32_t)inner), i = (int)(e - (int64_t)o * inner);
+                n = ms == 1 ? o : i;
+                m = (ms == 1 ? i : o) * 4;
                 from = pos ? pos[n] : n;
             }
             f32x4 s = {0.f, 0.f, 0.f, 0.f};
@@ -1002,11 +1017,14 @@ template <typename T> struct Join {
             for (int o = 1; o < 1 << lanes; o <<= 1)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) s[q] += __shfl_xor(s[q], o);
-            const float by = scale && from >= 0 ? u * scale[from] : u;
-            if (e < total && part == 0)
+            if (e < total && part == 0) {
+                s *= scale && from >= 0 ? u * scale[from] : u;
+                if (ms == 1) put4(out + m + n * ns, s, mmax - m);
+                else
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (m + q < mmax) out[(m + q) * ms + n * ns] = to<T>(s[q] * by);
+                    for (int q = 0; q < 4; ++q)
+                        if (m + q < mmax) out[(m + q) * ms + n * ns] = to<T>(s[q]);
+            }
         }
     }
 };
@@ -1170,7 +1188,8 @@ template <typename T, typename Epi> void product(tn::Args a, int64_t m, int64_t 
     }
     ops::hip_ok(hipGetLastError(), "product");
 }
-// the large tile, several tiles for every compute unit: their loads pass under one another's epilogues
+// the large tile, several tiles for every compute unit: their loads pass under one another's epilogues (131072 x 16384, k = 256: 1393 -> 1300 us;
+// 512 tiles of k = 1024: 68.5 -> 68.1; from fewer no gain)
 template <typename T, typename Epi> void stream(tn::Args a, int64_t m, int64_t n, const Choice &c, const Epi &epi, hipStream_t st) {
     grid(a, m, n, c);
     if (c.kind != 0 || blocks_of(a) < 2 * CUS) return product<T>(a, m, n, c, epi, st);
@@ -1293,9 +1312,10 @@ template <typename T> void run(const Call &c, const Shape &s) {
     const tn::Operand hop{h, s.kpad * es, (int)s.npad, (int)(s.kpad / per)};
     const Combine cb{reinterpret_cast<float2 *>(ws + s.o_part), s.o_zsum >= 0 ? f32(s.o_zsum) : nullptr, f32(s.o_zy), i32(s.o_idx), i32(s.o_y), info, tiles, (int)s.npad, p,
                      c.o.reduction, eps, f32(s.o_lse), f32(s.o_loss), c.lse, c.loss};
-    // dz's blocks join the tiles' statistics of their columns themselves where that is a few of them: less than a launch
+    // dz's blocks join the tiles' statistics of their columns themselves where that is a few of them: less than a launch (17 tiles, 83 columns:
+    // 27.0 -> 25.3 us a call; 32 tiles, 200 columns: 30.5 -> 28.6; 63 tiles, 1000 columns: 61 -> 67, left to combine_kernel)
     const bool keep = s.keep && !c.lse_given;
-    const bool few = c.grad && !c.lse_given && !keep && s.pieces == 1 && tiles <= 64 && (int64_t)tiles * ((n1 + KINDS[s.z.kind].n - 1) / KINDS[s.z.kind].n) <= 2 * CUS;
+    const bool few = c.grad && !c.lse_given && !keep && s.pieces == 1 && tiles <= 32 && (int64_t)tiles * ((n1 + KINDS[s.z.kind].n - 1) / KINDS[s.z.kind].n) <= 2 * CUS;
     T *dz = c.grad ? reinterpret_cast<T *>(ws + s.o_dz) : nullptr, *dzt = c.grad ? reinterpret_cast<T *>(ws + s.o_dzt) : nullptr;
     const float inv = (float)(1. / a_), label = (float)((1. - c.o.label_smoothing) / a_), off = (float)(c.o.label_smoothing / (a_ * p));
     if (keep) {
@@ -1334,11 +1354,9 @@ template <typename T> void run(const Call &c, const Shape &s) {
         const int mm = kfast ? k : pv, nn = kfast ? pv : k;
         tn::Args d{kfast ? top : zop, kfast ? zop : top, count, tn::LIMIT_C, 0, 0, 0, (int)(s.npad / step)};
         Join<T> jh{}, jw{};
-        const bool wide = ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * es - 1)) == 0;
-        const EpiOut<T> ew{out, ldo, info, mm, nn, wide, nullptr, nullptr, nullptr};
+        const EpiOut<T> ew{out, ldo, info, mm, nn, nullptr, nullptr, nullptr};
         if (direct) {
-            const bool hwide = c.dH.cs % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & (4 * es - 1)) == 0;
-            products<T>(b, k, n1, s.h, EpiOut<T>{dh, c.dH.cs, info, k, n, hwide, i32(s.o_idx), count, scale}, d, mm, nn, s.w, ew, Losses{f32(s.o_loss), info, c.o.reduction, add ? c.loss : nullptr}, c.st);
+            products<T>(b, k, n1, s.h, EpiOut<T>{dh, c.dH.cs, info, k, n, i32(s.o_idx), count, scale}, d, mm, nn, s.w, ew, Losses{f32(s.o_loss), info, c.o.reduction, add ? c.loss : nullptr}, c.st);
             return;
         }
         if (s.w_slots) {
