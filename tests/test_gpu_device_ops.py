@@ -477,6 +477,64 @@ def test_norm_stays_in_its_buffers():
         out_ok(), ws_ok(), got_ok(), flat_ok()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("p,n,k", [(70, 3, 9), (300, 40, 64), (900, 300, 129), (5000, 1000, 100)])
+@pytest.mark.parametrize("gw,gh", [("c", "r"), ("r+o", "c+"), ("c+", "r+o")])
+def test_xent_outputs_in_any_order(dtype, p, n, k, gw, gh):
+    """Outputs of another contiguous index than their inputs, padded, off by an element: the values of dense ones, nothing beside them."""
+    W, H, y = problem(p, n, k, dtype, seed=p, ignored=0.2)
+    want = nmfx.softmax_xent_grad(W, H, y)
+    dW, dH = lay(torch.zeros_like(W), gw), lay(torch.zeros_like(H), gh)
+
+    def around(t):
+        buf = torch.as_strided(t, (t.untyped_storage().nbytes() // t.element_size(),), (1,), 0)
+        return int(buf.isnan().sum())
+
+    pads = around(dW), around(dH)
+    loss, lse, a, b = nmfx.softmax_xent_grad(W, H, y, dW=dW, dH=dH)
+    assert a is dW and b is dH and (around(dW), around(dH)) == pads
+    assert torch.equal(loss, want[0]) and torch.equal(lse, want[1])
+    for name, got, dense in (("dW", dW, want[2]), ("dH", dH, want[3])):      # (the order decides the tiles: sums may differ in their last bits)
+        u = (4 * HALF_STEP[dtype] + n * V + p * V) * dense.abs().max().double()
+        assert ((got.double() - dense.double()).abs() <= u).all(), name
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [5, 60])
+def test_xent_ignored_label_that_is_a_class(dtype, n):
+    W, H, y = problem(40, n, 24, dtype, seed=n)
+    y[::3] = 7
+    check(W, H, y, dtype, ignore=7)
+
+
+@pytest.mark.parametrize("p,n,k", [(2 ** 21 - 1024, 3, 4), (2 ** 21 - 1024, 20, 4), (5, 2 ** 21 - 1024, 4), (2, 3, 2 ** 20 - 512)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_xent_largest_extents(dtype, p, n, k):
+    W, H, y = problem(p, n, k, dtype, seed=1, ignored=0.1 if n > 3 else 0.0)
+    check(W, H, y, dtype)
+
+
+@pytest.mark.parametrize("wl", ["r", "c"])
+@pytest.mark.parametrize("n", [4, 30])
+def test_xent_wide_strides_of_w(wl, n):
+    W, H, y = problem(300, n, 40, "bf16", seed=n)
+    ld = 2 ** 21 - 1024
+    buf = torch.full(((300 if wl == "r" else 40) * ld,), float("nan"), dtype=W.dtype, device=DEV).view(-1, ld)
+    v = buf[:, :40] if wl == "r" else buf[:, :300].t()
+    v.copy_(W)
+    check(v, H, y, "bf16")
+
+
+def test_an_error_left_behind_is_not_reported():
+    set_device = nmfx._lib.load().hipSetDevice                   # of the runtime that the library is linked to
+    W, H, y = problem(50, 4, 8, "f32")
+    for call in (lambda: nmfx.softmax_xent(W, H, y), lambda: nmfx.softmax_xent_grad(W, H, y), lambda: nmfx.grad_norm([W, H])):
+        call()
+        assert set_device(99) != 0
+        call()
+    torch.cuda.synchronize()
+
+
 # ---- norm and clipping ---------------------------------------------------------------------------------------------------------------
 def tensors(shapes, dtypes, seed=0, scale=0.1):
     g = torch.Generator(device=DEV)
@@ -585,6 +643,21 @@ def test_clip_not_finite(size):
         assert nmfx.clip_grad_norm([x, y], 1.0, kind).isnan() and x.isnan().all() and y.isnan().all()
     a[size // 2] = float("inf")
     assert nmfx.clip_grad_norm([a, b], 1.0).isinf() and (b == 0).all() and a[size // 2].isnan() and a.isnan().sum() == 1
+
+
+def test_norm_of_one_large_tensor_and_of_thousands():
+    big = torch.full((2 ** 31 + 2 ** 20 + 3,), 0.5, dtype=torch.bfloat16, device=DEV)
+    big[-1] = 3.0
+    want = math.sqrt((big.numel() - 1) * 0.25 + 9.0)
+    assert abs(float(nmfx.grad_norm(big)) - want) <= 2 * V * want
+    assert float(nmfx.grad_norm(big, norm_type=float("inf"))) == 3.0
+    norm = nmfx.clip_grad_norm([big], want / 2)
+    assert abs(float(norm) - want) <= 2 * V * want and float(big[-1]) == 1.5 and float(big[0]) == 0.25 and float(big[2 ** 31 + 7]) == 0.25
+    del big
+    many = [torch.full((i % 7 + 1,), 1.0, device=DEV) for i in range(3000)] + [torch.ones(5, 8, device=DEV)[:, :3] for _ in range(50)]
+    count = sum(t.numel() for t in many)
+    assert abs(float(nmfx.clip_grad_norm(many, 1.0)) - math.sqrt(count)) <= 2 * V * math.sqrt(count)
+    assert all(((t * math.sqrt(count) - 1).abs() <= 8 * V + 2e-6).all() for t in many[::97] + many[-3:])
 
 
 def test_clip_on_another_stream():
