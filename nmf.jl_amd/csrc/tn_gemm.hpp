@@ -15,7 +15,7 @@
 //         1985 TFLOP/s against 1745
 //   1318  the loads spread over 20 products, 8 of them in the next tile (12: 1290, 28: 1276, 44: 1198: the last ones then come too late)
 // A row stride that is a large power of two sends the rows of a tile to few memory channels (2048 x 8192 x 32768: 1137 TFLOP/s at 65536
-// bytes, 1317 at 256 more): images made for these products are padded.  Stages of 64-byte rows, 4 or 5 deep, were slower (1174-1195).
+// bytes, 1317 at 256 more): images made for these products are padded, or stored in blocks (Blocked).  Stages of 64-byte rows, 4 or 5 deep, were slower (1174-1195).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -57,6 +57,17 @@ struct Operand {
     int64_t ld;       // bytes between rows (a multiple of 16; p is 16-byte aligned)
     int rows;         // rows that exist; rows behind them repeat the last one
     int chunks;       // 16-byte chunks of a row that exist; chunks behind them read as zero
+    int kstep = ROW;       // bytes between a row's tiles of the contraction
+    int64_t block = 0;     // bytes between blocks of 256 rows; 0: 256 ld
+};
+// An operand of this project's own making is stored in blocks, block x tile x row: what a block of 256 rows has of one tile of the contraction
+// (256 x 128 bytes) lies together, so that a tile's loads go to a few pages of memory instead of one a row.  Element (row, c):
+template <typename T> struct Blocked {
+    static constexpr int CT = ROW / (int)sizeof(T);
+    T *p;
+    int ktiles;            // tiles of a row
+    __device__ __forceinline__ T *at(int row, int c) const { return p + ((int64_t)(row >> 8) * ktiles + c / CT) * (256 * CT) + (row & 255) * CT + c % CT; }
+    Operand operand(int rows) const { return Operand{p, ROW, rows, ktiles * (ROW / 16), 256 * ROW, (int64_t)ktiles * 256 * ROW}; }
 };
 enum { LIMIT_NONE = 0, LIMIT_N = 1, LIMIT_C = 2 };
 struct Args {
@@ -98,13 +109,15 @@ template <int TILE_ROWS, int NT> struct Loader {
     static constexpr int PER = TILE_ROWS * LPR / NT;       // 16-byte loads of a thread per tile
     static_assert(NT / LPR % 16 == 0, "a load of the block starts at a row that is a multiple of 16");
     u32x4 rsrc;
-    uint32_t off, apart;      // of the thread's first load; between one load's row and the next one's
+    uint32_t off, apart, kstep;   // of the thread's first load; between one load's row and the next one's
     int chunk, chunks;
     __device__ __forceinline__ void init(const Operand &o, int row0, int tid) {
         const int here = min(TILE_ROWS, o.rows - row0);                 // >= 1: the grid covers existing rows only
-        const uint64_t at = reinterpret_cast<uint64_t>(o.p) + (int64_t)row0 * o.ld;
-        // the buffer ends with the last row that exists: rows behind it read as zero
-        rsrc = u32x4{(uint32_t)at, (uint32_t)(at >> 32), (uint32_t)((int64_t)(here - 1) * o.ld + (int64_t)o.chunks * 16), 0x00020000u};
+        const uint64_t at = reinterpret_cast<uint64_t>(o.p) + (o.block ? (row0 >> 8) * o.block + (row0 & 255) * o.ld : (int64_t)row0 * o.ld);
+        // the buffer ends with the last row that exists: rows behind it read as zero (in blocks: as they are, they exist in memory)
+        const int64_t width = (int64_t)(o.chunks >> 3) * o.kstep + (o.chunks & 7) * 16;
+        rsrc = u32x4{(uint32_t)at, (uint32_t)(at >> 32), (uint32_t)((int64_t)(here - 1) * o.ld + width), 0x00020000u};
+        kstep = o.kstep;
 #pragma unroll
         for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
         const int row = tid / LPR;
@@ -114,7 +127,7 @@ template <int TILE_ROWS, int NT> struct Loader {
         apart = (uint32_t)(NT / LPR) * (uint32_t)o.ld;
     }
     // where tile kt's loads start; a chunk behind the row's end is asked for beyond the buffer and reads as zero
-    __device__ __forceinline__ uint32_t start(int kt) const { return kt * LPR + chunk < chunks ? off + kt * ROW : 0x80000000u; }
+    __device__ __forceinline__ uint32_t start(int kt) const { return kt * LPR + chunk < chunks ? off + kt * kstep : 0x80000000u; }
     __device__ __forceinline__ void load(char *lds, int tid, uint32_t start, int i) const { to_lds(rsrc, lds + (i * NT + (tid & ~63)) * 16, start + i * apart); }
 };
 

@@ -682,8 +682,7 @@ template <typename T> __device__ __forceinline__ T to(float x) { return (T)x; }
 
 // KEEP (f32): the same images of E = exp(z - r_j) instead, before the log-sum-exp is known, with the tiles' sums of E and the labels' logits.
 template <typename T, bool KEEP = false> struct EpiDz {
-    T *dz, *dzt;              // [npad][ldc] by packed column, [classes of the piece][ldn] by class
-    int64_t ldc, ldn;
+    tn::Blocked<T> dz, dzt;   // rows are packed columns, rows are classes of the piece
     const float *lse_c, *f;   // KEEP: lse_c is the reference, in units of log 2
     const int *y, *count;
     int p, v0;                // classes that exist in the piece; its first class
@@ -757,10 +756,10 @@ template <typename T, bool KEEP = false> struct EpiDz {
                 }
                 if constexpr (sizeof(T) == 2) *reinterpret_cast<T4 *>(patch + P::at(16 * j + (g.lane & 15), 2 * i + (g.lane >> 5)) + (g.lane >> 4 & 1) * 8) = o;
                 else {
-                    if (!at_edge || n < cnt) *reinterpret_cast<T4 *>(dz + (int64_t)n * ldc + g.m0 + 16 * i) = o;
+                    if (!at_edge || n < cnt) *reinterpret_cast<T4 *>(dz.at(n, g.m0 + 16 * i)) = o;
                     if (!at_edge || n < ends)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) dzt[(int64_t)(g.m0 + 16 * i + r) * ldn + n] = o[r];
+                        for (int r = 0; r < 4; ++r) *dzt.at(g.m0 + 16 * i + r, n) = o[r];
                 }
             }
             // the label's entry, where it is this lane's: written once more
@@ -776,8 +775,8 @@ template <typename T, bool KEEP = false> struct EpiDz {
                 const T v = to<T>(__builtin_fmaf(exp2_(__builtin_fmaf(z, LOG2E, ref)), mul, sub - fac * label));
                 if constexpr (sizeof(T) == 2) *reinterpret_cast<T *>(patch + P::at(16 * j + (g.lane & 15), 2 * (d >> 4) + (g.lane >> 5)) + (g.lane >> 4 & 1) * 8 + (d & 3) * 2) = v;
                 else {
-                    dz[(int64_t)n * ldc + g.m0 + d] = v;
-                    dzt[(int64_t)(g.m0 + d) * ldn + n] = v;
+                    *dz.at(n, g.m0 + d) = v;
+                    *dzt.at(g.m0 + d, n) = v;
                 }
                 }
             }
@@ -809,14 +808,14 @@ template <typename T, bool KEEP = false> struct EpiDz {
 #pragma unroll
             for (int e = 0; e < 16 * NJ * P::SLOTS / 64; ++e) {
                 const int at = e * 64 + g.lane, row = at / P::SLOTS, slot = at % P::SLOTS;
-                if (!edge || n0 + row < cnt) *reinterpret_cast<tn::u32x4 *>(dz + (int64_t)(n0 + row) * ldc + m0 + slot * 8) = *reinterpret_cast<const tn::u32x4 *>(patch + P::at(row, slot));
+                if (!edge || n0 + row < cnt) *reinterpret_cast<tn::u32x4 *>(dz.at(n0 + row, m0 + slot * 8)) = *reinterpret_cast<const tn::u32x4 *>(patch + P::at(row, slot));
             }
             const int l = g.lane & 15, rows8 = (g.lane >> 4) * 8;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
                 for (int h = 0; h < NJ / 2; ++h)
-                    if (!edge || n0 + 32 * h + rows8 < ends) *reinterpret_cast<tn::u32x4 *>(dzt + (int64_t)(m0 + 16 * i + l) * ldn + n0 + 32 * h + rows8) = P::transposed(patch, 32 * h + rows8, 16 * i, g.lane);
+                    if (!edge || n0 + 32 * h + rows8 < ends) *reinterpret_cast<tn::u32x4 *>(dzt.at(m0 + 16 * i + l, n0 + 32 * h + rows8)) = P::transposed(patch, 32 * h + rows8, 16 * i, g.lane);
         }
     }
 };
@@ -837,7 +836,8 @@ struct Keep {
     float *lse_c, *loss_c, *lse, *loss;
     float *scale, *again_f;   // of a column: f_j / S_j, and what its dz is multiplied by if it is formed again
     int *again;               // per tile: some column's sum is out of range
-    int64_t ldc, ldn;
+    tn::Blocked<float> dz, dzt;
+    int64_t ldn;              // of H's image
 };
 constexpr float SUM_MOST = 1e30f;
 // r_j, by a wave a column; and no tile is to be done again
@@ -858,7 +858,7 @@ __global__ __launch_bounds__(256) void label_kernel(Keep s, const float *w, int6
     if (lane == 0) ref[i] = d * LOG2E;
 }
 // joins the tiles' sums of 2^lc (at least 8) columns, finishes them, puts the label's entry right and scales H's image
-__global__ __launch_bounds__(256) void keep_kernel(Keep s, float *dz, float *dzt, float *ht, int lc) {
+__global__ __launch_bounds__(256) void keep_kernel(Keep s, float *ht, int lc) {
     __shared__ float ps[256], by[256];
     const int cols = 1 << lc, step = 256 >> lc, at = threadIdx.x & (cols - 1), slice = threadIdx.x >> lc;
     const int cnt = s.info->count, i0 = blockIdx.x * cols, i = i0 + at;
@@ -890,8 +890,8 @@ __global__ __launch_bounds__(256) void keep_kernel(Keep s, float *dz, float *dzt
                 c = good ? f / sum : 1.f;
                 if (lab >= s.v0) {
                     const float e = exp2_(__builtin_fmaf(s.zy[i], LOG2E, -r)) - sum;
-                    dz[i * s.ldc + (lab - s.v0)] = e;
-                    dzt[(lab - s.v0) * s.ldn + i] = e;
+                    *s.dz.at(i, lab - s.v0) = e;
+                    *s.dzt.at(lab - s.v0, i) = e;
                 }
             }
             if (!good) s.again[i / s.per] = 1;
@@ -1055,7 +1055,7 @@ struct Shape {
     int64_t wrs, wcs;             // strides of W
     bool w_rows_direct, w_cols_direct;   // W can be read in place as [class][component], as [component][class]
     int64_t npad, kpad, ppad;     // extents as the images have them
-    int64_t ldn, ldp, ldc;        // between rows of the images by columns (ht, dzt), by classes (wt), of dz: padded (tn_gemm.hpp)
+    int64_t ldn, ldp;             // between rows of the images ht, by columns, and wt, by classes: padded (tn_gemm.hpp)
     int64_t piece, pieces;        // classes of a piece (a multiple of 256)
     int64_t ldslot;
     Choice z, h, w;               // the products Z, W' dz, dz H'
@@ -1137,7 +1137,7 @@ Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     s.piece = up((s.ppad + s.pieces - 1) / s.pieces, 256);
     s.pieces = (s.ppad + s.piece - 1) / s.piece;
     s.ldslot = up(s.k, 4);
-    s.ldn = s.npad + 256 / s.es; s.ldp = s.ppad + 256 / s.es; s.ldc = s.piece + 256 / s.es;
+    s.ldn = s.npad + 256 / s.es; s.ldp = s.ppad + 256 / s.es;
     const int64_t n1 = std::max<int64_t>(s.n, 1);
     const int64_t pp = std::min(s.piece, s.p);
     const Guess z = choose(pp, n1, s.kpad / step, s.es);
@@ -1163,8 +1163,8 @@ Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     if (grad) {
         s.o_ht = take(s.k * s.ldn * s.es);
         s.o_wt = s.w_cols_direct ? -1 : take(s.k * s.ldp * s.es);
-        s.o_dz = take(s.npad * s.ldc * s.es);
-        s.o_dzt = take(s.piece * s.ldn * s.es);
+        s.o_dz = take(s.npad * s.piece * s.es);
+        s.o_dzt = take(s.npad * s.piece * s.es);
         s.o_hslot = take((int64_t)s.h.splits * s.npad * s.ldslot * 4);
         if (s.w_slots) s.o_wslot = take((int64_t)s.w.splits * std::max(up(s.piece, 4) * s.k, s.ldslot * s.piece) * 4);
     }
@@ -1242,7 +1242,7 @@ template <typename T> void score(const Call &c, const Shape &s) {
 
 // the first pass with E kept, up to the images that the gradient products read
 template <typename F, typename I>
-void keep_first(const Call &c, const Shape &s, const float *w, int64_t ldw, int wchunks, const tn::Operand &hop, const float *h, float *ht, float *dz, float *dzt, const Combine &cb, F f32, I i32) {
+void keep_first(const Call &c, const Shape &s, const float *w, int64_t ldw, int wchunks, const tn::Operand &hop, const float *h, float *ht, const tn::Blocked<float> &dz, const tn::Blocked<float> &dzt, const Combine &cb, F f32, I i32) {
     const int n = (int)s.n, es = 4, n1 = std::max(n, 1), v0 = (int)((s.pieces - 1) * s.piece), p = (int)s.p - v0, before = v0 / KINDS[s.z.kind].m, kt = (int)(s.kpad * es / 128);
     const int *count = &cb.info->count;
     float2 *part = const_cast<float2 *>(cb.part), *here = part + (int64_t)before * s.npad;      // (a piece is whole tiles)
@@ -1251,17 +1251,17 @@ void keep_first(const Call &c, const Shape &s, const float *w, int64_t ldw, int 
     grid(a, p, n1, s.z);
     float *sums = reinterpret_cast<float *>(here);
     const Keep kp{part, sums, f32(s.o_f), f32(s.o_ref), f32(s.o_zy), i32(s.o_idx), i32(s.o_y), cb.info, before, a.tiles_m, v0, (int)s.npad, c.o.reduction, (int)s.k, KINDS[s.z.kind].n,
-                  f32(s.o_lse), f32(s.o_loss), c.lse, c.loss, f32(s.o_scale), f32(s.o_again_f), i32(s.o_again), s.ldc, s.ldn};
+                  f32(s.o_lse), f32(s.o_loss), c.lse, c.loss, f32(s.o_scale), f32(s.o_again_f), i32(s.o_again), dz, dzt, s.ldn};
     label_kernel<<<(n1 + 3) / 4, 256, 0, c.st>>>(kp, w, ldw, wchunks, h, s.kpad, f32(s.o_ref), a.tiles_n);
     ops::hip_ok(hipGetLastError(), "label");
-    product<float>(a, p, n1, s.z, EpiDz<float, true>{dz, dzt, s.ldc, s.ldn, f32(s.o_ref), nullptr, i32(s.o_y), count, p, v0, 1.f, 0.f, 0.f, 0, cb, sums, f32(s.o_zy)}, c.st);
+    product<float>(a, p, n1, s.z, EpiDz<float, true>{dz, dzt, f32(s.o_ref), nullptr, i32(s.o_y), count, p, v0, 1.f, 0.f, 0.f, 0, cb, sums, f32(s.o_zy)}, c.st);
     int lc = 6;
     while (lc > 3 && (n1 >> lc) < CUS) --lc;
-    keep_kernel<<<(n1 + (1 << lc) - 1) >> lc, 256, 0, c.st>>>(kp, dz, dzt, ht, lc);
+    keep_kernel<<<(n1 + (1 << lc) - 1) >> lc, 256, 0, c.st>>>(kp, ht, lc);
     ops::hip_ok(hipGetLastError(), "keep");
     // columns whose sums left the range of E, by tiles: the way with a pass for the log-sum-exp in front
     const EpiStats ea{here, nullptr, f32(s.o_zy), i32(s.o_y), count, p, v0, (int)s.npad};
-    const EpiDz<float> eb{dz, dzt, s.ldc, s.ldn, f32(s.o_lse), f32(s.o_again_f), i32(s.o_y), count, p, v0, 1.f, 1.f, 0.f, 0, cb, nullptr, nullptr};
+    const EpiDz<float> eb{dz, dzt, f32(s.o_lse), f32(s.o_again_f), i32(s.o_y), count, p, v0, 1.f, 1.f, 0.f, 0, cb, nullptr, nullptr};
     switch (s.z.kind) {
         case 0: tn::tn_again_kernel<float, 256, 256, 2, 4, 2, EpiStats, Columnwise, EpiDz<float>><<<a.tiles_n, 512, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
         case 1: tn::tn_again_kernel<float, 128, 128, 2, 2, 2, EpiStats, Columnwise, EpiDz<float>><<<a.tiles_n, 256, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
@@ -1316,7 +1316,7 @@ template <typename T> void run(const Call &c, const Shape &s) {
     // 27.0 -> 25.3 us a call; 32 tiles, 200 columns: 30.5 -> 28.6; 63 tiles, 1000 columns: 61 -> 67, left to combine_kernel)
     const bool keep = s.keep && !c.lse_given;
     const bool few = c.grad && !c.lse_given && !keep && s.pieces == 1 && tiles <= 32 && (int64_t)tiles * ((n1 + KINDS[s.z.kind].n - 1) / KINDS[s.z.kind].n) <= 2 * CUS;
-    T *dz = c.grad ? reinterpret_cast<T *>(ws + s.o_dz) : nullptr, *dzt = c.grad ? reinterpret_cast<T *>(ws + s.o_dzt) : nullptr;
+    const tn::Blocked<T> dz{c.grad ? reinterpret_cast<T *>(ws + s.o_dz) : nullptr, (int)(s.piece / step)}, dzt{c.grad ? reinterpret_cast<T *>(ws + s.o_dzt) : nullptr, (int)(s.npad / step)};
     const float inv = (float)(1. / a_), label = (float)((1. - c.o.label_smoothing) / a_), off = (float)(c.o.label_smoothing / (a_ * p));
     if (keep) {
         if constexpr (std::is_same<T, float>::value) keep_first(c, s, w, ldw, wchunks, hop, h, ht, dz, dzt, cb, f32, i32);
@@ -1342,12 +1342,12 @@ template <typename T> void run(const Call &c, const Shape &s) {
         const bool last = t + 1 == s.pieces;
         tn::Args a{{w + v0 * ldw, ldw * es, pv, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt};
         if (!keep || t)
-            product<T>(a, pv, n1, s.z, EpiDz<T>{dz, dzt, s.ldc, s.ldn, f32(s.o_lse), f32(keep ? s.o_again_f : s.o_f), i32(s.o_y), count, pv, (int)v0, inv, label, off, few, cb, nullptr, nullptr}, c.st);
+            product<T>(a, pv, n1, s.z, EpiDz<T>{dz, dzt, f32(s.o_lse), f32(keep ? s.o_again_f : s.o_f), i32(s.o_y), count, pv, (int)v0, inv, label, off, few, cb, nullptr, nullptr}, c.st);
         // dH: rows are components, columns are packed columns
-        tn::Args b{{wt + v0, ldwt * es, k, (int)std::min<int64_t>((wtpad - v0) / per, s.piece / per)}, {dz, s.ldc * es, (int)s.npad, (int)(s.piece / per)}, count, tn::LIMIT_N, 0, 0, 0, pt / step};
+        tn::Args b{{wt + v0, ldwt * es, k, (int)std::min<int64_t>((wtpad - v0) / per, s.piece / per)}, dz.operand((int)s.npad), count, tn::LIMIT_N, 0, 0, 0, pt / step};
         const EpiSlot eh{f32(s.o_hslot), s.ldslot, s.npad * s.ldslot, (int)s.npad, t > 0};
         // dW: the contiguous index of dW is the row
-        const tn::Operand zop{dzt, s.ldn * es, pv, (int)(s.npad / per)}, top{ht, s.ldn * es, k, (int)(s.npad / per)};
+        const tn::Operand zop = dzt.operand(pv), top{ht, s.ldn * es, k, (int)(s.npad / per)};
         const bool kfast = c.dW.cs == 1;
         T *out = dw + v0 * c.dW.rs;
         const int64_t ldo = kfast ? c.dW.rs : c.dW.cs;
