@@ -54,20 +54,22 @@ constexpr int ROW = 128;   // bytes of a tile's row
 
 struct Operand {
     const void *p;
-    int64_t ld;       // bytes between rows (a multiple of 16; p is 16-byte aligned)
-    int rows;         // rows that exist; rows behind them repeat the last one
-    int chunks;       // 16-byte chunks of a row that exist; chunks behind them read as zero
-    int kstep = ROW;       // bytes between a row's tiles of the contraction
-    int64_t block = 0;     // bytes between blocks of 256 rows; 0: 256 ld
+    int64_t ld;            // bytes between rows (a multiple of 16; p is 16-byte aligned)
+    int64_t block;         // bytes between blocks of 256 rows
+    int rows;              // rows that exist; rows behind them read as zero (or as what is there: their results are nobody's)
+    int chunks;            // 16-byte chunks of a row that exist; chunks behind them read as zero
+    int kstep;             // bytes between a row's tiles of the contraction
+    uint32_t width;        // bytes from a row's start to where its last chunk ends
 };
+inline Operand plain(const void *p, int64_t ld, int rows, int chunks) { return Operand{p, ld, 256 * ld, rows, chunks, ROW, (uint32_t)chunks * 16}; }
 // An operand of this project's own making is stored in blocks, block x tile x row: what a block of 256 rows has of one tile of the contraction
 // (256 x 128 bytes) lies together, so that a tile's loads go to a few pages of memory instead of one a row.  Element (row, c):
 template <typename T> struct Blocked {
     static constexpr int CT = ROW / (int)sizeof(T);
     T *p;
     int ktiles;            // tiles of a row
-    __device__ __forceinline__ T *at(int row, int c) const { return p + ((int64_t)(row >> 8) * ktiles + c / CT) * (256 * CT) + (row & 255) * CT + c % CT; }
-    Operand operand(int rows) const { return Operand{p, ROW, rows, ktiles * (ROW / 16), 256 * ROW, (int64_t)ktiles * 256 * ROW}; }
+    __device__ __forceinline__ T *at(uint32_t row, uint32_t c) const { return p + ((int64_t)(row >> 8) * ktiles + c / CT) * (256 * CT) + ((row & 255) * CT + c % CT); }
+    Operand operand(int rows) const { return Operand{p, ROW, (int64_t)ktiles * 256 * ROW, rows, ktiles * (ROW / 16), 256 * ROW, (uint32_t)(ktiles - 1) * (256 * ROW) + ROW}; }
 };
 enum { LIMIT_NONE = 0, LIMIT_N = 1, LIMIT_C = 2 };
 struct Args {
@@ -113,10 +115,8 @@ template <int TILE_ROWS, int NT> struct Loader {
     int chunk, chunks;
     __device__ __forceinline__ void init(const Operand &o, int row0, int tid) {
         const int here = min(TILE_ROWS, o.rows - row0);                 // >= 1: the grid covers existing rows only
-        const uint64_t at = reinterpret_cast<uint64_t>(o.p) + (o.block ? (row0 >> 8) * o.block + (row0 & 255) * o.ld : (int64_t)row0 * o.ld);
-        // the buffer ends with the last row that exists: rows behind it read as zero (in blocks: as they are, they exist in memory)
-        const int64_t width = (int64_t)(o.chunks >> 3) * o.kstep + (o.chunks & 7) * 16;
-        rsrc = u32x4{(uint32_t)at, (uint32_t)(at >> 32), (uint32_t)((int64_t)(here - 1) * o.ld + width), 0x00020000u};
+        const uint64_t at = reinterpret_cast<uint64_t>(o.p) + (row0 >> 8) * o.block + (row0 & 255) * o.ld;
+        rsrc = u32x4{(uint32_t)at, (uint32_t)(at >> 32), (uint32_t)((here - 1) * o.ld) + o.width, 0x00020000u};
         kstep = o.kstep;
 #pragma unroll
         for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);

@@ -744,6 +744,8 @@ template <typename T, bool KEEP = false> struct EpiDz {
             const bool on = n < cnt;
             const float fac = early.f[j], mul = fac * inv, sub = -fac * off, ref = early.lse[j] * (KEEP ? -1.f : -LOG2E);
             float sum = 0.f;
+            // (a wave's part lies in one block of rows either way, and begins with a tile of them)
+            T *const zto = sizeof(T) == 4 ? dz.at(n, g.m0) : nullptr, *const tto = sizeof(T) == 4 ? dzt.at(g.m0, n) : nullptr;
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 T4 o;
@@ -756,10 +758,10 @@ template <typename T, bool KEEP = false> struct EpiDz {
                 }
                 if constexpr (sizeof(T) == 2) *reinterpret_cast<T4 *>(patch + P::at(16 * j + (g.lane & 15), 2 * i + (g.lane >> 5)) + (g.lane >> 4 & 1) * 8) = o;
                 else {
-                    if (!at_edge || n < cnt) *reinterpret_cast<T4 *>(dz.at(n, g.m0 + 16 * i)) = o;
+                    if (!at_edge || n < cnt) *reinterpret_cast<T4 *>(zto + i * 16 / CT * (256 * CT) + i * 16 % CT) = o;
                     if (!at_edge || n < ends)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) *dzt.at(g.m0 + 16 * i + r, n) = o[r];
+                        for (int r = 0; r < 4; ++r) tto[(16 * i + r) * CT] = o[r];
                 }
             }
             // the label's entry, where it is this lane's: written once more
@@ -805,17 +807,19 @@ template <typename T, bool KEEP = false> struct EpiDz {
         if constexpr (sizeof(T) == 2) {
             // from the patch both orders go out in 16-byte stores: its rows as they are, and transposed
             const int m0 = g.m0 - 4 * (g.lane >> 4), n0 = g.n0 - (g.lane & 15);
+            T *const zto = dz.at(n0 + g.lane / P::SLOTS, m0 + g.lane % P::SLOTS * 8);
 #pragma unroll
             for (int e = 0; e < 16 * NJ * P::SLOTS / 64; ++e) {
                 const int at = e * 64 + g.lane, row = at / P::SLOTS, slot = at % P::SLOTS;
-                if (!edge || n0 + row < cnt) *reinterpret_cast<tn::u32x4 *>(dz.at(n0 + row, m0 + slot * 8)) = *reinterpret_cast<const tn::u32x4 *>(patch + P::at(row, slot));
+                if (!edge || n0 + row < cnt) *reinterpret_cast<tn::u32x4 *>(zto + e * (64 / P::SLOTS) * CT) = *reinterpret_cast<const tn::u32x4 *>(patch + P::at(row, slot));
             }
             const int l = g.lane & 15, rows8 = (g.lane >> 4) * 8;
+            T *const tto = dzt.at(m0 + l, n0 + rows8);
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
                 for (int h = 0; h < NJ / 2; ++h)
-                    if (!edge || n0 + 32 * h + rows8 < ends) *reinterpret_cast<tn::u32x4 *>(dzt.at(m0 + 16 * i + l, n0 + 32 * h + rows8)) = P::transposed(patch, 32 * h + rows8, 16 * i, g.lane);
+                    if (!edge || n0 + 32 * h + rows8 < ends) *reinterpret_cast<tn::u32x4 *>(tto + i * 16 * CT + 32 * h) = P::transposed(patch, 32 * h + rows8, 16 * i, g.lane);
         }
     }
 };
@@ -1246,8 +1250,8 @@ void keep_first(const Call &c, const Shape &s, const float *w, int64_t ldw, int 
     const int n = (int)s.n, es = 4, n1 = std::max(n, 1), v0 = (int)((s.pieces - 1) * s.piece), p = (int)s.p - v0, before = v0 / KINDS[s.z.kind].m, kt = (int)(s.kpad * es / 128);
     const int *count = &cb.info->count;
     float2 *part = const_cast<float2 *>(cb.part), *here = part + (int64_t)before * s.npad;      // (a piece is whole tiles)
-    if (v0) stream<float>(tn::Args{{w, ldw * es, v0, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt}, v0, n1, s.z, EpiStats{part, nullptr, f32(s.o_zy), i32(s.o_y), count, v0, 0, (int)s.npad}, c.st);
-    tn::Args a{{w + v0 * ldw, ldw * es, p, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt};
+    if (v0) stream<float>(tn::Args{tn::plain(w, ldw * es, v0, wchunks), hop, count, tn::LIMIT_N, 0, 0, 1, kt}, v0, n1, s.z, EpiStats{part, nullptr, f32(s.o_zy), i32(s.o_y), count, v0, 0, (int)s.npad}, c.st);
+    tn::Args a{tn::plain(w + v0 * ldw, ldw * es, p, wchunks), hop, count, tn::LIMIT_N, 0, 0, 1, kt};
     grid(a, p, n1, s.z);
     float *sums = reinterpret_cast<float *>(here);
     const Keep kp{part, sums, f32(s.o_f), f32(s.o_ref), f32(s.o_zy), i32(s.o_idx), i32(s.o_y), cb.info, before, a.tiles_m, v0, (int)s.npad, c.o.reduction, (int)s.k, KINDS[s.z.kind].n,
@@ -1309,7 +1313,7 @@ template <typename T> void run(const Call &c, const Shape &s) {
     if (pwt) { wt = pwt; ldwt = s.ldp; wtpad = (int)s.ppad; }
 
     const int kt = (int)(s.kpad / step), n1 = std::max(n, 1), tiles = (p + KINDS[s.z.kind].m - 1) / KINDS[s.z.kind].m;
-    const tn::Operand hop{h, s.kpad * es, (int)s.npad, (int)(s.kpad / per)};
+    const tn::Operand hop = tn::plain(h, s.kpad * es, (int)s.npad, (int)(s.kpad / per));
     const Combine cb{reinterpret_cast<float2 *>(ws + s.o_part), s.o_zsum >= 0 ? f32(s.o_zsum) : nullptr, f32(s.o_zy), i32(s.o_idx), i32(s.o_y), info, tiles, (int)s.npad, p,
                      c.o.reduction, eps, f32(s.o_lse), f32(s.o_loss), c.lse, c.loss};
     // dz's blocks join the tiles' statistics of their columns themselves where that is a few of them: less than a launch (17 tiles, 83 columns:
@@ -1321,7 +1325,7 @@ template <typename T> void run(const Call &c, const Shape &s) {
     if (keep) {
         if constexpr (std::is_same<T, float>::value) keep_first(c, s, w, ldw, wchunks, hop, h, ht, dz, dzt, cb, f32, i32);
     } else if (!c.lse_given) {
-        tn::Args a{{w, ldw * es, p, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt};
+        tn::Args a{tn::plain(w, ldw * es, p, wchunks), hop, count, tn::LIMIT_N, 0, 0, 1, kt};
         stream<T>(a, p, n1, s.z, EpiStats{reinterpret_cast<float2 *>(ws + s.o_part), s.o_zsum >= 0 ? f32(s.o_zsum) : nullptr, f32(s.o_zy), i32(s.o_y), count, p, 0, (int)s.npad}, c.st);
         if (!few) {
             // as many threads for a column as leave every compute unit a block
@@ -1340,14 +1344,14 @@ template <typename T> void run(const Call &c, const Shape &s) {
         const int64_t q = keep ? s.pieces - 1 - t : t, v0 = q * s.piece;      // (the piece whose E was kept first)
         const int pv = (int)std::min(s.piece, s.p - v0), pt = (int)up(pv, step);
         const bool last = t + 1 == s.pieces;
-        tn::Args a{{w + v0 * ldw, ldw * es, pv, wchunks}, hop, count, tn::LIMIT_N, 0, 0, 1, kt};
+        tn::Args a{tn::plain(w + v0 * ldw, ldw * es, pv, wchunks), hop, count, tn::LIMIT_N, 0, 0, 1, kt};
         if (!keep || t)
             product<T>(a, pv, n1, s.z, EpiDz<T>{dz, dzt, f32(s.o_lse), f32(keep ? s.o_again_f : s.o_f), i32(s.o_y), count, pv, (int)v0, inv, label, off, few, cb, nullptr, nullptr}, c.st);
         // dH: rows are components, columns are packed columns
-        tn::Args b{{wt + v0, ldwt * es, k, (int)std::min<int64_t>((wtpad - v0) / per, s.piece / per)}, dz.operand((int)s.npad), count, tn::LIMIT_N, 0, 0, 0, pt / step};
+        tn::Args b{tn::plain(wt + v0, ldwt * es, k, (int)std::min<int64_t>((wtpad - v0) / per, s.piece / per)), dz.operand((int)s.npad), count, tn::LIMIT_N, 0, 0, 0, pt / step};
         const EpiSlot eh{f32(s.o_hslot), s.ldslot, s.npad * s.ldslot, (int)s.npad, t > 0};
         // dW: the contiguous index of dW is the row
-        const tn::Operand zop = dzt.operand(pv), top{ht, s.ldn * es, k, (int)(s.npad / per)};
+        const tn::Operand zop = dzt.operand(pv), top = tn::plain(ht, s.ldn * es, k, (int)(s.npad / per));
         const bool kfast = c.dW.cs == 1;
         T *out = dw + v0 * c.dW.rs;
         const int64_t ldo = kfast ? c.dW.rs : c.dW.cs;
