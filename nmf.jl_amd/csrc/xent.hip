@@ -689,7 +689,7 @@ template <typename T, bool KEEP = false> struct EpiDz {
     float inv, label, off;    // 1 / a, (1 - eps) / a, eps / (a p)
     int few;                  // the tiles' statistics are not joined yet: every block does it for its own columns
     Combine c;
-    float *part, *zy;         // KEEP: [tile_m][npad]; the labels' logits
+    float *part, *zy, *zsum;  // KEEP: [tile_m][npad]; the labels' logits; as part, or NULL
     // per column: log-sum-exp, factor, label's class in the piece.  The large tile has no registers for them to wait in: it reads them late.
     template <int MI, int NJ> struct Early { int cnt, y[NJ]; float lse[NJ], f[NJ]; };
     template <int BM, int BN, int WM, int WN> struct Shared { float lse[BN], t[WM * WN * 64]; float2 s[WM * WN * 64]; };
@@ -743,7 +743,7 @@ template <typename T, bool KEEP = false> struct EpiDz {
             const int n = g.n0 + 16 * j;
             const bool on = n < cnt;
             const float fac = early.f[j], mul = fac * inv, sub = -fac * off, ref = early.lse[j] * (KEEP ? -1.f : -LOG2E);
-            float sum = 0.f;
+            float sum = 0.f, zs = 0.f;
             // (a wave's part lies in one block of rows either way, and begins with a tile of them)
             T *const zto = sizeof(T) == 4 ? dz.at(n, g.m0) : nullptr, *const tto = sizeof(T) == 4 ? dzt.at(g.m0, n) : nullptr;
 #pragma unroll
@@ -753,7 +753,10 @@ template <typename T, bool KEEP = false> struct EpiDz {
                 for (int r = 0; r < 4; ++r) {
                     const float e = exp2_(__builtin_fmaf(acc[i][j][r], LOG2E, ref));
                     const float v = !at_edge || (on && g.m0 + 16 * i + r < p) ? (KEEP ? e : __builtin_fmaf(e, mul, sub)) : 0.f;
-                    sum += v;
+                    if (KEEP) {
+                        sum += v;
+                        if (zsum) zs += !at_edge || g.m0 + 16 * i + r < p ? acc[i][j][r] : 0.f;
+                    }
                     o[r] = to<T>(v);
                 }
                 if constexpr (sizeof(T) == 2) *reinterpret_cast<T4 *>(patch + P::at(16 * j + (g.lane & 15), 2 * i + (g.lane >> 5)) + (g.lane >> 4 & 1) * 8) = o;
@@ -785,7 +788,9 @@ template <typename T, bool KEEP = false> struct EpiDz {
             if constexpr (KEEP) {
                 sum += __shfl_xor(sum, 16);
                 sum += __shfl_xor(sum, 32);
-                if (g.lane < 16) sh.t[g.wm * BN + n - g.tile_n * BN] = sum;
+                zs += __shfl_xor(zs, 16);
+                zs += __shfl_xor(zs, 32);
+                if (g.lane < 16) sh.s[g.wm * BN + n - g.tile_n * BN] = make_float2(sum, zs);
             }
         };
         if (edge) {
@@ -798,10 +803,15 @@ template <typename T, bool KEEP = false> struct EpiDz {
         if constexpr (KEEP) {
             __syncthreads();
             if (g.tid < BN) {
-                float t = sh.t[g.tid];
+                float2 t = sh.s[g.tid];
 #pragma unroll
-                for (int w = 1; w < WM; ++w) t += sh.t[w * BN + g.tid];
-                part[(int64_t)g.tile_m * c.npad + g.tile_n * BN + g.tid] = t;
+                for (int w = 1; w < WM; ++w) {
+                    t.x += sh.s[w * BN + g.tid].x;
+                    t.y += sh.s[w * BN + g.tid].y;
+                }
+                const int64_t o = (int64_t)g.tile_m * c.npad + g.tile_n * BN + g.tid;
+                part[o] = t.x;
+                if (zsum) zsum[o] = t.y;
             }
         }
         if constexpr (sizeof(T) == 2) {
@@ -826,19 +836,20 @@ template <typename T, bool KEEP = false> struct EpiDz {
 
 // ---- E kept from the first pass ---------------------------------------------------------------------------------------------------------
 // (Of the last piece of the classes: the first ones' E would have to wait for its sums.)
-// Without smoothing dz_j = f_j / S_j (E_vj - S_j [v = y_j]) with E_vj = exp(z_vj - r_j), S_j = sum_v E_vj, whatever r_j is.  With r_j the
+// dz_j = f_j / S_j (E_vj - S_j (1 - eps) [v = y_j] - S_j eps / p) with E_vj = exp(z_vj - r_j), S_j = sum_v E_vj, whatever r_j is.  With r_j the
 // label's logit S_j = exp(l_j): between 1 and 10^30 for every loss that training sees.  So E is written by the pass that sums it, and the
 // logits are formed once: the column's factor f_j / S_j goes on dH's result and on H's image for dW.  The other pieces'
-// dz are formed to go with that: times S_j / f_j.
+// dz are formed to go with that: times S_j / f_j.  What smoothing takes from every entry is taken by a pass over the images (smooth_kernel).
 struct Keep {
     const float2 *before;     // [tile_m][npad]: statistics of the pieces in front
     const float *part;        // [tile_m][npad]: sums of E
-    const float *f, *ref, *zy;
+    const float *f, *ref, *zy, *zsum;     // zsum: [tile_m][npad] of all pieces, or NULL
     const int *idx, *y;
     const Info *info;
-    int tiles_before, tiles, v0, npad, reduction, k, per;   // v0: the piece's first class; per: columns of a tile of the product (what is done again)
+    float eps, a;
+    int p, tiles_before, tiles, v0, npad, reduction, k, per;   // v0: the piece's first class; per: columns of a tile of the product (what is done again)
     float *lse_c, *loss_c, *lse, *loss;
-    float *scale, *again_f;   // of a column: f_j / S_j, and what its dz is multiplied by if it is formed again
+    float *scale, *again_f, *shift;   // of a column: f_j / (a S_j); what its dz is multiplied by where it is formed again; S_j eps / p
     int *again;               // per tile: some column's sum is out of range
     tn::Blocked<float> dz, dzt;
     int64_t ldn;              // of H's image
@@ -863,7 +874,7 @@ __global__ __launch_bounds__(256) void label_kernel(Keep s, const float *w, int6
 }
 // joins the tiles' sums of 2^lc (at least 8) columns, finishes them, puts the label's entry right and scales H's image
 __global__ __launch_bounds__(256) void keep_kernel(Keep s, float *ht, int lc) {
-    __shared__ float ps[256], by[256];
+    __shared__ float ps[256], zs[256], by[256];
     const int cols = 1 << lc, step = 256 >> lc, at = threadIdx.x & (cols - 1), slice = threadIdx.x >> lc;
     const int cnt = s.info->count, i0 = blockIdx.x * cols, i = i0 + at;
     if (i0 >= cnt) return;
@@ -876,10 +887,17 @@ __global__ __launch_bounds__(256) void keep_kernel(Keep s, float *ht, int lc) {
         const float2 b = s.before[(int64_t)q * s.npad + i];
         a += b.y != 0.f ? b.y * exp2_(b.x - r) : 0.f;
     }
+    float t = 0.f;
+    if (s.zsum)
+        for (int q = slice; q < s.tiles_before + s.tiles; q += step) t += s.zsum[(int64_t)q * s.npad + i];
     ps[threadIdx.x] = a;
+    zs[threadIdx.x] = t;
     for (int o = step / 2; o; o >>= 1) {
         __syncthreads();
-        if (slice < o) ps[threadIdx.x] += ps[threadIdx.x + (o << lc)];
+        if (slice < o) {
+            ps[threadIdx.x] += ps[threadIdx.x + (o << lc)];
+            zs[threadIdx.x] += zs[threadIdx.x + (o << lc)];
+        }
     }
     if (slice == 0) {
         by[at] = 0.f;
@@ -890,10 +908,11 @@ __global__ __launch_bounds__(256) void keep_kernel(Keep s, float *ht, int lc) {
             float v = __builtin_nanf(""), l = v, c = v;
             if (lab >= 0) {
                 v = (r + log2f(sum)) * LN2;
-                l = v - s.zy[i];
-                c = good ? f / sum : 1.f;
+                l = v - (1.f - s.eps) * s.zy[i];
+                if (s.zsum) l -= s.eps * (zs[at] / (float)s.p);
+                c = good ? f / (sum * s.a) : 1.f;
                 if (lab >= s.v0) {
-                    const float e = exp2_(__builtin_fmaf(s.zy[i], LOG2E, -r)) - sum;
+                    const float e = exp2_(__builtin_fmaf(s.zy[i], LOG2E, -r)) - sum * (1.f - s.eps);
                     *s.dz.at(i, lab - s.v0) = e;
                     *s.dzt.at(lab - s.v0, i) = e;
                 }
@@ -905,7 +924,8 @@ __global__ __launch_bounds__(256) void keep_kernel(Keep s, float *ht, int lc) {
             if (s.lse) s.lse[col] = v;
             if (s.loss && s.reduction == NMFX_REDUCE_NONE) s.loss[col] = l;
             s.scale[i] = by[at] = c;
-            s.again_f[i] = good ? sum : f;
+            s.again_f[i] = good ? sum * s.a : f;
+            if (s.zsum) s.shift[i] = good ? sum * (s.eps / (float)s.p) : 0.f;
         }
     }
     __syncthreads();
@@ -914,6 +934,25 @@ __global__ __launch_bounds__(256) void keep_kernel(Keep s, float *ht, int lc) {
         const int c = e / chunks, o = e % chunks * 4;
         f32x4 *x = reinterpret_cast<f32x4 *>(ht + c * s.ldn + i0 + o);
         *x = *x * f32x4{by[o], by[o + 1], by[o + 2], by[o + 3]};
+    }
+}
+
+// what smoothing takes from every entry of the piece's images, by its column.  Read and written once each: cheaper than the logits again from
+// k = 256 or so on.
+__global__ __launch_bounds__(256) void smooth_kernel(Keep s, int classes, int64_t chunks) {
+    const int cnt = s.info->count;
+    for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < 2 * chunks; e += gridDim.x * 256ll) {
+        const bool turned = e >= chunks;                  // dzt: rows are classes
+        const int64_t q = turned ? e - chunks : e, tile = q >> 11;
+        const int kt = turned ? s.dzt.ktiles : s.dz.ktiles, block = (int)(tile / kt);
+        const int row = block * 256 + (int)(q >> 3 & 255), c = (int)(tile - (int64_t)block * kt) * 32 + (int)(q & 7) * 4;
+        if (row >= (turned ? classes : cnt) || c >= (turned ? cnt : classes)) continue;
+        f32x4 *x = reinterpret_cast<f32x4 *>(turned ? s.dzt.p : s.dz.p) + q;
+        f32x4 v = *x;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (c + u < (turned ? cnt : classes)) v[u] -= s.shift[turned ? c + u : row];
+        *x = v;
     }
 }
 
@@ -1066,7 +1105,7 @@ struct Shape {
     bool w_slots, direct;         // direct: dH need not be summed from slots
     bool keep;                    // E is kept from the first pass
     // workspace offsets
-    int64_t o_info, o_counts, o_idx, o_pos, o_y, o_f, o_lse, o_loss, o_zy, o_h, o_ht, o_w, o_wt, o_part, o_zsum, o_ref, o_scale, o_again_f, o_again, o_dz, o_dzt, o_hslot, o_wslot, bytes;
+    int64_t o_info, o_counts, o_idx, o_pos, o_y, o_f, o_lse, o_loss, o_zy, o_h, o_ht, o_w, o_wt, o_part, o_zsum, o_ref, o_scale, o_again_f, o_shift, o_again, o_dz, o_dzt, o_hslot, o_wslot, bytes;
 };
 
 constexpr int CUS = 256;
@@ -1120,8 +1159,10 @@ void choose_two(int64_t hm, int64_t hn, int64_t hk, int64_t wm, int64_t wn, int6
 // E is kept from the first pass in f32, where a pass over the logits takes longer than this estimate (us) and so more than the two launches
 // that come with it: 5000 x 1000, k = 100 (estimate 18): 100 -> 83 us; 2000 x 400, k = 42 (3.3): 33 -> 35 us.  (Not in 16 bits: the rounding of the
 // scaled H is not small there, and shows in the rows of dW that are mostly labels: bf16, 32768 x 4096, k = 1024, 1067 -> 894 us, but
-// gradients 2.9e-3 off instead of 1.7e-3.  Not with smoothing: it takes a part from every entry that E's rounding would show in.)
+// gradients 2.9e-3 off instead of 1.7e-3.)  With smoothing a pass over the images comes on top: 20000 x 3000, k = 256: 1181 -> 1107 us,
+// 32768 x 8192, k = 1024: 16.6 -> 13.1 ms (without: 14.4 -> 12.1).
 constexpr double KEEP_US = 6.;
+constexpr int KEEP_SMOOTHED = 256;
 
 Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     Shape s{};
@@ -1135,8 +1176,8 @@ Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     s.npad = up(std::max<int64_t>(s.n, 1), 256);
     s.kpad = up(s.k, step);
     s.ppad = up(s.p, 256);
-    // two images of dz of at most 512 MiB each, and pieces of one size
-    const int64_t most = std::max<int64_t>(256, ((512ll << 20) / (s.npad * s.es)) / 256 * 256);
+    // two images of dz of at most 2^28 elements each (or 256 classes), and pieces of one size
+    const int64_t most = std::max<int64_t>(256, ((1ll << 28) / s.npad) / 256 * 256);
     s.pieces = (s.ppad + most - 1) / most;
     s.piece = up((s.ppad + s.pieces - 1) / s.pieces, 256);
     s.pieces = (s.ppad + s.piece - 1) / s.piece;
@@ -1146,7 +1187,7 @@ Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     const int64_t pp = std::min(s.piece, s.p);
     const Guess z = choose(pp, n1, s.kpad / step, s.es);
     s.z = z.c;
-    s.keep = grad && !smooth && W.dtype == NMFX_F32 && z.us > KEEP_US;
+    s.keep = grad && W.dtype == NMFX_F32 && z.us > KEEP_US && (!smooth || s.k >= KEEP_SMOOTHED);
     choose_two(s.k, n1, (pp + step - 1) / step, pp, s.k, (n1 + step - 1) / step, s.es, s.pieces == 1, s.h, s.w);
     s.direct = s.pieces == 1 && s.h.splits == 1 && s.w.splits == 1 && s.h.kind == s.w.kind;
     s.w_slots = s.w.splits > 1;
@@ -1160,8 +1201,8 @@ Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     const int64_t tiles = (s.p + KINDS[s.z.kind].m - 1) / KINDS[s.z.kind].m, parts = std::max<int64_t>(tiles * s.npad, 16 * 4 * CUS);
     s.o_part = take(parts * sizeof(float2));
     s.o_zsum = smooth ? take(parts * 4) : -1;
-    s.o_ref = s.o_scale = s.o_again_f = s.o_again = -1;
-    if (s.keep) { s.o_ref = take(s.npad * 4); s.o_scale = take(s.npad * 4); s.o_again_f = take(s.npad * 4); s.o_again = take(s.npad / 64 * 4); }
+    s.o_ref = s.o_scale = s.o_again_f = s.o_shift = s.o_again = -1;
+    if (s.keep) { s.o_ref = take(s.npad * 4); s.o_scale = take(s.npad * 4); s.o_again_f = take(s.npad * 4); s.o_shift = take(s.npad * 4); s.o_again = take(s.npad / 64 * 4); }
     s.o_w = s.w_rows_direct ? -1 : take(s.p * s.kpad * s.es);
     s.o_ht = s.o_wt = s.o_dz = s.o_dzt = s.o_hslot = s.o_wslot = -1;
     if (grad) {
@@ -1246,26 +1287,32 @@ template <typename T> void score(const Call &c, const Shape &s) {
 
 // the first pass with E kept, up to the images that the gradient products read
 template <typename F, typename I>
-void keep_first(const Call &c, const Shape &s, const float *w, int64_t ldw, int wchunks, const tn::Operand &hop, const float *h, float *ht, const tn::Blocked<float> &dz, const tn::Blocked<float> &dzt, const Combine &cb, F f32, I i32) {
+void keep_first(const Call &c, const Shape &s, const float *w, int64_t ldw, int wchunks, const tn::Operand &hop, const float *h, float *ht, const tn::Blocked<float> &dz, const tn::Blocked<float> &dzt, const Combine &cb, float a_, float inv, float label, float off, F f32, I i32) {
     const int n = (int)s.n, es = 4, n1 = std::max(n, 1), v0 = (int)((s.pieces - 1) * s.piece), p = (int)s.p - v0, before = v0 / KINDS[s.z.kind].m, kt = (int)(s.kpad * es / 128);
     const int *count = &cb.info->count;
     float2 *part = const_cast<float2 *>(cb.part), *here = part + (int64_t)before * s.npad;      // (a piece is whole tiles)
-    if (v0) stream<float>(tn::Args{tn::plain(w, ldw * es, v0, wchunks), hop, count, tn::LIMIT_N, 0, 0, 1, kt}, v0, n1, s.z, EpiStats{part, nullptr, f32(s.o_zy), i32(s.o_y), count, v0, 0, (int)s.npad}, c.st);
+    float *zsum = const_cast<float *>(cb.zsum), *zhere = zsum ? zsum + (int64_t)before * s.npad : nullptr;
+    if (v0) stream<float>(tn::Args{tn::plain(w, ldw * es, v0, wchunks), hop, count, tn::LIMIT_N, 0, 0, 1, kt}, v0, n1, s.z, EpiStats{part, zsum, f32(s.o_zy), i32(s.o_y), count, v0, 0, (int)s.npad}, c.st);
     tn::Args a{tn::plain(w + v0 * ldw, ldw * es, p, wchunks), hop, count, tn::LIMIT_N, 0, 0, 1, kt};
     grid(a, p, n1, s.z);
     float *sums = reinterpret_cast<float *>(here);
-    const Keep kp{part, sums, f32(s.o_f), f32(s.o_ref), f32(s.o_zy), i32(s.o_idx), i32(s.o_y), cb.info, before, a.tiles_m, v0, (int)s.npad, c.o.reduction, (int)s.k, KINDS[s.z.kind].n,
-                  f32(s.o_lse), f32(s.o_loss), c.lse, c.loss, f32(s.o_scale), f32(s.o_again_f), i32(s.o_again), dz, dzt, s.ldn};
+    const Keep kp{part, sums, f32(s.o_f), f32(s.o_ref), f32(s.o_zy), zsum, i32(s.o_idx), i32(s.o_y), cb.info, cb.eps, a_, (int)s.p, before, a.tiles_m, v0, (int)s.npad, c.o.reduction, (int)s.k, KINDS[s.z.kind].n,
+                  f32(s.o_lse), f32(s.o_loss), c.lse, c.loss, f32(s.o_scale), f32(s.o_again_f), f32(s.o_shift), i32(s.o_again), dz, dzt, s.ldn};
     label_kernel<<<(n1 + 3) / 4, 256, 0, c.st>>>(kp, w, ldw, wchunks, h, s.kpad, f32(s.o_ref), a.tiles_n);
     ops::hip_ok(hipGetLastError(), "label");
-    product<float>(a, p, n1, s.z, EpiDz<float, true>{dz, dzt, f32(s.o_ref), nullptr, i32(s.o_y), count, p, v0, 1.f, 0.f, 0.f, 0, cb, sums, f32(s.o_zy)}, c.st);
+    product<float>(a, p, n1, s.z, EpiDz<float, true>{dz, dzt, f32(s.o_ref), nullptr, i32(s.o_y), count, p, v0, 1.f, 0.f, 0.f, 0, cb, sums, f32(s.o_zy), zhere}, c.st);
     int lc = 6;
     while (lc > 3 && (n1 >> lc) < CUS) --lc;
     keep_kernel<<<(n1 + (1 << lc) - 1) >> lc, 256, 0, c.st>>>(kp, ht, lc);
     ops::hip_ok(hipGetLastError(), "keep");
+    if (zsum) {
+        const int64_t chunks = s.npad * s.piece / 4;
+        smooth_kernel<<<(int)std::min<int64_t>(8 * CUS, (chunks + 127) / 128), 256, 0, c.st>>>(kp, p, chunks);
+        ops::hip_ok(hipGetLastError(), "smooth");
+    }
     // columns whose sums left the range of E, by tiles: the way with a pass for the log-sum-exp in front
-    const EpiStats ea{here, nullptr, f32(s.o_zy), i32(s.o_y), count, p, v0, (int)s.npad};
-    const EpiDz<float> eb{dz, dzt, f32(s.o_lse), f32(s.o_again_f), i32(s.o_y), count, p, v0, 1.f, 1.f, 0.f, 0, cb, nullptr, nullptr};
+    const EpiStats ea{here, zhere, f32(s.o_zy), i32(s.o_y), count, p, v0, (int)s.npad};
+    const EpiDz<float> eb{dz, dzt, f32(s.o_lse), f32(s.o_again_f), i32(s.o_y), count, p, v0, inv, label, off, 0, cb, nullptr, nullptr};
     switch (s.z.kind) {
         case 0: tn::tn_again_kernel<float, 256, 256, 2, 4, 2, EpiStats, Columnwise, EpiDz<float>><<<a.tiles_n, 512, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
         case 1: tn::tn_again_kernel<float, 128, 128, 2, 2, 2, EpiStats, Columnwise, EpiDz<float>><<<a.tiles_n, 256, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
@@ -1323,7 +1370,7 @@ template <typename T> void run(const Call &c, const Shape &s) {
     const tn::Blocked<T> dz{c.grad ? reinterpret_cast<T *>(ws + s.o_dz) : nullptr, (int)(s.piece / step)}, dzt{c.grad ? reinterpret_cast<T *>(ws + s.o_dzt) : nullptr, (int)(s.npad / step)};
     const float inv = (float)(1. / a_), label = (float)((1. - c.o.label_smoothing) / a_), off = (float)(c.o.label_smoothing / (a_ * p));
     if (keep) {
-        if constexpr (std::is_same<T, float>::value) keep_first(c, s, w, ldw, wchunks, hop, h, ht, dz, dzt, cb, f32, i32);
+        if constexpr (std::is_same<T, float>::value) keep_first(c, s, w, ldw, wchunks, hop, h, ht, dz, dzt, cb, (float)a_, inv, label, off, f32, i32);
     } else if (!c.lse_given) {
         tn::Args a{tn::plain(w, ldw * es, p, wchunks), hop, count, tn::LIMIT_N, 0, 0, 1, kt};
         stream<T>(a, p, n1, s.z, EpiStats{reinterpret_cast<float2 *>(ws + s.o_part), s.o_zsum >= 0 ? f32(s.o_zsum) : nullptr, f32(s.o_zy), i32(s.o_y), count, p, 0, (int)s.npad}, c.st);

@@ -231,9 +231,8 @@ def test_xent_no_columns():
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_xent_several_pieces_of_the_classes(dtype):
-    """600,001 classes: dz of all of them at 256 packed columns is over 512 MiB in Float32, so the gradients go in pieces."""
-    n = 256 if dtype == "f32" else 700
-    check(*problem(600001, n, 9, dtype, seed=6, ignored=0.1), dtype)
+    """600,001 classes: dz of all of them at 700 columns has over 2^28 entries, so the gradients go in pieces."""
+    check(*problem(600001, 700, 9, dtype, seed=6, ignored=0.1), dtype)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -276,7 +275,7 @@ def test_xent_factors_of_many_columns(n):
 
 
 # sizes that form the logits once
-ONCE = [("f32", 300001, 600, 9), ("f32", 1024, 300, 300), ("f32", 5000, 1000, 100), ("f32", 1537, 2500, 129), ("f32", 4097, 1100, 520)]
+ONCE = [("f32", 400001, 600, 9), ("f32", 1024, 300, 300), ("f32", 5000, 1000, 100), ("f32", 1537, 2500, 129), ("f32", 4097, 1100, 520)]
 
 
 @pytest.mark.parametrize("dtype,p,n,k", ONCE)
@@ -285,6 +284,13 @@ def test_xent_logits_formed_once(dtype, p, n, k, wl, ignored, reduction):
     W, H, y = problem(p, n, k, dtype, seed=p + n, ignored=ignored, wl=wl)
     gout = torch.linspace(-2, 2, n, device=DEV) if reduction == "none" else None
     check(W, H, y, dtype, reduction=reduction, gout=gout)
+
+
+@pytest.mark.parametrize("p,n,k", [(1024, 300, 300), (5001, 1000, 256), (4097, 1100, 520), (160001, 2000, 257)])
+@pytest.mark.parametrize("eps,ignored", [(0.1, 0.0), (0.7, 0.3), (1.0, 0.95), (0.1, 1.0)])
+def test_xent_logits_formed_once_with_smoothing(p, n, k, eps, ignored):
+    W, H, y = problem(p, n, k, "f32", seed=p + n, ignored=ignored, wl="r" if p % 2 else "c")
+    check(W, H, y, "f32", eps=eps, reduction="none", gout=torch.linspace(-2, 2, n, device=DEV))
 
 
 @pytest.mark.parametrize("dtype,p,n,k", [ONCE[0], ONCE[2], ONCE[4]])
@@ -298,6 +304,7 @@ def test_xent_losses_beyond_any_exponential(dtype, p, n, k):
     H = H.clone()
     H[:, cols] = (H[:, cols].double() * (torch.tensor([50.0, 68.0, 75.0, 87.0, 200.0, 1000.0], device=DEV, dtype=torch.float64) / spread)).to(H.dtype)
     check(W, H, y, dtype, reduction="none", gout=torch.linspace(-1, 1, n, device=DEV))
+    check(W, H, y, dtype, eps=0.2, reduction="none", gout=torch.linspace(-1, 1, n, device=DEV))
 
 
 @pytest.mark.parametrize("dtype,p,n,k", ONCE[2:4])
