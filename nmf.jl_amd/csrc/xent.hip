@@ -676,8 +676,9 @@ __global__ __launch_bounds__(1024) void score_join_kernel(Score a, int blocks, f
 
 // ---- dz of a piece of the classes, in both orders -----------------------------------------------------------------------------------
 // Both gradient products contract an index that has to be contiguous, so dz is written twice: 32768 x 8192, k = 2048: 995 us (1105 TFLOP/s
-// with 1.07 GB of stores); 16384 x 16384, k = 256, 400 us: bound by the stores (2.7 TB/s) and the exponentials.  It is rounded to the type of
-// W and H there, the one rounding in front of the products: in f32 they would run at an eighth of the rate.
+// with 1.07 GB of stores); 16384 x 16384, k = 256, f16: 353 us, bound by the stores (3.0 TB/s) and the exponentials.  It is rounded to the type of
+// W and H there, the one rounding in front of the products: in f32 they would run at an eighth of the rate.  Both images are in blocks
+// (tn::Blocked): with padded rows that case took 400 us here and the products that read them 465 instead of 326.
 template <typename T> __device__ __forceinline__ T to(float x) { return (T)x; }
 
 // KEEP (f32): the same images of E = exp(z - r_j) instead, before the log-sum-exp is known, with the tiles' sums of E and the labels' logits.

@@ -355,6 +355,71 @@ function pdrsolve!(ctx::Context{T}, A::Matrix{T}, B::Matrix{T}, x::Matrix{T}; la
     x
 end
 
+# ---- operators on device matrices (include/nmfx.h): softmax cross entropy of W*H with its gradients, gradient norm, clipping ----------
+# They take matrices that are in device memory (for example `pointer` of an AMDGPU.jl ROCArray), run on the caller's stream and return at
+# once; the workspace (device memory of the size the *_workspace function gives) and every output are the caller's and live until the
+# stream has passed them.
+struct DMat      # struct nmfx_dmat: element (i, j) at data + (i-1)*rs + (j-1)*cs, strides in elements
+    data::Ptr{Cvoid}
+    rows::Int64
+    cols::Int64
+    rs::Int64
+    cs::Int64
+    dtype::Int32      # 0 Float32, 1 Float64, 2 BFloat16, 3 Float16
+    reserved::Int32
+end
+DMat(data::Ptr, rows::Integer, cols::Integer, dtype::Integer; ld::Integer=rows) = DMat(convert(Ptr{Cvoid}, data), rows, cols, 1, ld, dtype, 0)   # column-major
+
+struct CXentOpts  # struct nmfx_xent_opts
+    label_smoothing::Float64
+    ignore_index::Int64
+    reduction::Int32  # 0 none, 1 sum, 2 mean
+    reserved0::Int32
+end
+CXentOpts(; label_smoothing::Real=0, ignore_index::Integer=-100, reduction::Integer=2) = CXentOpts(label_smoothing, ignore_index, reduction, 0)
+
+function opcheck(status::Cint)
+    status == 0 && return nothing
+    msg = unsafe_string(ccall((:nmfx_last_op_error, libnmfx), Cstring, ()))
+    status == 1 && throw(ArgumentError(msg))
+    status == 2 && throw(DimensionMismatch(msg))
+    error("nmfx status $status: $msg")
+end
+
+function xent_workspace(W::DMat, H::DMat, o::CXentOpts, grad::Bool)
+    n = Ref{Int64}(0)
+    opcheck(ccall((:nmfx_xent_workspace, libnmfx), Cint, (Ref{DMat}, Ref{DMat}, Ref{CXentOpts}, Cint, Ref{Int64}), W, H, o, grad, n))
+    n[]
+end
+# labels: n Int64 classes, counted from 0; loss, lse: Float32; all device pointers
+function xent!(loss::Ptr{Float32}, lse::Ptr{Float32}, W::DMat, H::DMat, labels::Ptr{Int64}, o::CXentOpts, ws::Ptr{Cvoid}, bytes::Integer, device::Integer, stream::Ptr{Cvoid})
+    opcheck(ccall((:nmfx_xent, libnmfx), Cint,
+                  (Ref{DMat}, Ref{DMat}, Ptr{Int64}, Ref{CXentOpts}, Ptr{Float32}, Ptr{Float32}, Ptr{Cvoid}, Int64, Cint, Ptr{Cvoid}),
+                  W, H, labels, o, loss, lse, ws, bytes, device, stream))
+end
+# lse_given: lse holds what xent! gave, and only dW and dH are written; gout: the gradient in the loss, or C_NULL for 1
+function xent_grad!(dW::DMat, dH::DMat, loss::Ptr{Float32}, lse::Ptr{Float32}, W::DMat, H::DMat, labels::Ptr{Int64}, o::CXentOpts, gout::Ptr{Float32}, lse_given::Bool,
+                    ws::Ptr{Cvoid}, bytes::Integer, device::Integer, stream::Ptr{Cvoid})
+    opcheck(ccall((:nmfx_xent_grad, libnmfx), Cint,
+                  (Ref{DMat}, Ref{DMat}, Ptr{Int64}, Ref{CXentOpts}, Ptr{Float32}, Cint, Ptr{Float32}, Ptr{Float32}, Ref{DMat}, Ref{DMat}, Ptr{Cvoid}, Int64, Cint, Ptr{Cvoid}),
+                  W, H, labels, o, gout, lse_given, loss, lse, dW, dH, ws, bytes, device, stream))
+end
+
+function grad_norm_workspace(count::Integer)
+    n = Ref{Int64}(0)
+    opcheck(ccall((:nmfx_grad_norm_workspace, libnmfx), Cint, (Cint, Ref{Int64}), count, n))
+    n[]
+end
+# kind: 2, or 0 for the largest magnitude; norm: one Float32 on the device
+function grad_norm!(norm::Ptr{Float32}, grads::Vector{DMat}, kind::Integer, ws::Ptr{Cvoid}, bytes::Integer, device::Integer, stream::Ptr{Cvoid})
+    opcheck(ccall((:nmfx_grad_norm, libnmfx), Cint, (Cint, Ptr{DMat}, Cint, Ptr{Float32}, Ptr{Cvoid}, Int64, Cint, Ptr{Cvoid}),
+                  length(grads), grads, kind, norm, ws, bytes, device, stream))
+end
+function clip_grad_norm!(norm::Ptr{Float32}, grads::Vector{DMat}, max_norm::Real, kind::Integer, ws::Ptr{Cvoid}, bytes::Integer, device::Integer, stream::Ptr{Cvoid})
+    opcheck(ccall((:nmfx_clip_grad_norm, libnmfx), Cint, (Cint, Ptr{DMat}, Ptr{DMat}, Float64, Cint, Ptr{Float32}, Ptr{Cvoid}, Int64, Cint, Ptr{Cvoid}),
+                  length(grads), grads, C_NULL, max_norm, kind, norm, ws, bytes, device, stream))
+end
+
 # ---- multi-GPU from ONE Julia process: one task (thread) per Context, all attached to a local group (include/nmfx.h) --------
 # g = local_group(nranks); Threads.@spawn per rank: ctx = Context{T}(...) on its device; attach!(ctx, g, rank) BEFORE the X upload
 # changes anything (the row padding depends on nranks); then solve! as usual with the rank's column shard of X and H.
