@@ -380,12 +380,14 @@ int nmfx_xent_workspace(const nmfx_dmat *W, const nmfx_dmat *H, const nmfx_xent_
 int nmfx_xent(const nmfx_dmat *W, const nmfx_dmat *H, const int64_t *labels, const nmfx_xent_opts *opts, float *loss, float *lse,
               void *workspace, int64_t workspace_bytes, int device, void *stream);
 
-/* Its gradients dW (p x k) and dH (k x n), of the types of W and H, any strides of their own; overlapping no input.
+/* Its gradients dW (p x k) and dH (k x n), of the types of W and H, any strides of their own; they may share no element with each other, W or H
+ * (NMFX_ERR_BAD_ARG; matrices that interleave with different strides count as sharing).
  *   gout       the gradient of what follows in the loss: n values for NMFX_REDUCE_NONE, else one; NULL stands for 1
  *   lse_given  0: loss (or NULL) and lse (or NULL) are computed and written as nmfx_xent does
  *              1: lse holds what nmfx_xent gave for the same W, H and labels, and is read; loss is not written
  * dZ is formed per piece of the classes and rounded to the type of W and H in front of the two products (Float16: scaled by a power of two
- * into its range first); the sums are Float32 and rounded once. */
+ * into its range first); the sums are Float32 and rounded once.  (Float32: where that is faster exp(Z - Z[label]) is kept from the first pass
+ * and scaled afterwards.) */
 int nmfx_xent_grad(const nmfx_dmat *W, const nmfx_dmat *H, const int64_t *labels, const nmfx_xent_opts *opts, const float *gout,
                    int lse_given, float *loss, float *lse, const nmfx_dmat *dW, const nmfx_dmat *dH, void *workspace,
                    int64_t workspace_bytes, int device, void *stream);
@@ -395,7 +397,7 @@ int nmfx_xent_grad(const nmfx_dmat *W, const nmfx_dmat *H, const int64_t *labels
  * The list may mix all four types; a vector is a matrix of one row.  Squares are summed in Float64.  *norm (device memory) is Float32.
  * out = NULL: in place (nothing is written where coef = 1); else out[i] has grads[i]'s shape, type and contiguous index.  No two matrices
  * written may share elements, and none may be part of another's gradient (NMFX_ERR_BAD_ARG).  A NaN among the gradients makes the norm
- * and every result NaN; an infinite norm makes coef 0. */
+ * and every result NaN; an infinite norm makes coef 0 (NaN where max_norm is infinite too). */
 enum { NMFX_NORM_2 = 2, NMFX_NORM_INF = 0 };
 int nmfx_grad_norm_workspace(int count, int64_t *bytes);
 int nmfx_grad_norm(int count, const nmfx_dmat *grads, int norm_type, float *norm, void *workspace, int64_t workspace_bytes, int device,

@@ -191,6 +191,23 @@ def _list(ts, name, device):
     return a, sizes
 
 
+def _few(ts, index):
+    """The descriptors of a short list (2 us for two tensors; _list, made for hundreds, takes 6), or None where a tensor is not contiguous or
+    not what it should be: _list then says what."""
+    codes, sizes = _state["dtypes"], []
+    a = (L.DMat * len(ts))()
+    try:
+        for d, t in zip(a, ts):
+            if t.get_device() != index or not t.is_contiguous():
+                return None
+            n = t.numel()
+            sizes.append(n)
+            d.data, d.rows, d.cols, d.rs, d.cs, d.dtype = t.data_ptr(), 1, n, n, 1, codes[t.dtype]
+    except (TypeError, AttributeError, KeyError):
+        return None
+    return a, sizes
+
+
 def _strided(a, i, t, name):
     if t.dim() == 1:
         a[i] = (t.data_ptr(), t.shape[0], 1, t.stride(0), 1, a[i]["dtype"], 0)
@@ -208,6 +225,29 @@ def _norm_type(norm_type):
     raise ArgumentError(f"norm_type must be 2 or inf, not {norm_type!r}")
 
 
+def _lists(grads, out, dev):
+    """The descriptors of grads and of out (or None), as pointers to arrays that live as long as they do."""
+    a, sizes = _list(grads, "grads", dev)
+    if out is None:
+        return _pointer(a), None
+    b, counts = _list(out, "out", dev)
+    if sizes != counts:
+        raise DimensionMismatch("one of out has another number of elements than its gradient")
+    # where one of the two is not contiguous both go by the strides of their matrix
+    odd = (a["rows"] != 1) | (b["rows"] != 1)
+    if odd.any():
+        for i in np.nonzero(odd)[0]:
+            if grads[i].shape != out[i].shape:
+                raise DimensionMismatch("one of out has another shape than its gradient")
+            _strided(a, i, grads[i], "grads")
+            _strided(b, i, out[i], "out")
+    return _pointer(a), _pointer(b)
+
+
+def _pointer(a):
+    return (L.DMat * len(a)).from_buffer(a)
+
+
 def _norm(grads, max_norm, norm_type, out):
     torch = _torch()
     kind = _norm_type(norm_type)
@@ -217,23 +257,21 @@ def _norm(grads, max_norm, norm_type, out):
     if not isinstance(grads[0], torch.Tensor):
         raise ArgumentError("grads must be torch tensors")
     dev = grads[0].device
-    a, sizes = _list(grads, "grads", dev)
-    b = None
     if out is not None:
         out = [out] if isinstance(out, torch.Tensor) else list(out)
         if len(out) != len(grads):
             raise DimensionMismatch(f"out has {len(out)} tensors, grads {len(grads)}")
-        b, counts = _list(out, "out", dev)
-        if sizes != counts:
-            raise DimensionMismatch("one of out has another number of elements than its gradient")
-        # where one of the two is not contiguous both go by the strides of their matrix
-        odd = (a["rows"] != 1) | (b["rows"] != 1)
-        if odd.any():
-            for i in np.nonzero(odd)[0]:
-                if grads[i].shape != out[i].shape:
-                    raise DimensionMismatch("one of out has another shape than its gradient")
-                _strided(a, i, grads[i], "grads")
-                _strided(b, i, out[i], "out")
+    few = len(grads) <= 8
+    a = few and _few(grads, dev.index)
+    b = few and out is not None and _few(out, dev.index)
+    if a and (b or out is None):
+        a, sizes = a
+        if b:
+            b, counts = b
+            if sizes != counts:
+                raise DimensionMismatch("one of out has another number of elements than its gradient")
+    else:
+        a, b = _lists(grads, out, dev)
     lib = L.load()
     size = C.c_int64()
     _ck(lib.nmfx_grad_norm_workspace(len(grads), size))
@@ -241,9 +279,9 @@ def _norm(grads, max_norm, norm_type, out):
     norm = torch.empty((), dtype=torch.float32, device=dev)
     common = (norm.data_ptr(), ws.data_ptr(), size.value, dev.index, _stream(dev.index))
     if max_norm is None:
-        _ck(lib.nmfx_grad_norm(len(grads), a.ctypes.data, kind, *common))
+        _ck(lib.nmfx_grad_norm(len(grads), a, kind, *common))
     else:
-        _ck(lib.nmfx_clip_grad_norm(len(grads), a.ctypes.data, None if b is None else b.ctypes.data, float(max_norm), kind, *common))
+        _ck(lib.nmfx_clip_grad_norm(len(grads), a, b or None, float(max_norm), kind, *common))
     return norm
 
 

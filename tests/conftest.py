@@ -38,8 +38,9 @@ def pytest_collection_modifyitems(items):
 
 @pytest.fixture(scope="session")
 def built():
-    """Make sure libnmfx.so and the C oracle exist (cross-compiles on CPU)."""
+    """Make sure libnmfx.so and the C oracle exist (cross-compiles on CPU).  What is there is loaded: after a change to a source, build."""
     sys.path.insert(0, ROOT)
     import __graft_entry__ as g
-    g.build()
+    if not (os.path.exists(g.LIB) and os.path.exists(os.path.join(ROOT, "oracle", "libnmf_oracle.so"))):
+        g.build()
     return True
