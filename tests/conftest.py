@@ -7,7 +7,9 @@ import pytest
 # spins on the device until its peers' signal kernels have run, so no two ranks' streams may share a hardware queue (HIP multiplexes a
 # process's streams onto GPU_MAX_HW_QUEUES = 4 queues by default; a signal queued behind a spinning wait would never run).  Read by
 # the HIP runtime at initialisation, hence before torch.  One process per GPU -- the production layout -- needs nothing of the kind.
-# (At least 24: an environment that states the runtime's own default of 4 would leave the ranks sharing queues.)
+# (With an environment that states the default of 4 four ranks time out, with 8 now and then.  torch's own streams, which are of several
+# priorities with as many queues each, come on top once a test uses one, and then there are more queues than the card has: work of several
+# streams has stood still after that.  Such tests are in test_operators_gpu.py, which runs behind all of these.)
 if not os.environ.get("GPU_MAX_HW_QUEUES", "").isdigit() or int(os.environ["GPU_MAX_HW_QUEUES"]) < 24:
     os.environ["GPU_MAX_HW_QUEUES"] = "24"
 # the library's development switches (NMFX_POTRS, NMFX_K_GRANULE, NMFX_RS_FUSED, ...: alternative kernels the tests run against each
@@ -28,12 +30,11 @@ def pytest_configure(config):
 
 
 def pytest_collection_modifyitems(items):
-    """Four and more PROCESSES that exchange over peer windows on one GPU: a run with four (multmse, 1024 x 1100, k = 256) stood still
-    for 180 s and was ended, where two processes, and four ranks within one process, pass.  The cause is not known; until it is, these
-    stay off."""
+    """Four and more PROCESSES that exchange over peer windows on one GPU: a run with four (multmse, 1024 x 1100, k = 256; 24 queues a process)
+    stood still for 180 s and was ended, where two processes, and four ranks within one process, pass.  Until its cause is shown they stay off."""
     for item in items:
         if getattr(item, "originalname", "") == "test_peer_windows_across_processes_on_one_device" and item.callspec.params["G"] >= 4:
-            item.add_marker(pytest.mark.skip(reason="four and more processes that wait for each other on one GPU stood still; cause not known"))
+            item.add_marker(pytest.mark.skip(reason="four and more processes that wait for each other on one GPU stood still; cause not shown"))
 
 
 @pytest.fixture(scope="session")
