@@ -45,15 +45,18 @@
 #include <vector>
 
 #include "comm.hpp"
+#include "peer_rules.hpp"
 
 namespace nmfx {
 
 constexpr size_t PEER_HDR_BYTES = 16384;
 constexpr size_t PEER_FLAG_OFF = 0;       // u32 flag[LOCAL_MAX_RANKS]
 constexpr size_t PEER_ABORT_OFF = 256;    // u32
+constexpr size_t PEER_ENDED_OFF = 320;    // u32 ended[LOCAL_MAX_RANKS]: rank q has done its last access to this window (peer_rules.hpp)
 constexpr size_t PEER_TINYCNT_OFF = 512;  // u64: in-kernel all-reduces EXECUTED by this rank so far (the next one's tag - 1)
 constexpr size_t PEER_TINY_OFF = 1024;    // TinyGran inbox[2][LOCAL_MAX_RANKS][PEER_TINY_MAX]
 constexpr int PEER_TINY_MAX = 8;
+static_assert(PEER_ENDED_OFF + 4 * LOCAL_MAX_RANKS <= PEER_TINYCNT_OFF, "the header's words");
 
 struct __attribute__((aligned(16))) TinyGran {
     double v;
@@ -261,35 +264,25 @@ struct PeerHandle {
 static_assert(sizeof(PeerHandle) <= 128, "NMFX_P2P_HANDLE_BYTES");
 constexpr uint64_t PEER_MAGIC = 0x4e4d465850325031ull;
 
-// Windows are kept for the process's next communicator instead of being freed: memory that was allocated uncached and read by a kernel must
-// not go back to the runtime (allocations that got it afterwards have held wrong values), and a rank whose peer has failed may still store into
-// the peer's window.  What is kept is at most what was in use at once.
-struct WindowPool {
-    struct Kept { int dev; unsigned flags; size_t bytes; unsigned char *p; };
-    std::mutex m;
-    std::vector<Kept> kept;
-    static WindowPool &get() {
-        static WindowPool *pool = new WindowPool;       // never destroyed: contexts may outlive static destructors
-        return *pool;
-    }
-    hipError_t take(int dev, unsigned flags, size_t &bytes, unsigned char *&p) {
-        {
-            std::lock_guard<std::mutex> lock(m);
-            for (size_t i = 0; i < kept.size(); ++i)
-                if (kept[i].dev == dev && kept[i].flags == flags && kept[i].bytes >= bytes) {
-                    p = kept[i].p;
-                    bytes = kept[i].bytes;
-                    kept.erase(kept.begin() + (ptrdiff_t)i);
-                    return hipSuccess;
-                }
-        }
-        return hipExtMallocWithFlags(reinterpret_cast<void **>(&p), bytes, flags);
-    }
-    void give(int dev, unsigned flags, size_t bytes, unsigned char *p) {
-        std::lock_guard<std::mutex> lock(m);
-        kept.push_back(Kept{dev, flags, bytes, p});
-    }
-};
+// the process's windows that no communicator uses (peer_rules.hpp)
+static inline WindowPool &window_pool() {
+    static WindowPool *pool = new WindowPool;       // never destroyed: contexts may outlive static destructors
+    return *pool;
+}
+// behind a rank's last exchange, on its stream: every peer may use its window for something else (on = 1), or this rank maps them again (0)
+static __global__ void peer_end_kernel(PeerWin w, int rank, int n, unsigned on) {
+    const int q = threadIdx.x;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "");
+    if (q < n && w.p[q] && w.p[q] != w.p[rank]) peer_store_u32(reinterpret_cast<unsigned *>(w.p[q] + PEER_ENDED_OFF) + rank, on);
+}
+// the ranks that have let go of a window (an error: none)
+static inline uint32_t window_ended(const unsigned char *p) {
+    unsigned words[LOCAL_MAX_RANKS];
+    if (hipMemcpy(words, p + PEER_ENDED_OFF, sizeof words, hipMemcpyDeviceToHost) != hipSuccess) { (void)hipGetLastError(); return 0; }
+    uint32_t m = 0;
+    for (int q = 0; q < LOCAL_MAX_RANKS; ++q) m |= words[q] ? 1u << q : 0u;
+    return m;
+}
 
 struct PeerComm : Comm {
     Comm *base;                       // bootstrap transport; carries whatever does not fit a slot (owned)
@@ -301,6 +294,7 @@ struct PeerComm : Comm {
     PeerWin win;                      // every rank's window as mapped HERE
     bool opened[LOCAL_MAX_RANKS] = {};
     bool attached = false, sim = false;
+    bool exported = false, mapped = false;   // the handle was given out; a peer's window is mapped
     unsigned seq = 0;
     unsigned long long timeout_ticks;
     // group state
@@ -324,23 +318,35 @@ struct PeerComm : Comm {
         const char *kind = dev_env("NMFX_P2P_MEM");
         mem_flags = kind && std::strcmp(kind, "plain") == 0 ? hipDeviceMallocDefault : kind && std::strcmp(kind, "finegrained") == 0 ? hipDeviceMallocFinegrained : hipDeviceMallocUncached;
         mem_bytes = win_bytes;
-        const hipError_t e = WindowPool::get().take(dev, mem_flags, mem_bytes, mine);
+        mine = window_pool().take(dev, mem_flags, mem_bytes, window_ended);
+        const hipError_t e = mine ? hipSuccess : hipExtMallocWithFlags(reinterpret_cast<void **>(&mine), mem_bytes, mem_flags);
         if (e != hipSuccess) throw CommError{std::string("peer window allocation failed: ") + hipGetErrorString(e)};
         if (hipMemset(mine, 0, win_bytes) != hipSuccess || hipDeviceSynchronize() != hipSuccess) throw CommError{"peer window memset failed"};
         for (int q = 0; q < LOCAL_MAX_RANKS; ++q) win.p[q] = nullptr;
         win.p[rank] = mine;
     }
     ~PeerComm() override {
+        let_go();
         for (int q = 0; q < nranks; ++q)
             if (opened[q] && win.p[q]) (void)hipIpcCloseMemHandle(win.p[q]);
-        // (a window that saw a time-out stays mapped and is not used again: a rank that has not failed yet may still store into it)
-        unsigned aborted = 1;
-        if (mine && hipMemcpy(&aborted, mine + PEER_ABORT_OFF, 4, hipMemcpyDeviceToHost) == hipSuccess && !aborted) WindowPool::get().give(dev, mem_flags, mem_bytes, mine);
+        // who may have the window: everyone the handle went to, but this rank itself (the timing stand-in is its own peer)
+        const uint32_t others = exported && !sim ? (uint32_t)((1ull << nranks) - 1) & ~(1u << rank) : 0u;
+        if (mine) window_pool().give(dev, mem_flags, mem_bytes, mine, others);
         delete base;
     }
     const char *transport() const override { return "peer"; }
 
+    // This rank's accesses to the peers' windows are over: behind everything on the stream that made them.  (An error leaves the peers' windows
+    // held, and so unused, for good.)
+    void let_go() {
+        if (!mapped) return;
+        mapped = false;
+        (void)hipSetDevice(dev);
+        hipLaunchKernelGGL(peer_end_kernel, dim3(1), dim3(64), 0, home, win, rank, nranks, 1u);
+        if (hipStreamSynchronize(home) != hipSuccess) (void)hipGetLastError();
+    }
     void export_handle(void *out128) {
+        exported = true;
         PeerHandle h;
         std::memset(&h, 0, sizeof h);
         h.magic = PEER_MAGIC;
@@ -361,6 +367,7 @@ struct PeerComm : Comm {
             if (h.magic != PEER_MAGIC) throw CommError{"peer attach: bad handle (rank " + std::to_string(q) + ")"};
             if (h.bytes != win_bytes || h.slot_bytes != slot_bytes) throw CommError{"peer attach: the ranks' windows differ in size (different p, k or dtype?)"};
             if (q == rank) continue;
+            mapped = true;
             if (h.pid == (int32_t)getpid()) {
                 if (h.device != dev) {
                     const hipError_t e = hipDeviceEnablePeerAccess(h.device, 0);
@@ -376,12 +383,16 @@ struct PeerComm : Comm {
                 opened[q] = true;
             }
         }
+        // (this rank may have let go of them before)
+        hipLaunchKernelGGL(peer_end_kernel, dim3(1), dim3(64), 0, home, win, rank, nranks, 0u);
+        ck(hipStreamSynchronize(home), "peer attach");
         attached = true;
     }
     // Back to the wrapped transport: unmap the peers' windows, every later collective goes to `base`.  For the case where mapping
     // failed on SOME rank (no IPC support, no peer access): the ranks where it succeeded must not keep routing through windows the
     // others do not use -- their collectives would no longer pair up.  The caller makes this collective (nmfx/dist.py::attach_p2p).
     void detach() {
+        let_go();
         for (int q = 0; q < nranks; ++q) {
             if (opened[q] && win.p[q]) (void)hipIpcCloseMemHandle(win.p[q]);
             opened[q] = false;

@@ -1,0 +1,23 @@
+// csrc/peer_rules.hpp behind plain C functions, for tests/test_peer_rules.py (no device is used: a window is a number here)
+#include <map>
+
+#include "../../nmf.jl_amd/csrc/peer_rules.hpp"
+
+static std::map<unsigned char *, uint32_t> ended;
+
+extern "C" {
+void *pool_new() { ended.clear(); return new nmfx::WindowPool; }
+void pool_delete(void *pool) { delete static_cast<nmfx::WindowPool *>(pool); }
+void pool_give(void *pool, int dev, unsigned flags, uint64_t bytes, uint64_t window, unsigned held) {
+    static_cast<nmfx::WindowPool *>(pool)->give(dev, flags, (size_t)bytes, reinterpret_cast<unsigned char *>(window), held);
+}
+// rank q stores its word into a window
+void window_end(uint64_t window, int q) { ended[reinterpret_cast<unsigned char *>(window)] |= 1u << q; }
+// 0: none; *bytes: what is asked for, and what it has
+uint64_t pool_take(void *pool, int dev, unsigned flags, uint64_t *bytes) {
+    size_t b = (size_t)*bytes;
+    unsigned char *p = static_cast<nmfx::WindowPool *>(pool)->take(dev, flags, b, [](const unsigned char *w) { return ended[const_cast<unsigned char *>(w)]; });
+    *bytes = b;
+    return reinterpret_cast<uint64_t>(p);
+}
+}
