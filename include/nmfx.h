@@ -300,7 +300,10 @@ int nmfx_comm_set_mode(nmfx_ctx *ctx, int mode);
  *                         the windows are unmapped and every collective goes to the wrapped transport again (what every rank
  *                         must do when mapping failed on ANY rank, so that the ranks keep routing by the same rule).
  *   nmfx_comm_init_p2p    a communicator with NO other transport (then export + attach as above): no RCCL involved; also works
- *                         with several processes on ONE device, where RCCL refuses duplicate GPUs (tests/test_gpu_peer.py).
+ *                         with two processes on ONE device, where RCCL refuses duplicate GPUs (tests/test_gpu_peer.py).
+ * Ranks that share a device wait for each other on it, so nmfx_comm_p2p_attach refuses (NMFX_ERR_RCCL, on every rank) more than two
+ * processes on one device, and several ranks of one process on one device where its GPU_MAX_HW_QUEUES gives their streams no hardware queue
+ * each: two ranks need 4 (the runtime's default), more need 3 a rank and one more.  Set it before the process first uses the GPU.
  * Waits are bounded (NMFX_P2P_TIMEOUT_S, default 30): a rank that never arrives turns into NMFX_ERR_RCCL ("peer exchange timed
  * out") at the end of the solve instead of a hung GPU -- on EVERY rank: the rank whose wait expires raises the abort word in all
  * mapped windows.  The state is sticky: destroy the contexts and build a new communicator.  nmfx_comm_p2p_stats: collectives served by the windows / by the fallback. */

@@ -255,14 +255,16 @@ static __global__ __launch_bounds__(256) void peer_gather_kernel(unsigned char *
 
 // ---- bootstrap handle (what the host ships between the ranks: nmfx_comm_p2p_export / nmfx_comm_p2p_attach) ---------------
 struct PeerHandle {
-    uint64_t magic;        // 'NMFXP2P1'
+    uint64_t magic;        // 'NMFXP2P2'
     int32_t pid, device;
     uint64_t ptr, bytes;
     uint64_t slot_bytes;
     hipIpcMemHandle_t ipc;
+    uint64_t place;        // of the device, whatever the process calls it: a hash of its PCI address
+    int32_t queues, reserved;
 };
 static_assert(sizeof(PeerHandle) <= 128, "NMFX_P2P_HANDLE_BYTES");
-constexpr uint64_t PEER_MAGIC = 0x4e4d465850325031ull;
+constexpr uint64_t PEER_MAGIC = 0x4e4d465850325032ull;
 
 // the process's windows that no communicator uses (peer_rules.hpp)
 static inline WindowPool &window_pool() {
@@ -355,17 +357,32 @@ struct PeerComm : Comm {
         h.ptr = (uint64_t)(uintptr_t)mine;
         h.bytes = win_bytes;
         h.slot_bytes = slot_bytes;
+        char pci[64] = {};
+        ck(hipDeviceGetPCIBusId(pci, sizeof pci - 1, dev), "hipDeviceGetPCIBusId");
+        h.place = 0xcbf29ce484222325ull;
+        for (const char *c = pci; *c; ++c) h.place = (h.place ^ (unsigned char)*c) * 0x100000001b3ull;
+        h.queues = hw_queues(std::getenv("GPU_MAX_HW_QUEUES"));
         const hipError_t e = hipIpcGetMemHandle(&h.ipc, mine);
         if (e != hipSuccess) { (void)hipGetLastError(); std::memset(&h.ipc, 0, sizeof h.ipc); }   // same-process peers need the pointer only
         std::memset(out128, 0, 128);
         std::memcpy(out128, &h, sizeof h);
     }
     void attach(const void *all_handles) {
+        PeerPlace at[LOCAL_MAX_RANKS];
         for (int q = 0; q < nranks; ++q) {
             PeerHandle h;
             std::memcpy(&h, reinterpret_cast<const unsigned char *>(all_handles) + (size_t)q * 128, sizeof h);
+            at[q] = PeerPlace{h.pid, h.queues, h.place, h.ptr};
             if (h.magic != PEER_MAGIC) throw CommError{"peer attach: bad handle (rank " + std::to_string(q) + ")"};
             if (h.bytes != win_bytes || h.slot_bytes != slot_bytes) throw CommError{"peer attach: the ranks' windows differ in size (different p, k or dtype?)"};
+        }
+        if (const char *why = peer_layout_refusal(at, nranks)) {
+            exported = mapped;                     // (every rank refuses it: nobody maps this window)
+            throw CommError{why};
+        }
+        for (int q = 0; q < nranks; ++q) {
+            PeerHandle h;
+            std::memcpy(&h, reinterpret_cast<const unsigned char *>(all_handles) + (size_t)q * 128, sizeof h);
             if (q == rank) continue;
             mapped = true;
             if (h.pid == (int32_t)getpid()) {

@@ -1,8 +1,9 @@
 // peer_rules.hpp -- decisions of the peer transport (peer.hpp) that need no device, apart from it so that they are tested without one:
-// when a window may be used again.
+// when a window may be used again, and which layouts of ranks over devices and processes are refused.
 #pragma once
 #include <cstddef>
 #include <cstdint>
+#include <cstdlib>
 #include <mutex>
 #include <vector>
 
@@ -39,5 +40,42 @@ struct WindowPool {
         kept.push_back(Kept{dev, flags, bytes, p, held});
     }
 };
+
+// Where a rank is.  device: the same number for the same physical device, whatever a process calls it; queues: hardware queues that the rank's
+// process has on a device.
+struct PeerPlace {
+    int32_t pid, queues;
+    uint64_t device, window;
+};
+// HIP spreads a process's streams over GPU_MAX_HW_QUEUES hardware queues, 4 unless it says otherwise.
+inline int hw_queues(const char *setting) {
+    const int n = setting ? std::atoi(setting) : 0;
+    return n > 0 ? n : 4;
+}
+// Ranks that share a device wait for each other with kernels that spin, so what a wait is for must get to run beside it.
+//  * In one process a signal that sits in one hardware queue behind another rank's wait never runs (the wait ends by its time-out).  A rank has
+//    up to three streams and the process its default one: with a queue for each nothing sits behind anything.  Four ranks: with 4 queues they
+//    time out, with 8 now and then, with 24 never.  Two ranks' exchanging streams have queues of their own with the default 4 as well.
+//  * Of processes on one device two run; with four of them the GPU has stood still, and the cause is not known.
+// Every rank has the same places and comes to the same answer.  NULL: the layout is fine.
+inline const char *peer_layout_refusal(const PeerPlace *at, int n) {
+    for (int i = 0; i < n; ++i) {
+        int processes = 0, ranks = 0;
+        for (int q = 0; q < n; ++q) {
+            if (at[q].device != at[i].device) continue;
+            bool new_process = true, new_rank = at[q].pid == at[i].pid;      // (the timing stand-in names one window several times)
+            for (int r = 0; r < q; ++r) {
+                new_process = new_process && !(at[r].device == at[q].device && at[r].pid == at[q].pid);
+                new_rank = new_rank && !(at[r].device == at[q].device && at[r].pid == at[q].pid && at[r].window == at[q].window);
+            }
+            processes += new_process;
+            ranks += new_rank;
+        }
+        if (processes > 2) return "peer attach: more than two processes on one device (their kernels wait for each other and may never run side by side): use one device per process";
+        if (ranks > 1 && at[i].queues < (ranks == 2 ? 4 : 3 * ranks + 1))
+            return "peer attach: several ranks of one process on one device need a hardware queue for each of their streams: set GPU_MAX_HW_QUEUES to 3 a rank and one more before the process uses the GPU, or use the in-process group";
+    }
+    return nullptr;
+}
 
 }  // namespace nmfx

@@ -446,7 +446,7 @@ class Context:
 
     def comm_init_p2p(self, rank: int, nranks: int):
         """Rank `rank` of `nranks` with the peer windows as the ONLY transport (no RCCL): follow with comm_p2p_export /
-        comm_p2p_attach.  Works with several processes on one device (where RCCL refuses duplicate GPUs)."""
+        comm_p2p_attach.  Works with two processes on one device (where RCCL refuses duplicate GPUs)."""
         self._ck(self.lib.nmfx_comm_init_p2p(self.h, rank, nranks))
 
     def comm_p2p_export(self) -> bytes:

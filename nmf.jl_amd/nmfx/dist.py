@@ -38,7 +38,7 @@ def init_comm(ctx, group=None, transport="rccl"):
     """Attach a communicator spanning `group` (default: world) to a Context.
     transport = "rccl": RCCL over xGMI.  "p2p": RCCL for the bootstrap and as the fallback, the exchange itself over the ranks'
     peer-mapped windows (all xGMI links at once, device-side flags; csrc/peer.hpp).  "p2p_only": the windows alone, no RCCL
-    communicator at all (also works with several ranks on ONE device, where RCCL refuses duplicate GPUs)."""
+    communicator at all (also works with two ranks on ONE device, where RCCL refuses duplicate GPUs)."""
     import torch.distributed as dist
     from .api import comm_unique_id
     if transport not in ("rccl", "p2p", "p2p_only"):      # before any collective work: a typo must not leave a half-built communicator

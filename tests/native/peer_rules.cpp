@@ -20,4 +20,11 @@ uint64_t pool_take(void *pool, int dev, unsigned flags, uint64_t *bytes) {
     *bytes = b;
     return reinterpret_cast<uint64_t>(p);
 }
+int queues_of(const char *setting) { return nmfx::hw_queues(setting); }
+// ranks as pid, queues, device, window
+const char *layout_refusal(const uint64_t *ranks, int n) {
+    std::vector<nmfx::PeerPlace> at;
+    for (int i = 0; i < n; ++i) at.push_back(nmfx::PeerPlace{(int32_t)ranks[4 * i], (int32_t)ranks[4 * i + 1], ranks[4 * i + 2], ranks[4 * i + 3]});
+    return nmfx::peer_layout_refusal(at.data(), n);
+}
 }

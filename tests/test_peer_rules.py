@@ -15,6 +15,7 @@ def rules(tmp_path_factory):
     lib = C.CDLL(so)
     lib.pool_new.restype = C.c_void_p
     lib.pool_take.restype = C.c_uint64
+    lib.layout_refusal.restype = C.c_char_p
     return lib
 
 
@@ -79,3 +80,46 @@ def test_a_window_of_another_device_or_kind_of_memory_does_not_serve(pool):
     pool.give(0x2000, 512, held=0, dev=0, flags=2)
     assert pool.take(512, dev=0, flags=1) is None
     assert pool.take(512, dev=1, flags=1) == (0x1000, 512) and pool.take(512, dev=0, flags=2) == (0x2000, 512)
+
+
+def refusal(lib, ranks):
+    """ranks: (process, hardware queues, device); every rank has a window of its own."""
+    flat = [v for i, (pid, queues, device) in enumerate(ranks) for v in (pid, queues, device, 0x1000 * (i + 1))]
+    why = lib.layout_refusal((C.c_uint64 * len(flat))(*flat), len(ranks))
+    return why.decode() if why else None
+
+
+def test_one_process_per_device_is_fine(rules):
+    for n in (1, 2, 8, 16):
+        assert refusal(rules, [(100 + r, 4, 7000 + r) for r in range(n)]) is None
+
+
+def test_two_processes_share_a_device_and_more_are_refused(rules):
+    assert refusal(rules, [(1, 4, 7), (2, 4, 7)]) is None
+    assert refusal(rules, [(1, 24, 7), (2, 24, 7), (3, 4, 8), (4, 4, 8)]) is None          # two each on two devices
+    for queues in (1, 4, 24):
+        for n in (3, 4, 8):
+            assert "two processes" in refusal(rules, [(r, queues, 7) for r in range(n)])
+    crowd = [(1, 4, 8), (2, 4, 7), (3, 4, 7), (4, 4, 7)]                                  # the rank on device 8 answers as the others do
+    assert all("two processes" in refusal(rules, crowd[i:] + crowd[:i]) for i in range(4))
+
+
+def test_ranks_of_one_process_on_one_device_need_queues(rules):
+    assert refusal(rules, [(1, 4, 7)] * 2) is None and "GPU_MAX_HW_QUEUES" in refusal(rules, [(1, 3, 7)] * 2)
+    for n, enough in ((3, 10), (4, 13), (8, 25)):
+        assert refusal(rules, [(1, enough, 7)] * n) is None
+        for queues in (1, 4, enough - 1):
+            assert "GPU_MAX_HW_QUEUES" in refusal(rules, [(1, queues, 7)] * n)
+    assert refusal(rules, [(1, 4, 7 + r) for r in range(8)]) is None                      # a device each: a queue each
+    mixed = [(1, 24, 7)] * 4 + [(2, 4, 7)] * 3
+    assert "GPU_MAX_HW_QUEUES" in refusal(rules, mixed) and "GPU_MAX_HW_QUEUES" in refusal(rules, mixed[::-1])
+
+
+def test_the_timing_stand_in_is_its_own_peer(rules):
+    """One rank's handle for all of them: one window, one stream that never waits."""
+    flat = [1, 4, 7, 0x1000] * 8
+    assert rules.layout_refusal((C.c_uint64 * len(flat))(*flat), 8) is None
+
+
+def test_the_runtime_s_number_of_queues(rules):
+    assert [rules.queues_of(s) for s in (None, b"", b"4", b"24", b"x", b"-1", b"0")] == [4, 4, 4, 24, 4, 4, 4]
