@@ -179,7 +179,7 @@ template <int NT> __device__ __forceinline__ void select_columns(const Select &s
         float g = 1.f;
         if (!per && s.gout) g = s.gout[0];
         if (s.reduction == NMFX_REDUCE_MEAN) g /= (float)max(base + all, 1);
-        *s.info = Info{base + all, g * s.a / scale, 0, 0};
+        *s.info = Info{base + all, base + all ? g * s.a / scale : 0.f, 0, 0};      // (of no columns the gradients are zero whatever g is)
     }
 }
 __global__ __launch_bounds__(256) void count_kernel(Select s) {
@@ -1062,7 +1062,7 @@ template <typename T> struct Join {
 #pragma unroll
                 for (int q = 0; q < 4; ++q) s[q] += __shfl_xor(s[q], o);
             if (e < total && part == 0) {
-                s *= scale && from >= 0 ? u * scale[from] : u;
+                if (from >= 0) s *= scale ? u * scale[from] : u;            // (a zero stays one whatever u is)
                 if (ms == 1) put4(out + m + n * ns, s, mmax - m);
                 else
 #pragma unroll
