@@ -851,11 +851,14 @@ struct Keep {
     int p, tiles_before, tiles, v0, npad, reduction, k, per;   // v0: the piece's first class; per: columns of a tile of the product (what is done again)
     float *lse_c, *loss_c, *lse, *loss;
     float *scale, *again_f, *shift;   // of a column: f_j / (a S_j); what its dz is multiplied by where it is formed again; S_j eps / p
-    int *again;               // per tile: some column's sum is out of range
+    int *again;               // per tile: some column's sum or factor is out of range
     tn::Blocked<float> dz, dzt;
     int64_t ldn;              // of H's image
 };
 constexpr float SUM_MOST = 1e30f;
+// f_j / S_j too goes on H's image only where it leaves H's elements normal numbers (of 2^-78 to 2^80): below, the image would lose their last bits
+// (f = 10^-30 and losses of 60: dW 3e-33 off where its rounding is 3e-34)
+constexpr float FACTOR_LEAST = 0x1p-48f, FACTOR_MOST = 0x1p48f;
 // r_j, by a wave a column; and no tile is to be done again
 __global__ __launch_bounds__(256) void label_kernel(Keep s, const float *w, int64_t ldw, int chunks, const float *h, int64_t ldh, float *ref, int tiles_n) {
     if (blockIdx.x == 0)
@@ -905,13 +908,14 @@ __global__ __launch_bounds__(256) void keep_kernel(Keep s, float *ht, int lc) {
         if (i < cnt) {
             const float sum = ps[at], f = s.f[i];
             const int lab = s.y[i];
-            const bool good = sum < SUM_MOST;
+            const float factor = f / (sum * s.a), size = fabsf(factor);
+            const bool good = sum < SUM_MOST && (f == 0.f || !(size < FACTOR_LEAST || (size > FACTOR_MOST && size < __builtin_inff())));
             float v = __builtin_nanf(""), l = v, c = v;
             if (lab >= 0) {
                 v = (r + log2f(sum)) * LN2;
                 l = v - (1.f - s.eps) * s.zy[i];
                 if (s.zsum) l -= s.eps * (zs[at] / (float)s.p);
-                c = good ? f / (sum * s.a) : 1.f;
+                c = good ? factor : 1.f;
                 if (lab >= s.v0) {
                     const float e = exp2_(__builtin_fmaf(s.zy[i], LOG2E, -r)) - sum * (1.f - s.eps);
                     *s.dz.at(i, lab - s.v0) = e;
@@ -1311,7 +1315,7 @@ void keep_first(const Call &c, const Shape &s, const float *w, int64_t ldw, int 
         smooth_kernel<<<(int)std::min<int64_t>(8 * CUS, (chunks + 127) / 128), 256, 0, c.st>>>(kp, p, chunks);
         ops::hip_ok(hipGetLastError(), "smooth");
     }
-    // columns whose sums left the range of E, by tiles: the way with a pass for the log-sum-exp in front
+    // columns whose sums or factors left the range of E, by tiles: the way with a pass for the log-sum-exp in front
     const EpiStats ea{here, zhere, f32(s.o_zy), i32(s.o_y), count, p, v0, (int)s.npad};
     const EpiDz<float> eb{dz, dzt, f32(s.o_lse), f32(s.o_again_f), i32(s.o_y), count, p, v0, inv, label, off, 0, cb, nullptr, nullptr};
     switch (s.z.kind) {

@@ -27,3 +27,21 @@ def test_an_ignored_column_has_a_zero_gradient_whatever_the_factor(dtype, p, n, 
     y[:] = -100
     _, _, dW, dH = nmfx.softmax_xent_grad(W, H, y, reduction=reduction, gout=torch.tensor(math.inf, device=DEV))
     assert (dW == 0).all() and (dH == 0).all()
+
+
+@pytest.mark.parametrize("p,n,k", [(1024, 300, 300), (5000, 1000, 100)])
+@pytest.mark.parametrize("gout", [1e-12, 1e-30, 1e20])
+def test_small_and_large_factors_of_badly_predicted_columns(p, n, k, gout):
+    """Sizes that form the logits once.  Columns with losses of 60, H of 10^-3 and factors far from 1 among well predicted ones: rows of dW that
+    hold little else must keep their bits.  (10^-30: dW's entries are of 10^-33, far above the smallest step of 2^-149.)"""
+    W, H, y = problem(p, n, k, "f32", seed=k)
+    z = W.double() @ H.double()
+    scale = 60.0 / (z.max(0).values - z.min(0).values).mean()
+    W, H = (W.double() * scale * 1e3).float(), (H.double() * 1e-3).float()
+    z = W.double() @ H.double()
+    y = z.argmax(0)
+    bad = torch.tensor([2, 3, n // 2, n - 1], device=DEV)
+    y[bad] = z.argmin(0)[bad]
+    g = torch.ones(n, device=DEV) * min(1.0, gout * 1e3)
+    g[bad] = gout
+    check(W, H, y, "f32", reduction="none", gout=g)
