@@ -362,34 +362,23 @@ __global__ __launch_bounds__(WM *WN * 64) void tn_stream_kernel(Args g, Epi epi)
 #endif
 }
 
-// A block for each column of tiles that `on` names: all its tiles with one epilogue, between(tile_n), then all with the other.
-template <typename T, int BM, int BN, int WM, int WN, int ST, typename EpiA, typename Between, typename EpiB>
-__global__ __launch_bounds__(WM *WN * 64) void tn_again_kernel(Args g, EpiA ea, Between between, EpiB eb, const int *on) {
+// The tiles of those columns of tiles that `on` names, dealt out to the blocks one by one: one column's tiles are as many blocks' work.
+template <typename T, int BM, int BN, int WM, int WN, int ST, typename Epi>
+__global__ __launch_bounds__(WM *WN * 64) void tn_some_kernel(Args g, Epi epi, const int *on) {
 #ifdef __HIP_DEVICE_COMPILE__
-    if (!on[blockIdx.x]) return;
+    int any = 0;
+    for (int t = threadIdx.x; t < g.tiles_n; t += WM * WN * 64) any |= on[t];
+    if (!__syncthreads_or(any)) return;
     NMFX_TN_STAGES(BM, BN, ST)
+    __shared__ typename Epi::template Shared<BM, BN, WM, WN> sh;
+    typename Epi::template Early<BM / WM / 16, BN / WN / 16> early;
     f32x4 acc[BM / WM / 16][BN / WN / 16];
-    auto all = [&](const auto &epi, auto &sh, auto &early) {
-        for (int m = 0; m < g.tiles_m; ++m) {
-            walk<T, BM, BN, WM, WN, ST>(g, Place{m, (int)blockIdx.x, 0}, st, acc, [](Place &) { return false; }, [&](const Geom &at) { epi.template begin<BM, BN, WM, WN>(at, early, sh); },
-                                        [&](auto &sums, const Geom &at) { epi.template finish<BM, BN, WM, WN>(sums, at, early, sh, st0, st1); });
-            __syncthreads();
-        }
-        __threadfence();
+    for (int id = blockIdx.x; id < g.tiles_m * g.tiles_n; id += gridDim.x) {
+        const int tile_n = id / g.tiles_m;
+        if (!on[tile_n]) continue;
+        walk<T, BM, BN, WM, WN, ST>(g, Place{id - tile_n * g.tiles_m, tile_n, 0}, st, acc, [](Place &) { return false; }, [&](const Geom &at) { epi.template begin<BM, BN, WM, WN>(at, early, sh); },
+                                    [&](auto &sums, const Geom &at) { epi.template finish<BM, BN, WM, WN>(sums, at, early, sh, st0, st1); });
         __syncthreads();
-    };
-    {
-        __shared__ typename EpiA::template Shared<BM, BN, WM, WN> sh;
-        typename EpiA::template Early<BM / WM / 16, BN / WN / 16> early;
-        all(ea, sh, early);
-    }
-    between.template run<BN>(blockIdx.x * BN);
-    __threadfence();
-    __syncthreads();
-    {
-        __shared__ typename EpiB::template Shared<BM, BN, WM, WN> sh;
-        typename EpiB::template Early<BM / WM / 16, BN / WN / 16> early;
-        all(eb, sh, early);
     }
 #endif
 }

@@ -460,19 +460,6 @@ struct Combine {
     }
 };
 
-// the columns from n0 on of a tile, by a thread each
-struct Columnwise {
-    Combine c;
-    template <int BN> __device__ __forceinline__ void run(int n0) const {
-        const int i = n0 + threadIdx.x;
-        if (threadIdx.x >= BN || i >= c.info->count) return;
-        float2 a;
-        float t;
-        c.some(i, 0, 1, a, t);
-        c.finish(i, a, t, true);
-    }
-};
-
 // the losses' sum or mean, by one block: Float64, a fixed order
 template <int NT> __device__ __forceinline__ void reduce_losses(const float *loss_c, int cnt, int reduction, float *loss) {
     __shared__ double sh[NT / 64];
@@ -680,9 +667,11 @@ __global__ __launch_bounds__(1024) void score_join_kernel(Score a, int blocks, f
 // W and H there, the one rounding in front of the products: in f32 they would run at an eighth of the rate.  Both images are in blocks
 // (tn::Blocked): with padded rows that case took 400 us here and the products that read them 465 instead of 326.
 template <typename T> __device__ __forceinline__ T to(float x) { return (T)x; }
+constexpr float SUM_MOST = 1e30f;      // of the E of a column
 
-// KEEP (f32): the same images of E = exp(z - r_j) instead, before the log-sum-exp is known, with the tiles' sums of E and the labels' logits.
-template <typename T, bool KEEP = false> struct EpiDz {
+// KEEP (f32): the same images of E = exp(z - r_j) instead, before the log-sum-exp is known, with the tiles' statistics and the labels' logits.
+// SOME (f32): dz of the columns that `only` names, the others' entries stay.
+template <typename T, bool KEEP = false, bool SOME = false> struct EpiDz {
     tn::Blocked<T> dz, dzt;   // rows are packed columns, rows are classes of the piece
     const float *lse_c, *f;   // KEEP: lse_c is the reference, in units of log 2
     const int *y, *count;
@@ -690,7 +679,9 @@ template <typename T, bool KEEP = false> struct EpiDz {
     float inv, label, off;    // 1 / a, (1 - eps) / a, eps / (a p)
     int few;                  // the tiles' statistics are not joined yet: every block does it for its own columns
     Combine c;
-    float *part, *zy, *zsum;  // KEEP: [tile_m][npad]; the labels' logits; as part, or NULL
+    float2 *part;             // KEEP: [tile_m][npad], as EpiStats'
+    float *zy, *zsum;         // KEEP: the labels' logits; [tile_m][npad] or NULL
+    const int *only;          // SOME: of every packed column
     // per column: log-sum-exp, factor, label's class in the piece.  The large tile has no registers for them to wait in: it reads them late.
     template <int MI, int NJ> struct Early { int cnt, y[NJ]; float lse[NJ], f[NJ]; };
     template <int BM, int BN, int WM, int WN> struct Shared { float lse[BN], t[WM * WN * 64]; float2 s[WM * WN * 64]; };
@@ -743,6 +734,7 @@ template <typename T, bool KEEP = false> struct EpiDz {
         auto column = [&](int j, auto at_edge) {
             const int n = g.n0 + 16 * j;
             const bool on = n < cnt;
+            if (SOME && (!on || !only[n])) return;
             const float fac = early.f[j], mul = fac * inv, sub = -fac * off, ref = early.lse[j] * (KEEP ? -1.f : -LOG2E);
             float sum = 0.f, zs = 0.f;
             // (a wave's part lies in one block of rows either way, and begins with a tile of them)
@@ -791,7 +783,29 @@ template <typename T, bool KEEP = false> struct EpiDz {
                 sum += __shfl_xor(sum, 32);
                 zs += __shfl_xor(zs, 16);
                 zs += __shfl_xor(zs, 32);
-                if (g.lane < 16) sh.s[g.wm * BN + n - g.tile_n * BN] = make_float2(sum, zs);
+                float2 s = make_float2(early.lse[j], sum);
+                if (!(sum < SUM_MOST)) {                   // (seldom) E is of no use here: the statistics with the maximum for a reference
+                    auto there = [&](int i, int r) { return !at_edge || (on && g.m0 + 16 * i + r < p); };
+                    float mx = -__builtin_inff();
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, there(i, r) ? acc[i][j][r] : mx);
+                    mx = fmaxf(mx, __shfl_xor(mx, 16));
+                    mx = fmaxf(mx, __shfl_xor(mx, 32));
+                    s = make_float2(mx * LOG2E, 0.f);
+                    const float from = s.x == -__builtin_inff() ? 0.f : s.x;
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s.y += there(i, r) ? exp2_(__builtin_fmaf(acc[i][j][r], LOG2E, -from)) : 0.f;
+                    s.y += __shfl_xor(s.y, 16);
+                    s.y += __shfl_xor(s.y, 32);
+                }
+                if (g.lane < 16) {
+                    sh.s[g.wm * BN + n - g.tile_n * BN] = s;
+                    sh.t[g.wm * BN + n - g.tile_n * BN] = zs;
+                }
             }
         };
         if (edge) {
@@ -804,15 +818,16 @@ template <typename T, bool KEEP = false> struct EpiDz {
         if constexpr (KEEP) {
             __syncthreads();
             if (g.tid < BN) {
-                float2 t = sh.s[g.tid];
+                float2 s = sh.s[g.tid];
+                float t = sh.t[g.tid];
 #pragma unroll
                 for (int w = 1; w < WM; ++w) {
-                    t.x += sh.s[w * BN + g.tid].x;
-                    t.y += sh.s[w * BN + g.tid].y;
+                    s = join(s, sh.s[w * BN + g.tid]);
+                    t += sh.t[w * BN + g.tid];
                 }
                 const int64_t o = (int64_t)g.tile_m * c.npad + g.tile_n * BN + g.tid;
-                part[o] = t.x;
-                if (zsum) zsum[o] = t.y;
+                part[o] = s;
+                if (zsum) zsum[o] = t;
             }
         }
         if constexpr (sizeof(T) == 2) {
@@ -841,21 +856,22 @@ template <typename T, bool KEEP = false> struct EpiDz {
 // label's logit S_j = exp(l_j): between 1 and 10^30 for every loss that training sees.  So E is written by the pass that sums it, and the
 // logits are formed once: the column's factor f_j / S_j goes on dH's result and on H's image for dW.  The other pieces'
 // dz are formed to go with that: times S_j / f_j.  What smoothing takes from every entry is taken by a pass over the images (smooth_kernel).
+// Where a tile's sum of E leaves its range the tile's statistics take the maximum for a reference, while the logits are in registers, and dz of
+// such a column is formed again, its column of tiles by as many blocks (16384 x 2048, k = 512: 855 us, with one such column 979, with nothing
+// else 1166; by one block for the whole column of tiles it was 18500).
 struct Keep {
-    const float2 *before;     // [tile_m][npad]: statistics of the pieces in front
-    const float *part;        // [tile_m][npad]: sums of E
+    const float2 *part;       // [tile_m][npad]: statistics of all pieces; the reference of the last one's is r_j where its sum is in range
     const float *f, *ref, *zy, *zsum;     // zsum: [tile_m][npad] of all pieces, or NULL
     const int *idx, *y;
     const Info *info;
     float eps, a;
-    int p, tiles_before, tiles, v0, npad, reduction, k, per;   // v0: the piece's first class; per: columns of a tile of the product (what is done again)
+    int p, tiles, v0, npad, reduction, k, per;   // v0: the piece's first class; per: columns of a tile of the product (what is done again)
     float *lse_c, *loss_c, *lse, *loss;
     float *scale, *again_f, *shift;   // of a column: f_j / (a S_j); what its dz is multiplied by where it is formed again; S_j eps / p
-    int *again;               // per tile: some column's sum or factor is out of range
+    int *again, *only;        // per tile, per column: some column's, the column's sum or factor is out of range
     tn::Blocked<float> dz, dzt;
     int64_t ldn;              // of H's image
 };
-constexpr float SUM_MOST = 1e30f;
 // f_j / S_j too goes on H's image only where it leaves H's elements normal numbers (of 2^-78 to 2^80): below, the image would lose their last bits
 // (f = 10^-30 and losses of 60: dW 3e-33 off where its rounding is 3e-34)
 constexpr float FACTOR_LEAST = 0x1p-48f, FACTOR_MOST = 0x1p48f;
@@ -876,43 +892,39 @@ __global__ __launch_bounds__(256) void label_kernel(Keep s, const float *w, int6
     for (int o = 32; o; o >>= 1) d += __shfl_xor(d, o);
     if (lane == 0) ref[i] = d * LOG2E;
 }
-// joins the tiles' sums of 2^lc (at least 8) columns, finishes them, puts the label's entry right and scales H's image
+// joins the tiles' statistics of 2^lc (at least 8) columns, finishes them, puts the label's entry right and scales H's image
 __global__ __launch_bounds__(256) void keep_kernel(Keep s, float *ht, int lc) {
-    __shared__ float ps[256], zs[256], by[256];
+    __shared__ float2 ps[256];
+    __shared__ float zs[256], by[256];
     const int cols = 1 << lc, step = 256 >> lc, at = threadIdx.x & (cols - 1), slice = threadIdx.x >> lc;
     const int cnt = s.info->count, i0 = blockIdx.x * cols, i = i0 + at;
     if (i0 >= cnt) return;
-    float a = 0.f;
+    float2 a = make_float2(-__builtin_inff(), 0.f);
 #pragma unroll 4
-    for (int q = slice; q < s.tiles; q += step) a += s.part[(int64_t)q * s.npad + i];
-    const float r = i < cnt ? s.ref[i] : 0.f;
-#pragma unroll 4
-    for (int q = slice; q < s.tiles_before; q += step) {
-        const float2 b = s.before[(int64_t)q * s.npad + i];
-        a += b.y != 0.f ? b.y * exp2_(b.x - r) : 0.f;
-    }
+    for (int q = slice; q < s.tiles; q += step) a = join(a, s.part[(int64_t)q * s.npad + i]);
     float t = 0.f;
     if (s.zsum)
-        for (int q = slice; q < s.tiles_before + s.tiles; q += step) t += s.zsum[(int64_t)q * s.npad + i];
+        for (int q = slice; q < s.tiles; q += step) t += s.zsum[(int64_t)q * s.npad + i];
     ps[threadIdx.x] = a;
     zs[threadIdx.x] = t;
     for (int o = step / 2; o; o >>= 1) {
         __syncthreads();
         if (slice < o) {
-            ps[threadIdx.x] += ps[threadIdx.x + (o << lc)];
+            ps[threadIdx.x] = join(ps[threadIdx.x], ps[threadIdx.x + (o << lc)]);
             zs[threadIdx.x] += zs[threadIdx.x + (o << lc)];
         }
     }
     if (slice == 0) {
         by[at] = 0.f;
         if (i < cnt) {
-            const float sum = ps[at], f = s.f[i];
+            a = ps[at];
+            const float r = s.ref[i], sum = a.x == r ? a.y : a.y * exp2_(a.x - r), f = s.f[i];
             const int lab = s.y[i];
             const float factor = f / (sum * s.a), size = fabsf(factor);
             const bool good = sum < SUM_MOST && (f == 0.f || !(size < FACTOR_LEAST || (size > FACTOR_MOST && size < __builtin_inff())));
             float v = __builtin_nanf(""), l = v, c = v;
             if (lab >= 0) {
-                v = (r + log2f(sum)) * LN2;
+                v = (a.x + log2f(a.y)) * LN2;
                 l = v - (1.f - s.eps) * s.zy[i];
                 if (s.zsum) l -= s.eps * (zs[at] / (float)s.p);
                 c = good ? factor : 1.f;
@@ -923,6 +935,7 @@ __global__ __launch_bounds__(256) void keep_kernel(Keep s, float *ht, int lc) {
                 }
             }
             if (!good) s.again[i / s.per] = 1;
+            s.only[i] = !good;
             s.lse_c[i] = v;
             s.loss_c[i] = l;
             const int col = s.idx[i];
@@ -1110,7 +1123,7 @@ struct Shape {
     bool w_slots, direct;         // direct: dH need not be summed from slots
     bool keep;                    // E is kept from the first pass
     // workspace offsets
-    int64_t o_info, o_counts, o_idx, o_pos, o_y, o_f, o_lse, o_loss, o_zy, o_h, o_ht, o_w, o_wt, o_part, o_zsum, o_ref, o_scale, o_again_f, o_shift, o_again, o_dz, o_dzt, o_hslot, o_wslot, bytes;
+    int64_t o_info, o_counts, o_idx, o_pos, o_y, o_f, o_lse, o_loss, o_zy, o_h, o_ht, o_w, o_wt, o_part, o_zsum, o_ref, o_scale, o_again_f, o_shift, o_again, o_only, o_dz, o_dzt, o_hslot, o_wslot, bytes;
 };
 
 constexpr int CUS = 256;
@@ -1206,8 +1219,8 @@ Shape shape_of(const nmfx_dmat &W, const nmfx_dmat &H, bool grad, bool smooth) {
     const int64_t tiles = (s.p + KINDS[s.z.kind].m - 1) / KINDS[s.z.kind].m, parts = std::max<int64_t>(tiles * s.npad, 16 * 4 * CUS);
     s.o_part = take(parts * sizeof(float2));
     s.o_zsum = smooth ? take(parts * 4) : -1;
-    s.o_ref = s.o_scale = s.o_again_f = s.o_shift = s.o_again = -1;
-    if (s.keep) { s.o_ref = take(s.npad * 4); s.o_scale = take(s.npad * 4); s.o_again_f = take(s.npad * 4); s.o_shift = take(s.npad * 4); s.o_again = take(s.npad / 64 * 4); }
+    s.o_ref = s.o_scale = s.o_again_f = s.o_shift = s.o_again = s.o_only = -1;
+    if (s.keep) { s.o_ref = take(s.npad * 4); s.o_scale = take(s.npad * 4); s.o_again_f = take(s.npad * 4); s.o_shift = take(s.npad * 4); s.o_again = take(s.npad / 64 * 4); s.o_only = take(s.npad * 4); }
     s.o_w = s.w_rows_direct ? -1 : take(s.p * s.kpad * s.es);
     s.o_ht = s.o_wt = s.o_dz = s.o_dzt = s.o_hslot = s.o_wslot = -1;
     if (grad) {
@@ -1300,12 +1313,11 @@ void keep_first(const Call &c, const Shape &s, const float *w, int64_t ldw, int 
     if (v0) stream<float>(tn::Args{tn::plain(w, ldw * es, v0, wchunks), hop, count, tn::LIMIT_N, 0, 0, 1, kt}, v0, n1, s.z, EpiStats{part, zsum, f32(s.o_zy), i32(s.o_y), count, v0, 0, (int)s.npad}, c.st);
     tn::Args a{tn::plain(w + v0 * ldw, ldw * es, p, wchunks), hop, count, tn::LIMIT_N, 0, 0, 1, kt};
     grid(a, p, n1, s.z);
-    float *sums = reinterpret_cast<float *>(here);
-    const Keep kp{part, sums, f32(s.o_f), f32(s.o_ref), f32(s.o_zy), zsum, i32(s.o_idx), i32(s.o_y), cb.info, cb.eps, a_, (int)s.p, before, a.tiles_m, v0, (int)s.npad, c.o.reduction, (int)s.k, KINDS[s.z.kind].n,
-                  f32(s.o_lse), f32(s.o_loss), c.lse, c.loss, f32(s.o_scale), f32(s.o_again_f), f32(s.o_shift), i32(s.o_again), dz, dzt, s.ldn};
+    const Keep kp{part, f32(s.o_f), f32(s.o_ref), f32(s.o_zy), zsum, i32(s.o_idx), i32(s.o_y), cb.info, cb.eps, a_, (int)s.p, before + a.tiles_m, v0, (int)s.npad, c.o.reduction, (int)s.k, KINDS[s.z.kind].n,
+                  f32(s.o_lse), f32(s.o_loss), c.lse, c.loss, f32(s.o_scale), f32(s.o_again_f), f32(s.o_shift), i32(s.o_again), i32(s.o_only), dz, dzt, s.ldn};
     label_kernel<<<(n1 + 3) / 4, 256, 0, c.st>>>(kp, w, ldw, wchunks, h, s.kpad, f32(s.o_ref), a.tiles_n);
     ops::hip_ok(hipGetLastError(), "label");
-    product<float>(a, p, n1, s.z, EpiDz<float, true>{dz, dzt, f32(s.o_ref), nullptr, i32(s.o_y), count, p, v0, 1.f, 0.f, 0.f, 0, cb, sums, f32(s.o_zy), zhere}, c.st);
+    product<float>(a, p, n1, s.z, EpiDz<float, true>{dz, dzt, f32(s.o_ref), nullptr, i32(s.o_y), count, p, v0, 1.f, 0.f, 0.f, 0, cb, here, f32(s.o_zy), zhere, nullptr}, c.st);
     int lc = 6;
     while (lc > 3 && (n1 >> lc) < CUS) --lc;
     keep_kernel<<<(n1 + (1 << lc) - 1) >> lc, 256, 0, c.st>>>(kp, ht, lc);
@@ -1315,13 +1327,13 @@ void keep_first(const Call &c, const Shape &s, const float *w, int64_t ldw, int 
         smooth_kernel<<<(int)std::min<int64_t>(8 * CUS, (chunks + 127) / 128), 256, 0, c.st>>>(kp, p, chunks);
         ops::hip_ok(hipGetLastError(), "smooth");
     }
-    // columns whose sums or factors left the range of E, by tiles: the way with a pass for the log-sum-exp in front
-    const EpiStats ea{here, zhere, f32(s.o_zy), i32(s.o_y), count, p, v0, (int)s.npad};
-    const EpiDz<float> eb{dz, dzt, f32(s.o_lse), f32(s.o_again_f), i32(s.o_y), count, p, v0, inv, label, off, 0, cb, nullptr, nullptr};
+    // dz of the columns whose sums or factors left the range of E, from logits formed again
+    const EpiDz<float, false, true> again{dz, dzt, f32(s.o_lse), f32(s.o_again_f), i32(s.o_y), count, p, v0, inv, label, off, 0, cb, nullptr, nullptr, nullptr, i32(s.o_only)};
+    const int blocks = std::min(a.tiles_m * a.tiles_n, KINDS[s.z.kind].cap * CUS);
     switch (s.z.kind) {
-        case 0: tn::tn_again_kernel<float, 256, 256, 2, 4, 2, EpiStats, Columnwise, EpiDz<float>><<<a.tiles_n, 512, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
-        case 1: tn::tn_again_kernel<float, 128, 128, 2, 2, 2, EpiStats, Columnwise, EpiDz<float>><<<a.tiles_n, 256, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
-        default: tn::tn_again_kernel<float, 64, 64, 2, 2, 4, EpiStats, Columnwise, EpiDz<float>><<<a.tiles_n, 256, 0, c.st>>>(a, ea, Columnwise{cb}, eb, kp.again); break;
+        case 0: tn::tn_some_kernel<float, 256, 256, 2, 4, 2, EpiDz<float, false, true>><<<blocks, 512, 0, c.st>>>(a, again, kp.again); break;
+        case 1: tn::tn_some_kernel<float, 128, 128, 2, 2, 2, EpiDz<float, false, true>><<<blocks, 256, 0, c.st>>>(a, again, kp.again); break;
+        default: tn::tn_some_kernel<float, 64, 64, 2, 2, 4, EpiDz<float, false, true>><<<blocks, 256, 0, c.st>>>(a, again, kp.again); break;
     }
     ops::hip_ok(hipGetLastError(), "again");
 }
@@ -1398,7 +1410,7 @@ template <typename T> void run(const Call &c, const Shape &s) {
         const bool last = t + 1 == s.pieces;
         tn::Args a{tn::plain(w + v0 * ldw, ldw * es, pv, wchunks), hop, count, tn::LIMIT_N, 0, 0, 1, kt};
         if (!keep || t)
-            product<T>(a, pv, n1, s.z, EpiDz<T>{dz, dzt, f32(s.o_lse), f32(keep ? s.o_again_f : s.o_f), i32(s.o_y), count, pv, (int)v0, inv, label, off, few, cb, nullptr, nullptr}, c.st);
+            product<T>(a, pv, n1, s.z, EpiDz<T>{dz, dzt, f32(s.o_lse), f32(keep ? s.o_again_f : s.o_f), i32(s.o_y), count, pv, (int)v0, inv, label, off, few, cb, nullptr, nullptr, nullptr, nullptr}, c.st);
         // dH: rows are components, columns are packed columns
         tn::Args b{tn::plain(wt + v0, ldwt * es, k, (int)std::min<int64_t>((wtpad - v0) / per, s.piece / per)), dz.operand((int)s.npad), count, tn::LIMIT_N, 0, 0, 0, pt / step};
         const EpiSlot eh{f32(s.o_hslot), s.ldslot, s.npad * s.ldslot, (int)s.npad, t > 0};

@@ -45,3 +45,45 @@ def test_small_and_large_factors_of_badly_predicted_columns(p, n, k, gout):
     g = torch.ones(n, device=DEV) * min(1.0, gout * 1e3)
     g[bad] = gout
     check(W, H, y, "f32", reduction="none", gout=g)
+
+
+def outlier(W, H, y, column):
+    """H and y with a loss in one column that no exponential holds."""
+    H, y = H.clone(), y.clone()
+    H[:, column] *= 300
+    y[column] = (W.double() @ H[:, column].double()).argmin()
+    return H, y
+
+
+@pytest.mark.parametrize("p,n,k", [(5000, 1000, 100), (4097, 1100, 520)])
+@pytest.mark.parametrize("eps", [0.0, 0.1])
+def test_an_outlier_leaves_the_other_columns_as_they_were(p, n, k, eps):
+    W, H, y = problem(p, n, k, "f32", seed=k, ignored=0.2)
+    y[77] = 5
+    kw = dict(reduction="none", label_smoothing=eps)
+    clean = nmfx.softmax_xent_grad(W, H, y, **kw)
+    H2, y2 = outlier(W, H, y, 77)
+    assert float(oracle(W, H2, y2, eps, "none")["loss"][77]) > 100 * (1 - eps)
+    got = nmfx.softmax_xent_grad(W, H2, y2, **kw)
+    others = torch.arange(n, device=DEV) != 77
+    for a, b in zip((got[0], got[1], got[3]), (clean[0], clean[1], clean[3])):
+        assert torch.equal(a[..., others], b[..., others])
+    check(W, H2, y2, "f32", eps=eps, reduction="none")
+
+
+def test_an_outlier_does_not_hold_up_the_call():
+    """One column whose logits are formed again, among 2048: a few more microseconds, not another kernel's length for every tile of classes."""
+    W, H, y = problem(16384, 2048, 512, "f32")
+    times = {}
+    for name, (h, labels) in {"none": (H, y), "one": outlier(W, H, y, 700)}.items():
+        nmfx.softmax_xent_grad(W, h, labels)
+        best = math.inf
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            nmfx.softmax_xent_grad(W, h, labels)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        times[name] = best
+    assert times["one"] < 2 * times["none"], times
