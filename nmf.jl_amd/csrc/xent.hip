@@ -328,13 +328,24 @@ template <typename T> __global__ __launch_bounds__(256) void prepare_kernel(Sele
     pack_tile<T>(h, tile, from, rows, r0, c0);
 }
 
-// Statistics are kept in units of log 2: (reference r, sum of 2^(z log2(e) - r)), one multiply-add and one exp2 a logit, where r is some
-// set's maximum as it was rounded: its rounding cancels.  Of two sets: an empty one, or one of minus infinities, is (-inf, 0) and changes nothing; a NaN sum
-// is not 0 and goes through.
+// exp(z - r) with one multiply-add and one exp2 a logit: 2^(z log2(e) - x), where x is r log2(e) as it was rounded, is exp(z - r) 2^rest.  rest
+// goes into the column's factor: without it exp(z - lse) of logits of 10^8 comes out e^6 and more times too large.  From BIG on rest would leave
+// exp2's range: logits are then taken relative to r beforehand, and x = rest = 0 (as for a NaN, and the minus infinity of no logits).
+constexpr float BIG = 0x1p26f;
+__device__ __forceinline__ bool big(float r) { return !(fabsf(r) < BIG); }
+struct Scaled { float x, rest; };
+__device__ __forceinline__ Scaled scaled(float r) {
+    const float x = big(r) ? 0.f : r * LOG2E;
+    return Scaled{x, big(r) ? 0.f : __builtin_fmaf(r, LOG2E, -x)};
+}
+
+// Statistics of a set of logits: (reference r, sum of exp(z - r)), r its maximum in most places.  Of two sets: an empty one, or one of minus
+// infinities, is (-inf, 0) and changes nothing; a NaN sum is not 0 and goes through.
 __device__ __forceinline__ float2 join(float2 a, float2 b) {
     const float m = fmaxf(a.x, b.x);
-    return make_float2(m, (a.y != 0.f ? a.y * exp2_(a.x - m) : 0.f) + (b.y != 0.f ? b.y * exp2_(b.x - m) : 0.f));
+    return make_float2(m, (a.y != 0.f ? a.y * exp2_((a.x - m) * LOG2E) : 0.f) + (b.y != 0.f ? b.y * exp2_((b.x - m) * LOG2E) : 0.f));
 }
+__device__ __forceinline__ float lse_of(float2 a) { return __builtin_fmaf(log2f(a.y), LN2, a.x); }
 
 // ---- statistics of the logits: rows of D are classes, columns are packed columns ----------------------------------------------------
 // Bound by the product where k is long (131072 x 8192, k = 2048: 3.26 ms, 1350 TFLOP/s); where it is short by the exponentials, which go in
@@ -368,25 +379,7 @@ struct EpiStats {
         }
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const int n = g.n0 + 16 * j;
-            float mx = -__builtin_inff();
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            mx *= LOG2E;
-            const float ref = mx == -__builtin_inff() ? 0.f : mx;
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) s += exp2_(__builtin_fmaf(acc[i][j][r], LOG2E, -ref));
-            s += __shfl_xor(s, 16);
-            s += __shfl_xor(s, 32);
-            const int col = g.wn * (BN / WN) + 16 * j + (g.lane & 15);
-            if (g.lane < 16) ps[g.wm * BN + col] = make_float2(mx, s);
+            const int n = g.n0 + 16 * j, col = g.wn * (BN / WN) + 16 * j + (g.lane & 15);
             if (zsum) {
                 float t = 0.f;
 #pragma unroll
@@ -407,6 +400,39 @@ struct EpiStats {
                             if (d == 16 * i + r) zy[n] = acc[i][j][r];
                 }
             }
+        }
+        float mx[NJ];
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            mx[j] = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mx[j] = fmaxf(mx[j], acc[i][j][r]);
+            mx[j] = fmaxf(mx[j], __shfl_xor(mx[j], 16));
+            mx[j] = fmaxf(mx[j], __shfl_xor(mx[j], 32));
+            any |= big(mx[j]);
+        }
+        if (__any(any)) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[i][j][r] -= big(mx[j]) && mx[j] != -__builtin_inff() ? mx[j] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const Scaled ref = scaled(mx[j]);
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s += exp2_(__builtin_fmaf(acc[i][j][r], LOG2E, -ref.x));
+            s += __shfl_xor(s, 16);
+            s += __shfl_xor(s, 32);
+            if (g.lane < 16) ps[g.wm * BN + g.wn * (BN / WN) + 16 * j + g.lane] = make_float2(mx[j], s * exp2_(-ref.rest));
         }
         __syncthreads();
         if (g.tid < BN) {
@@ -446,7 +472,7 @@ struct Combine {
     }
     __device__ __forceinline__ float finish(int i, float2 a, float t, bool write) const {
         const int lab = y[i];
-        const float v = lab < 0 ? __builtin_nanf("") : (a.x + log2f(a.y)) * LN2;     // a label that is no class: the column's loss is NaN
+        const float v = lab < 0 ? __builtin_nanf("") : lse_of(a);     // a label that is no class: the column's loss is NaN
         if (write) {
             float l = v - (1.f - eps) * (lab < 0 ? 0.f : zy[i]);
             if (zsum) l -= eps * (t / (float)p);
@@ -565,7 +591,8 @@ template <typename T> __global__ __launch_bounds__(512) void score_kernel(Score 
         *reinterpret_cast<tn::u32x4 *>(hs + e * 16) = v;
     }
     __syncthreads();
-    float ref = -__builtin_inff(), sum = 0.f, zsum = 0.f;
+    float top = -__builtin_inff(), sum = 0.f, zsum = 0.f, fix = 1.f;      // fix: what a group's sum is multiplied by
+    Scaled ref = {0.f, 0.f};
     f32x4 z = {0.f, 0.f, 0.f, 0.f};
     auto work = [&](int set) {
         const int gn = q + 1 < parts ? g : g + 1, qn = q + 1 < parts ? q + 1 : 0;
@@ -587,14 +614,19 @@ template <typename T> __global__ __launch_bounds__(512) void score_kernel(Score 
                 if (v == lab) a.zy[col] = z[r];
                 mx = fmaxf(mx, z[r]);
             }
-            mx *= LOG2E;
-            if (mx > ref) {
-                sum *= sum != 0.f ? exp2_(ref - mx) : 0.f;
-                ref = mx;
+            if (mx > top) {
+                sum *= sum != 0.f ? exp2_((top - mx) * LOG2E) : 0.f;
+                top = mx;
+                ref = scaled(top);
+                fix = exp2_(-ref.rest);
             }
-            const float at = ref == -__builtin_inff() ? 0.f : ref;
+            if (big(top) && top != -__builtin_inff())
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sum += exp2_(__builtin_fmaf(z[r], LOG2E, -at));
+                for (int r = 0; r < 4; ++r) z[r] -= top;
+            float s = 0.f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s += exp2_(__builtin_fmaf(z[r], LOG2E, -ref.x));
+            sum = __builtin_fmaf(s, fix, sum);
             z = f32x4{0.f, 0.f, 0.f, 0.f};
         }
         g = gn;
@@ -604,7 +636,7 @@ template <typename T> __global__ __launch_bounds__(512) void score_kernel(Score 
         work(0);
         if (g < last) work(1);
     }
-    float2 s = make_float2(ref, sum);
+    float2 s = make_float2(top, sum);
 #pragma unroll
     for (int o = 16; o < 64; o <<= 1) {
         s = join(s, make_float2(__shfl_xor(s.x, o), __shfl_xor(s.y, o)));
@@ -641,7 +673,7 @@ __global__ __launch_bounds__(1024) void score_join_kernel(Score a, int blocks, f
         float v = 0.f, l = 0.f;
         if (lab != a.ignore) {
             const bool bad = lab < 0 || lab >= a.p;
-            v = bad ? __builtin_nanf("") : (s.x + log2f(s.y)) * LN2;
+            v = bad ? __builtin_nanf("") : lse_of(s);
             l = v - (1.f - eps) * (bad ? 0.f : a.zy[col]);
             if (a.zsum) l -= eps * (t / (float)a.p);
         }
@@ -673,7 +705,7 @@ constexpr float SUM_MOST = 1e30f;      // of the E of a column
 // SOME (f32): dz of the columns that `only` names, the others' entries stay.
 template <typename T, bool KEEP = false, bool SOME = false> struct EpiDz {
     tn::Blocked<T> dz, dzt;   // rows are packed columns, rows are classes of the piece
-    const float *lse_c, *f;   // KEEP: lse_c is the reference, in units of log 2
+    const float *lse_c, *f;   // KEEP: lse_c is the reference
     const int *y, *count;
     int p, v0;                // classes that exist in the piece; its first class
     float inv, label, off;    // 1 / a, (1 - eps) / a, eps / (a p)
@@ -735,7 +767,8 @@ template <typename T, bool KEEP = false, bool SOME = false> struct EpiDz {
             const int n = g.n0 + 16 * j;
             const bool on = n < cnt;
             if (SOME && (!on || !only[n])) return;
-            const float fac = early.f[j], mul = fac * inv, sub = -fac * off, ref = early.lse[j] * (KEEP ? -1.f : -LOG2E);
+            const Scaled from = scaled(early.lse[j]);
+            const float fac = early.f[j], mul = KEEP ? 1.f : fac * inv * exp2_(-from.rest), sub = -fac * off, ref = -from.x;
             float sum = 0.f, zs = 0.f;
             // (a wave's part lies in one block of rows either way, and begins with a tile of them)
             T *const zto = sizeof(T) == 4 ? dz.at(n, g.m0) : nullptr, *const tto = sizeof(T) == 4 ? dzt.at(g.m0, n) : nullptr;
@@ -783,8 +816,8 @@ template <typename T, bool KEEP = false, bool SOME = false> struct EpiDz {
                 sum += __shfl_xor(sum, 32);
                 zs += __shfl_xor(zs, 16);
                 zs += __shfl_xor(zs, 32);
-                float2 s = make_float2(early.lse[j], sum);
-                if (!(sum < SUM_MOST)) {                   // (seldom) E is of no use here: the statistics with the maximum for a reference
+                float2 s = make_float2(early.lse[j], sum * exp2_(-from.rest));
+                if (!(sum < SUM_MOST) || big(early.lse[j])) {              // (seldom) E is of no use here: the statistics with the maximum for a reference
                     auto there = [&](int i, int r) { return !at_edge || (on && g.m0 + 16 * i + r < p); };
                     float mx = -__builtin_inff();
 #pragma unroll
@@ -793,12 +826,12 @@ template <typename T, bool KEEP = false, bool SOME = false> struct EpiDz {
                         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, there(i, r) ? acc[i][j][r] : mx);
                     mx = fmaxf(mx, __shfl_xor(mx, 16));
                     mx = fmaxf(mx, __shfl_xor(mx, 32));
-                    s = make_float2(mx * LOG2E, 0.f);
-                    const float from = s.x == -__builtin_inff() ? 0.f : s.x;
+                    s = make_float2(mx, 0.f);
+                    const float at = mx == -__builtin_inff() ? 0.f : mx;
 #pragma unroll
                     for (int i = 0; i < MI; ++i)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s.y += there(i, r) ? exp2_(__builtin_fmaf(acc[i][j][r], LOG2E, -from)) : 0.f;
+                        for (int r = 0; r < 4; ++r) s.y += there(i, r) ? exp2_((acc[i][j][r] - at) * LOG2E) : 0.f;
                     s.y += __shfl_xor(s.y, 16);
                     s.y += __shfl_xor(s.y, 32);
                 }
@@ -808,6 +841,19 @@ template <typename T, bool KEEP = false, bool SOME = false> struct EpiDz {
                 }
             }
         };
+        if (!KEEP) {
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) any |= big(early.lse[j]);
+            if (__any(any)) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[i][j][r] -= big(early.lse[j]) ? early.lse[j] : 0.f;
+            }
+        }
         if (edge) {
 #pragma unroll
             for (int j = 0; j < NJ; ++j) column(j, std::true_type{});
@@ -853,7 +899,7 @@ template <typename T, bool KEEP = false, bool SOME = false> struct EpiDz {
 // ---- E kept from the first pass ---------------------------------------------------------------------------------------------------------
 // (Of the last piece of the classes: the first ones' E would have to wait for its sums.)
 // dz_j = f_j / S_j (E_vj - S_j (1 - eps) [v = y_j] - S_j eps / p) with E_vj = exp(z_vj - r_j), S_j = sum_v E_vj, whatever r_j is.  With r_j the
-// label's logit S_j = exp(l_j): between 1 and 10^30 for every loss that training sees.  So E is written by the pass that sums it, and the
+// label's logit (or a little less) S_j = exp(l_j): between 1 and 10^30 for every loss that training sees.  So E is written by the pass that sums it, and the
 // logits are formed once: the column's factor f_j / S_j goes on dH's result and on H's image for dW.  The other pieces'
 // dz are formed to go with that: times S_j / f_j.  What smoothing takes from every entry is taken by a pass over the images (smooth_kernel).
 // Where a tile's sum of E leaves its range the tile's statistics take the maximum for a reference, while the logits are in registers, and dz of
@@ -882,15 +928,23 @@ __global__ __launch_bounds__(256) void label_kernel(Keep s, const float *w, int6
     const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (i >= s.info->count) return;
     const int v = s.y[i];
-    float d = 0.f;
+    float d = 0.f, size = 0.f;
     if (v >= 0)
         for (int q = lane; q < chunks; q += 64) {
             const f32x4 a = reinterpret_cast<const f32x4 *>(w + v * ldw)[q], b = reinterpret_cast<const f32x4 *>(h + i * ldh)[q];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) d = __builtin_fmaf(a[u], b[u], d);
+            for (int u = 0; u < 4; ++u) {
+                d = __builtin_fmaf(a[u], b[u], d);
+                size = __builtin_fmaf(fabsf(a[u]), fabsf(b[u]), size);
+            }
         }
-    for (int o = 32; o; o >>= 1) d += __shfl_xor(d, o);
-    if (lane == 0) ref[i] = d * LOG2E;
+    for (int o = 32; o; o >>= 1) {
+        d += __shfl_xor(d, o);
+        size += __shfl_xor(size, o);
+    }
+    // not above the label's logit as the product forms it, whose terms are added in another order: so S_j is at least 1.  (Both orders' errors, and
+    // that of scaling by log2(e); a few thousandths for ordinary logits.)
+    if (lane == 0) ref[i] = d - size * ((4 * chunks + 8) * 0x1p-23f);
 }
 // joins the tiles' statistics of 2^lc (at least 8) columns, finishes them, puts the label's entry right and scales H's image
 __global__ __launch_bounds__(256) void keep_kernel(Keep s, float *ht, int lc) {
@@ -918,18 +972,20 @@ __global__ __launch_bounds__(256) void keep_kernel(Keep s, float *ht, int lc) {
         by[at] = 0.f;
         if (i < cnt) {
             a = ps[at];
-            const float r = s.ref[i], sum = a.x == r ? a.y : a.y * exp2_(a.x - r), f = s.f[i];
+            const float r = s.ref[i], f = s.f[i];
+            const Scaled from = scaled(r);
+            const float sum = a.y * exp2_(__builtin_fmaf(a.x - r, LOG2E, from.rest));      // of E as it is stored
             const int lab = s.y[i];
             const float factor = f / (sum * s.a), size = fabsf(factor);
-            const bool good = sum < SUM_MOST && (f == 0.f || !(size < FACTOR_LEAST || (size > FACTOR_MOST && size < __builtin_inff())));
+            const bool good = sum < SUM_MOST && !big(r) && (f == 0.f || !(size < FACTOR_LEAST || (size > FACTOR_MOST && size < __builtin_inff())));
             float v = __builtin_nanf(""), l = v, c = v;
             if (lab >= 0) {
-                v = (a.x + log2f(a.y)) * LN2;
+                v = lse_of(a);
                 l = v - (1.f - s.eps) * s.zy[i];
                 if (s.zsum) l -= s.eps * (zs[at] / (float)s.p);
                 c = good ? factor : 1.f;
                 if (lab >= s.v0) {
-                    const float e = exp2_(__builtin_fmaf(s.zy[i], LOG2E, -r)) - sum * (1.f - s.eps);
+                    const float e = exp2_(__builtin_fmaf(s.zy[i], LOG2E, -from.x)) - sum * (1.f - s.eps);
                     *s.dz.at(i, lab - s.v0) = e;
                     *s.dzt.at(lab - s.v0, i) = e;
                 }

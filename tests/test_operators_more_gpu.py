@@ -87,3 +87,37 @@ def test_an_outlier_does_not_hold_up_the_call():
             best = min(best, a.elapsed_time(b))
         times[name] = best
     assert times["one"] < 2 * times["none"], times
+
+
+@pytest.mark.parametrize("dtype,k", [(d, k) for d in ("bf16", "f16") for k in (264, 512, 1000, 2048)] + [("f32", k) for k in (132, 500, 1024)])
+@pytest.mark.parametrize("n", [1, 7, 16])
+@pytest.mark.parametrize("p", [1031, 70001])
+def test_scoring_of_many_components(dtype, k, n, p):
+    """Up to 16 columns against rows of W that a wave reads in several parts (up to all of H's 64 KB), in one and in several groups of rows."""
+    W, H, y = problem(p, n, k, dtype, seed=k + n)
+    if n > 1:
+        y[n // 2] = -100
+    for eps in (0.0, 0.1):
+        want = oracle(W, H, y, eps, "none", dtype=dtype)
+        loss, lse = nmfx.softmax_xent(W, H, y, label_smoothing=eps, reduction="none")
+        near("loss", loss, want["loss"], want["eloss"])
+        near("lse", lse, want["lse"], want["else_"])
+    want = oracle(W, H, y, 0.1, "mean", dtype=dtype)
+    near("mean", nmfx.softmax_xent(W, H, y, label_smoothing=0.1)[0], want["loss"], want["eloss"])
+
+
+@pytest.mark.parametrize("p,n,k", [(300, 40, 64), (1024, 300, 300), (5000, 1000, 100)])
+@pytest.mark.parametrize("size", [1e6, 1e8, 1e9, 1e12])
+def test_logits_so_large_that_their_rounding_is(p, n, k, size):
+    """Float32 logits whose own rounding is beyond any exponential: exp(z - lse) still is between 0 and 1 (as the bounds take for granted), and
+    everything finite."""
+    W, H, y = problem(p, n, k, "f32", seed=3)
+    W, H = W * math.sqrt(size), H * math.sqrt(size)
+    loss, lse = nmfx.softmax_xent(W, H, y, reduction="none")
+    for eps in (0.0, 0.1):
+        loss, lse, dW, dH = nmfx.softmax_xent_grad(W, H, y, label_smoothing=eps, reduction="none")
+        want = oracle(W, H, y, eps, "none")
+        near("lse", lse, want["lse"], want["else_"])
+        near("loss", loss, want["loss"], want["eloss"])
+        near("dW", dW, want["dW"], want["edW"])
+        near("dH", dH, want["dH"], want["edH"])
