@@ -40,8 +40,11 @@ def pytest_collection_modifyitems(items):
 @pytest.fixture(scope="session")
 def built():
     """Make sure libnmfx.so and the C oracle exist (cross-compiles on CPU).  What is there is loaded: after a change to a source, build."""
+    # (a library of other sources would pass or fail for what they say)
     sys.path.insert(0, ROOT)
     import __graft_entry__ as g
     if not (os.path.exists(g.LIB) and os.path.exists(os.path.join(ROOT, "oracle", "libnmf_oracle.so"))):
         g.build()
+    if g.stale():
+        pytest.fail("libnmfx.so was built from other sources than are in csrc/ and include/ now: run build() of __graft_entry__.py first")
     return True
