@@ -95,14 +95,44 @@ def _stream(index):
     return raw(index) if raw else _torch().cuda.current_stream(index).cuda_stream
 
 
+def _no_graph():
+    """Outputs that torch's autograd takes for a function of W and H, and whose gradient it is refused: left out, it would be missing from a sum of
+    losses without a word."""
+    if "no_graph" not in _state:
+        torch = _torch()
+
+        class NoGraph(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, W, H, call):
+                return call()
+
+            @staticmethod
+            def backward(ctx, *grads):
+                raise ArgumentError("softmax_xent has no autograd graph: its gradients come from softmax_xent_grad or softmax_xent_backward "
+                                    "(detach() its results where they are to be constants)")
+
+        _state["no_graph"] = NoGraph
+    return _state["no_graph"]
+
+
 def softmax_xent(W, H, labels, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
     """Softmax cross entropy of the logits W @ H against one class per column, without keeping the logits: (loss, lse).
 
     W (p x k) and H (k x n) are float32, bfloat16 or float16 with one contiguous index each; labels has n int64 values, classes 0..p-1 or
     ignore_index.  loss is float32: n values for reduction 'none' (-loss is the label's log-probability), else one, the sum or the mean over
     the columns that are not ignored (0 where there is none).  lse, the log-sum-exp of every column's logits, has n values; both are 0 in
-    ignored columns.  A label that is no class makes its column's loss NaN."""
+    ignored columns.  A label that is no class makes its column's loss NaN.
+
+    There is no autograd graph behind them: a backward pass that reaches W or H through them (both count as functions of W and H while torch
+    records gradients) is refused.  softmax_xent_grad gives the gradients."""
     torch = _torch()
+    if (getattr(W, "requires_grad", False) or getattr(H, "requires_grad", False)) and torch.is_grad_enabled():
+        return _no_graph().apply(W, H, lambda: _forward(W, H, labels, ignore_index, label_smoothing, reduction))
+    return _forward(W, H, labels, ignore_index, label_smoothing, reduction)
+
+
+def _forward(W, H, labels, ignore_index, label_smoothing, reduction):
+    torch = _state["torch"]
     w, h, labels, o, index = _xent_args(W, H, labels, ignore_index, label_smoothing, reduction)
     lib, dev, n = L.load(), W.device, h.cols
     ws, size = _workspace(lib, w, h, o, 0, dev)
@@ -148,7 +178,9 @@ def softmax_xent_grad(W, H, labels, ignore_index=-100, label_smoothing=0.0, redu
     """softmax_xent with its gradients: (loss, lse, dW, dH).
 
     gout is the gradient with respect to the loss (float32; n values for reduction 'none', else one; None: 1; with float16 gradients a loss
-    scale belongs here).  dW and dH have the types of W and H and their contiguous index; matrices to write them to can be given."""
+    scale belongs here).  dW and dH have the types of W and H and their contiguous index; matrices to write them to can be given.
+
+    The results are constants to torch's autograd: dW and dH are the gradients, and go on from there as `H.backward(dH)` or into W.grad."""
     return _grad(W, H, labels, ignore_index, label_smoothing, reduction, gout, None, dW, dH)
 
 

@@ -140,3 +140,31 @@ def test_clip_by_a_coefficient_that_is_no_normal_float32(dtype, size):
             for b, t in zip(before, res):
                 want = b.double() * (max_norm / (norm + 1e-6))
                 assert ((t.double() - want).abs() <= (u + (3 * V if dtype != torch.float64 else 0.0)) * want.abs() + tiny).all()
+
+
+@pytest.mark.parametrize("n", [3, 100])
+def test_a_backward_pass_through_softmax_xent_is_refused(n):
+    """Its results have no graph: added to another loss, their part of the gradient must not be left out without a word."""
+    W, H, y = problem(200, n, 40, "f32")
+    want = nmfx.softmax_xent(W, H, y)
+    hidden = H.t().detach().clone().requires_grad_()
+    for a, b in ((W.clone().requires_grad_(), H), (W, hidden.t()), (torch.nn.Parameter(W), hidden.t())):
+        leaf = a if a.requires_grad else hidden
+        for part in (0, 1):
+            got = nmfx.softmax_xent(a, b, y)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+            with pytest.raises(nmfx.ArgumentError, match="softmax_xent_grad"):
+                (got[part].sum() + leaf.sum()).backward()
+            with pytest.raises(nmfx.ArgumentError, match="softmax_xent_grad"):
+                torch.autograd.grad(got[part].sum(), leaf)
+        with torch.no_grad():
+            assert not nmfx.softmax_xent(a, b, y)[0].requires_grad
+        leaf.grad = None
+        loss, lse = (t.detach() for t in nmfx.softmax_xent(a, b, y))
+        (loss + lse.sum() + leaf.sum()).backward()                    # a constant, and said to be one
+        assert (leaf.grad == 1).all()
+        for call in (lambda w, h: nmfx.softmax_xent_grad(w, h, y), lambda w, h: nmfx.softmax_xent_backward(w, h, y, lse)):
+            for g, x in zip(call(a, b), call(W, H)):
+                assert not g.requires_grad and torch.equal(g, x)
+    with pytest.raises(nmfx.DimensionMismatch):
+        nmfx.softmax_xent(torch.nn.Parameter(W), H[:, :2], y)
