@@ -23,7 +23,7 @@ _dtype_of = attrgetter("dtype")
 def _torch():
     if not _state:
         import torch
-        _state.update(raw=getattr(torch._C, "_cuda_getCurrentRawStream", None), torch=torch, bytes=torch.uint8, dtypes={torch.float32: L.F32, torch.float64: L.F64, torch.bfloat16: L.BF16, torch.float16: L.F16})
+        _state.update(raw=getattr(torch._C, "_cuda_getCurrentRawStream", None), torch=torch, bytes=torch.uint8, written=torch.autograd.graph.increment_version, dtypes={torch.float32: L.F32, torch.float64: L.F64, torch.bfloat16: L.BF16, torch.float16: L.F16})
     return _state["torch"]
 
 
@@ -163,6 +163,7 @@ def _grad(W, H, labels, ignore_index, label_smoothing, reduction, gout, lse, dW,
     else:
         lse = torch.empty(n, dtype=torch.float32, device=dev)
         loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=dev)
+    theirs = [t for t in (dW, dH) if t is not None]
     dW = _like(W, w, dev) if dW is None else dW
     dH = _like(H, h, dev) if dH is None else dH
     gw, gh = _matrix(dW, "dW", index), _matrix(dH, "dH", index)
@@ -171,6 +172,8 @@ def _grad(W, H, labels, ignore_index, label_smoothing, reduction, gout, lse, dW,
                                 ws.data_ptr(), size, index, _stream(index))
     if status:
         _ck(status)
+    if theirs:
+        _state["written"](theirs)
     return loss, lse, dW, dH
 
 
@@ -216,11 +219,12 @@ def _list(ts, name, device):
     a["rows"] = a["cs"] = 1
     a["dtype"] = codes[dtypes[0]] if len(kinds) == 1 else [codes[d] for d in dtypes]
     dense = list(map(T.is_contiguous, ts))
-    if not all(dense):
+    plain = all(dense)
+    if not plain:
         for i in range(len(ts)):
             if not dense[i]:
                 _strided(a, i, ts[i], name)
-    return a, sizes
+    return a, sizes, plain
 
 
 def _few(ts, index):
@@ -259,16 +263,15 @@ def _norm_type(norm_type):
 
 def _lists(grads, out, dev):
     """The descriptors of grads and of out (or None), as pointers to arrays that live as long as they do."""
-    a, sizes = _list(grads, "grads", dev)
+    a, sizes, plain = _list(grads, "grads", dev)
     if out is None:
         return _pointer(a), None
-    b, counts = _list(out, "out", dev)
+    b, counts, plain_too = _list(out, "out", dev)
     if sizes != counts:
         raise DimensionMismatch("one of out has another number of elements than its gradient")
     # where one of the two is not contiguous both go by the strides of their matrix
-    odd = (a["rows"] != 1) | (b["rows"] != 1)
-    if odd.any():
-        for i in np.nonzero(odd)[0]:
+    if not (plain and plain_too):
+        for i in np.nonzero((a["rows"] != 1) | (b["rows"] != 1))[0]:
             if grads[i].shape != out[i].shape:
                 raise DimensionMismatch("one of out has another shape than its gradient")
             _strided(a, i, grads[i], "grads")
@@ -306,14 +309,20 @@ def _norm(grads, max_norm, norm_type, out):
         a, b = _lists(grads, out, dev)
     lib = L.load()
     size = C.c_int64()
-    _ck(lib.nmfx_grad_norm_workspace(len(grads), size))
+    status = lib.nmfx_grad_norm_workspace(len(grads), size)
+    if status:
+        _ck(status)
     ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     common = (norm.data_ptr(), ws.data_ptr(), size.value, dev.index, _stream(dev.index))
     if max_norm is None:
         _ck(lib.nmfx_grad_norm(len(grads), a, kind, *common))
     else:
-        _ck(lib.nmfx_clip_grad_norm(len(grads), a, b or None, float(max_norm), kind, *common))
+        status = lib.nmfx_clip_grad_norm(len(grads), a, b or None, float(max_norm), kind, *common)
+        if status:
+            _ck(status)
+        # autograd is told what was written in place: a graph that has saved it refuses its backward pass then (0.05 us a tensor)
+        _state["written"](grads if out is None else out)
     return norm
 
 

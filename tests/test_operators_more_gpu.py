@@ -168,3 +168,35 @@ def test_a_backward_pass_through_softmax_xent_is_refused(n):
                 assert not g.requires_grad and torch.equal(g, x)
     with pytest.raises(nmfx.DimensionMismatch):
         nmfx.softmax_xent(torch.nn.Parameter(W), H[:, :2], y)
+
+
+def test_what_is_written_in_place_shows_to_autograd():
+    """A graph that has saved a tensor which is then written over must not go on with the new values."""
+    W, H, y = problem(60, 20, 16, "f32")
+
+    def saved(t):
+        x = torch.ones_like(t).requires_grad_()
+        return (x * t).sum()
+
+    t, u = torch.randn(40, 30, device=DEV), torch.randn(300, device=DEV)
+    out = [torch.empty_like(t), torch.empty_like(u)]
+    dW, dH = torch.empty_like(W), torch.empty_like(H)
+    with torch.inference_mode():
+        apart = torch.randn(10, device=DEV)
+    for targets, call in (([t, u], lambda: nmfx.clip_grad_norm([t, u, apart], 1.0)), (out, lambda: nmfx.clip_grad_norm([t, u], 1.0, out=out)),
+                          ([t[:, :7]], lambda: nmfx.clip_grad_norm([t[:, :7]], 1.0)), ([dW, dH], lambda: nmfx.softmax_xent_grad(W, H, y, dW=dW, dH=dH)),
+                          ([dH], lambda: nmfx.softmax_xent_backward(W, H, y, torch.zeros(20, device=DEV), dH=dH))):
+        graphs = [saved(x) for x in targets]
+        call()
+        for g in graphs:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                g.backward()
+    read = [saved(t), saved(u)]
+    nmfx.grad_norm([t, u])                                            # reads only
+    nmfx.clip_grad_norm([t, u], 1.0, out=out)
+    for g in read:
+        g.backward()
+    graph = saved(t)
+    with pytest.raises(nmfx.ArgumentError):
+        nmfx.clip_grad_norm([t], -1.0)                                # refused: nothing is written
+    graph.backward()
