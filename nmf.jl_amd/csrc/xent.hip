@@ -345,6 +345,8 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
     const float m = fmaxf(a.x, b.x);
     return make_float2(m, (a.y != 0.f ? a.y * exp2_((a.x - m) * LOG2E) : 0.f) + (b.y != 0.f ? b.y * exp2_((b.x - m) * LOG2E) : 0.f));
 }
+// the same where the references are mostly one
+__device__ __forceinline__ float2 join_same(float2 a, float2 b) { return a.x == b.x ? make_float2(a.x, a.y + b.y) : join(a, b); }
 __device__ __forceinline__ float lse_of(float2 a) { return __builtin_fmaf(log2f(a.y), LN2, a.x); }
 
 // ---- statistics of the logits: rows of D are classes, columns are packed columns ----------------------------------------------------
@@ -868,7 +870,7 @@ template <typename T, bool KEEP = false, bool SOME = false> struct EpiDz {
                 float t = sh.t[g.tid];
 #pragma unroll
                 for (int w = 1; w < WM; ++w) {
-                    s = join(s, sh.s[w * BN + g.tid]);
+                    s = join_same(s, sh.s[w * BN + g.tid]);
                     t += sh.t[w * BN + g.tid];
                 }
                 const int64_t o = (int64_t)g.tile_m * c.npad + g.tile_n * BN + g.tid;
@@ -955,7 +957,7 @@ __global__ __launch_bounds__(256) void keep_kernel(Keep s, float *ht, int lc) {
     if (i0 >= cnt) return;
     float2 a = make_float2(-__builtin_inff(), 0.f);
 #pragma unroll 4
-    for (int q = slice; q < s.tiles; q += step) a = join(a, s.part[(int64_t)q * s.npad + i]);
+    for (int q = slice; q < s.tiles; q += step) a = join_same(a, s.part[(int64_t)q * s.npad + i]);
     float t = 0.f;
     if (s.zsum)
         for (int q = slice; q < s.tiles; q += step) t += s.zsum[(int64_t)q * s.npad + i];
