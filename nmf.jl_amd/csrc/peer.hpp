@@ -260,7 +260,7 @@ struct PeerHandle {
     uint64_t ptr, bytes;
     uint64_t slot_bytes;
     hipIpcMemHandle_t ipc;
-    uint64_t place;        // of the device, whatever the process calls it: a hash of its PCI address
+    uint64_t place;        // of the device (device_place)
     int32_t queues, reserved;
 };
 static_assert(sizeof(PeerHandle) <= 128, "NMFX_P2P_HANDLE_BYTES");
@@ -359,8 +359,7 @@ struct PeerComm : Comm {
         h.slot_bytes = slot_bytes;
         char pci[64] = {};
         ck(hipDeviceGetPCIBusId(pci, sizeof pci - 1, dev), "hipDeviceGetPCIBusId");
-        h.place = 0xcbf29ce484222325ull;
-        for (const char *c = pci; *c; ++c) h.place = (h.place ^ (unsigned char)*c) * 0x100000001b3ull;
+        h.place = device_place(pci, dev, std::getenv("HIP_VISIBLE_DEVICES"), std::getenv("ROCR_VISIBLE_DEVICES"));
         h.queues = hw_queues(std::getenv("GPU_MAX_HW_QUEUES"));
         const hipError_t e = hipIpcGetMemHandle(&h.ipc, mine);
         if (e != hipSuccess) { (void)hipGetLastError(); std::memset(&h.ipc, 0, sizeof h.ipc); }   // same-process peers need the pointer only

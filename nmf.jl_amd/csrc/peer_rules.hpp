@@ -5,6 +5,7 @@
 #include <cstdint>
 #include <cstdlib>
 #include <mutex>
+#include <string>
 #include <vector>
 
 namespace nmfx {
@@ -41,8 +42,21 @@ struct WindowPool {
     }
 };
 
-// Where a rank is.  device: the same number for the same physical device, whatever a process calls it; queues: hardware queues that the rank's
-// process has on a device.
+// A number for a device, the same for two ranks only where they certainly use the same one: partitions of a card are devices of their own with one
+// PCI address, so a process's number of the device and what it sees of them count too.
+inline uint64_t device_place(const char *pci, int number, const char *visible, const char *visible_to_rocr) {
+    uint64_t h = 0xcbf29ce484222325ull;
+    auto add = [&](const char *s) {
+        for (; s && *s; ++s) h = (h ^ (unsigned char)*s) * 0x100000001b3ull;
+        h = (h ^ 0x1ffu) * 0x100000001b3ull;          // (no character)
+    };
+    add(pci);
+    add(std::to_string(number).c_str());
+    add(visible);
+    add(visible_to_rocr);
+    return h;
+}
+// Where a rank is.  device: as above; queues: hardware queues that the rank's process has on a device.
 struct PeerPlace {
     int32_t pid, queues;
     uint64_t device, window;

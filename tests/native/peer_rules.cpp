@@ -20,6 +20,7 @@ uint64_t pool_take(void *pool, int dev, unsigned flags, uint64_t *bytes) {
     *bytes = b;
     return reinterpret_cast<uint64_t>(p);
 }
+uint64_t place_of(const char *pci, int number, const char *visible, const char *visible_to_rocr) { return nmfx::device_place(pci, number, visible, visible_to_rocr); }
 int queues_of(const char *setting) { return nmfx::hw_queues(setting); }
 // ranks as pid, queues, device, window
 const char *layout_refusal(const uint64_t *ranks, int n) {

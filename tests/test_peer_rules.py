@@ -16,6 +16,7 @@ def rules(tmp_path_factory):
     lib.pool_new.restype = C.c_void_p
     lib.pool_take.restype = C.c_uint64
     lib.layout_refusal.restype = C.c_char_p
+    lib.place_of.restype = C.c_uint64
     return lib
 
 
@@ -123,3 +124,16 @@ def test_the_timing_stand_in_is_its_own_peer(rules):
 
 def test_the_runtime_s_number_of_queues(rules):
     assert [rules.queues_of(s) for s in (None, b"", b"4", b"24", b"x", b"-1", b"0")] == [4, 4, 4, 24, 4, 4, 4]
+
+
+def test_partitions_of_a_card_are_devices_of_their_own(rules):
+    """One PCI address, numbers or visible devices of their own: eight processes, one on each, are one process per device."""
+    pci = b"0000:05:00.0"
+    by_number = [rules.place_of(pci, r, None, None) for r in range(8)]
+    by_hip = [rules.place_of(pci, 0, b"%d" % r, None) for r in range(8)]
+    by_rocr = [rules.place_of(pci, 0, None, b"%d" % r) for r in range(8)]
+    assert len(set(by_number + by_hip + by_rocr)) >= 22 and len(set(by_number)) == len(set(by_hip)) == len(set(by_rocr)) == 8
+    for places in (by_number, by_hip, by_rocr):
+        assert refusal(rules, [(100 + r, 4, d) for r, d in enumerate(places)]) is None
+    assert rules.place_of(pci, 0, None, None) == rules.place_of(pci, 0, None, None) != rules.place_of(b"0000:06:00.0", 0, None, None)
+    assert rules.place_of(pci, 1, b"2", None) != rules.place_of(pci, 1, None, b"2") != rules.place_of(pci, 12, None, None)
