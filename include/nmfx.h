@@ -370,8 +370,8 @@ const char *nmfx_last_op_error(void);
  *                     (0 where there is none)
  *   lse               n values, or NULL
  * Types: W and H are both NMFX_F32, NMFX_BF16 or NMFX_F16 (NMFX_F64: NMFX_ERR_UNSUPPORTED); products are summed in Float32, loss and lse are
- * Float32.  p, n and the stride of W at most
- * 2^21 - 1024, k half of that.  n = 0 is allowed. */
+ * Float32.  p, n and the stride of W at most 2^21 - 1024, k half of that.  n = 0 is allowed.
+ * Workspace: copies of W and H where their orders do not serve the products, and statistics of about p n / 32 bytes. */
 typedef struct {
     double label_smoothing;   /* in [0, 1] */
     int64_t ignore_index;
@@ -390,7 +390,9 @@ int nmfx_xent(const nmfx_dmat *W, const nmfx_dmat *H, const int64_t *labels, con
  *              1: lse holds what nmfx_xent gave for the same W, H and labels, and is read; loss is not written
  * dZ is formed per piece of the classes and rounded to the type of W and H in front of the two products (Float16: scaled by a power of two
  * into its range first); the sums are Float32 and rounded once.  (Float32: where that is faster exp(Z - Z[label]) is kept from the first pass
- * and scaled afterwards.) */
+ * and scaled afterwards.)
+ * Workspace: as above, and two images of a piece's dZ of the type of W and H, at most 2^28 entries (or 256 classes) each: Z is not kept, but where it
+ * fits a piece the images are larger than it. */
 int nmfx_xent_grad(const nmfx_dmat *W, const nmfx_dmat *H, const int64_t *labels, const nmfx_xent_opts *opts, const float *gout,
                    int lse_given, float *loss, float *lse, const nmfx_dmat *dW, const nmfx_dmat *dH, void *workspace,
                    int64_t workspace_bytes, int device, void *stream);

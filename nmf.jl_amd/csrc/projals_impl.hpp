@@ -206,7 +206,7 @@ template <typename T> void Solver<T>::enqueue_projals(const nmfx_opts &o, long l
     // takes one CU from one engine slows the whole product by 1/8 -- scripts/kbench/cu_mask_probe.hip).  What works: the Gram
     // by its own small launch first, then the product launched `chol_slots` blocks SHORT (plan_short_grid: the missing items
     // ride as tail pieces, +1.6 % work per block) -- that leaves chol_slots half-empty CUs -- and the factorisation on a
-    // high-priority side stream with a 512-thread Cholesky workgroup (2 waves per SIMD x 128 registers = the free half of a
+    // side stream with a 512-thread Cholesky workgroup (2 waves per SIMD x 128 registers = the free half of a
     // CU).  Sharing its CU with a GEMM block the chain runs 4x slower (potrf 650 us, trtri 400 us), which still fits under the
     // 1.02 ms product: 2.75 -> 2.36 ms per iteration at 16384 x 16384, k = 256.  Replicated-W multi-GPU mode keeps the serial
     // order (its Gram travels inside the one packed all-reduce that follows the product).

@@ -133,7 +133,7 @@ template <typename T> class Solver : public SolverBase {
         num_cu = prop.multiProcessorCount;
         HIP_TRY(hipStreamCreateWithFlags(&stream, hipStreamNonBlocking));
         // ProjectedALS runs its single-workgroup factorisations UNDER the big products (projals_impl.hpp): the products launch
-        // `chol_slots` blocks short of two per CU, a high-priority side stream owns the half-empty CUs that leaves.
+        // `chol_slots` blocks short of two per CU, a side stream owns the half-empty CUs that leaves.
         // NMFX_CHOL_SLOTS=0 turns it off (factorisations between the products, as in round 1).
         if (const char *e = dev_env("NMFX_CHOL_SLOTS")) chol_slots = std::max(0, std::min(128, std::atoi(e)));
         if (const char *e = dev_env("NMFX_FORCE_SHARDED")) force_sharded = std::atoi(e) != 0;

@@ -351,7 +351,7 @@ __device__ __forceinline__ float lse_of(float2 a) { return __builtin_fmaf(log2f(
 
 // ---- statistics of the logits: rows of D are classes, columns are packed columns ----------------------------------------------------
 // Bound by the product where k is long (131072 x 8192, k = 2048: 3.26 ms, 1350 TFLOP/s); where it is short by the exponentials, which go in
-// the products' shadow only between blocks (131072 x 16384, k = 256: 1.30 ms, 845 TFLOP/s: 1.65 10^12 logits a second).
+// the products' shadow only between blocks (131072 x 16384, k = 256: 1.25 to 1.39 ms on several cards, 790 to 880 TFLOP/s).
 struct EpiStats {
     float2 *part;         // [tile_m][npad]: reference and sum over the tile's classes
     float *zsum;          // [tile_m][npad] or NULL
