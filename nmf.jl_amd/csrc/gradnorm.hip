@@ -141,7 +141,7 @@ struct Coef {
     float c1, c2;
 };
 __device__ __forceinline__ Coef coef_parts(double c) {
-    const bool tiny = c < 0x1p-100;
+    const bool tiny = c < 0x1p-126;      // (so c1 is below 1 either way, and x c1 does not overflow)
     return Coef{c, (float)(tiny ? c * 0x1p126 : c), tiny ? 0x1p-126f : 1.f};
 }
 template <typename T> __device__ __forceinline__ T scaled(T x, const Coef &c) {

@@ -126,9 +126,10 @@ def test_logits_so_large_that_their_rounding_is(p, n, k, size):
 @pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("size", [300, 50001])
 def test_clip_by_a_coefficient_that_is_no_normal_float32(dtype, size):
-    """Gradients near the largest numbers of their type and small norms to clip to: the coefficient is below 2^-126, the results are not."""
+    """Gradients near the largest numbers of their type and norms to clip to that are small beside them: the coefficient is near and below 2^-126,
+    the results are not."""
     big = {torch.float32: 3e38, torch.bfloat16: 3e38, torch.float16: 65504.0, torch.float64: 1e100}[dtype]
-    for max_norm in (1e-3, 1e-20, 1e-30):
+    for max_norm in (1e10, 1e6, 1e4, 100.0, 10.0, 1.0, 1e-3, 1e-20, 1e-30):
         for out in (False, True):
             ts = [torch.full((size,), big, device=DEV, dtype=torch.float64).to(dtype), torch.linspace(-big, big, 77, device=DEV, dtype=torch.float64).to(dtype)]
             ts[0][::3] = 0
@@ -138,7 +139,7 @@ def test_clip_by_a_coefficient_that_is_no_normal_float32(dtype, size):
             u = {torch.float32: V, torch.float64: 2.0 ** -50, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
             tiny = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 2.0 ** -150, torch.float64: 0.0}[dtype]   # half the smallest step
             for b, t in zip(before, res):
-                want = b.double() * (max_norm / (norm + 1e-6))
+                want = b.double() * min(1.0, max_norm / (norm + 1e-6))
                 assert ((t.double() - want).abs() <= (u + (3 * V if dtype != torch.float64 else 0.0)) * want.abs() + tiny).all()
 
 
